@@ -8,9 +8,13 @@ selection and the bf16 mixed-precision linear.  ``AXS6Linear`` aliases
 aliases of the HIP ones so existing call sites keep working; they run the
 HIP kernels, not Triton.  The training pipeline (``AXSTrainingPipelineUnified``,
 ``AmaxEMA``) runs its gradient unscale, overflow check and clipping as one
-fused device pass.  The distributed gradient hooks are not part of this
+fused device pass.  A decoder's operators beyond the reference's -- rotary
+positions, attention without the score matrix, the 8-bit cache and attention
+over it, distillation from a teacher's top logits -- run on HIP kernels of
+their own.  The distributed gradient hooks are not part of this
 package (the NF5 gradient codec is, in ``axs.unified.distributed``).
 """
+from axs.unified.attention_unified import AXSCausalSelfAttentionUnified, axs_attention_unified
 from axs.unified.backend import (
     BackendType,
     accelerated_fake_quantize,
@@ -22,6 +26,7 @@ from axs.unified.backend import (
     get_backend,
     set_backend,
 )
+from axs.unified.distillation_unified import axs_distillation_loss_unified
 from axs.unified.functional_unified import (
     axs_linear_group_unified,
     axs_linear_unified,
@@ -29,6 +34,12 @@ from axs.unified.functional_unified import (
     fake_quantize_unified,
 )
 from axs.unified.hip_kernels import has_hip, hip_fused_fake_quantize, hip_fused_linear
+from axs.unified.kv_cache_unified import (
+    AXSKVCacheUnified,
+    axs_cache_append_unified,
+    axs_cache_attention_unified,
+    axs_cache_read_unified,
+)
 from axs.unified.mixed_precision import (
     AXSLinearMixedPrecision,
     axs_linear_mixed_precision,
@@ -43,6 +54,7 @@ from axs.unified.modules_unified import (
     AXSMultiheadAttentionUnified,
     convert_to_axs_unified,
 )
+from axs.unified.rotary_unified import axs_rotary_unified, rotary_table
 from axs.unified.training_unified import AmaxEMA, AXSTrainingPipelineUnified
 from axs.unified.quantize_unified import (
     FUSED_NF5_LUT,
@@ -100,4 +112,13 @@ __all__ = [
     "estimate_memory_savings",
     "AXSTrainingPipelineUnified",
     "AmaxEMA",
+    "axs_rotary_unified",
+    "rotary_table",
+    "axs_attention_unified",
+    "AXSCausalSelfAttentionUnified",
+    "AXSKVCacheUnified",
+    "axs_cache_append_unified",
+    "axs_cache_read_unified",
+    "axs_cache_attention_unified",
+    "axs_distillation_loss_unified",
 ]

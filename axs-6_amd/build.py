@@ -7,10 +7,10 @@ axs._C in-tree.
 Each csrc/*.hip file is compiled with hipcc to an object in axs-6_amd/_build/
 (in parallel), then linked into axs-6_amd/axs/_lib/libaxs6.so, which exposes
 the C ABI declared in include/axs6.h (bound with ctypes by axs/_lib.py).
-csrc/torch_ext.cpp is compiled with the host C++ compiler against torch's
+csrc/torch_ext*.cpp are compiled with the host C++ compiler against torch's
 headers into axs-6_amd/axs/_C.so, a thin extension that calls that C ABI
-(the linear's host logic and autograd node); it links libaxs6.so through an
-$ORIGIN-relative run path.
+(the linear's and the decoder operators' host logic and autograd nodes); it
+links libaxs6.so through an $ORIGIN-relative run path.
 """
 from __future__ import annotations
 
@@ -27,7 +27,7 @@ CSRC = os.path.join(PKG, "csrc")
 BUILD = os.path.join(PKG, "_build")
 OUT_DIR = os.path.join(PKG, "axs", "_lib")
 OUT = os.path.join(OUT_DIR, "libaxs6.so")
-EXT_SRC = os.path.join(CSRC, "torch_ext.cpp")
+EXT_SRCS = [os.path.join(CSRC, f) for f in ("torch_ext.cpp", "torch_ext_decoder.cpp")]
 EXT_OUT = os.path.join(PKG, "axs", "_C.so")
 CXX = os.environ.get("CXX", "g++")
 
@@ -43,9 +43,9 @@ COMMON = [
 ]
 
 
-def ext_compile_command(obj: str) -> list[str]:
-    """g++ command line compiling the torch extension (torch's include paths
-    and C++ ABI flag; HIP headers for the current-stream query)."""
+def ext_compile_command(src: str, obj: str) -> list[str]:
+    """g++ command line compiling a source of the torch extension (torch's include
+    paths and C++ ABI flag; HIP headers for the current-stream query)."""
     import sysconfig
 
     import torch
@@ -58,16 +58,16 @@ def ext_compile_command(obj: str) -> list[str]:
     for inc in (*ce.include_paths(), sysconfig.get_paths()["include"], "/opt/rocm/include",
                 os.path.join(ROOT, "include")):
         cmd += ["-I", inc]
-    return cmd + ["-c", EXT_SRC, "-o", obj]
+    return cmd + ["-c", src, "-o", obj]
 
 
-def ext_link_command(obj: str, out: str) -> list[str]:
+def ext_link_command(objs: list[str], out: str) -> list[str]:
     """Links the extension against torch and libaxs6.so (found beside it at
     run time through $ORIGIN/_lib)."""
     from torch.utils import cpp_extension as ce
 
     torch_lib = ce.library_paths()[0]
-    return [CXX, "-shared", "-fPIC", obj, "-o", out,
+    return [CXX, "-shared", "-fPIC", *objs, "-o", out,
             "-L", torch_lib, "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10_hip",
             "-L", OUT_DIR, "-laxs6", "-Wl,-rpath,$ORIGIN/_lib", f"-Wl,-rpath,{torch_lib}"]
 
@@ -82,15 +82,15 @@ def _run(cmd: list[str], what: str, verbose: bool) -> None:
         print(r.stderr, file=sys.stderr)
 
 
-def compile_ext(verbose: bool) -> str:
-    obj = os.path.join(BUILD, "torch_ext.cpp.o")
-    _run(ext_compile_command(obj), "torch extension compile", verbose)
+def compile_ext(src: str, verbose: bool) -> str:
+    obj = os.path.join(BUILD, os.path.basename(src) + ".o")
+    _run(ext_compile_command(src, obj), "torch extension compile", verbose)
     return obj
 
 
-def link_ext(obj: str, verbose: bool) -> str:
+def link_ext(objs: list[str], verbose: bool) -> str:
     tmp = EXT_OUT + ".tmp"
-    _run(ext_link_command(obj, tmp), "torch extension link", verbose)
+    _run(ext_link_command(objs, tmp), "torch extension link", verbose)
     os.replace(tmp, EXT_OUT)
     return EXT_OUT
 
@@ -122,10 +122,10 @@ def build(verbose: bool = False, jobs: int | None = None) -> str:
     os.makedirs(OUT_DIR, exist_ok=True)
     srcs = sources()
     jobs = jobs or min(len(srcs), os.cpu_count() or 1, 16)
-    with cf.ThreadPoolExecutor(max_workers=jobs + 1) as ex:
-        ext_obj = ex.submit(compile_ext, verbose)
+    with cf.ThreadPoolExecutor(max_workers=jobs + len(EXT_SRCS)) as ex:
+        ext = [ex.submit(compile_ext, s, verbose) for s in EXT_SRCS]
         objs = list(ex.map(lambda s: compile_one(s, verbose), srcs))
-        ext_obj = ext_obj.result()
+        ext_objs = [e.result() for e in ext]
     tmp = OUT + ".tmp"
     cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-Wl,-soname,libaxs6.so", "-o", tmp, *objs]
     if verbose:
@@ -134,7 +134,7 @@ def build(verbose: bool = False, jobs: int | None = None) -> str:
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, OUT)
-    link_ext(ext_obj, verbose)
+    link_ext(ext_objs, verbose)
     return OUT
 
 

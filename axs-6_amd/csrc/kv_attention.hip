@@ -1,0 +1,366 @@
+// Attention of the newest tokens over the 8-bit cache (generation).
+//
+// Sequence b holds n_b tokens, the last Tq of which are the queries: query t
+// of head h sees keys j <= n_b - Tq + t of the key head h / G, G = Hq / Hkv:
+//   x_j = scale * ks * (q . kc_j),  o = sum_j softmax(x)_j vs * vc_j
+// with codes kc, vc and the block's scales ks, vs.  A query that sees nothing
+// gives 0.
+//
+// Bound by HBM: each code is read once, 2 D bytes a token and key head, for
+// all G * Tq rows that share them.  The products run on the matrix cores in
+// f16, where the codes are exact (|code| <= 127): a query row is scaled by a
+// power of two to [128, 256) and rounded to f16 (bf16 and f16 queries exactly,
+// but for values 2^-21 below the row's largest), a float32 query split in two
+// f16 terms (22 bits); probabilities go in as f16 times 2^14 (11 bits; for
+// float32 in two terms), so that one of 2^-28 of the largest still counts.
+// Maximum, sums and outputs are float32.
+//
+// S^T = K q^T by 16x16x32 instructions with the keys as rows: a lane then
+// holds 8 consecutive keys of one query row, which is the order in which the
+// second product takes them, so the probabilities never leave their registers.
+// A workgroup's four waves take every fourth block of its range; where there
+// are few rows the blocks are split over more workgroups and joined by a
+// second launch.
+#include <math.h>
+
+#include "axs6_internal.h"
+#include "kv_cache.h"
+#include "nf5_device.h"
+
+namespace axs6 {
+namespace {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kProbScale = 16384.0f;   // 2^14
+constexpr float kSumScale = 1048576.0f;  // 2^20: sums are held as 2^-20 of themselves, so that values near
+                                         // float32's largest, summed before they are divided, stay finite
+constexpr int kWaves = 4;
+
+struct KvAttnArgs {
+    const void* q;
+    int64_t qs[3];            // batch, token, head, in elements
+    const int8_t *kc, *vc;
+    const float *ks, *vs;
+    const int64_t* lengths;
+    void* out;                // (B, Tq, Hq, D) contiguous
+    float *part, *stat;       // of each split and row: the sums of D values; maximum and sum
+    int64_t rows_all;         // B * H * rows
+    int H, G, Tq, D, nb, rows, row_tiles, splits;
+    int qvec;
+    float scale;
+};
+
+// Eight int8 codes as f16: with the sign bit flipped a byte u is code + 128,
+// and the f16 with the bits 0x6400 | u is 1024 + u.
+__device__ __forceinline__ f16x8 codes_f16(uint32_t a, uint32_t b) {
+    union { uint32_t w[4]; f16x2 h[4]; f16x8 v; } r;
+    a ^= 0x80808080u;
+    b ^= 0x80808080u;
+    r.w[0] = __builtin_amdgcn_perm(0x64646464u, a, 0x04010400u);
+    r.w[1] = __builtin_amdgcn_perm(0x64646464u, a, 0x04030402u);
+    r.w[2] = __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u);
+    r.w[3] = __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u);
+    const f16x2 bias = {(_Float16)1152.0f, (_Float16)1152.0f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.h[i] = r.h[i] - bias;
+    return r.v;
+}
+
+__device__ __forceinline__ f32x4 mma(f16x8 a, f16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// Sixteen values of a query from element i.
+template <int DT>
+__device__ __forceinline__ void load16(const void* p, int64_t i, bool vec, float* f) {
+    using E = Elem<DT>;
+    const auto* q = reinterpret_cast<const typename E::S*>(p) + i;
+    if (vec) {
+#pragma unroll
+        for (int j = 0; j < 16; j += E::V) E::unpack(*reinterpret_cast<const u32x4*>(q + j), f + j);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) f[j] = E::to_f(q[j]);
+    }
+}
+
+// NC: 64-value pieces of a head.
+template <int DT, int NC>
+__global__ __launch_bounds__(64 * kWaves) void kv_attention_kernel(KvAttnArgs a) {
+    constexpr int TERMS = DT == AXS6_F32 ? 2 : 1;
+    constexpr int ND = NC * 4;   // 16-value pieces of a head
+    __shared__ float sh_o[2][ND * 4][64];
+    __shared__ float sh_m[kWaves][16], sh_l[kWaves][16];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n16 = lane & 15, g4 = lane >> 4;
+    const int rt = blockIdx.x % a.row_tiles, bh = blockIdx.x / a.row_tiles, h = bh % a.H, b = bh / a.H;
+    const int64_t cap = (int64_t)a.nb * kKvBlock;
+    int64_t len = a.lengths[b];
+    len = len < 0 ? 0 : len > cap ? cap : len;
+    const int r = rt * 16 + n16, rr = r < a.rows ? r : a.rows - 1, t = rr / a.G, hq = h * a.G + rr % a.G;
+    const int last = (int)(len - a.Tq) + t;   // the last key that this lane's row sees
+    const int r_top = rt * 16 + 15 < a.rows ? rt * 16 + 15 : a.rows - 1;
+    const int keys = (int)(len - a.Tq) + r_top / a.G + 1;
+    const int blocks = keys <= 0 ? 0 : (keys + kKvBlock - 1) / kKvBlock;
+    const int per = (blocks + a.splits - 1) / a.splits;
+    const int b0 = blockIdx.y * per, b1 = b0 + per < blocks ? b0 + per : blocks;
+
+    // the row's query, scaled, in the products' order: piece c, value 16 g4 + j
+    f16x8 qf[TERMS][NC][2];
+    float rs;
+    {
+        float f[NC][16], amax = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) f[c][j] = 0.0f;
+            if (64 * c + 16 * g4 < a.D)
+                load16<DT>(a.q, b * a.qs[0] + t * a.qs[1] + hq * a.qs[2] + 64 * c + 16 * g4, a.qvec, f[c]);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) amax = fmaxf(amax, fabsf(f[c][j]));
+        }
+        amax = fmaxf(amax, __shfl_xor(amax, 16, 64));
+        amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
+        const int e = amax > 0.0f && isfinite(amax) ? ilogbf(amax) - 7 : 0;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const float x = ldexpf(f[c][j], -e);
+                const _Float16 hi = (_Float16)x;
+                qf[0][c][j >> 3][j & 7] = hi;
+                if constexpr (TERMS == 2) qf[1][c][j >> 3][j & 7] = (_Float16)(x - (float)hi);
+            }
+        rs = ldexpf(a.scale * kLog2e, e);
+    }
+
+    f32x4 o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -INFINITY, l = 0.0f;
+    for (int blk = b0 + w; blk < b1; blk += kWaves) {
+        const int64_t cell = (int64_t)bh * a.nb + blk;
+        const int8_t* kc = a.kc + cell * kKvBlock * a.D;
+        const int8_t* vc = a.vc + cell * kKvBlock * a.D;
+        const float ks = a.ks[cell];
+        u32x4 kr[2][NC];
+        uint2 vr[ND];
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                kr[tt][c] = u32x4{0, 0, 0, 0};
+                const int key = 8 * (n16 >> 2) + 4 * tt + (n16 & 3);
+                if (64 * c + 16 * g4 < a.D)
+                    kr[tt][c] = *reinterpret_cast<const u32x4*>(kc + key * a.D + 64 * c + 16 * g4);
+            }
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+            vr[d] = make_uint2(0, 0);
+            if (16 * d < a.D) vr[d] = *reinterpret_cast<const uint2*>(vc + (16 * d + n16) * kKvBlock + 8 * g4);
+        }
+        // a row that sees none of the block takes nothing of it, whatever its scale
+        const float vs = blk * kKvBlock > last ? 0.0f : a.vs[cell] * (1.0f / (kProbScale * kSumScale));
+        float x[8], mx = -INFINITY;
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt) {
+            f32x4 s = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const f16x8 k0 = codes_f16(kr[tt][c].x, kr[tt][c].y), k1 = codes_f16(kr[tt][c].z, kr[tt][c].w);
+#pragma unroll
+                for (int u = 0; u < TERMS; ++u) {
+                    s = mma(k0, qf[u][c][0], s);
+                    s = mma(k1, qf[u][c][1], s);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int key = blk * kKvBlock + 8 * g4 + 4 * tt + i;
+                x[4 * tt + i] = key <= last ? s[i] * (rs * ks) : -INFINITY;
+                mx = fmaxf(mx, x[4 * tt + i]);
+            }
+        }
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float mn = fmaxf(m, mx), ref = mn == -INFINITY ? 0.0f : mn;
+        const float alpha = __builtin_amdgcn_exp2f(m - ref);
+        m = mn;
+        l *= alpha;
+        f16x8 pf[TERMS];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float p = __builtin_amdgcn_exp2f(x[j] - ref);
+            l += p;
+            const float y = p * kProbScale;
+            pf[0][j] = (_Float16)y;
+            if constexpr (TERMS == 2) pf[1][j] = (_Float16)(y - (float)pf[0][j]);
+        }
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+            if (16 * d >= a.D) continue;
+            const f16x8 vf = codes_f16(vr[d].x, vr[d].y);
+            f32x4 s = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int u = 0; u < TERMS; ++u) s = mma(vf, pf[u], s);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[d][i] = o[d][i] * alpha + s[i] * vs;
+        }
+    }
+    // join the waves: the four lanes of a row, then waves 2, 3 into 0, 1, then 1 into 0
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    if (g4 == 0) { sh_m[w][n16] = m; sh_l[w][n16] = l; }
+    __syncthreads();
+    float mt = sh_m[0][n16];
+#pragma unroll
+    for (int i = 1; i < kWaves; ++i) mt = fmaxf(mt, sh_m[i][n16]);
+    const float ref = mt == -INFINITY ? 0.0f : mt;
+    float lt = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) lt += sh_l[i][n16] * __builtin_amdgcn_exp2f(sh_m[i][n16] - ref);
+    const float f = __builtin_amdgcn_exp2f(m - ref);
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[d][i] *= f;
+#pragma unroll
+    for (int step = kWaves / 2; step >= 1; step >>= 1) {
+        if (w >= step && w < 2 * step)
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sh_o[w - step][d * 4 + i][lane] = o[d][i];
+        __syncthreads();
+        if (w < step)
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[d][i] += sh_o[w][d * 4 + i][lane];
+        __syncthreads();
+    }
+    if (w != 0 || r >= a.rows) return;
+    const int64_t row = (int64_t)bh * a.rows + r;
+    if (a.splits > 1) {
+        const int64_t at = blockIdx.y * a.rows_all + row;
+        if (g4 == 0) { a.stat[2 * at] = mt; a.stat[2 * at + 1] = lt; }
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+            if (16 * d < a.D) *reinterpret_cast<f32x4*>(a.part + at * a.D + 16 * d + 4 * g4) = o[d];
+        return;
+    }
+    const float rl = lt == 0.0f ? 0.0f : kSumScale / lt;
+    using E = Elem<DT>;
+    auto* out = reinterpret_cast<typename E::S*>(a.out) + (((int64_t)b * a.Tq + t) * a.H * a.G + hq) * a.D + 4 * g4;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+        if (16 * d < a.D)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) out[16 * d + i] = E::from_f(o[d][i] * rl);
+}
+
+// One wave a row: the splits' sums joined in order.
+template <int DT>
+__global__ __launch_bounds__(64) void kv_join_kernel(KvAttnArgs a) {
+    using E = Elem<DT>;
+    const int64_t row = blockIdx.x, bh = row / a.rows;
+    const int r = (int)(row - bh * a.rows), t = r / a.G, hq = (int)(bh % a.H) * a.G + r % a.G;
+    float mt = -INFINITY;
+    for (int s = 0; s < a.splits; ++s) mt = fmaxf(mt, a.stat[2 * (s * a.rows_all + row)]);
+    const float ref = mt == -INFINITY ? 0.0f : mt;
+    float lt = 0.0f;
+    const int d = threadIdx.x * 4;
+    f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = 0; s < a.splits; ++s) {
+        const int64_t at = s * a.rows_all + row;
+        const float f = __builtin_amdgcn_exp2f(a.stat[2 * at] - ref);
+        lt += a.stat[2 * at + 1] * f;
+        if (d < a.D) o += *reinterpret_cast<const f32x4*>(a.part + at * a.D + d) * f;
+    }
+    if (d >= a.D) return;
+    const float rl = lt == 0.0f ? 0.0f : kSumScale / lt;
+    auto* out = reinterpret_cast<typename E::S*>(a.out) +
+                (((bh / a.H) * a.Tq + t) * a.H * a.G + hq) * a.D + d;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = E::from_f(o[i] * rl);
+}
+
+template <int DT>
+void launch_attention(const KvAttnArgs& a, int64_t B, hipStream_t st) {
+    const dim3 grid((unsigned)(B * a.H * a.row_tiles), (unsigned)a.splits);
+    switch ((a.D + 63) / 64) {
+        case 1: kv_attention_kernel<DT, 1><<<grid, 64 * kWaves, 0, st>>>(a); break;
+        case 2: kv_attention_kernel<DT, 2><<<grid, 64 * kWaves, 0, st>>>(a); break;
+        case 3: kv_attention_kernel<DT, 3><<<grid, 64 * kWaves, 0, st>>>(a); break;
+        default: kv_attention_kernel<DT, 4><<<grid, 64 * kWaves, 0, st>>>(a); break;
+    }
+    if (a.splits > 1) kv_join_kernel<DT><<<(unsigned)a.rows_all, 64, 0, st>>>(a);
+}
+
+// Workgroups that share one set of rows: enough to give the chip's 256 CUs
+// four each, as long as a wave keeps two blocks.
+int split_count(int64_t groups, int64_t blocks) {
+    int64_t s = (1024 + groups - 1) / (groups > 0 ? groups : 1);
+    const int64_t most = blocks / (2 * kWaves);
+    s = s < most ? s : most;
+    return s < 1 ? 1 : (int)s;
+}
+
+}  // namespace
+}  // namespace axs6
+
+using namespace axs6;
+
+extern "C" int64_t axs6_kv_attention_workspace(int64_t B, int64_t Tq, int64_t Hq, int64_t H, int64_t D, int64_t blocks) {
+    if (B <= 0 || Tq <= 0 || H <= 0 || Hq <= 0 || Hq % H || D <= 0 || blocks <= 0) return 0;
+    const int64_t rows = Tq * (Hq / H), s = split_count(B * H * ((rows + 15) / 16), blocks);
+    return s == 1 ? 0 : s * B * H * rows * (D + 2) * (int64_t)sizeof(float);
+}
+
+extern "C" int axs6_kv_attention(const void* q, int32_t dtype, int64_t B, int64_t Tq, int64_t Hq, int64_t H, int64_t D,
+                                 const int64_t* q_strides, const void* k_codes, const float* k_scales,
+                                 const void* v_codes, const float* v_scales, int64_t blocks, const int64_t* lengths,
+                                 float scale, void* out, void* workspace, int64_t workspace_bytes, void* stream) {
+    const char* fn = "axs6_kv_attention";
+    if (!valid_dtype(dtype)) return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: unknown dtype code %d", fn, dtype);
+    int rc = check_cache(fn, B, H, D, blocks, k_codes, k_scales, v_codes, v_scales);
+    if (rc) return rc;
+    if (Tq < 0 || Hq < 0 || (H > 0 && Hq % H))
+        return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: %lld query heads for %lld key heads", fn, (long long)Hq, (long long)H);
+    if (!isfinite(scale)) return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: the scale must be finite", fn);
+    if (B * Tq * Hq == 0) return AXS6_OK;
+    if (H == 0 || blocks == 0) return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: an empty cache", fn);
+    if (!q || !q_strides || !lengths || !out) return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: null operand", fn);
+    const int64_t es = dtype == AXS6_F32 ? 4 : 2, vl = 16 / es, rows = Tq * (Hq / H);
+    if (rows > (1 << 24) || B * H * ((rows + 15) / 16) > ((int64_t)1 << 31) - 1 || B * H * rows > ((int64_t)1 << 31) - 1)
+        return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: dimension too large", fn);
+    if ((uintptr_t)q % es || (uintptr_t)out % es)
+        return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: pointer not element-aligned", fn);
+    KvAttnArgs a{};
+    a.q = q; a.kc = reinterpret_cast<const int8_t*>(k_codes); a.vc = reinterpret_cast<const int8_t*>(v_codes);
+    a.ks = k_scales; a.vs = v_scales; a.lengths = lengths; a.out = out;
+    a.qvec = (uintptr_t)q % 16 == 0;
+    for (int i = 0; i < 3; ++i) {
+        a.qs[i] = q_strides[i];
+        a.qvec = a.qvec && q_strides[i] % vl == 0;
+    }
+    a.H = (int)H; a.G = (int)(Hq / H); a.Tq = (int)Tq; a.D = (int)D; a.nb = (int)blocks; a.rows = (int)rows;
+    a.row_tiles = (int)((rows + 15) / 16); a.rows_all = B * H * rows; a.scale = scale;
+    a.splits = split_count(B * H * a.row_tiles, blocks);
+    if (a.splits > 1) {
+        const int64_t need = axs6_kv_attention_workspace(B, Tq, Hq, H, D, blocks);
+        if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16)
+            return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: a 16-byte aligned workspace of %lld bytes required, got %lld", fn,
+                        (long long)need, (long long)workspace_bytes);
+        a.part = reinterpret_cast<float*>(workspace);
+        a.stat = a.part + a.splits * a.rows_all * D;
+    }
+    hipStream_t st = (hipStream_t)stream;
+    if (dtype == AXS6_F32) launch_attention<AXS6_F32>(a, B, st);
+    else if (dtype == AXS6_BF16) launch_attention<AXS6_BF16>(a, B, st);
+    else launch_attention<AXS6_F16>(a, B, st);
+    return check_launch(fn);
+}

@@ -33,44 +33,23 @@
 //     records a graph it adds a per-device counter read on the device, which
 //     the graph advances once (after its first such call), so replays draw
 //     fresh dither values.
-#include <torch/extension.h>
-
-#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
-#include <c10/hip/HIPStream.h>
 
 #include <cstdint>
 #include <mutex>
 #include <optional>
 #include <unordered_map>
 
-#include "axs6.h"
+#include "torch_ext_common.h"
+
+using namespace axs6_ext;
 
 namespace {
 
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-int dtype_code(at::ScalarType t) {
-    switch (t) {
-        case at::kFloat: return AXS6_F32;
-        case at::kBFloat16: return AXS6_BF16;
-        case at::kHalf: return AXS6_F16;
-        default: return -1;
-    }
-}
-
 at::ScalarType compute_dtype(at::ScalarType t) { return dtype_code(t) >= 0 ? t : at::kFloat; }
-
-void check_rc(int rc, const char* fn) {
-    TORCH_CHECK(rc == 0, fn, " failed (status ", rc, "): ", axs6_last_error());
-}
-
-void require_device(const at::Tensor& t, const char* fn) {
-    TORCH_CHECK(t.is_cuda(), fn, " requires a CUDA (ROCm/HIP) device tensor, got device ", t.device());
-}
-
-void* stream_of(const at::Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 
 int64_t pad_amount(int64_t n, int64_t mult) { return (mult - n % mult) % mult; }
 
@@ -81,11 +60,8 @@ at::Tensor rows2d(const at::Tensor& t, int64_t cols) {
     return t.reshape({rows, cols});
 }
 
-// Row lengths the kernels take without a copy: whole 16-byte vectors (4
-// float32 or 8 bfloat16 / float16 values); a ragged last NF5 block is
-// zero-padded by the kernels themselves.
-int64_t vec_multiple(at::ScalarType dtype) { return dtype == at::kFloat ? 4 : 8; }
-
+// A ragged last NF5 block is zero-padded by the kernels themselves, so rows are
+// padded to whole vectors (vec_multiple) at most.
 at::Tensor pad_last(const at::Tensor& t, int64_t mult) {
     const int64_t p = pad_amount(t.size(-1), mult);
     return p ? at::constant_pad_nd(t, {0, p}) : t;
@@ -604,5 +580,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("graph_counter_advance", &advance_counter,
           "records the device's counter advance after a graph-recorded stochastic call (once per capture)",
           py::arg("device"));
+    register_decoder(m);
     m.def("next_seed", &next_seed, "a dither seed from torch's default CPU generator");
 }

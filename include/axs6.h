@@ -383,6 +383,103 @@ int axs6_layer_norm_backward(const void* dy, const void* x, int32_t dtype, int64
                              const float* mean, const float* rstd, const void* gamma, void* dx, float* dgamma,
                              float* dbeta, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- rotary positions --------------------------------------------------------
+ * Queries (B, T, Hq, D) and keys (B, T, Hkv, D) rotated by their positions, in
+ * one launch; the reference has no counterpart.  With c, s the cosines and
+ * sines of row p of the table (R/2 of each, float32) a pair (x0, x1) of a head's
+ * first R values becomes (x0 c - x1 s, x1 c + x0 s); a pair is x[i], x[i + R/2],
+ * or x[2i], x[2i + 1] with `interleaved`; x[R..D) is copied.  `inverse` negates s
+ * (the gradient).  Strides (host arrays of 3: batch, token, head) in elements,
+ * a head's values adjacent; outputs contiguous.  positions NULL: 0..T-1 of every
+ * sequence, else positions[b * pos_stride_b + t * pos_stride_t]; one outside the
+ * table gives NaN.  q or k may be NULL.  R even, D <= 512. */
+int axs6_rotary(const void* q, const void* k, void* q_out, void* k_out, int32_t dtype, int64_t B, int64_t T,
+                int64_t Hq, int64_t Hkv, int64_t D, int64_t R, const int64_t* q_strides, const int64_t* k_strides,
+                const float* table, int64_t table_rows, const int64_t* positions, int64_t pos_stride_b,
+                int64_t pos_stride_t, int32_t interleaved, int32_t inverse, void* stream);
+
+/* ---- attention ---------------------------------------------------------------
+ * out = softmax(scale q k^T + mask) v for queries (B, Tq, Hq, D) and keys and
+ * values (B, Tk, Hkv, D), Hq a multiple of Hkv (query head h reads key head
+ * h / (Hq / Hkv)); the core of the attention module without the reference's
+ * fake-quantized probabilities (axs/unified/modules_unified.py:245-262).
+ *   causal: query i sees keys j <= i + Tk - Tq;
+ *   mask_type -1: bytes, nonzero where a query sees a key; a dtype code: values
+ *   added to the scores (-inf: not seen); mask_strides (host array of 4: batch,
+ *   head, query, key) in elements, 0 for a broadcast dim;
+ *   a query that sees no key gives 0, and no gradient.
+ * D <= AXS6_ATTENTION_MAX_HEAD, D, every stride and pointer whole 16-byte vectors, a
+ * head's values adjacent; out and the gradients contiguous.  lse (B, Hq, Tq)
+ * floats is written by the forward (may be NULL there) and read by the
+ * backward, which overwrites delta (B, Hq, Tq) floats.  Products run on the
+ * matrix cores in the operands' type with float32 sums; no atomics, fixed
+ * orders.  scale positive and finite. */
+#define AXS6_ATTENTION_MAX_HEAD 128
+int axs6_attention_forward(const void* q, const void* k, const void* v, int32_t dtype, int64_t B, int64_t Tq,
+                           int64_t Tk, int64_t Hq, int64_t Hkv, int64_t D, const int64_t* q_strides,
+                           const int64_t* k_strides, const int64_t* v_strides, const void* mask, int32_t mask_type,
+                           const int64_t* mask_strides, int32_t causal, float scale, void* out, float* lse,
+                           void* stream);
+int axs6_attention_backward(const void* dout, const void* q, const void* k, const void* v, const void* out,
+                            const float* lse, int32_t dtype, int64_t B, int64_t Tq, int64_t Tk, int64_t Hq,
+                            int64_t Hkv, int64_t D, const int64_t* dout_strides, const int64_t* q_strides,
+                            const int64_t* k_strides, const int64_t* v_strides, const void* mask, int32_t mask_type,
+                            const int64_t* mask_strides, int32_t causal, float scale, float* delta, void* dq,
+                            void* dk, void* dv, void* stream);
+
+/* ---- 8-bit cache of keys and values --------------------------------------------
+ * Blocks of AXS6_KV_BLOCK tokens; for each block and head of keys and of values
+ * one float32 scale (the largest magnitude of the block's tokens over 127; NaN
+ * where the block holds a NaN or infinity) and int8 codes (value / scale rounded
+ * to even):
+ *   k_codes (B, H, blocks, AXS6_KV_BLOCK, D), v_codes (B, H, blocks, D, AXS6_KV_BLOCK),
+ *   k_scales, v_scales (B, H, blocks), and k_tail, v_tail (B, H, AXS6_KV_BLOCK, D) of
+ * `dtype`, the raw values of the block that is not full yet.
+ * append: k, v (B, n, H, D) (strides as above) become tokens starts[b].. of
+ *   sequence b; tokens past the capacity are dropped, and all of a sequence whose
+ *   start lies outside the cache; a start inside a block takes the block's earlier
+ *   tokens from the tail.
+ * read: tokens first[b] .. first[b] + count - 1 as float32 (B, count, H, D), code
+ *   times scale; 0 outside the cache.
+ * attention: q (B, Tq, Hq, D), the last Tq of the lengths[b] tokens of sequence b;
+ *   query t sees keys j <= lengths[b] - Tq + t (none: 0); out (B, Tq, Hq, D)
+ *   contiguous.  Needs axs6_kv_attention_workspace(...) bytes, 16-byte aligned.
+ * D a multiple of 16 up to AXS6_KV_MAX_HEAD; codes and tails 16-byte aligned;
+ * starts, first and lengths are read on the device. */
+#define AXS6_KV_BLOCK 32
+#define AXS6_KV_MAX_HEAD 256
+int axs6_kv_append(const void* k, const void* v, int32_t dtype, int64_t B, int64_t n, int64_t H, int64_t D,
+                   const int64_t* k_strides, const int64_t* v_strides, const int64_t* starts, int64_t blocks,
+                   void* k_codes, float* k_scales, void* v_codes, float* v_scales, void* k_tail, void* v_tail,
+                   void* stream);
+int axs6_kv_read(const void* k_codes, const float* k_scales, const void* v_codes, const float* v_scales, int64_t B,
+                 int64_t H, int64_t D, int64_t blocks, const int64_t* first, int64_t count, float* k_out, float* v_out,
+                 void* stream);
+int64_t axs6_kv_attention_workspace(int64_t B, int64_t Tq, int64_t Hq, int64_t H, int64_t D, int64_t blocks);
+int axs6_kv_attention(const void* q, int32_t dtype, int64_t B, int64_t Tq, int64_t Hq, int64_t H, int64_t D,
+                      const int64_t* q_strides, const void* k_codes, const float* k_scales, const void* v_codes,
+                      const float* v_scales, int64_t blocks, const int64_t* lengths, float scale, void* out,
+                      void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- distillation ----------------------------------------------------------------
+ * Loss of student logits (N, V) (rows ld apart) against a teacher's top K logits
+ * of each row (values, indices (N, K); an index below 0 leaves its entry out):
+ *   p = softmax(values / T) over the entries,  q = softmax(logits / T),
+ *   rows[r] = T^2 sum_k p_k (log p_k - log q_index_k),
+ *   loss = sum_r w_r rows[r], divided by sum_r w_r with `mean` (0 where that is 0).
+ * weights NULL: all 1; a row of weight 0 is not read.  An index at or past V
+ * gives the row NaN.  rows: N floats, stats: 2 N floats kept for the backward,
+ * loss and norm: one float each (loss may be NULL).  The backward writes
+ * dlogits (N, V) contiguous: T w_r (q - sum of p over an index) times grad_out
+ * (one float, or N with grad_rows) and norm[0] (NULL: 1). */
+int axs6_distill_forward(const void* logits, int32_t dtype, int64_t ld, int64_t N, int64_t V, const float* values,
+                         const int64_t* indices, int64_t K, float temperature, const float* weights, int32_t mean,
+                         float* rows, float* stats, float* loss, float* norm, void* stream);
+int axs6_distill_backward(const void* logits, int32_t dtype, int64_t ld, int64_t N, int64_t V, const float* values,
+                          const int64_t* indices, int64_t K, float temperature, const float* weights,
+                          const float* stats, const float* grad_out, int32_t grad_rows, const float* norm,
+                          void* dlogits, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
