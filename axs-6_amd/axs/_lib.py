@@ -80,9 +80,11 @@ _SIGNATURES: dict[str, list] = {
     "axs6_rotary": [_vp, _vp, _vp, _vp, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _i64,
                     _i64, _i32, _i32, _vp],
     "axs6_attention_forward": [_vp, _vp, _vp, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i32,
-                               _vp, _i32, ctypes.c_float, _vp, _vp, _vp],
+                               _vp, _i32, ctypes.c_float, _vp, _vp, _vp, _i64, _vp],
+    "axs6_attention_forward_workspace": [_i64, _i64, _i64, _i64, _i64],
+    "axs6_attention_backward_workspace": [_i64, _i64, _i64, _i64, _i64, _i64, _i32],
     "axs6_attention_backward": [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp,
-                                _vp, _vp, _vp, _i32, _vp, _i32, ctypes.c_float, _vp, _vp, _vp, _vp, _vp],
+                                _vp, _vp, _vp, _i32, _vp, _i32, ctypes.c_float, _vp, _vp, _vp, _vp, _vp, _i64, _vp],
     "axs6_kv_append": [_vp, _vp, _i32, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp,
                        _vp],
     "axs6_kv_read": [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp],
@@ -100,7 +102,8 @@ _RESTYPES = {"axs6_linear_padded_k": _i64, "axs6_nf5_linear_backward_workspace":
              "axs6_nf5_row_stats_workspace": _i64, "axs6_nf5_fused_linear_split_x": ctypes.c_int32,
              "axs6_nf5_fused_linear_split_workspace": _i64, "axs6_nf5_linear_infer_workspace": _i64,
              "axs6_nf5_linear_infer_stacked_workspace": _i64,
-             "axs6_layer_norm_backward_workspace": _i64, "axs6_kv_attention_workspace": _i64}
+             "axs6_layer_norm_backward_workspace": _i64, "axs6_kv_attention_workspace": _i64,
+             "axs6_attention_forward_workspace": _i64, "axs6_attention_backward_workspace": _i64}
 
 
 class LibraryError(RuntimeError):

@@ -26,6 +26,10 @@ struct AttnArgs {
     void *o, *dq, *dk, *dv;            // contiguous (B, T, H, D)
     int64_t qs[3], ks[3], vs[3], os[3], gs[3];   // strides of batch, token, head (q, k, v, out, dout)
     float *lse, *delta;                // (B, Hq, Tq); lse in units of log2, +inf where a row sees nothing
+    // Splits of the walked axis and their partial results: of the forward each
+    // row's sums, maximum and sum; of the backward dq, and dk and dv.
+    int splits, splits_kv;
+    float *part, *stat, *part_kv;
     const void* mask;
     int64_t ms[4];                     // strides of batch, head, query, key
     int mask_type;                     // -1: bytes, true where a query sees a key; else a type code: added
@@ -109,6 +113,22 @@ struct Tile {
         return *reinterpret_cast<const u32x4*>(tile + at(row0 + (lane & 31), 2 * s + (lane >> 5)));
     }
 
+    // Column 32 d + l % 32 of the 16 rows from row0 (16-bit types).
+    __device__ static u32x4 col_fragment(const char* tile, int row0, int d, int lane) {
+        const int h = lane >> 5, s = lane & 15, chunk = 4 * d + 2 * ((lane >> 4) & 1) + ((s & 3) >> 1);
+        u32x4 a;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int row = row0 + 8 * e + 4 * h + (s >> 2);
+            const s16x4 x =
+                __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + at(row, chunk) + (s & 1) * 8));
+            const u32x2 w = __builtin_bit_cast(u32x2, x);
+            a[2 * e] = w[0];
+            a[2 * e + 1] = w[1];
+        }
+        return a;
+    }
+
     // c += (columns 32 d .. 32 d + 31 of the 32 rows from row0)^T p, p a result
     // whose rows are these rows; pf: p in fragments (16-bit types).
     __device__ static f32x16 cols(const char* tile, int row0, int d, const f32x16& p, const u32x4 (&pf)[2], f32x16 c,
@@ -122,23 +142,35 @@ struct Tile {
                 c = __builtin_amdgcn_mfma_f32_32x32x2f32(x, p[i], c, 0, 0, 0);
             }
         } else {
-            const int s = lane & 15, chunk = 4 * d + 2 * ((lane >> 4) & 1) + ((s & 3) >> 1);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                u32x4 a;
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int row = row0 + 16 * j + 8 * e + 4 * h + (s >> 2);
-                    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (lds_s16x4*)(tile + at(row, chunk) + (s & 1) * 8));
-                    const u32x2 w = __builtin_bit_cast(u32x2, x);
-                    a[2 * e] = w[0];
-                    a[2 * e + 1] = w[1];
-                }
-                c = mma<DT>(a, pf[j], c);
-            }
+            for (int j = 0; j < 2; ++j) c = mma<DT>(col_fragment(tile, row0 + 16 * j, d, lane), pf[j], c);
         }
         return c;
+    }
+
+    // The same for the results p[n][j] of N sets of columns, into o[n][d]: the
+    // tile is read once.
+    template <int N, int NK, int ND>
+    __device__ static void cols_n(const char* tile, int j, int d, const f32x16 (&p)[N][NK], const u32x4 (&pf)[N][NK][2],
+                                  f32x16 (&o)[N][ND], int lane) {
+        const int h = lane >> 5;
+        if constexpr (DT == AXS6_F32) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int row = 32 * j + 8 * (i >> 2) + 4 * h + (i & 3), col = 32 * d + (lane & 31);
+                const float x = *reinterpret_cast<const float*>(tile + at(row, col >> 2) + (col & 3) * 4);
+#pragma unroll
+                for (int n = 0; n < N; ++n)
+                    o[n][d] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, p[n][j][i], o[n][d], 0, 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const u32x4 x = col_fragment(tile, 32 * j + 16 * e, d, lane);
+#pragma unroll
+                for (int n = 0; n < N; ++n) o[n][d] = mma<DT>(x, pf[n][j][e], o[n][d]);
+            }
+        }
     }
 };
 
@@ -153,32 +185,84 @@ __device__ __forceinline__ void fragments(const f32x16& p, u32x4 (&pf)[2]) {
     }
 }
 
-// A tile of R rows on its way from memory through registers into LDS; rows at
-// or past `rows` and values at or past D are zeros.
-template <int DT, int DC, int R, int THREADS>
-struct Stage {
+// The buffer descriptor of `bytes` bytes from p: loads past it give zeros.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* p, int64_t bytes) {
+    const int n = bytes < 0 ? 0 : bytes > 0x7fffffff ? 0x7fffffff : (int)bytes;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, n, 0x00020000);
+}
+typedef __attribute__((address_space(3))) void lds_void;
+
+// A tile of R rows straight from memory into LDS (16 bytes a lane, 1 KB a wave
+// and instruction, in slot order): rows past the last and values past D arrive
+// as zeros.  The caller waits on vmcnt and a barrier.
+template <int DT, int DC, int R, int WAVES>
+struct Direct {
     using T = Tile<DT, DC>;
-    static constexpr int kAll = R * T::kChunks, kN = (kAll + THREADS - 1) / THREADS;
-    u32x4 r[kN];
-    __device__ void load(const void* base, int64_t stride, int row0, int rows, int D) {
+    static constexpr int kSlots = T::kPitch / 16, kN = R * kSlots / 64 / WAVES;
+    static_assert(R * kSlots % (64 * WAVES) == 0, "whole instructions a wave");
+    int off[kN];
+    int pitch;   // bytes from a row to the next
+    __device__ void init(int64_t stride, int D, int lane, int w) {
+        pitch = (int)(stride * T::kBytes);
 #pragma unroll
         for (int i = 0; i < kN; ++i) {
-            const int c = threadIdx.x + i * THREADS, row = c / T::kChunks, ch = c % T::kChunks;
-            r[i] = u32x4{0, 0, 0, 0};
-            if (c < kAll && row0 + row < rows && ch * T::kVals < D)
-                r[i] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(base) +
-                                                       ((row0 + row) * stride + ch * T::kVals) * T::kBytes);
+            const int p = (i * WAVES + w) * 64 + lane, row = p / kSlots, chunk = (p % kSlots) ^ T::key(row);
+            off[i] = chunk * T::kVals < D ? row * pitch + chunk * 16 : 0x7fffffff;
         }
     }
-    __device__ void store(char* tile) const {
+    // rows row0 .. row0 + R - 1 of `rows`
+    __device__ void load(char* tile, const char* base, int row0, int rows, int D, int w) const {
+        const int left = rows - row0 < R ? rows - row0 : R;
+#if defined(__HIP_DEVICE_COMPILE__)   // the host pass knows no 16-byte form and would drop the kernel's stub
+        const auto rsrc = buffer_of(base + (int64_t)row0 * pitch, left <= 0 ? 0 : (int64_t)(left - 1) * pitch + D * T::kBytes);
 #pragma unroll
-        for (int i = 0; i < kN; ++i) {
-            const int c = threadIdx.x + i * THREADS;
-            if (kAll % THREADS == 0 || c < kAll)
-                *reinterpret_cast<u32x4*>(tile + T::at(c / T::kChunks, c % T::kChunks)) = r[i];
-        }
+        for (int i = 0; i < kN; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(tile + (i * WAVES + w) * 1024), 16, off[i], 0, 0, 0);
+#endif
     }
 };
+
+// Every load of this wave has arrived and every LDS read of it is done, then
+// the workgroup meets: tiles on their way may be read, read ones overwritten.
+__device__ __forceinline__ void tile_barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070);   // vmcnt(0) lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// The head and the piece (of `pieces`, the longest first) that workgroup `id`
+// takes.  Consecutive ids go round the 8 XCDs: where the heads divide by 8 each
+// XCD takes whole heads, one after another, whose keys its L2 then holds
+// (by_piece: all heads' first pieces, then their second ones); else the pieces go
+// round all heads, so that every XCD gets long and short ones.
+__device__ __forceinline__ void work_item(int id, int heads, int pieces, bool by_piece, int& head, int& piece) {
+    if (heads % 8 == 0) {
+        const int per = heads / 8, i = id >> 3;
+        head = (id & 7) * per + (by_piece ? i % per : i / pieces);
+        piece = by_piece ? i / per : i % pieces;
+    } else {
+        head = id % heads;
+        piece = id / heads;
+    }
+}
+
+// l + the sum of a fragment's values, as they are in the type.
+template <int DT>
+__device__ __forceinline__ float add_fragment(u32x4 f, float l) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t x = f[i];
+        if constexpr (DT == AXS6_F16) {
+            typedef _Float16 x2 __attribute__((ext_vector_type(2)));
+            l = __builtin_amdgcn_fdot2(__builtin_bit_cast(x2, x), x2{(_Float16)1.0f, (_Float16)1.0f}, l, false);
+        } else {
+            typedef __bf16 x2 __attribute__((ext_vector_type(2)));
+            l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(x2, x), x2{(__bf16)1.0f, (__bf16)1.0f}, l, false);
+        }
+    }
+    return l;
+}
 
 // One row of memory as row fragments: the lane's row is l % 32.
 template <int DT, int DC, int N>
@@ -194,18 +278,62 @@ __device__ __forceinline__ void load_rows(u32x4 (&f)[N], const void* base, int64
     }
 }
 
-// What the mask makes of x (the score times scale log2(e)); -inf where the
-// query does not see the key.  An added value below -1e38 counts as that: times
-// log2(e) it would be -inf, and a row of the type's lowest values, which
-// averages all its keys, would be taken for an empty one.
-__device__ __forceinline__ float masked(const AttnArgs& a, const char* row, int64_t k, float x) {
-    if (a.mask_type < 0) return row[k * a.ms[3]] ? x : -INFINITY;
+// How a mask is read: not at all; by key (the same for all queries of a head: a
+// tile's terms lie in LDS); by query and key.
+enum MaskKind { kNoMask, kKeyMask, kFullMask };
+
+// What the mask adds to a score in units of log2: -inf where the query does not
+// see the key.  An added value below -1e38 counts as that: times log2(e) it
+// would be -inf, and a row of the type's lowest values, which averages all its
+// keys, would be taken for an empty one.
+__device__ __forceinline__ float mask_term(const AttnArgs& a, const char* row, int64_t k) {
+    if (a.mask_type < 0) return row[k * a.ms[3]] ? 0.0f : -INFINITY;
     const float add = load_elem(row, a.mask_type, k * a.ms[3]);
-    return add == -INFINITY ? -INFINITY : x + fmaxf(add, -1e38f) * kLog2e + (add != add ? add : 0.0f);
+    return add == -INFINITY || add != add ? add : fmaxf(add, -1e38f) * kLog2e;
 }
 __device__ __forceinline__ const char* mask_row(const AttnArgs& a, int b, int h, int64_t q) {
     const int64_t bytes = a.mask_type < 0 ? 1 : a.mask_type == AXS6_F32 ? 4 : 2;
     return reinterpret_cast<const char*>(a.mask) + (b * a.ms[0] + h * a.ms[1] + q * a.ms[2]) * bytes;
+}
+// The terms of the four keys from k (those below Tk): one load where the mask is
+// bytes, adjacent and aligned.
+__device__ __forceinline__ void mask_terms(const AttnArgs& a, const char* row, int k, float (&f)[4]) {
+    const char* p = row + k;
+    if (a.mask_type < 0 && a.ms[3] == 1 && k + 4 <= a.Tk && (reinterpret_cast<uintptr_t>(p) & 3) == 0) {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[e] = (w >> (8 * e)) & 0xff ? 0.0f : -INFINITY;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[e] = k + e < a.Tk ? mask_term(a, row, k + e) : -INFINITY;
+    }
+}
+
+// The scores s of 32 keys from k0 (rows of the result) against the lane's
+// query, in units of log2, with the mask; `edge`: keys at or past limit are
+// not seen.  term: the keys' terms in LDS (by key).
+template <int MASK>
+__device__ __forceinline__ void apply_mask(const AttnArgs& a, f32x16& s, float c, int k0, const float* term,
+                                           const char* row, bool edge, int limit, int lane) {
+    const int h4 = 4 * (lane >> 5);
+    if constexpr (MASK != kNoMask) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            float f[4];
+            if constexpr (MASK == kKeyMask) {
+                const float4 t = *reinterpret_cast<const float4*>(term + 8 * g + h4);
+                f[0] = t.x; f[1] = t.y; f[2] = t.z; f[3] = t.w;
+            } else {
+                mask_terms(a, row, k0 + 8 * g + h4, f);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[4 * g + e] = f[e] == -INFINITY ? -INFINITY : __builtin_fmaf(s[4 * g + e], c, f[e]);
+        }
+    }
+    if (edge)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            s[i] = k0 + 8 * (i >> 2) + h4 + (i & 3) < limit ? s[i] : -INFINITY;
 }
 
 // A 32x32 result whose lanes are rows of memory: out[row][32 d + ...] of the

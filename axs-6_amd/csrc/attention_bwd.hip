@@ -9,35 +9,70 @@
 // The first holds 32 queries a wave and walks over the keys (dq, and delta for
 // the second); the second holds 32 keys a wave and walks over the queries of
 // all heads of the group (dk, dv).  Scores and do . v are computed in both: 7
-// products a pair instead of 5.
+// products a pair instead of 5.  Tiles travel as in the forward.
+// Under a causal mask the first keys are seen by far more queries than the
+// last: their queries are split over workgroups, whose float32 sums a third
+// launch adds (1 x 16384, 2 key heads for 16, bf16: 9072 -> 3824 us for both
+// launches; 2 x 4096, 8 for 32: 1511 -> 1127, of which dq 453).
 #include "attention.h"
 
 namespace axs6 {
 namespace {
 
-constexpr int kBwdThreads = 256, kBwdHeld = 128, kBwdWalk = 32;
+constexpr int kWaves = 4, kThr = 64 * kWaves, kHeld = 32 * kWaves;
+
+template <int DT, int DC> struct DqShape {
+    static constexpr int kKeys = DT == AXS6_F32 ? 32 : 64;
+    static constexpr int kOccupancy = DT == AXS6_F32 ? 1 : 2;
+};
 
 // dq of 128 queries; the loop is the forward's.
-template <int DT, int DC, bool MASK>
-__global__ __launch_bounds__(kBwdThreads) void attn_dq_kernel(AttnArgs a) {
+template <int DT, int DC, int MASK>
+__global__ __launch_bounds__(kThr, (DqShape<DT, DC>::kOccupancy)) void attn_dq_kernel(AttnArgs a) {
     using T = Tile<DT, DC>;
-    __shared__ __attribute__((aligned(16))) char kt[kBwdWalk * T::kPitch];
-    __shared__ __attribute__((aligned(16))) char vt[kBwdWalk * T::kPitch];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int heads = a.B * a.Hq, bh = blockIdx.x % heads, b = bh / a.Hq, hq = bh % a.Hq, h = hq / a.G;
-    const int q0 = ((int)(gridDim.x / heads) - 1 - (int)(blockIdx.x / heads)) * kBwdHeld;
-    const int q = q0 + 32 * w + (lane & 31), qr = q < a.Tq ? q : a.Tq - 1;
+    constexpr int KEYS = DqShape<DT, DC>::kKeys, NK = KEYS / 32;
+    __shared__ __attribute__((aligned(1024))) char kt[2][KEYS * T::kPitch];
+    __shared__ __attribute__((aligned(1024))) char vt[2][KEYS * T::kPitch];
+    __shared__ __attribute__((aligned(16))) float term[2][MASK == kKeyMask ? KEYS : 1];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int q_tiles = (a.Tq + kHeld - 1) / kHeld;
+    int bh, piece;
+    work_item(blockIdx.x, a.B * a.Hq, q_tiles * a.splits, false, bh, piece);
+    const int b = bh / a.Hq, hq = bh % a.Hq, h = hq / a.G, split = piece % a.splits;
+    const int q0 = (q_tiles - 1 - piece / a.splits) * kHeld;
     const int off = a.Tk - a.Tq;
-    const int q_last = q0 + kBwdHeld < a.Tq ? q0 + kBwdHeld - 1 : a.Tq - 1;
+    const int q_last = q0 + kHeld < a.Tq ? q0 + kHeld - 1 : a.Tq - 1;
     int keys = a.causal ? q_last + off + 1 : a.Tk;
     keys = keys < 0 ? 0 : keys > a.Tk ? a.Tk : keys;
-    const int tiles = (keys + kBwdWalk - 1) / kBwdWalk;
-    const int limit = a.causal ? (qr + off + 1 < a.Tk ? qr + off + 1 : a.Tk) : a.Tk;
+    int first = 0, tiles = (keys + KEYS - 1) / KEYS;
+    if (a.splits > 1) {
+        const int per = (tiles + a.splits - 1) / a.splits;
+        first = split * per < tiles ? split * per : tiles;
+        tiles = first + per < tiles ? first + per : tiles;
+    }
     const int free_keys = a.causal ? q0 + off + 1 : a.Tk;
+    const int free_tiles = free_keys <= 0 ? 0 : (free_keys < a.Tk ? free_keys : a.Tk) / KEYS;
 
     const char* kb = reinterpret_cast<const char*>(a.k) + (b * a.ks[0] + h * a.ks[2]) * T::kBytes;
     const char* vb = reinterpret_cast<const char*>(a.v) + (b * a.vs[0] + h * a.vs[2]) * T::kBytes;
-    const char* mrow = MASK ? mask_row(a, b, hq, qr) : nullptr;
+    Direct<DT, DC, KEYS, kWaves> dk, dv;
+    dk.init(a.ks[1], a.D, lane, w);
+    dv.init(a.vs[1], a.D, lane, w);
+    auto key_term = [&](int t) {
+        const int key = t * KEYS + threadIdx.x;
+        return threadIdx.x < KEYS && key < a.Tk ? mask_term(a, mask_row(a, b, hq, 0), key) : -INFINITY;
+    };
+    if (first < tiles) {
+        dk.load(kt[first & 1], kb, first * KEYS, a.Tk, a.D, w);
+        dv.load(vt[first & 1], vb, first * KEYS, a.Tk, a.D, w);
+        if constexpr (MASK == kKeyMask) {
+            const float f = key_term(first);
+            if (threadIdx.x < KEYS) term[first & 1][threadIdx.x] = f;
+        }
+    }
+    const int q = q0 + 32 * w + (lane & 31), qr = q < a.Tq ? q : a.Tq - 1;
+    const int limit = a.causal && qr + off + 1 < a.Tk ? qr + off + 1 : a.Tk;
+    const char* mrow = MASK == kFullMask ? mask_row(a, b, hq, qr) : nullptr;
     u32x4 qf[T::kSteps], gf[T::kSteps];
     load_rows<DT, DC>(qf, a.q, b * a.qs[0] + qr * a.qs[1] + hq * a.qs[2], a.D, lane);
     load_rows<DT, DC>(gf, a.dout, b * a.gs[0] + qr * a.gs[1] + hq * a.gs[2], a.D, lane);
@@ -55,136 +90,200 @@ __global__ __launch_bounds__(kBwdThreads) void attn_dq_kernel(AttnArgs a) {
             for (int i = 0; i < T::kVals; ++i) delta += x[i] * y[i];
         }
         delta += __shfl_xor(delta, 32, 64);
-        if (lane < 32 && q < a.Tq) a.delta[row] = delta;
+        if (lane < 32 && q < a.Tq && split == 0) a.delta[row] = delta;
     }
     const float lse = a.lse[row], c = a.scale * kLog2e;
 
     f32x16 dq[DC / 32];
 #pragma unroll
     for (int d = 0; d < DC / 32; ++d) dq[d] = zero16();
-    Stage<DT, DC, kBwdWalk, kBwdThreads> sk, sv;
-    if (tiles) {
-        sk.load(kb, a.ks[1], 0, a.Tk, a.D);
-        sv.load(vb, a.vs[1], 0, a.Tk, a.D);
-    }
-    for (int t = 0; t < tiles; ++t) {
-        __syncthreads();
-        sk.store(kt);
-        sv.store(vt);
-        __syncthreads();
-        const int k0 = t * kBwdWalk;
+    for (int t = first; t < tiles; ++t) {
+        tile_barrier();
+        float next_term = 0.0f;
         if (t + 1 < tiles) {
-            sk.load(kb, a.ks[1], k0 + kBwdWalk, a.Tk, a.D);
-            sv.load(vb, a.vs[1], k0 + kBwdWalk, a.Tk, a.D);
+            dk.load(kt[(t + 1) & 1], kb, (t + 1) * KEYS, a.Tk, a.D, w);
+            dv.load(vt[(t + 1) & 1], vb, (t + 1) * KEYS, a.Tk, a.D, w);
+            if constexpr (MASK == kKeyMask) next_term = key_term(t + 1);
         }
-        f32x16 s = zero16(), dp = zero16();
+        const char *ks = kt[t & 1], *vs = vt[t & 1];
+        const int k0 = t * KEYS;
+        bool any = true;
+        if constexpr (MASK == kKeyMask) any = __any(!(term[t & 1][lane & (KEYS - 1)] == -INFINITY));
+        if (any) {
 #pragma unroll
-        for (int i = 0; i < T::kSteps; ++i) s = mma<DT>(T::rows(kt, 0, i, lane), qf[i], s);
+            for (int j = 0; j < NK; ++j) {
+                f32x16 s = zero16(), dp = zero16();
 #pragma unroll
-        for (int i = 0; i < T::kSteps; ++i) dp = mma<DT>(T::rows(vt, 0, i, lane), gf[i], dp);
-        const bool whole = k0 + kBwdWalk <= free_keys && k0 + kBwdWalk <= a.Tk;
+                for (int i = 0; i < T::kSteps; ++i) s = mma<DT>(T::rows(ks, 32 * j, i, lane), qf[i], s);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int key = k0 + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3);
-            float x = s[i] * c;
-            if constexpr (MASK) x = key < limit ? masked(a, mrow, key, x) : -INFINITY;
-            else if (!whole) x = key < limit ? x : -INFINITY;
-            s[i] = __builtin_amdgcn_exp2f(x - lse) * (dp[i] - delta);
+                for (int i = 0; i < T::kSteps; ++i) dp = mma<DT>(T::rows(vs, 32 * j, i, lane), gf[i], dp);
+                apply_mask<MASK>(a, s, c, k0 + 32 * j, &term[t & 1][MASK == kKeyMask ? 32 * j : 0], mrow,
+                                 t >= free_tiles, limit, lane);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float x = MASK == kNoMask ? __builtin_fmaf(s[i], c, -lse) : s[i] - lse;
+                    s[i] = __builtin_amdgcn_exp2f(x) * (dp[i] - delta);
+                }
+                u32x4 pf[2];
+                fragments<DT>(s, pf);
+#pragma unroll
+                for (int d = 0; d < DC / 32; ++d) dq[d] = T::cols(ks, 32 * j, d, s, pf, dq[d], lane);
+            }
         }
-        u32x4 pf[2];
-        fragments<DT>(s, pf);
-#pragma unroll
-        for (int d = 0; d < DC / 32; ++d) dq[d] = T::cols(kt, 0, d, s, pf, dq[d], lane);
+        if constexpr (MASK == kKeyMask)
+            if (threadIdx.x < KEYS) term[(t + 1) & 1][threadIdx.x] = next_term;
     }
     if (q >= a.Tq) return;
     const int64_t out = (((int64_t)b * a.Tq + q) * a.Hq + hq) * a.D;
+    if (a.splits > 1) {
+        float* part = a.part + split * ((int64_t)a.B * a.Tq * a.Hq * a.D);
+#pragma unroll
+        for (int d = 0; d < DC / 32; ++d) store_cols<AXS6_F32>(part, out, d, dq[d], a.scale, a.D, lane);
+        return;
+    }
 #pragma unroll
     for (int d = 0; d < DC / 32; ++d) store_cols<DT>(a.dq, out, d, dq[d], a.scale, a.D, lane);
 }
 
+constexpr int kWalk = 32;   // queries of a tile
+
+template <int DT, int DC> struct DkvShape {
+    // the values held stay in LDS where their fragments would leave a wave more
+    // than half of a SIMD's registers
+    static constexpr bool kVInLds = DC > 96;
+    static constexpr int kOccupancy = DT == AXS6_F32 ? 1 : 2;
+};
+
 // dk and dv of 128 keys of one key head.
-template <int DT, int DC, bool MASK>
-__global__ __launch_bounds__(kBwdThreads) void attn_dkv_kernel(AttnArgs a) {
+template <int DT, int DC, int MASK>
+__global__ __launch_bounds__(kThr, (DkvShape<DT, DC>::kOccupancy)) void attn_dkv_kernel(AttnArgs a) {
     using T = Tile<DT, DC>;
-    __shared__ __attribute__((aligned(16))) char qt[kBwdWalk * T::kPitch];
-    __shared__ __attribute__((aligned(16))) char gt[kBwdWalk * T::kPitch];
-    __shared__ __attribute__((aligned(16))) float lt[kBwdWalk], dt[kBwdWalk];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int heads = a.B * a.H, bh = blockIdx.x % heads, b = bh / a.H, h = bh % a.H;
-    const int k0 = blockIdx.x / heads * kBwdHeld;   // the first keys have the most queries under a causal mask
+    constexpr bool VL = DkvShape<DT, DC>::kVInLds;
+    __shared__ __attribute__((aligned(1024))) char qt[2][kWalk * T::kPitch];
+    __shared__ __attribute__((aligned(1024))) char gt[2][kWalk * T::kPitch];
+    __shared__ __attribute__((aligned(1024))) char vt[VL ? kHeld * T::kPitch : 16];
+    __shared__ __attribute__((aligned(16))) float lt[2][kWalk], dt[2][kWalk];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int k_tiles = (a.Tk + kHeld - 1) / kHeld;
+    int bh, piece;
+    work_item(blockIdx.x, a.B * a.H, k_tiles * a.splits_kv, true, bh, piece);
+    const int b = bh / a.H, h = bh % a.H, split = piece % a.splits_kv;
+    const int k0 = piece / a.splits_kv * kHeld;   // the first keys have the most queries under a causal mask
     const int key = k0 + 32 * w + (lane & 31), kr = key < a.Tk ? key : a.Tk - 1;
     const int off = a.Tk - a.Tq;
     int q_first = a.causal ? k0 - off : 0;   // the first query that sees one of the keys
-    q_first = q_first < 0 ? 0 : q_first / kBwdWalk * kBwdWalk;
-    const int per_head = q_first < a.Tq ? (a.Tq - q_first + kBwdWalk - 1) / kBwdWalk : 0;
-    const int tiles = per_head * a.G;
-    const int free_q = a.causal ? k0 + kBwdHeld - 1 - off : 0;   // from here on every query sees every key held
+    q_first = q_first < 0 ? 0 : q_first / kWalk * kWalk;
+    const int per_head = q_first < a.Tq ? (a.Tq - q_first + kWalk - 1) / kWalk : 0;
+    int first = 0, tiles = per_head * a.G;   // the group's heads one after another
+    if (a.splits_kv > 1) {
+        const int per = (tiles + a.splits_kv - 1) / a.splits_kv;
+        first = split * per < tiles ? split * per : tiles;
+        tiles = first + per < tiles ? first + per : tiles;
+    }
+    const int free_q = a.causal ? k0 + kHeld - 1 - off : 0;   // from here on every query sees every key held
 
-    u32x4 kf[T::kSteps], vf[T::kSteps];
-    load_rows<DT, DC>(kf, a.k, b * a.ks[0] + kr * a.ks[1] + h * a.ks[2], a.D, lane);
-    load_rows<DT, DC>(vf, a.v, b * a.vs[0] + kr * a.vs[1] + h * a.vs[2], a.D, lane);
-    f32x16 dk[DC / 32], dv[DC / 32];
-#pragma unroll
-    for (int d = 0; d < DC / 32; ++d) { dk[d] = zero16(); dv[d] = zero16(); }
-    const float c = a.scale * kLog2e;
-    Stage<DT, DC, kBwdWalk, kBwdThreads> sq, sg;
-    float sl = INFINITY, sd = 0.0f;
-    auto load = [&](int t) {
-        const int hq = h * a.G + t / per_head, i0 = q_first + t % per_head * kBwdWalk;
-        sq.load(reinterpret_cast<const char*>(a.q) + (b * a.qs[0] + hq * a.qs[2]) * T::kBytes, a.qs[1], i0, a.Tq, a.D);
-        sg.load(reinterpret_cast<const char*>(a.dout) + (b * a.gs[0] + hq * a.gs[2]) * T::kBytes, a.gs[1], i0, a.Tq, a.D);
-        if (threadIdx.x < kBwdWalk) {
+    Direct<DT, DC, kWalk, kWaves> lq, lg;
+    lq.init(a.qs[1], a.D, lane, w);
+    lg.init(a.gs[1], a.D, lane, w);
+    const char* vb = reinterpret_cast<const char*>(a.v) + (b * a.vs[0] + h * a.vs[2]) * T::kBytes;
+    if constexpr (VL) {
+        Direct<DT, DC, kHeld, kWaves> lv;
+        lv.init(a.vs[1], a.D, lane, w);
+        lv.load(vt, vb, k0, a.Tk, a.D, w);
+    }
+    // head and first query of the tile on its way
+    int hq = h * a.G + (per_head ? first / per_head : 0), i0 = q_first + (per_head ? first % per_head : 0) * kWalk;
+    float sl = 0.0f, sd = 0.0f;
+    auto load = [&](int buf) {
+        lq.load(qt[buf], reinterpret_cast<const char*>(a.q) + (b * a.qs[0] + hq * a.qs[2]) * T::kBytes, i0, a.Tq, a.D, w);
+        lg.load(gt[buf], reinterpret_cast<const char*>(a.dout) + (b * a.gs[0] + hq * a.gs[2]) * T::kBytes, i0, a.Tq, a.D, w);
+        if (threadIdx.x < kWalk) {
             const int i = i0 + threadIdx.x;
             const int64_t row = ((int64_t)b * a.Hq + hq) * a.Tq + i;
             sl = i < a.Tq ? a.lse[row] : INFINITY;   // rows past the end have no probabilities
             sd = i < a.Tq ? a.delta[row] : 0.0f;
         }
     };
-    if (tiles) load(0);
-    for (int t = 0; t < tiles; ++t) {
-        __syncthreads();
-        sq.store(qt);
-        sg.store(gt);
-        if (threadIdx.x < kBwdWalk) { lt[threadIdx.x] = sl; dt[threadIdx.x] = sd; }
-        __syncthreads();
-        const int hq = h * a.G + t / per_head, i0 = q_first + t % per_head * kBwdWalk;
-        if (t + 1 < tiles) load(t + 1);
-        f32x16 s = zero16(), dp = zero16();
+    auto store = [&](int buf) {
+        if (threadIdx.x < kWalk) { lt[buf][threadIdx.x] = sl; dt[buf][threadIdx.x] = sd; }
+    };
+    if (first < tiles) {
+        load(first & 1);
+        store(first & 1);
+    }
+    u32x4 kf[T::kSteps], vf[VL ? 1 : T::kSteps];
+    load_rows<DT, DC>(kf, a.k, b * a.ks[0] + kr * a.ks[1] + h * a.ks[2], a.D, lane);
+    if constexpr (!VL) load_rows<DT, DC>(vf, a.v, b * a.vs[0] + kr * a.vs[1] + h * a.vs[2], a.D, lane);
+    f32x16 dk[DC / 32], dv[DC / 32];
 #pragma unroll
-        for (int i = 0; i < T::kSteps; ++i) s = mma<DT>(T::rows(qt, 0, i, lane), kf[i], s);
+    for (int d = 0; d < DC / 32; ++d) { dk[d] = zero16(); dv[d] = zero16(); }
+    const float c = a.scale * kLog2e;
+    float term = 0.0f;   // the mask's of the lane's key
+    for (int t = first; t < tiles; ++t) {
+        tile_barrier();
+        const int hq_now = hq, i_now = i0;
+        if constexpr (MASK == kKeyMask)
+            if (t == first || i_now == q_first) term = mask_term(a, mask_row(a, b, hq_now, 0), kr);
+        i0 += kWalk;
+        if (i0 >= a.Tq) { i0 = q_first; ++hq; }
+        if (t + 1 < tiles) load((t + 1) & 1);
+        const char *qs = qt[t & 1], *gs = gt[t & 1];
+        bool any = true;
+        if constexpr (MASK == kKeyMask) any = __any(!(term == -INFINITY));
+        if (any) {
+            f32x16 s = zero16(), dp = zero16();
 #pragma unroll
-        for (int i = 0; i < T::kSteps; ++i) dp = mma<DT>(T::rows(gt, 0, i, lane), vf[i], dp);
-        const bool whole = i0 >= free_q;
+            for (int i = 0; i < T::kSteps; ++i) s = mma<DT>(T::rows(qs, 0, i, lane), kf[i], s);
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const float4 lse = *reinterpret_cast<const float4*>(lt + 8 * g + 4 * (lane >> 5));
-            const float4 del = *reinterpret_cast<const float4*>(dt + 8 * g + 4 * (lane >> 5));
-            const float ls[4] = {lse.x, lse.y, lse.z, lse.w}, ds[4] = {del.x, del.y, del.z, del.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int i = 4 * g + e, q = i0 + 8 * g + 4 * (lane >> 5) + e;
-                float x = s[i] * c;
-                if constexpr (MASK) {
-                    const int qr = q < a.Tq ? q : a.Tq - 1;
-                    x = !a.causal || kr <= q + off ? masked(a, mask_row(a, b, hq, qr), kr, x) : -INFINITY;
-                } else if (!whole) {
-                    x = kr <= q + off ? x : -INFINITY;
-                }
-                s[i] = __builtin_amdgcn_exp2f(x - ls[e]);
-                dp[i] = s[i] * (dp[i] - ds[e]);
+            for (int i = 0; i < T::kSteps; ++i) {
+                u32x4 v;
+                if constexpr (VL) v = T::rows(vt, 32 * w, i, lane);
+                else v = vf[i];
+                dp = mma<DT>(T::rows(gs, 0, i, lane), v, dp);
             }
-        }
-        u32x4 pf[2], df[2];
-        fragments<DT>(s, pf);
-        fragments<DT>(dp, df);
+            const bool edge = i_now < free_q;
 #pragma unroll
-        for (int d = 0; d < DC / 32; ++d) {
-            dv[d] = T::cols(gt, 0, d, s, pf, dv[d], lane);
-            dk[d] = T::cols(qt, 0, d, dp, df, dk[d], lane);
+            for (int g = 0; g < 4; ++g) {
+                const float4 lse = *reinterpret_cast<const float4*>(&lt[t & 1][8 * g + 4 * (lane >> 5)]);
+                const float4 del = *reinterpret_cast<const float4*>(&dt[t & 1][8 * g + 4 * (lane >> 5)]);
+                const float ls[4] = {lse.x, lse.y, lse.z, lse.w}, ds[4] = {del.x, del.y, del.z, del.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int i = 4 * g + e, q = i_now + 8 * g + 4 * (lane >> 5) + e;
+                    float x;
+                    if constexpr (MASK == kNoMask) {
+                        x = __builtin_fmaf(s[i], c, -ls[e]);
+                    } else {
+                        const float f = MASK == kKeyMask ? term
+                                                         : mask_term(a, mask_row(a, b, hq_now, q < a.Tq ? q : a.Tq - 1), kr);
+                        x = f == -INFINITY ? f : __builtin_fmaf(s[i], c, f) - ls[e];
+                    }
+                    if (edge) x = kr <= q + off ? x : -INFINITY;
+                    s[i] = __builtin_amdgcn_exp2f(x);
+                    dp[i] = s[i] * (dp[i] - ds[e]);
+                }
+            }
+            u32x4 pf[2], df[2];
+            fragments<DT>(s, pf);
+            fragments<DT>(dp, df);
+#pragma unroll
+            for (int d = 0; d < DC / 32; ++d) dv[d] = T::cols(gs, 0, d, s, pf, dv[d], lane);
+#pragma unroll
+            for (int d = 0; d < DC / 32; ++d) dk[d] = T::cols(qs, 0, d, dp, df, dk[d], lane);
         }
+        if (t + 1 < tiles) store((t + 1) & 1);
     }
     if (key >= a.Tk) return;
     const int64_t out = (((int64_t)b * a.Tk + key) * a.H + h) * a.D;
+    if (a.splits_kv > 1) {
+        const int64_t all = (int64_t)a.B * a.Tk * a.H * a.D;
+#pragma unroll
+        for (int d = 0; d < DC / 32; ++d) {
+            store_cols<AXS6_F32>(a.part_kv + split * all, out, d, dk[d], a.scale, a.D, lane);
+            store_cols<AXS6_F32>(a.part_kv + (a.splits_kv + split) * all, out, d, dv[d], 1.0f, a.D, lane);
+        }
+        return;
+    }
 #pragma unroll
     for (int d = 0; d < DC / 32; ++d) {
         store_cols<DT>(a.dk, out, d, dk[d], a.scale, a.D, lane);
@@ -192,25 +291,55 @@ __global__ __launch_bounds__(kBwdThreads) void attn_dkv_kernel(AttnArgs a) {
     }
 }
 
-template <int DT, int DC>
+// Sums of the splits in order, four values a thread.
+template <int DT>
+__global__ __launch_bounds__(256) void attn_sum_kernel(const float* part, int splits, int64_t n, void* out) {
+    using E = Elem<DT>;
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= n) return;
+    float4 x = *reinterpret_cast<const float4*>(part + i);
+    for (int s = 1; s < splits; ++s) {
+        const float4 y = *reinterpret_cast<const float4*>(part + s * n + i);
+        x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+    }
+    auto* p = reinterpret_cast<typename E::S*>(out) + i;
+    if constexpr (DT == AXS6_F32) *reinterpret_cast<float4*>(p) = x;
+    else *reinterpret_cast<uint2*>(p) = make_uint2(pack2<DT>(x.x, x.y), pack2<DT>(x.z, x.w));
+}
+
+template <int DT>
+void sum_splits(const float* part, int splits, int64_t n, void* out, hipStream_t st) {
+    attn_sum_kernel<DT><<<(unsigned)((n / 4 + 255) / 256), 256, 0, st>>>(part, splits, n, out);
+}
+
+template <int DT, int DC, int MASK>
 void launch(const AttnArgs& a, hipStream_t st) {
     if (a.Tq) {
-        const unsigned grid = (unsigned)((a.Tq + kBwdHeld - 1) / kBwdHeld * a.B * a.Hq);
-        if (a.mask) attn_dq_kernel<DT, DC, true><<<grid, kBwdThreads, 0, st>>>(a);
-        else attn_dq_kernel<DT, DC, false><<<grid, kBwdThreads, 0, st>>>(a);
+        attn_dq_kernel<DT, DC, MASK><<<(unsigned)((a.Tq + kHeld - 1) / kHeld * a.B * a.Hq * a.splits), kThr, 0, st>>>(a);
+        if (a.splits > 1) sum_splits<DT>(a.part, a.splits, (int64_t)a.B * a.Tq * a.Hq * a.D, a.dq, st);
     }
     if (a.Tk) {
-        const unsigned grid = (unsigned)((a.Tk + kBwdHeld - 1) / kBwdHeld * a.B * a.H);
-        if (a.mask) attn_dkv_kernel<DT, DC, true><<<grid, kBwdThreads, 0, st>>>(a);
-        else attn_dkv_kernel<DT, DC, false><<<grid, kBwdThreads, 0, st>>>(a);
+        attn_dkv_kernel<DT, DC, MASK><<<(unsigned)((a.Tk + kHeld - 1) / kHeld * a.B * a.H * a.splits_kv), kThr, 0, st>>>(a);
+        if (a.splits_kv > 1) {
+            const int64_t n = (int64_t)a.B * a.Tk * a.H * a.D;
+            sum_splits<DT>(a.part_kv, a.splits_kv, n, a.dk, st);
+            sum_splits<DT>(a.part_kv + a.splits_kv * n, a.splits_kv, n, a.dv, st);
+        }
     }
+}
+
+template <int DT, int DC>
+void pick(const AttnArgs& a, hipStream_t st) {
+    if (!a.mask) launch<DT, DC, kNoMask>(a, st);
+    else if (a.ms[2] == 0) launch<DT, DC, kKeyMask>(a, st);
+    else launch<DT, DC, kFullMask>(a, st);
 }
 
 template <int DT>
 void dispatch(const AttnArgs& a, hipStream_t st) {
-    if (a.D <= 64) launch<DT, 64>(a, st);
-    else if (a.D <= 96) launch<DT, 96>(a, st);
-    else launch<DT, 128>(a, st);
+    if (a.D <= 64) pick<DT, 64>(a, st);
+    else if (a.D <= 96) pick<DT, 96>(a, st);
+    else pick<DT, 128>(a, st);
 }
 
 }  // namespace

@@ -11,104 +11,169 @@
 // beside them.  A wave holds 32 queries in registers; S^T = K q^T puts a
 // query's scores in one lane and the lane 32 further on, so maximum and sum
 // take one exchange, and the probabilities are the second product's operand
-// in place.  A workgroup's four waves share the keys' tiles in LDS.
+// in place.  The waves of a workgroup share the keys' tiles, which go from
+// memory into the other of two LDS buffers while one is computed on: one
+// barrier a tile.  Two waves a SIMD (at most 256 registers each) let one
+// multiply while the other exponentiates: 1 x 16384, 16 heads of 128, causal,
+// bf16: 1816 us with one, 1063 with two (2179 through registers with two
+// barriers), 998 with 128 keys a tile and 256 queries a workgroup, 1102
+// TFLOP/s, where a bf16 matrix product of 8192^3 reaches 1139 on this card.
+// The row's reference is only raised when a score passes it by 2^8, so the
+// output is hardly ever rescaled; the sum is taken of the probabilities as they
+// are rounded for the product.
+// Few rows against many keys: the keys are split over workgroups, whose sums a
+// second launch joins (4 x 4 queries of 16 heads, 8000 keys: 165 -> 41 us).
 #include "attention.h"
 
 namespace axs6 {
 namespace {
 
-constexpr int kFwdThreads = 256, kFwdQ = 128, kFwdK = 64;
+// Scores may grow this far (a factor of 2^8 of a probability) past a row's
+// reference before the row is rescaled, which then hardly ever happens.
+constexpr float kSlack = 8.0f;
 
-template <int DT, int DC, bool MASK>
-__global__ __launch_bounds__(kFwdThreads) void attn_fwd_kernel(AttnArgs a) {
+// Queries and keys of a workgroup's tile.
+template <int DT, int DC, bool LARGE> struct FwdShape {
+    static constexpr int kWaves = LARGE ? 8 : 4;
+    static constexpr int kKeys = DT == AXS6_F32 ? 64 : LARGE || DC <= 64 ? 128 : 64;
+    static constexpr int kQ = 32 * kWaves, kThreads = 64 * kWaves;
+    // two waves a SIMD, of which one computes softmax while the other multiplies
+    static constexpr int kOccupancy = DT == AXS6_F32 ? 1 : 2;
+};
+
+template <int DT, int DC, int MASK, bool LARGE>
+__global__ __launch_bounds__((FwdShape<DT, DC, LARGE>::kThreads), (FwdShape<DT, DC, LARGE>::kOccupancy)) void
+attn_fwd_kernel(AttnArgs a) {
     using T = Tile<DT, DC>;
-    __shared__ __attribute__((aligned(16))) char kt[kFwdK * T::kPitch];
-    __shared__ __attribute__((aligned(16))) char vt[kFwdK * T::kPitch];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int heads = a.B * a.Hq, bh = blockIdx.x % heads, b = bh / a.Hq, hq = bh % a.Hq, h = hq / a.G;
-    const int q0 = ((int)(gridDim.x / heads) - 1 - (int)(blockIdx.x / heads)) * kFwdQ;   // a causal mask's longest rows first
-    const int q = q0 + 32 * w + (lane & 31), qr = q < a.Tq ? q : a.Tq - 1;
+    using S = FwdShape<DT, DC, LARGE>;
+    constexpr int NK = S::kKeys / 32, W = S::kWaves;
+    __shared__ __attribute__((aligned(1024))) char kt[2][S::kKeys * T::kPitch];
+    __shared__ __attribute__((aligned(1024))) char vt[2][S::kKeys * T::kPitch];
+    __shared__ __attribute__((aligned(16))) float term[2][MASK == kKeyMask ? S::kKeys : 1];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int q_tiles = (a.Tq + S::kQ - 1) / S::kQ;
+    int bh, piece;
+    work_item(blockIdx.x, a.B * a.Hq, q_tiles * a.splits, false, bh, piece);
+    const int b = bh / a.Hq, hq = bh % a.Hq, h = hq / a.G, split = piece % a.splits;
+    const int q0 = (q_tiles - 1 - piece / a.splits) * S::kQ;   // a causal mask's longest rows first
     const int off = a.Tk - a.Tq;
-    const int q_last = q0 + kFwdQ < a.Tq ? q0 + kFwdQ - 1 : a.Tq - 1;
+    const int q_last = q0 + S::kQ < a.Tq ? q0 + S::kQ - 1 : a.Tq - 1;
     int keys = a.causal ? q_last + off + 1 : a.Tk;
     keys = keys < 0 ? 0 : keys > a.Tk ? a.Tk : keys;
-    const int tiles = (keys + kFwdK - 1) / kFwdK;
-    const int limit = a.causal ? (qr + off + 1 < a.Tk ? qr + off + 1 : a.Tk) : a.Tk;   // keys that the lane's row sees
-    const int free_keys = a.causal ? q0 + off + 1 : a.Tk;   // below it every row of the workgroup sees every key
+    int first = 0, tiles = (keys + S::kKeys - 1) / S::kKeys;
+    if (a.splits > 1) {   // this workgroup's part of the keys
+        const int per = (tiles + a.splits - 1) / a.splits;
+        first = split * per < tiles ? split * per : tiles;
+        tiles = first + per < tiles ? first + per : tiles;
+    }
+    // tiles whose every key every row of the workgroup sees, but for the mask
+    const int free_keys = a.causal ? q0 + off + 1 : a.Tk;
+    const int free_tiles = free_keys <= 0 ? 0 : (free_keys < a.Tk ? free_keys : a.Tk) / S::kKeys;
 
     const char* kb = reinterpret_cast<const char*>(a.k) + (b * a.ks[0] + h * a.ks[2]) * T::kBytes;
     const char* vb = reinterpret_cast<const char*>(a.v) + (b * a.vs[0] + h * a.vs[2]) * T::kBytes;
-    const char* mrow = MASK ? mask_row(a, b, hq, qr) : nullptr;
+    Direct<DT, DC, S::kKeys, W> dk, dv;
+    dk.init(a.ks[1], a.D, lane, w);
+    dv.init(a.vs[1], a.D, lane, w);
+    // the mask's term of key threadIdx.x of tile t
+    auto key_term = [&](int t) {
+        const int key = t * S::kKeys + threadIdx.x;
+        return threadIdx.x < S::kKeys && key < a.Tk ? mask_term(a, mask_row(a, b, hq, 0), key) : -INFINITY;
+    };
+    if (first < tiles) {
+        dk.load(kt[first & 1], kb, first * S::kKeys, a.Tk, a.D, w);
+        dv.load(vt[first & 1], vb, first * S::kKeys, a.Tk, a.D, w);
+        if constexpr (MASK == kKeyMask) {
+            const float f = key_term(first);
+            if (threadIdx.x < S::kKeys) term[first & 1][threadIdx.x] = f;
+        }
+    }
+    const int q = q0 + 32 * w + (lane & 31), qr = q < a.Tq ? q : a.Tq - 1;
+    const int limit = a.causal && qr + off + 1 < a.Tk ? qr + off + 1 : a.Tk;   // keys that the lane's row sees
+    const char* mrow = MASK == kFullMask ? mask_row(a, b, hq, qr) : nullptr;
     u32x4 qf[T::kSteps];
     load_rows<DT, DC>(qf, a.q, b * a.qs[0] + qr * a.qs[1] + hq * a.qs[2], a.D, lane);
-
     f32x16 o[DC / 32];
 #pragma unroll
     for (int d = 0; d < DC / 32; ++d) o[d] = zero16();
-    float m = -INFINITY, l = 0.0f;
+    float m = -INFINITY, l = 0.0f;   // the reference that scores are taken from; the sum of exponentials
     const float c = a.scale * kLog2e;
-    Stage<DT, DC, kFwdK, kFwdThreads> sk, sv;
-    if (tiles) {
-        sk.load(kb, a.ks[1], 0, a.Tk, a.D);
-        sv.load(vb, a.vs[1], 0, a.Tk, a.D);
-    }
-    for (int t = 0; t < tiles; ++t) {
-        __syncthreads();
-        sk.store(kt);
-        sv.store(vt);
-        __syncthreads();
-        const int k0 = t * kFwdK;
+
+    for (int t = first; t < tiles; ++t) {
+        tile_barrier();   // tile t is there, and nobody reads the other buffers any more
+        float next_term = 0.0f;
         if (t + 1 < tiles) {
-            sk.load(kb, a.ks[1], k0 + kFwdK, a.Tk, a.D);
-            sv.load(vb, a.vs[1], k0 + kFwdK, a.Tk, a.D);
+            dk.load(kt[(t + 1) & 1], kb, (t + 1) * S::kKeys, a.Tk, a.D, w);
+            dv.load(vt[(t + 1) & 1], vb, (t + 1) * S::kKeys, a.Tk, a.D, w);
+            if constexpr (MASK == kKeyMask) next_term = key_term(t + 1);
         }
-        f32x16 s[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            s[j] = zero16();
-#pragma unroll
-            for (int i = 0; i < T::kSteps; ++i) s[j] = mma<DT>(T::rows(kt, 32 * j, i, lane), qf[i], s[j]);
+        const char *ks = kt[t & 1], *vs = vt[t & 1];
+        const int k0 = t * S::kKeys;
+        bool any = true;   // a tile of keys that nobody sees is passed over
+        if constexpr (MASK == kKeyMask) {
+            float f = term[t & 1][lane];
+            if constexpr (S::kKeys > 64) f = fmaxf(f, term[t & 1][lane + 64]);
+            any = __any(!(f == -INFINITY));
         }
-        const bool whole = k0 + kFwdK <= free_keys && k0 + kFwdK <= a.Tk;
-        float mx = m;
+        if (any) {
+            f32x16 s[NK];
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+            for (int j = 0; j < NK; ++j) {
+                s[j] = zero16();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int key = k0 + 32 * j + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3);
-                float x = s[j][i] * c;
-                if constexpr (MASK) {
-                    x = key < limit ? masked(a, mrow, key, x) : -INFINITY;
-                } else if (!whole) {
-                    x = key < limit ? x : -INFINITY;
+                for (int i = 0; i < T::kSteps; ++i) s[j] = mma<DT>(T::rows(ks, 32 * j, i, lane), qf[i], s[j]);
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < NK; ++j)
+                apply_mask<MASK>(a, s[j], c, k0 + 32 * j, &term[t & 1][MASK == kKeyMask ? 32 * j : 0], mrow,
+                                 t >= free_tiles, limit, lane);
+#pragma unroll
+            for (int j = 0; j < NK; ++j)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[j][i]);
+            if constexpr (MASK == kNoMask) mx *= c;
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            if (__any(mx > m + kSlack)) {   // m is -inf until the row sees a key
+                const float mn = fmaxf(m, mx), alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn));
+                m = mn;
+                l *= alpha;
+#pragma unroll
+                for (int d = 0; d < DC / 32; ++d) o[d] *= alpha;
+            }
+            const float ref = m == -INFINITY ? 0.0f : m;
+            u32x4 pf[NK][2];
+#pragma unroll
+            for (int j = 0; j < NK; ++j) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    s[j][i] = __builtin_amdgcn_exp2f(MASK == kNoMask ? __builtin_fmaf(s[j][i], c, -ref) : s[j][i] - ref);
+                fragments<DT>(s[j], pf[j]);
+                if constexpr (DT == AXS6_F32) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) l += s[j][i];
+                } else {   // the values as the product takes them
+                    l = add_fragment<DT>(pf[j][0], l);
+                    l = add_fragment<DT>(pf[j][1], l);
                 }
-                s[j][i] = x;
-                mx = fmaxf(mx, x);
             }
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const float ref = mx == -INFINITY ? 0.0f : mx;
-        const float alpha = __builtin_amdgcn_exp2f(m - ref);
-        m = mx;
-        l *= alpha;
-        u32x4 pf[2][2];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+            for (int d = 0; d < DC / 32; ++d)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                s[j][i] = __builtin_amdgcn_exp2f(s[j][i] - ref);
-                l += s[j][i];
-            }
-            fragments<DT>(s[j], pf[j]);
+                for (int j = 0; j < NK; ++j) o[d] = T::cols(vs, 32 * j, d, s[j], pf[j], o[d], lane);
         }
-#pragma unroll
-        for (int d = 0; d < DC / 32; ++d) {
-            o[d] *= alpha;
-#pragma unroll
-            for (int j = 0; j < 2; ++j) o[d] = T::cols(vt, 32 * j, d, s[j], pf[j], o[d], lane);
-        }
+        if constexpr (MASK == kKeyMask)
+            if (threadIdx.x < S::kKeys) term[(t + 1) & 1][threadIdx.x] = next_term;
     }
     l += __shfl_xor(l, 32, 64);
     if (q >= a.Tq) return;
+    if (a.splits > 1) {
+        const int64_t at = split * ((int64_t)a.B * a.Hq * a.Tq) + ((int64_t)b * a.Hq + hq) * a.Tq + q;
+        if (lane < 32) { a.stat[2 * at] = m; a.stat[2 * at + 1] = l; }
+#pragma unroll
+        for (int d = 0; d < DC / 32; ++d) store_cols<AXS6_F32>(a.part, at * a.D, d, o[d], 1.0f, a.D, lane);
+        return;
+    }
     const float rl = l == 0.0f ? 0.0f : 1.0f / l;
     const int64_t row = (((int64_t)b * a.Tq + q) * a.Hq + hq) * a.D;
 #pragma unroll
@@ -117,18 +182,85 @@ __global__ __launch_bounds__(kFwdThreads) void attn_fwd_kernel(AttnArgs a) {
         a.lse[((int64_t)b * a.Hq + hq) * a.Tq + q] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
-template <int DT, int DC>
+// Joins the splits of a row in order: one wave a row.
+template <int DT>
+__global__ __launch_bounds__(64) void attn_join_kernel(AttnArgs a) {
+    using E = Elem<DT>;
+    const int64_t rows = (int64_t)a.B * a.Hq * a.Tq, row = blockIdx.x, bh = row / a.Tq;
+    const int q = (int)(row - bh * a.Tq);
+    float m = -INFINITY;
+    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.stat[2 * (s * rows + row)]);
+    const float ref = m == -INFINITY ? 0.0f : m;
+    const int d = threadIdx.x * 2;
+    float l = 0.0f, x = 0.0f, y = 0.0f;
+    for (int s = 0; s < a.splits; ++s) {
+        const int64_t at = s * rows + row;
+        const float f = __builtin_amdgcn_exp2f(a.stat[2 * at] - ref);
+        l += a.stat[2 * at + 1] * f;
+        if (d < a.D) {
+            const float2 p = *reinterpret_cast<const float2*>(a.part + at * a.D + d);
+            x += p.x * f;
+            y += p.y * f;
+        }
+    }
+    if (a.lse && threadIdx.x == 0) a.lse[row] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
+    if (d >= a.D) return;
+    const float rl = l == 0.0f ? 0.0f : 1.0f / l;
+    auto* out = reinterpret_cast<typename E::S*>(a.o) + (((bh / a.Hq) * a.Tq + q) * a.Hq + bh % a.Hq) * a.D + d;
+    out[0] = E::from_f(x * rl);
+    out[1] = E::from_f(y * rl);
+}
+
+template <int DT, int DC, int MASK, bool LARGE>
 void launch(const AttnArgs& a, hipStream_t st) {
-    const unsigned grid = (unsigned)((a.Tq + kFwdQ - 1) / kFwdQ * a.B * a.Hq);
-    if (a.mask) attn_fwd_kernel<DT, DC, true><<<grid, kFwdThreads, 0, st>>>(a);
-    else attn_fwd_kernel<DT, DC, false><<<grid, kFwdThreads, 0, st>>>(a);
+    using S = FwdShape<DT, DC, LARGE>;
+    const unsigned grid = (unsigned)((a.Tq + S::kQ - 1) / S::kQ * a.B * a.Hq * a.splits);
+    attn_fwd_kernel<DT, DC, MASK, LARGE><<<grid, S::kThreads, 0, st>>>(a);
+    if (a.splits > 1) attn_join_kernel<DT><<<(unsigned)(a.B * a.Hq * a.Tq), 64, 0, st>>>(a);
+}
+
+template <int DT, int DC>
+void pick(const AttnArgs& a, hipStream_t st) {
+    if (a.mask && a.ms[2] == 0) return launch<DT, DC, kKeyMask, false>(a, st);
+    if (a.mask) return launch<DT, DC, kFullMask, false>(a, st);
+    if constexpr (DT != AXS6_F32 && DC > 64) {
+        // 256 queries a workgroup and 128 keys a tile from two workgroups a CU on:
+        // fewer barriers (1 x 16384, 16 heads of 128, causal 990 us against 1063,
+        // 2 x 4096 x 32 heads 333 against 327, without the mask 526 against 562)
+        if ((int64_t)((a.Tq + 255) / 256) * a.B * a.Hq >= 512) return launch<DT, DC, kNoMask, true>(a, st);
+    }
+    launch<DT, DC, kNoMask, false>(a, st);
 }
 
 template <int DT>
 void dispatch(const AttnArgs& a, hipStream_t st) {
-    if (a.D <= 64) launch<DT, 64>(a, st);
-    else if (a.D <= 96) launch<DT, 96>(a, st);
-    else launch<DT, 128>(a, st);
+    if (a.D <= 64) pick<DT, 64>(a, st);
+    else if (a.D <= 96) pick<DT, 96>(a, st);
+    else pick<DT, 128>(a, st);
+}
+
+// Parts that an axis of `steps` tiles is split in, so that `groups` workgroups
+// become `want`, of `least` tiles each at the least.
+int split_count(int64_t groups, int64_t steps, int64_t want, int64_t least, int64_t most) {
+    if (groups <= 0) return 1;
+    int64_t s = (want + groups - 1) / groups;
+    s = s < steps / least ? s : steps / least;
+    s = s < most ? s : most;
+    return s < 1 ? 1 : (int)s;
+}
+
+// Few rows against many keys: the keys are split until the 256 CUs have work,
+// 256 keys a part at the least.
+int forward_splits(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq) {
+    const int64_t groups = (Tq + 127) / 128 * B * Hq;
+    return groups >= 256 ? 1 : split_count(groups, Tk / 256, 512, 1, 64);
+}
+// The backward walks over keys for dq, as the forward, and over the queries of a
+// group's heads for dk and dv.  There a causal mask gives some keys' workgroups
+// far more queries than others': four workgroups for each place on the chip's
+// CUs even that out, where two fill it.
+int key_splits(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t H, bool causal) {
+    return split_count((Tk + 127) / 128 * B * H, (Tq + 31) / 32 * (H ? Hq / H : 1), causal ? 1024 : 512, 8, 16);
 }
 
 // The arguments of both directions, checked.
@@ -167,6 +299,17 @@ int operand(const char* fn, const char* name, const void* p, const int64_t* stri
         if (strides[i] % v) return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: a stride of %s is not whole vectors", fn, name);
         to[i] = strides[i];
     }
+    // a tile's rows are addressed by 32-bit byte offsets from its first
+    if (strides[1] < 0 || strides[1] >= AXS6_ATTENTION_MAX_TOKEN_STRIDE)
+        return fail(AXS6_ERR_UNSUPPORTED, "%s: the tokens of %s are not 0 to %d elements apart", fn, name,
+                    AXS6_ATTENTION_MAX_TOKEN_STRIDE - 1);
+    return AXS6_OK;
+}
+
+int scratch(const char* fn, const void* workspace, int64_t bytes, int64_t need) {
+    if (need && (!workspace || bytes < need || (uintptr_t)workspace % 16))
+        return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: a 16-byte aligned workspace of %lld bytes required, got %lld", fn,
+                    (long long)need, (long long)bytes);
     return AXS6_OK;
 }
 
@@ -175,11 +318,24 @@ int operand(const char* fn, const char* name, const void* p, const int64_t* stri
 
 using namespace axs6;
 
+extern "C" int64_t axs6_attention_forward_workspace(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t D) {
+    if (B <= 0 || Tq <= 0 || Tk <= 0 || Hq <= 0 || D <= 0) return 0;
+    const int64_t s = forward_splits(B, Tq, Tk, Hq);
+    return s == 1 ? 0 : s * B * Hq * Tq * (D + 2) * (int64_t)sizeof(float);
+}
+
+extern "C" int64_t axs6_attention_backward_workspace(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t H, int64_t D,
+                                                     int32_t causal) {
+    if (B <= 0 || Tq <= 0 || Tk <= 0 || Hq <= 0 || H <= 0 || D <= 0) return 0;
+    const int64_t s = forward_splits(B, Tq, Tk, Hq), kv = key_splits(B, Tq, Tk, Hq, H, causal);
+    return ((s == 1 ? 0 : s * B * Tq * Hq * D) + (kv == 1 ? 0 : 2 * kv * B * Tk * H * D)) * (int64_t)sizeof(float);
+}
+
 extern "C" int axs6_attention_forward(const void* q, const void* k, const void* v, int32_t dtype, int64_t B, int64_t Tq,
                                       int64_t Tk, int64_t Hq, int64_t H, int64_t D, const int64_t* q_strides,
                                       const int64_t* k_strides, const int64_t* v_strides, const void* mask,
                                       int32_t mask_type, const int64_t* mask_strides, int32_t causal, float scale,
-                                      void* out, float* lse, void* stream) {
+                                      void* out, float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
     const char* fn = "axs6_attention_forward";
     AttnArgs a{};
     int rc = fill(fn, a, dtype, B, Tq, Tk, Hq, H, D, mask, mask_type, mask_strides, causal, scale);
@@ -190,6 +346,11 @@ extern "C" int axs6_attention_forward(const void* q, const void* k, const void* 
         return rc;
     if (!out || (uintptr_t)out % 16) return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: output null or not aligned", fn);
     a.q = q; a.k = k; a.v = v; a.o = out; a.lse = lse;
+    a.splits = forward_splits(B, Tq, Tk, Hq);
+    const int64_t need = axs6_attention_forward_workspace(B, Tq, Tk, Hq, D);
+    if ((rc = scratch(fn, workspace, workspace_bytes, need))) return rc;
+    a.part = reinterpret_cast<float*>(workspace);
+    a.stat = a.part + a.splits * B * Hq * Tq * D;
     hipStream_t st = (hipStream_t)stream;
     if (dtype == AXS6_F32) dispatch<AXS6_F32>(a, st);
     else if (dtype == AXS6_BF16) dispatch<AXS6_BF16>(a, st);
@@ -202,7 +363,8 @@ extern "C" int axs6_attention_backward(const void* dout, const void* q, const vo
                                        int64_t H, int64_t D, const int64_t* dout_strides, const int64_t* q_strides,
                                        const int64_t* k_strides, const int64_t* v_strides, const void* mask,
                                        int32_t mask_type, const int64_t* mask_strides, int32_t causal, float scale,
-                                       float* delta, void* dq, void* dk, void* dv, void* stream) {
+                                       float* delta, void* dq, void* dk, void* dv, void* workspace,
+                                       int64_t workspace_bytes, void* stream) {
     const char* fn = "axs6_attention_backward";
     AttnArgs a{};
     int rc = fill(fn, a, dtype, B, Tq, Tk, Hq, H, D, mask, mask_type, mask_strides, causal, scale);
@@ -221,6 +383,12 @@ extern "C" int axs6_attention_backward(const void* dout, const void* q, const vo
         return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: gradients not aligned to 16 bytes", fn);
     a.q = q; a.k = k; a.v = v; a.out = out; a.dout = dout; a.lse = const_cast<float*>(lse); a.delta = delta;
     a.dq = dq; a.dk = dk; a.dv = dv;
+    a.splits = forward_splits(B, Tq, Tk, Hq);
+    a.splits_kv = key_splits(B, Tq, Tk, Hq, H, causal);
+    if ((rc = scratch(fn, workspace, workspace_bytes, axs6_attention_backward_workspace(B, Tq, Tk, Hq, H, D, causal))))
+        return rc;
+    a.part = reinterpret_cast<float*>(workspace);
+    a.part_kv = a.part + (a.splits == 1 ? 0 : a.splits * B * Tq * Hq * D);
     attention_backward(a, dtype, (hipStream_t)stream);
     return check_launch(fn);
 }

@@ -45,7 +45,7 @@ at::Tensor vectors(const at::Tensor& t) {
     const int64_t v = vec_multiple(t.scalar_type()), d = t.size(3), pad = (v - d % v) % v;
     if (pad) return at::constant_pad_nd(t, {0, pad});
     if (t.numel() == 0) return t;
-    const bool ok = t.stride(3) == 1 && t.stride(0) % v == 0 && t.stride(1) % v == 0 && t.stride(2) % v == 0;
+    const bool ok = t.stride(3) == 1 && t.stride(1) < AXS6_ATTENTION_MAX_TOKEN_STRIDE && t.stride(0) % v == 0 && t.stride(1) % v == 0 && t.stride(2) % v == 0;
     if (!ok) return t.contiguous();
     return aligned(t) ? t : t.clone(at::MemoryFormat::Contiguous);
 }
@@ -58,6 +58,13 @@ at::Tensor int64s(const at::Tensor& t, at::IntArrayRef shape, const at::Tensor& 
                 " must be int64 or int32, got ", t.scalar_type());
     return t.to(at::kLong).contiguous();
 }
+
+// `bytes` of workspace beside `like`; undefined for 0.
+at::Tensor workspace(int64_t bytes, const at::Tensor& like) {
+    return bytes ? at::empty({bytes}, like.options().dtype(at::kByte)) : at::Tensor();
+}
+void* data_of(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+int64_t size_of(const at::Tensor& t) { return t.defined() ? t.numel() : 0; }
 
 // ---- rotary positions ---------------------------------------------------------------
 
@@ -182,10 +189,11 @@ std::pair<at::Tensor, at::Tensor> attention_fwd(const at::Tensor& q, const at::T
     const Mask m = mask_of(mask, B, Hq, Tq, Tk);
     at::Tensor out = at::empty({B, Tq, Hq, D}, q.options());
     at::Tensor l = lse ? at::empty({B, Hq, Tq}, q.options().dtype(at::kFloat)) : at::Tensor();
+    const at::Tensor ws = workspace(axs6_attention_forward_workspace(B, Tq, Tk, Hq, D), q);
     check_rc(axs6_attention_forward(q.data_ptr(), k.data_ptr(), v.data_ptr(), dtype_code(q.scalar_type()), B, Tq, Tk, Hq,
                                     H, D, q.strides().data(), k.strides().data(), v.strides().data(), m.data(), m.type,
                                     m.strides, causal, (float)scale, out.data_ptr(),
-                                    lse ? l.data_ptr<float>() : nullptr, stream_of(q)),
+                                    lse ? l.data_ptr<float>() : nullptr, data_of(ws), size_of(ws), stream_of(q)),
              "axs6_attention_forward");
     return {out, l};
 }
@@ -217,12 +225,14 @@ struct AttentionFunction : public torch::autograd::Function<AttentionFunction> {
         const Mask m = mask_of(s[5], B, Hq, Tq, Tk);
         at::Tensor dq = at::empty({B, Tq, Hq, D}, q.options()), dk = at::empty({B, Tk, H, D}, q.options());
         at::Tensor dv = at::empty({B, Tk, H, D}, q.options()), delta = at::empty_like(lse);
+        const bool causal = d["causal"].toBool();
+        const at::Tensor ws = workspace(axs6_attention_backward_workspace(B, Tq, Tk, Hq, H, D, causal), q);
         check_rc(axs6_attention_backward(
                      g.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr<float>(),
                      dtype_code(q.scalar_type()), B, Tq, Tk, Hq, H, D, g.strides().data(), q.strides().data(),
-                     k.strides().data(), v.strides().data(), m.data(), m.type, m.strides, d["causal"].toBool(),
+                     k.strides().data(), v.strides().data(), m.data(), m.type, m.strides, causal,
                      (float)d["scale"].toDouble(), delta.data_ptr<float>(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                     stream_of(q)),
+                     data_of(ws), size_of(ws), stream_of(q)),
                  "axs6_attention_backward");
         const at::Tensor got[3] = {dq, dk, dv};
         for (int i = 0; i < 3; ++i)
@@ -348,11 +358,10 @@ at::Tensor kv_attention(const at::Tensor& q, const at::Tensor& k_codes, const at
     c10::DeviceGuard guard(q.device());
     at::Tensor out = at::empty({c.B, Tq, Hq, c.D}, q.options());
     if (c.nb == 0) return out.zero_();
-    const int64_t bytes = axs6_kv_attention_workspace(c.B, Tq, Hq, c.H, c.D, c.nb);
-    at::Tensor ws = bytes ? at::empty({bytes}, q.options().dtype(at::kByte)) : at::Tensor();
+    const at::Tensor ws = workspace(axs6_kv_attention_workspace(c.B, Tq, Hq, c.H, c.D, c.nb), q);
     check_rc(axs6_kv_attention(qp.data_ptr(), dtype_code(q.scalar_type()), c.B, Tq, Hq, c.H, c.D, qp.strides().data(),
                                c.kc.data_ptr(), c.ks.data_ptr<float>(), c.vc.data_ptr(), c.vs.data_ptr<float>(), c.nb,
-                               n.data_ptr<int64_t>(), (float)s, out.data_ptr(), bytes ? ws.data_ptr() : nullptr, bytes,
+                               n.data_ptr<int64_t>(), (float)s, out.data_ptr(), data_of(ws), size_of(ws),
                                stream_of(q)),
              "axs6_kv_attention");
     return out;

@@ -61,7 +61,7 @@ def test_c_entries_check_their_arguments():
     st = ctypes.cast(_i64(256, 64, 64, 1), ctypes.c_void_p)
     p, odd = 4096, 4098   # never read: every call below is refused, or has nothing to do
     fwd = L.axs6_attention_forward
-    good = [p, p, p, 0, 1, 4, 4, 2, 1, 64, st, st, st, None, 0, None, 0, 0.1, p, p, None]
+    good = [p, p, p, 0, 1, 4, 4, 2, 1, 64, st, st, st, None, 0, None, 0, 0.1, p, p, None, 0, None]
 
     def call(fn, args, **changes):
         a = list(args)
@@ -72,12 +72,13 @@ def test_c_entries_check_their_arguments():
     for change, rc in (({"a3": 9}, 1), ({"a7": 3, "a8": 2}, 1), ({"a9": 136}, 2), ({"a9": 63}, 2), ({"a17": 0.0}, 1),
                        ({"a17": math.inf}, 1), ({"a0": None}, 1), ({"a1": odd}, 1), ({"a18": None}, 1), ({"a4": -1}, 1),
                        ({"a13": p}, 1), ({"a13": p, "a14": 7, "a15": st}, 1), ({"a5": 1 << 31}, 2), ({"a5": 0}, 0),
-                       ({"a10": ctypes.cast(_i64(256, 63, 64), ctypes.c_void_p)}, 1)):
+                       ({"a10": ctypes.cast(_i64(256, 63, 64), ctypes.c_void_p)}, 1),
+                       ({"a11": ctypes.cast(_i64(256, 1 << 22, 64), ctypes.c_void_p)}, 2)):
         assert call(fwd, good, **change) == rc, change
         assert rc == 0 or L.axs6_last_error()
-    bwd = [p, p, p, p, p, p, 0, 1, 4, 4, 2, 1, 64, st, st, st, st, None, 0, None, 0, 0.1, p, p, p, p, None]
+    bwd = [p, p, p, p, p, p, 0, 1, 4, 4, 2, 1, 64, st, st, st, st, None, 0, None, 0, 0.1, p, p, p, p, p, 1 << 20, None]
     for change, rc in (({"a6": 5}, 1), ({"a0": None}, 1), ({"a5": None}, 1), ({"a23": odd}, 1), ({"a22": None}, 1),
-                       ({"a7": 0}, 0)):
+                       ({"a7": 0}, 0), ({"a8": 1 << 14, "a9": 1 << 14}, 1)):
         assert call(L.axs6_attention_backward, bwd, **change) == rc, change
     rot = [p, p, p, p, 0, 1, 4, 2, 1, 64, 32, st, st, p, 10, None, 0, 0, 0, 0, None]
     for change, rc in (({"a10": 31}, 1), ({"a10": 66}, 1), ({"a9": 600}, 2), ({"a13": None}, 1), ({"a2": None}, 1),
@@ -94,6 +95,10 @@ def test_c_entries_check_their_arguments():
     for change, rc in (({"a4": 3}, 1), ({"a12": 0}, 1), ({"a14": math.nan}, 1), ({"a12": 4096}, 1), ({"a3": 0}, 0),
                        ({"a15": None}, 1), ({"a1": 3}, 1)):
         assert call(L.axs6_kv_attention, att, **change) == rc, change
+    assert call(fwd, good, a6=8192) == 1   # split keys need a workspace
+    assert L.axs6_attention_forward_workspace(1, 4, 8192, 2, 64) > 0
+    assert L.axs6_attention_forward_workspace(1, 4, 64, 2, 64) == 0
+    assert L.axs6_attention_backward_workspace(0, 4, 64, 2, 1, 64, 1) == 0
     need = L.axs6_kv_attention_workspace(1, 1, 4, 2, 64, 4096)
     assert need > 0 and L.axs6_kv_attention_workspace(0, 1, 4, 2, 64, 4096) == 0
     dis = [p, 0, 100, 4, 100, p, p, 8, 1.0, None, 1, p, p, p, p, None]

@@ -64,6 +64,28 @@ def test_shapes(shape, causal, dtype):
 
 
 @pytest.mark.parametrize("dtype", ref.DTYPES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("shape", [(1, 3, 2100, 2, 1, 64), (2, 1, 1030, 8, 2, 128), (1, 700, 333, 4, 1, 80), (1, 600, 600, 8, 8, 96)])
+def test_split_axes(shape, causal, dtype):
+    """Few rows against many keys (keys split), few keys against many queries (queries split); heads that divide by
+    the chip's 8 dies."""
+    _check(*_inputs(*shape, dtype), causal=causal)
+    mask = torch.rand(shape[0], 1, 1, shape[2], generator=torch.Generator().manual_seed(1)) < 0.4
+    mask[..., :300] = False     # whole tiles that nobody sees
+    _check(*_inputs(*shape, dtype), mask=mask.to(DEV), causal=causal)
+
+
+@pytest.mark.parametrize("dtype", ref.DTYPES)
+def test_many_workgroups(dtype):
+    """The form of large problems: 256 queries a workgroup."""
+    from axs.unified import axs_attention_unified
+
+    q, k, v, _ = _inputs(8, 300, 280, 32, 4, 72, dtype)
+    for causal in (False, True):
+        assert ref.rel(axs_attention_unified(q, k, v, causal=causal), ref.attention(q, k, v, causal=causal)) <= _bounds(dtype)[0]
+
+
+@pytest.mark.parametrize("dtype", ref.DTYPES)
 @pytest.mark.parametrize("D", [1, 3, 33, 72, 127])
 def test_odd_heads(D, dtype):
     _check(*_inputs(1, 70, 70, 2, 1, D, dtype), causal=True)
