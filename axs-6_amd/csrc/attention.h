@@ -212,8 +212,8 @@ struct Direct {
     }
     // rows row0 .. row0 + R - 1 of `rows`
     __device__ void load(char* tile, const char* base, int row0, int rows, int D, int w) const {
-        const int left = rows - row0 < R ? rows - row0 : R;
 #if defined(__HIP_DEVICE_COMPILE__)   // the host pass knows no 16-byte form and would drop the kernel's stub
+        const int left = rows - row0 < R ? rows - row0 : R;
         const auto rsrc = buffer_of(base + (int64_t)row0 * pitch, left <= 0 ? 0 : (int64_t)(left - 1) * pitch + D * T::kBytes);
 #pragma unroll
         for (int i = 0; i < kN; ++i)
@@ -353,6 +353,55 @@ __device__ __forceinline__ void store_cols(void* out, int64_t row, int d, const 
                 make_uint2(pack2<DT>(c[4 * g] * f, c[4 * g + 1] * f), pack2<DT>(c[4 * g + 2] * f, c[4 * g + 3] * f));
         }
     }
+}
+
+// ---- rows again -------------------------------------------------------------
+// A key that a query does not see has no part in its results, whatever key and
+// value hold there.  The products over a tile's rows give it a weight of 0, which
+// an infinity or NaN turns into NaN; so a result that is not finite is made
+// again from the pairs that see each other alone, one pair at a time by one wave.
+// Where those give a NaN everywhere there is nothing more to find.
+
+// Whether any of the results of the lane's column is not finite.
+template <int N>
+__device__ __forceinline__ bool not_finite(const f32x16 (&c)[N]) {
+    float z = 0.0f;
+#pragma unroll
+    for (int d = 0; d < N; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) z = __builtin_fmaf(c[d][i], 0.0f, z);
+    z += __shfl_xor(z, 32, 64);
+    return z != z;
+}
+
+// Values l and l + 64 of a row of D.
+struct Two { float x, y; };
+template <int DT>
+__device__ __forceinline__ Two load_two(const void* p, int64_t i, int D, int lane) {
+    using E = Elem<DT>;
+    const auto* q = reinterpret_cast<const typename E::S*>(p) + i;
+    return {lane < D ? E::to_f(q[lane]) : 0.0f, lane + 64 < D ? E::to_f(q[lane + 64]) : 0.0f};
+}
+template <int DT>
+__device__ __forceinline__ void store_two(void* p, int64_t i, Two v, int D, int lane) {
+    using E = Elem<DT>;
+    auto* q = reinterpret_cast<typename E::S*>(p) + i;
+    if (lane < D) q[lane] = E::from_f(v.x);
+    if (lane + 64 < D) q[lane + 64] = E::from_f(v.y);
+}
+__device__ __forceinline__ float dot(Two a, Two b) {
+    float s = a.x * b.x + a.y * b.y;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
+    return s;
+}
+__device__ __forceinline__ bool all_nan(Two v, int D, int lane) {
+    return __all((lane >= D || v.x != v.x) && (lane + 64 >= D || v.y != v.y));
+}
+// What the masks add to the score of the pair, -inf where it is not seen.
+__device__ __forceinline__ float pair_term(const AttnArgs& a, int b, int hq, int q, int key) {
+    if (a.causal && key > q + a.Tk - a.Tq) return -INFINITY;
+    return a.mask ? mask_term(a, mask_row(a, b, hq, q), key) : 0.0f;
 }
 
 }  // namespace

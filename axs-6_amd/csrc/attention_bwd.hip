@@ -21,6 +21,67 @@ namespace {
 
 constexpr int kWaves = 4, kThr = 64 * kWaves, kHeld = 32 * kWaves;
 
+constexpr int kWalk = 32;   // queries of a tile that the held keys walk over
+
+// dq of a query from the keys k0 .. k1 - 1 that it sees, one by one.
+template <int DT>
+__device__ void dq_row(const AttnArgs& a, int b, int hq, int q, int k0, int k1, int split, float lse, float delta,
+                       int lane) {
+    const int h = hq / a.G;
+    const float c = a.scale * kLog2e;
+    const Two qv = load_two<DT>(a.q, b * a.qs[0] + q * a.qs[1] + hq * a.qs[2], a.D, lane);
+    const Two gv = load_two<DT>(a.dout, b * a.gs[0] + q * a.gs[1] + hq * a.gs[2], a.D, lane);
+    Two r = {0.0f, 0.0f};
+    for (int key = k0; key < k1 && !all_nan(r, a.D, lane); ++key) {
+        const float f = pair_term(a, b, hq, q, key);
+        if (f == -INFINITY) continue;
+        const Two kv = load_two<DT>(a.k, b * a.ks[0] + key * a.ks[1] + h * a.ks[2], a.D, lane);
+        const Two vv = load_two<DT>(a.v, b * a.vs[0] + key * a.vs[1] + h * a.vs[2], a.D, lane);
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(dot(qv, kv), c, f) - lse);
+        const float ds = p * (dot(gv, vv) - delta);
+        r = {r.x + ds * kv.x, r.y + ds * kv.y};
+    }
+    r = {r.x * a.scale, r.y * a.scale};
+    const int64_t out = (((int64_t)b * a.Tq + q) * a.Hq + hq) * a.D;
+    if (a.splits > 1) store_two<AXS6_F32>(a.part + split * ((int64_t)a.B * a.Tq * a.Hq * a.D), out, r, a.D, lane);
+    else store_two<DT>(a.dq, out, r, a.D, lane);
+}
+
+// dk and dv of a key from the queries of the group's tiles first .. tiles - 1
+// that see it, one by one.
+template <int DT>
+__device__ void dkv_row(const AttnArgs& a, int b, int h, int key, int first, int tiles, int q_first, int per_head,
+                        int split, int lane) {
+    const float c = a.scale * kLog2e;
+    const Two kv = load_two<DT>(a.k, b * a.ks[0] + key * a.ks[1] + h * a.ks[2], a.D, lane);
+    const Two vv = load_two<DT>(a.v, b * a.vs[0] + key * a.vs[1] + h * a.vs[2], a.D, lane);
+    Two rk = {0.0f, 0.0f}, rv = {0.0f, 0.0f};
+    for (int t = first; t < tiles && !(all_nan(rk, a.D, lane) && all_nan(rv, a.D, lane)); ++t) {
+        const int hq = h * a.G + t / per_head, i0 = q_first + t % per_head * kWalk;
+        for (int q = i0; q < i0 + kWalk && q < a.Tq; ++q) {
+            const float f = pair_term(a, b, hq, q, key);
+            if (f == -INFINITY) continue;
+            const int64_t row = ((int64_t)b * a.Hq + hq) * a.Tq + q;
+            const Two qv = load_two<DT>(a.q, b * a.qs[0] + q * a.qs[1] + hq * a.qs[2], a.D, lane);
+            const Two gv = load_two<DT>(a.dout, b * a.gs[0] + q * a.gs[1] + hq * a.gs[2], a.D, lane);
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(dot(qv, kv), c, f) - a.lse[row]);
+            const float ds = p * (dot(gv, vv) - a.delta[row]);
+            rk = {rk.x + ds * qv.x, rk.y + ds * qv.y};
+            rv = {rv.x + p * gv.x, rv.y + p * gv.y};
+        }
+    }
+    rk = {rk.x * a.scale, rk.y * a.scale};
+    const int64_t out = (((int64_t)b * a.Tk + key) * a.H + h) * a.D;
+    if (a.splits_kv > 1) {
+        const int64_t all = (int64_t)a.B * a.Tk * a.H * a.D;
+        store_two<AXS6_F32>(a.part_kv + split * all, out, rk, a.D, lane);
+        store_two<AXS6_F32>(a.part_kv + (a.splits_kv + split) * all, out, rv, a.D, lane);
+    } else {
+        store_two<DT>(a.dk, out, rk, a.D, lane);
+        store_two<DT>(a.dv, out, rv, a.D, lane);
+    }
+}
+
 template <int DT, int DC> struct DqShape {
     static constexpr int kKeys = DT == AXS6_F32 ? 32 : 64;
     static constexpr int kOccupancy = DT == AXS6_F32 ? 1 : 2;
@@ -133,19 +194,22 @@ __global__ __launch_bounds__(kThr, (DqShape<DT, DC>::kOccupancy)) void attn_dq_k
         if constexpr (MASK == kKeyMask)
             if (threadIdx.x < KEYS) term[(t + 1) & 1][threadIdx.x] = next_term;
     }
-    if (q >= a.Tq) return;
-    const int64_t out = (((int64_t)b * a.Tq + q) * a.Hq + hq) * a.D;
-    if (a.splits > 1) {
+    const bool bad = not_finite(dq);
+    const int64_t out = (((int64_t)b * a.Tq + qr) * a.Hq + hq) * a.D;
+    if (q < a.Tq) {
         float* part = a.part + split * ((int64_t)a.B * a.Tq * a.Hq * a.D);
 #pragma unroll
-        for (int d = 0; d < DC / 32; ++d) store_cols<AXS6_F32>(part, out, d, dq[d], a.scale, a.D, lane);
-        return;
+        for (int d = 0; d < DC / 32; ++d) {
+            if (a.splits > 1) store_cols<AXS6_F32>(part, out, d, dq[d], a.scale, a.D, lane);
+            else store_cols<DT>(a.dq, out, d, dq[d], a.scale, a.D, lane);
+        }
     }
-#pragma unroll
-    for (int d = 0; d < DC / 32; ++d) store_cols<DT>(a.dq, out, d, dq[d], a.scale, a.D, lane);
+    for (uint64_t rows = __ballot(bad && lane < 32 && q < a.Tq); rows; rows &= rows - 1) {
+        const int r = __builtin_ctzll(rows);
+        dq_row<DT>(a, b, hq, q0 + 32 * w + r, first * KEYS, tiles * KEYS < a.Tk ? tiles * KEYS : a.Tk, split,
+                   __shfl(lse, r, 64), __shfl(delta, r, 64), lane);
+    }
 }
-
-constexpr int kWalk = 32;   // queries of a tile
 
 template <int DT, int DC> struct DkvShape {
     // the values held stay in LDS where their fragments would leave a wave more
@@ -273,22 +337,22 @@ __global__ __launch_bounds__(kThr, (DkvShape<DT, DC>::kOccupancy)) void attn_dkv
         }
         if (t + 1 < tiles) store((t + 1) & 1);
     }
-    if (key >= a.Tk) return;
-    const int64_t out = (((int64_t)b * a.Tk + key) * a.H + h) * a.D;
-    if (a.splits_kv > 1) {
-        const int64_t all = (int64_t)a.B * a.Tk * a.H * a.D;
+    const bool bad = not_finite(dk) || not_finite(dv);
+    if (key < a.Tk) {
+        const int64_t out = (((int64_t)b * a.Tk + key) * a.H + h) * a.D, all = (int64_t)a.B * a.Tk * a.H * a.D;
 #pragma unroll
         for (int d = 0; d < DC / 32; ++d) {
-            store_cols<AXS6_F32>(a.part_kv + split * all, out, d, dk[d], a.scale, a.D, lane);
-            store_cols<AXS6_F32>(a.part_kv + (a.splits_kv + split) * all, out, d, dv[d], 1.0f, a.D, lane);
+            if (a.splits_kv > 1) {
+                store_cols<AXS6_F32>(a.part_kv + split * all, out, d, dk[d], a.scale, a.D, lane);
+                store_cols<AXS6_F32>(a.part_kv + (a.splits_kv + split) * all, out, d, dv[d], 1.0f, a.D, lane);
+            } else {
+                store_cols<DT>(a.dk, out, d, dk[d], a.scale, a.D, lane);
+                store_cols<DT>(a.dv, out, d, dv[d], 1.0f, a.D, lane);
+            }
         }
-        return;
     }
-#pragma unroll
-    for (int d = 0; d < DC / 32; ++d) {
-        store_cols<DT>(a.dk, out, d, dk[d], a.scale, a.D, lane);
-        store_cols<DT>(a.dv, out, d, dv[d], 1.0f, a.D, lane);
-    }
+    for (uint64_t rows = __ballot(bad && lane < 32 && key < a.Tk); rows; rows &= rows - 1)
+        dkv_row<DT>(a, b, h, k0 + 32 * w + __builtin_ctzll(rows), first, tiles, q_first, per_head, split, lane);
 }
 
 // Sums of the splits in order, four values a thread.

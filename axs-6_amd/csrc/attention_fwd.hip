@@ -32,6 +32,43 @@ namespace {
 // reference before the row is rescaled, which then hardly ever happens.
 constexpr float kSlack = 8.0f;
 
+// A row of a split's partial results.
+__device__ __forceinline__ int64_t split_row(const AttnArgs& a, int split, int b, int hq, int q) {
+    return (((int64_t)split * a.B + b) * a.Hq + hq) * a.Tq + q;
+}
+
+// A row's results from the keys k0 .. k1 - 1 that it sees, one by one.
+template <int DT>
+__device__ void forward_row(const AttnArgs& a, int b, int hq, int q, int k0, int k1, int split, int lane) {
+    const int h = hq / a.G;
+    const float c = a.scale * kLog2e;
+    const Two qv = load_two<DT>(a.q, b * a.qs[0] + q * a.qs[1] + hq * a.qs[2], a.D, lane);
+    Two o = {0.0f, 0.0f};
+    float m = -INFINITY, l = 0.0f;
+    for (int key = k0; key < k1 && !all_nan(o, a.D, lane); ++key) {
+        const float f = pair_term(a, b, hq, q, key);
+        if (f == -INFINITY) continue;
+        const Two v = load_two<DT>(a.v, b * a.vs[0] + key * a.vs[1] + h * a.vs[2], a.D, lane);
+        const float x =
+            __builtin_fmaf(dot(qv, load_two<DT>(a.k, b * a.ks[0] + key * a.ks[1] + h * a.ks[2], a.D, lane)), c, f);
+        const float mn = fmaxf(m, x), ref = mn == -INFINITY ? 0.0f : mn;
+        const float alpha = __builtin_amdgcn_exp2f(m - ref), p = __builtin_amdgcn_exp2f(x - ref);
+        m = mn;
+        l = l * alpha + p;
+        o = {o.x * alpha + p * v.x, o.y * alpha + p * v.y};
+    }
+    if (a.splits > 1) {
+        const int64_t at = split_row(a, split, b, hq, q);
+        if (lane == 0) { a.stat[2 * at] = m; a.stat[2 * at + 1] = l; }
+        store_two<AXS6_F32>(a.part, at * a.D, o, a.D, lane);
+        return;
+    }
+    const float rl = l == 0.0f ? 0.0f : 1.0f / l;
+    store_two<DT>(a.o, (((int64_t)b * a.Tq + q) * a.Hq + hq) * a.D, {o.x * rl, o.y * rl}, a.D, lane);
+    if (a.lse && lane == 0)
+        a.lse[((int64_t)b * a.Hq + hq) * a.Tq + q] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
+}
+
 // Queries and keys of a workgroup's tile.
 template <int DT, int DC, bool LARGE> struct FwdShape {
     static constexpr int kWaves = LARGE ? 8 : 4;
@@ -166,20 +203,25 @@ attn_fwd_kernel(AttnArgs a) {
             if (threadIdx.x < S::kKeys) term[(t + 1) & 1][threadIdx.x] = next_term;
     }
     l += __shfl_xor(l, 32, 64);
-    if (q >= a.Tq) return;
-    if (a.splits > 1) {
-        const int64_t at = split * ((int64_t)a.B * a.Hq * a.Tq) + ((int64_t)b * a.Hq + hq) * a.Tq + q;
-        if (lane < 32) { a.stat[2 * at] = m; a.stat[2 * at + 1] = l; }
+    const bool bad = not_finite(o);
+    if (q < a.Tq) {
+        if (a.splits > 1) {
+            const int64_t at = split_row(a, split, b, hq, q);
+            if (lane < 32) { a.stat[2 * at] = m; a.stat[2 * at + 1] = l; }
 #pragma unroll
-        for (int d = 0; d < DC / 32; ++d) store_cols<AXS6_F32>(a.part, at * a.D, d, o[d], 1.0f, a.D, lane);
-        return;
+            for (int d = 0; d < DC / 32; ++d) store_cols<AXS6_F32>(a.part, at * a.D, d, o[d], 1.0f, a.D, lane);
+        } else {
+            const float rl = l == 0.0f ? 0.0f : 1.0f / l;
+            const int64_t row = (((int64_t)b * a.Tq + q) * a.Hq + hq) * a.D;
+#pragma unroll
+            for (int d = 0; d < DC / 32; ++d) store_cols<DT>(a.o, row, d, o[d], rl, a.D, lane);
+            if (a.lse && lane < 32)
+                a.lse[((int64_t)b * a.Hq + hq) * a.Tq + q] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
+        }
     }
-    const float rl = l == 0.0f ? 0.0f : 1.0f / l;
-    const int64_t row = (((int64_t)b * a.Tq + q) * a.Hq + hq) * a.D;
-#pragma unroll
-    for (int d = 0; d < DC / 32; ++d) store_cols<DT>(a.o, row, d, o[d], rl, a.D, lane);
-    if (a.lse && lane < 32)
-        a.lse[((int64_t)b * a.Hq + hq) * a.Tq + q] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
+    for (uint64_t rows = __ballot(bad && lane < 32 && q < a.Tq); rows; rows &= rows - 1)
+        forward_row<DT>(a, b, hq, q0 + 32 * w + __builtin_ctzll(rows), first * S::kKeys,
+                        tiles * S::kKeys < a.Tk ? tiles * S::kKeys : a.Tk, split, lane);
 }
 
 // Joins the splits of a row in order: one wave a row.

@@ -54,6 +54,13 @@ def seen(B, Hq, Tq, Tk, causal, mask):
     return ok, add
 
 
+def seen_product(w, m, x):
+    """w x over the pairs of m alone: a weight of 0 elsewhere would turn an infinity or NaN of x into NaN."""
+    if x.isfinite().all():
+        return w @ x
+    return torch.where(m[:, :, None], w[:, :, None] * x[None], 0.0).sum(1)
+
+
 def attention(q, k, v, go=None, mask=None, causal=False, scale=None):
     """out, or (out, dq, dk, dv) for the output's gradient go; unseen keys have no part in a row."""
     q, k, v = (x.detach().double().cpu() for x in (q, k, v))
@@ -71,15 +78,16 @@ def attention(q, k, v, go=None, mask=None, causal=False, scale=None):
             top = x.amax(-1, keepdim=True) if Tk else x.new_zeros(Tq, 1)
             e = torch.where(m, (x - torch.where(top == -math.inf, 0.0, top)).exp(), 0.0)
             total = e.sum(-1, keepdim=True)
-            p = torch.where(total > 0, e / torch.where(total > 0, total, 1.0), 0.0) if Tk else e
-            out[b, :, h] = p @ vh
+            p = torch.where(total == 0, 0.0, e / total) if Tk else e   # a NaN total stays
+            out[b, :, h] = seen_product(p, m, vh)
             if go is not None:
                 gh = go[b, :, h].detach().double().cpu()
                 dp = gh @ vh.T
-                ds = p * (dp - (p * dp).sum(-1, keepdim=True)) * scale
-                dq[b, :, h] = ds @ kh
-                dk[b, :, h // g] += ds.T @ qh
-                dv[b, :, h // g] += p.T @ gh
+                pdp = torch.where(m, p * dp, 0.0)
+                ds = torch.where(m, (pdp - p * pdp.sum(-1, keepdim=True)) * scale, 0.0)
+                dq[b, :, h] = seen_product(ds, m, kh)
+                dk[b, :, h // g] += seen_product(ds.T, m.T, qh)
+                dv[b, :, h // g] += seen_product(p.T, m.T, gh)
     return out if go is None else (out, dq, dk, dv)
 
 

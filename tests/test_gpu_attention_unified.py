@@ -165,6 +165,45 @@ def test_layouts_and_strides(dtype):
     _check(*one, go)
 
 
+@pytest.mark.parametrize("dtype", ref.DTYPES)
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("Tk", [90, 2100])
+def test_bad_values_where_nobody_looks(Tk, bad, dtype):
+    """Infinities and NaN in keys and values that a query does not see have no part in its results, and queries that
+    see nothing none in the keys'."""
+    Tq = 70 if Tk == 90 else 6      # the longer keys are split over workgroups
+    q, k, v, go = _inputs(2, Tq, Tk, 4, 2, 64, dtype)
+    keep = torch.rand(2, 1, Tq, Tk, generator=torch.Generator().manual_seed(3)) < 0.7
+    keep[..., 60:75] = False
+    keep[:, :, 4] = False
+    k[:, 60:70], v[0, 65:75, :, 5] = bad, bad
+    q[:, 4], go[1, 4] = bad, bad
+    _check(q, k, v, go, keep.to(DEV))
+    pad = torch.ones(2, 1, 1, Tk, dtype=torch.bool)
+    pad[..., 60:75] = False
+    _check(*(torch.where(x.isfinite(), x, 0.5) if i in (0, 3) else x for i, x in enumerate((q, k, v, go))), pad.to(DEV))
+
+
+@pytest.mark.parametrize("dtype", ref.DTYPES)
+def test_bad_values_that_are_seen(dtype):
+    """A NaN key or an infinite value reaches the rows that see it and no others."""
+    from axs.unified import axs_attention_unified
+
+    q, k, v, go = _inputs(1, 80, 80, 2, 2, 64, dtype)
+    k[0, 50, 0], v[0, 40, 1, 7] = math.nan, math.inf
+    xs = [x.requires_grad_(True) for x in (q, k, v)]
+    out = axs_attention_unified(*xs, causal=True)
+    want, dq, dk, dv = ref.attention(q, k, v, go, causal=True)
+    got = out.detach().double().cpu()
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf(), want.isinf())
+    fine = want.isfinite()
+    assert ref.rel(torch.where(fine, got, 0.0), torch.where(fine, want, 0.0)) <= _bounds(dtype)[0]
+    for x, y in zip(torch.autograd.grad(out, xs, go), (dq, dk, dv)):
+        x = x.double().cpu()
+        assert torch.equal(x.isfinite(), y.isfinite())
+        assert ref.rel(torch.where(y.isfinite(), x, 0.0), torch.where(y.isfinite(), y, 0.0)) <= _bounds(dtype)[1]
+
+
 def test_scale():
     q, k, v, go = _inputs(1, 40, 50, 2, 2, 64, torch.float32)
     for s in (1e-4, 0.5):
