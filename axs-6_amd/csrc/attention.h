@@ -129,47 +129,76 @@ struct Tile {
         return a;
     }
 
-    // c += (columns 32 d .. 32 d + 31 of the 32 rows from row0)^T p, p a result
-    // whose rows are these rows; pf: p in fragments (16-bit types).
-    __device__ static f32x16 cols(const char* tile, int row0, int d, const f32x16& p, const u32x4 (&pf)[2], f32x16 c,
-                                  int lane) {
-        const int h = lane >> 5;
+    // Results over a tile's columns: DC / 32 of them.  Row r of result d is
+    // column 32 d + r of the tile in the 16-bit types.  In float32 a lane reads
+    // the columns of several results at once: column 4 r + d of four, 2 r + d of
+    // the first two, 64 + r of the third of three.
+    static constexpr int kResults = DC / 32;
+
+    // o += (the 32 rows from row0)^T p, p a result whose rows are these rows; pf: p
+    // in fragments (16-bit types).
+    __device__ static void accumulate(const char* tile, int row0, const f32x16& p, const u32x4 (&pf)[2],
+                                      f32x16 (&o)[kResults], int lane) {
         if constexpr (DT == AXS6_F32) {
+            const int m = lane & 31;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const int row = row0 + 8 * (i >> 2) + 4 * h + (i & 3), col = 32 * d + (lane & 31);
-                const float x = *reinterpret_cast<const float*>(tile + at(row, col >> 2) + (col & 3) * 4);
-                c = __builtin_amdgcn_mfma_f32_32x32x2f32(x, p[i], c, 0, 0, 0);
+                const int row = row0 + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3);
+                float x[4];
+                if constexpr (kResults == 4) {
+                    const float4 v = *reinterpret_cast<const float4*>(tile + at(row, m));
+                    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+                } else {
+                    const float2 v = *reinterpret_cast<const float2*>(tile + at(row, m >> 1) + (m & 1) * 8);
+                    x[0] = v.x; x[1] = v.y;
+                    if constexpr (kResults == 3)
+                        x[2] = *reinterpret_cast<const float*>(tile + at(row, 16 + (m >> 2)) + (m & 3) * 4);
+                }
+#pragma unroll
+                for (int d = 0; d < kResults; ++d)
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[d], p[i], o[d], 0, 0, 0);
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) c = mma<DT>(col_fragment(tile, row0 + 16 * j, d, lane), pf[j], c);
+            for (int d = 0; d < kResults; ++d)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) o[d] = mma<DT>(col_fragment(tile, row0 + 16 * j, d, lane), pf[j], o[d]);
         }
-        return c;
     }
 
-    // The same for the results p[n][j] of N sets of columns, into o[n][d]: the
-    // tile is read once.
-    template <int N, int NK, int ND>
-    __device__ static void cols_n(const char* tile, int j, int d, const f32x16 (&p)[N][NK], const u32x4 (&pf)[N][NK][2],
-                                  f32x16 (&o)[N][ND], int lane) {
-        const int h = lane >> 5;
+    // The results, times f, as the lane's row of memory (element `row` of out) in
+    // the type OUT.
+    template <int OUT>
+    __device__ static void store(void* out, int64_t row, const f32x16 (&o)[kResults], float f, int D, int lane) {
+        auto* p = reinterpret_cast<typename Elem<OUT>::S*>(out) + row;
+        const int h4 = 4 * (lane >> 5);
         if constexpr (DT == AXS6_F32) {
+            static_assert(OUT == AXS6_F32, "float32 results");
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const int row = 32 * j + 8 * (i >> 2) + 4 * h + (i & 3), col = 32 * d + (lane & 31);
-                const float x = *reinterpret_cast<const float*>(tile + at(row, col >> 2) + (col & 3) * 4);
-#pragma unroll
-                for (int n = 0; n < N; ++n)
-                    o[n][d] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, p[n][j][i], o[n][d], 0, 0, 0);
+                const int r = 8 * (i >> 2) + h4 + (i & 3);
+                if constexpr (kResults == 4) {
+                    if (4 * r < D)
+                        *reinterpret_cast<float4*>(p + 4 * r) =
+                            make_float4(o[0][i] * f, o[1][i] * f, o[2][i] * f, o[3][i] * f);
+                } else {
+                    if (2 * r < D) *reinterpret_cast<float2*>(p + 2 * r) = make_float2(o[0][i] * f, o[1][i] * f);
+                    if constexpr (kResults == 3)
+                        if (64 + r < D) p[64 + r] = o[2][i] * f;
+                }
             }
         } else {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const u32x4 x = col_fragment(tile, 32 * j + 16 * e, d, lane);
+            for (int d = 0; d < kResults; ++d)
 #pragma unroll
-                for (int n = 0; n < N; ++n) o[n][d] = mma<DT>(x, pf[n][j][e], o[n][d]);
-            }
+                for (int g = 0; g < 4; ++g) {
+                    const int col = 32 * d + 8 * g + h4;
+                    const float x = o[d][4 * g] * f, y = o[d][4 * g + 1] * f, z = o[d][4 * g + 2] * f,
+                                w = o[d][4 * g + 3] * f;
+                    if (col >= D) continue;
+                    if constexpr (OUT == AXS6_F32) *reinterpret_cast<float4*>(p + col) = make_float4(x, y, z, w);
+                    else *reinterpret_cast<uint2*>(p + col) = make_uint2(pack2<OUT>(x, y), pack2<OUT>(z, w));
+                }
         }
     }
 };
@@ -334,25 +363,6 @@ __device__ __forceinline__ void apply_mask(const AttnArgs& a, f32x16& s, float c
 #pragma unroll
         for (int i = 0; i < 16; ++i)
             s[i] = k0 + 8 * (i >> 2) + h4 + (i & 3) < limit ? s[i] : -INFINITY;
-}
-
-// A 32x32 result whose lanes are rows of memory: out[row][32 d + ...] of the
-// type, 4 values at a time.
-template <int DT>
-__device__ __forceinline__ void store_cols(void* out, int64_t row, int d, const f32x16& c, float f, int D, int lane) {
-    using E = Elem<DT>;
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-        const int col = 32 * d + 8 * g + 4 * (lane >> 5);
-        if (col >= D) continue;
-        auto* p = reinterpret_cast<typename E::S*>(out) + row + col;
-        if constexpr (DT == AXS6_F32) {
-            *reinterpret_cast<float4*>(p) = make_float4(c[4 * g] * f, c[4 * g + 1] * f, c[4 * g + 2] * f, c[4 * g + 3] * f);
-        } else {
-            *reinterpret_cast<uint2*>(p) =
-                make_uint2(pack2<DT>(c[4 * g] * f, c[4 * g + 1] * f), pack2<DT>(c[4 * g + 2] * f, c[4 * g + 3] * f));
-        }
-    }
 }
 
 // ---- rows again -------------------------------------------------------------

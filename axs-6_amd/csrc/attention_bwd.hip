@@ -158,6 +158,8 @@ __global__ __launch_bounds__(kThr, (DqShape<DT, DC>::kOccupancy)) void attn_dq_k
     f32x16 dq[DC / 32];
 #pragma unroll
     for (int d = 0; d < DC / 32; ++d) dq[d] = zero16();
+    const int w_last = q0 + 32 * w + 31 < a.Tq ? q0 + 32 * w + 31 : a.Tq - 1;   // the wave's last row and its keys
+    const int w_keys = a.causal && w_last + off + 1 < a.Tk ? w_last + off + 1 : a.Tk;
     for (int t = first; t < tiles; ++t) {
         tile_barrier();
         float next_term = 0.0f;
@@ -173,6 +175,7 @@ __global__ __launch_bounds__(kThr, (DqShape<DT, DC>::kOccupancy)) void attn_dq_k
         if (any) {
 #pragma unroll
             for (int j = 0; j < NK; ++j) {
+                if (k0 + 32 * j >= w_keys) break;   // none of the wave's rows sees them
                 f32x16 s = zero16(), dp = zero16();
 #pragma unroll
                 for (int i = 0; i < T::kSteps; ++i) s = mma<DT>(T::rows(ks, 32 * j, i, lane), qf[i], s);
@@ -187,8 +190,7 @@ __global__ __launch_bounds__(kThr, (DqShape<DT, DC>::kOccupancy)) void attn_dq_k
                 }
                 u32x4 pf[2];
                 fragments<DT>(s, pf);
-#pragma unroll
-                for (int d = 0; d < DC / 32; ++d) dq[d] = T::cols(ks, 32 * j, d, s, pf, dq[d], lane);
+                T::accumulate(ks, 32 * j, s, pf, dq, lane);
             }
         }
         if constexpr (MASK == kKeyMask)
@@ -198,11 +200,8 @@ __global__ __launch_bounds__(kThr, (DqShape<DT, DC>::kOccupancy)) void attn_dq_k
     const int64_t out = (((int64_t)b * a.Tq + qr) * a.Hq + hq) * a.D;
     if (q < a.Tq) {
         float* part = a.part + split * ((int64_t)a.B * a.Tq * a.Hq * a.D);
-#pragma unroll
-        for (int d = 0; d < DC / 32; ++d) {
-            if (a.splits > 1) store_cols<AXS6_F32>(part, out, d, dq[d], a.scale, a.D, lane);
-            else store_cols<DT>(a.dq, out, d, dq[d], a.scale, a.D, lane);
-        }
+        if (a.splits > 1) T::template store<AXS6_F32>(part, out, dq, a.scale, a.D, lane);
+        else T::template store<DT>(a.dq, out, dq, a.scale, a.D, lane);
     }
     for (uint64_t rows = __ballot(bad && lane < 32 && q < a.Tq); rows; rows &= rows - 1) {
         const int r = __builtin_ctzll(rows);
@@ -292,8 +291,9 @@ __global__ __launch_bounds__(kThr, (DkvShape<DT, DC>::kOccupancy)) void attn_dkv
         if (i0 >= a.Tq) { i0 = q_first; ++hq; }
         if (t + 1 < tiles) load((t + 1) & 1);
         const char *qs = qt[t & 1], *gs = gt[t & 1];
-        bool any = true;
-        if constexpr (MASK == kKeyMask) any = __any(!(term == -INFINITY));
+        // none of the tile's queries sees the wave's keys: they are before them, or the mask hides them
+        bool any = !a.causal || i_now + kWalk - 1 + off >= k0 + 32 * w;
+        if constexpr (MASK == kKeyMask) any = any && __any(!(term == -INFINITY));
         if (any) {
             f32x16 s = zero16(), dp = zero16();
 #pragma unroll
@@ -330,25 +330,20 @@ __global__ __launch_bounds__(kThr, (DkvShape<DT, DC>::kOccupancy)) void attn_dkv
             u32x4 pf[2], df[2];
             fragments<DT>(s, pf);
             fragments<DT>(dp, df);
-#pragma unroll
-            for (int d = 0; d < DC / 32; ++d) dv[d] = T::cols(gs, 0, d, s, pf, dv[d], lane);
-#pragma unroll
-            for (int d = 0; d < DC / 32; ++d) dk[d] = T::cols(qs, 0, d, dp, df, dk[d], lane);
+            T::accumulate(gs, 0, s, pf, dv, lane);
+            T::accumulate(qs, 0, dp, df, dk, lane);
         }
         if (t + 1 < tiles) store((t + 1) & 1);
     }
     const bool bad = not_finite(dk) || not_finite(dv);
     if (key < a.Tk) {
         const int64_t out = (((int64_t)b * a.Tk + key) * a.H + h) * a.D, all = (int64_t)a.B * a.Tk * a.H * a.D;
-#pragma unroll
-        for (int d = 0; d < DC / 32; ++d) {
-            if (a.splits_kv > 1) {
-                store_cols<AXS6_F32>(a.part_kv + split * all, out, d, dk[d], a.scale, a.D, lane);
-                store_cols<AXS6_F32>(a.part_kv + (a.splits_kv + split) * all, out, d, dv[d], 1.0f, a.D, lane);
-            } else {
-                store_cols<DT>(a.dk, out, d, dk[d], a.scale, a.D, lane);
-                store_cols<DT>(a.dv, out, d, dv[d], 1.0f, a.D, lane);
-            }
+        if (a.splits_kv > 1) {
+            T::template store<AXS6_F32>(a.part_kv + split * all, out, dk, a.scale, a.D, lane);
+            T::template store<AXS6_F32>(a.part_kv + (a.splits_kv + split) * all, out, dv, 1.0f, a.D, lane);
+        } else {
+            T::template store<DT>(a.dk, out, dk, a.scale, a.D, lane);
+            T::template store<DT>(a.dv, out, dv, 1.0f, a.D, lane);
         }
     }
     for (uint64_t rows = __ballot(bad && lane < 32 && key < a.Tk); rows; rows &= rows - 1)
