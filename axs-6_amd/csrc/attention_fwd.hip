@@ -24,6 +24,7 @@
 // Few rows against many keys: the keys are split over workgroups, whose sums a
 // second launch joins (4 x 4 queries of 16 heads, 8000 keys: 165 -> 41 us).
 #include "attention.h"
+#include "split_join.h"
 
 namespace axs6 {
 namespace {
@@ -236,33 +237,18 @@ attn_fwd_kernel(AttnArgs a) {
                         tiles * S::kKeys < a.Tk ? tiles * S::kKeys : a.Tk, split, lane);
 }
 
-// Joins the splits of a row in order: one wave a row.
 template <int DT>
-__global__ __launch_bounds__(64) void attn_join_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kJoinThreads) void attn_join_kernel(AttnArgs a) {
     using E = Elem<DT>;
-    const int64_t rows = (int64_t)a.B * a.Hq * a.Tq, row = blockIdx.x, bh = row / a.Tq;
+    const int64_t row = blockIdx.x, bh = row / a.Tq;
     const int q = (int)(row - bh * a.Tq);
-    float m = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.stat[2 * (s * rows + row)]);
-    const float ref = m == -INFINITY ? 0.0f : m;
-    const int d = threadIdx.x * 2;
-    float l = 0.0f, x = 0.0f, y = 0.0f;
-    for (int s = 0; s < a.splits; ++s) {
-        const int64_t at = s * rows + row;
-        const float f = __builtin_amdgcn_exp2f(a.stat[2 * at] - ref);
-        l += a.stat[2 * at + 1] * f;
-        if (d < a.D) {
-            const float2 p = *reinterpret_cast<const float2*>(a.part + at * a.D + d);
-            x += p.x * f;
-            y += p.y * f;
-        }
-    }
-    if (a.lse && threadIdx.x == 0) a.lse[row] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
-    if (d >= a.D) return;
-    const float rl = l == 0.0f ? 0.0f : 1.0f / l;
-    auto* out = reinterpret_cast<typename E::S*>(a.o) + (((bh / a.Hq) * a.Tq + q) * a.Hq + bh % a.Hq) * a.D + d;
-    out[0] = E::from_f(x * rl);
-    out[1] = E::from_f(y * rl);
+    const Joined j = join_row(a.part, a.stat, (int64_t)a.B * a.Hq * a.Tq, row, a.splits, a.D);
+    if (j.d < 0) return;
+    if (a.lse && j.d == 0) a.lse[row] = j.l == 0.0f ? INFINITY : j.m + __builtin_amdgcn_logf(j.l);
+    const float rl = j.l == 0.0f ? 0.0f : 1.0f / j.l;
+    auto* out = reinterpret_cast<typename E::S*>(a.o) + (((bh / a.Hq) * a.Tq + q) * a.Hq + bh % a.Hq) * a.D + j.d;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = E::from_f(j.o[i] * rl);
 }
 
 template <int DT, int DC, int MASK, bool LARGE>
@@ -270,7 +256,7 @@ void launch(const AttnArgs& a, hipStream_t st) {
     using S = FwdShape<DT, DC, LARGE>;
     const unsigned grid = (unsigned)((a.Tq + S::kQ - 1) / S::kQ * a.B * a.Hq * a.splits);
     attn_fwd_kernel<DT, DC, MASK, LARGE><<<grid, S::kThreads, 0, st>>>(a);
-    if (a.splits > 1) attn_join_kernel<DT><<<(unsigned)(a.B * a.Hq * a.Tq), 64, 0, st>>>(a);
+    if (a.splits > 1) attn_join_kernel<DT><<<(unsigned)(a.B * a.Hq * a.Tq), kJoinThreads, 0, st>>>(a);
 }
 
 template <int DT, int DC>
@@ -307,7 +293,7 @@ int split_count(int64_t groups, int64_t steps, int64_t want, int64_t least, int6
 // 256 keys a part at the least.
 int forward_splits(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq) {
     const int64_t groups = (Tq + 127) / 128 * B * Hq;
-    return groups >= 256 ? 1 : split_count(groups, Tk / 256, 512, 1, 64);
+    return groups >= 256 ? 1 : split_count(groups, Tk / 256, 512, 1, kMaxSplits);
 }
 // The backward walks over keys for dq, as the forward, and over the queries of a
 // group's heads for dk and dv.  There a causal mask gives some keys' workgroups

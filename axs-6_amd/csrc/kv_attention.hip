@@ -18,14 +18,22 @@
 // S^T = K q^T by 16x16x32 instructions with the keys as rows: a lane then
 // holds 8 consecutive keys of one query row, which is the order in which the
 // second product takes them, so the probabilities never leave their registers.
-// A workgroup's four waves take every fourth block of its range; where there
-// are few rows the blocks are split over more workgroups and joined by a
-// second launch.
+// A workgroup's waves take every so-many-th block of its range; where there are
+// few rows the blocks are split over more workgroups and joined by a second
+// launch, in which a thread takes one split's factor and groups of threads every
+// so-many-th sum (one wave a row that walked over the splits took three times the
+// attention: 1 x 16384 tokens, 8 key heads for 32, 48 us against 15).
+// Measured: 64 sequences of 4096 to 16383 tokens, 8 key heads of 128 for 64,
+// 290 us, 4.6 TB/s (a copy of 4 GiB runs at 4.7 on this card); one of 131072
+// 55 us; one of 300, where launches and latency count, 8.7 us.  Holding the next
+// block's codes on their way costs registers and with them waves: 64 x 2048
+// tokens 22.8 -> 25.7 us.
 #include <math.h>
 
 #include "axs6_internal.h"
 #include "kv_cache.h"
 #include "nf5_device.h"
+#include "split_join.h"
 
 namespace axs6 {
 namespace {
@@ -38,7 +46,6 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kProbScale = 16384.0f;   // 2^14
 constexpr float kSumScale = 1048576.0f;  // 2^20: sums are held as 2^-20 of themselves, so that values near
                                          // float32's largest, summed before they are divided, stay finite
-constexpr int kWaves = 4;
 
 struct KvAttnArgs {
     const void* q;
@@ -88,30 +95,60 @@ __device__ __forceinline__ void load16(const void* p, int64_t i, bool vec, float
     }
 }
 
-// NC: 64-value pieces of a head.
-template <int DT, int NC>
-__global__ __launch_bounds__(64 * kWaves) void kv_attention_kernel(KvAttnArgs a) {
+// A block's codes as a lane takes them.
+template <int NC>
+__device__ __forceinline__ void load_block(u32x4 (&k)[2][NC], uint2 (&v)[NC * 4], const KvAttnArgs& a, int64_t cell,
+                                           int n16, int g4) {
+    const int8_t* kc = a.kc + cell * kKvBlock * a.D;
+    const int8_t* vc = a.vc + cell * kKvBlock * a.D;
+#pragma unroll
+    for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            k[tt][c] = u32x4{0, 0, 0, 0};
+            const int key = 8 * (n16 >> 2) + 4 * tt + (n16 & 3);
+            if (64 * c + 16 * g4 < a.D)
+                k[tt][c] = *reinterpret_cast<const u32x4*>(kc + key * a.D + 64 * c + 16 * g4);
+        }
+#pragma unroll
+    for (int d = 0; d < NC * 4; ++d) {
+        v[d] = make_uint2(0, 0);
+        if (16 * d < a.D) v[d] = *reinterpret_cast<const uint2*>(vc + (16 * d + n16) * kKvBlock + 8 * g4);
+    }
+}
+
+// NC: 64-value pieces of a head.  NR: 16-row pieces of queries that a wave takes
+// against each block.  WAVES: of a workgroup, each of which takes every WAVES-th
+// block of its range.
+template <int DT, int NC, int NR, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void kv_attention_kernel(KvAttnArgs a) {
     constexpr int TERMS = DT == AXS6_F32 ? 2 : 1;
     constexpr int ND = NC * 4;   // 16-value pieces of a head
-    __shared__ float sh_o[2][ND * 4][64];
-    __shared__ float sh_m[kWaves][16], sh_l[kWaves][16];
+    __shared__ float sh_o[WAVES / 2][NR * ND * 4][64];
+    __shared__ float sh_m[WAVES][NR * 16], sh_l[WAVES][NR * 16];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n16 = lane & 15, g4 = lane >> 4;
     const int rt = blockIdx.x % a.row_tiles, bh = blockIdx.x / a.row_tiles, h = bh % a.H, b = bh / a.H;
     const int64_t cap = (int64_t)a.nb * kKvBlock;
     int64_t len = a.lengths[b];
     len = len < 0 ? 0 : len > cap ? cap : len;
-    const int r = rt * 16 + n16, rr = r < a.rows ? r : a.rows - 1, t = rr / a.G, hq = h * a.G + rr % a.G;
-    const int last = (int)(len - a.Tq) + t;   // the last key that this lane's row sees
-    const int r_top = rt * 16 + 15 < a.rows ? rt * 16 + 15 : a.rows - 1;
+    const int r0 = rt * NR * 16, r_top = r0 + NR * 16 < a.rows ? r0 + NR * 16 - 1 : a.rows - 1;
     const int keys = (int)(len - a.Tq) + r_top / a.G + 1;
     const int blocks = keys <= 0 ? 0 : (keys + kKvBlock - 1) / kKvBlock;
     const int per = (blocks + a.splits - 1) / a.splits;
     const int b0 = blockIdx.y * per, b1 = b0 + per < blocks ? b0 + per : blocks;
+    const int64_t cell0 = (int64_t)bh * a.nb;
+    u32x4 kr[2][NC];
+    uint2 vr[ND];
+    if (b0 + w < b1) load_block<NC>(kr, vr, a, cell0 + b0 + w, n16, g4);
 
-    // the row's query, scaled, in the products' order: piece c, value 16 g4 + j
-    f16x8 qf[TERMS][NC][2];
-    float rs;
-    {
+    // the rows' queries, scaled, in the products' order: piece c, value 16 g4 + j
+    f16x8 qf[NR][TERMS][NC][2];
+    float rs[NR];
+    int last[NR];   // the last key that the lane's row sees
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+        const int r = r0 + 16 * n + n16, rr = r < a.rows ? r : a.rows - 1, t = rr / a.G, hq = h * a.G + rr % a.G;
+        last[n] = (int)(len - a.Tq) + t;
         float f[NC][16], amax = 0.0f;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
@@ -131,182 +168,208 @@ __global__ __launch_bounds__(64 * kWaves) void kv_attention_kernel(KvAttnArgs a)
             for (int j = 0; j < 16; ++j) {
                 const float x = ldexpf(f[c][j], -e);
                 const _Float16 hi = (_Float16)x;
-                qf[0][c][j >> 3][j & 7] = hi;
-                if constexpr (TERMS == 2) qf[1][c][j >> 3][j & 7] = (_Float16)(x - (float)hi);
+                qf[n][0][c][j >> 3][j & 7] = hi;
+                if constexpr (TERMS == 2) qf[n][1][c][j >> 3][j & 7] = (_Float16)(x - (float)hi);
             }
-        rs = ldexpf(a.scale * kLog2e, e);
+        rs[n] = ldexpf(a.scale * kLog2e, e);
     }
 
-    f32x4 o[ND];
+    f32x4 o[NR][ND];
+    float m[NR], l[NR];
 #pragma unroll
-    for (int d = 0; d < ND; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    float m = -INFINITY, l = 0.0f;
-    for (int blk = b0 + w; blk < b1; blk += kWaves) {
-        const int64_t cell = (int64_t)bh * a.nb + blk;
-        const int8_t* kc = a.kc + cell * kKvBlock * a.D;
-        const int8_t* vc = a.vc + cell * kKvBlock * a.D;
-        const float ks = a.ks[cell];
-        u32x4 kr[2][NC];
-        uint2 vr[ND];
+    for (int n = 0; n < NR; ++n) {
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                kr[tt][c] = u32x4{0, 0, 0, 0};
-                const int key = 8 * (n16 >> 2) + 4 * tt + (n16 & 3);
-                if (64 * c + 16 * g4 < a.D)
-                    kr[tt][c] = *reinterpret_cast<const u32x4*>(kc + key * a.D + 64 * c + 16 * g4);
-            }
-#pragma unroll
-        for (int d = 0; d < ND; ++d) {
-            vr[d] = make_uint2(0, 0);
-            if (16 * d < a.D) vr[d] = *reinterpret_cast<const uint2*>(vc + (16 * d + n16) * kKvBlock + 8 * g4);
-        }
-        // a row that sees none of the block takes nothing of it, whatever its scale
-        const float vs = blk * kKvBlock > last ? 0.0f : a.vs[cell] * (1.0f / (kProbScale * kSumScale));
-        float x[8], mx = -INFINITY;
+        for (int d = 0; d < ND; ++d) o[n][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        m[n] = -INFINITY;
+        l[n] = 0.0f;
+    }
+    for (int blk = b0 + w; blk < b1; blk += WAVES) {
+        const int64_t cell = cell0 + blk;
+        if (blk != b0 + w) load_block<NC>(kr, vr, a, cell, n16, g4);   // the first came before the queries
+        const float ks = a.ks[cell], vs = a.vs[cell] * (1.0f / (kProbScale * kSumScale));
+        f32x4 s[NR][2];
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt) {
-            f32x4 s = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int n = 0; n < NR; ++n) s[n][tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
                 const f16x8 k0 = codes_f16(kr[tt][c].x, kr[tt][c].y), k1 = codes_f16(kr[tt][c].z, kr[tt][c].w);
 #pragma unroll
-                for (int u = 0; u < TERMS; ++u) {
-                    s = mma(k0, qf[u][c][0], s);
-                    s = mma(k1, qf[u][c][1], s);
-                }
-            }
+                for (int n = 0; n < NR; ++n)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int key = blk * kKvBlock + 8 * g4 + 4 * tt + i;
-                x[4 * tt + i] = key <= last ? s[i] * (rs * ks) : -INFINITY;
-                mx = fmaxf(mx, x[4 * tt + i]);
+                    for (int u = 0; u < TERMS; ++u) {
+                        s[n][tt] = mma(k0, qf[n][u][c][0], s[n][tt]);
+                        s[n][tt] = mma(k1, qf[n][u][c][1], s[n][tt]);
+                    }
             }
         }
-        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const float mn = fmaxf(m, mx), ref = mn == -INFINITY ? 0.0f : mn;
-        const float alpha = __builtin_amdgcn_exp2f(m - ref);
-        m = mn;
-        l *= alpha;
-        f16x8 pf[TERMS];
+        f16x8 pf[NR][TERMS];
+        float alpha[NR], vsn[NR];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float p = __builtin_amdgcn_exp2f(x[j] - ref);
-            l += p;
-            const float y = p * kProbScale;
-            pf[0][j] = (_Float16)y;
-            if constexpr (TERMS == 2) pf[1][j] = (_Float16)(y - (float)pf[0][j]);
+        for (int n = 0; n < NR; ++n) {
+            // a row that sees none of the block takes nothing of it, whatever its scale
+            vsn[n] = blk * kKvBlock > last[n] ? 0.0f : vs;
+            float x[8], mx = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                x[j] = blk * kKvBlock + 8 * g4 + j <= last[n] ? s[n][j >> 2][j & 3] * (rs[n] * ks) : -INFINITY;
+                mx = fmaxf(mx, x[j]);
+            }
+            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            const float mn = fmaxf(m[n], mx), ref = mn == -INFINITY ? 0.0f : mn;
+            alpha[n] = __builtin_amdgcn_exp2f(m[n] - ref);
+            m[n] = mn;
+            l[n] *= alpha[n];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float p = __builtin_amdgcn_exp2f(x[j] - ref);
+                l[n] += p;
+                const float y = p * kProbScale;
+                pf[n][0][j] = (_Float16)y;
+                if constexpr (TERMS == 2) pf[n][1][j] = (_Float16)(y - (float)pf[n][0][j]);
+            }
         }
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
             if (16 * d >= a.D) continue;
             const f16x8 vf = codes_f16(vr[d].x, vr[d].y);
-            f32x4 s = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int u = 0; u < TERMS; ++u) s = mma(vf, pf[u], s);
+            for (int n = 0; n < NR; ++n) {
+                f32x4 y = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[d][i] = o[d][i] * alpha + s[i] * vs;
+                for (int u = 0; u < TERMS; ++u) y = mma(vf, pf[n][u], y);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[n][d][i] = o[n][d][i] * alpha[n] + y[i] * vsn[n];
+            }
         }
     }
-    // join the waves: the four lanes of a row, then waves 2, 3 into 0, 1, then 1 into 0
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
-    if (g4 == 0) { sh_m[w][n16] = m; sh_l[w][n16] = l; }
+    // join the waves: the four lanes of a row, then the upper half of the waves
+    // into the lower, and again
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+        l[n] += __shfl_xor(l[n], 16, 64);
+        l[n] += __shfl_xor(l[n], 32, 64);
+        if (g4 == 0) { sh_m[w][16 * n + n16] = m[n]; sh_l[w][16 * n + n16] = l[n]; }
+    }
     __syncthreads();
-    float mt = sh_m[0][n16];
+    float lt[NR], mt[NR];
 #pragma unroll
-    for (int i = 1; i < kWaves; ++i) mt = fmaxf(mt, sh_m[i][n16]);
-    const float ref = mt == -INFINITY ? 0.0f : mt;
-    float lt = 0.0f;
+    for (int n = 0; n < NR; ++n) {
+        mt[n] = sh_m[0][16 * n + n16];
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) lt += sh_l[i][n16] * __builtin_amdgcn_exp2f(sh_m[i][n16] - ref);
-    const float f = __builtin_amdgcn_exp2f(m - ref);
+        for (int i = 1; i < WAVES; ++i) mt[n] = fmaxf(mt[n], sh_m[i][16 * n + n16]);
+        const float ref = mt[n] == -INFINITY ? 0.0f : mt[n];
+        lt[n] = 0.0f;
 #pragma unroll
-    for (int d = 0; d < ND; ++d)
+        for (int i = 0; i < WAVES; ++i)
+            lt[n] += sh_l[i][16 * n + n16] * __builtin_amdgcn_exp2f(sh_m[i][16 * n + n16] - ref);
+        const float f = __builtin_amdgcn_exp2f(m[n] - ref);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[d][i] *= f;
+        for (int d = 0; d < ND; ++d) o[n][d] *= f;
+    }
 #pragma unroll
-    for (int step = kWaves / 2; step >= 1; step >>= 1) {
+    for (int step = WAVES / 2; step >= 1; step >>= 1) {
         if (w >= step && w < 2 * step)
 #pragma unroll
-            for (int d = 0; d < ND; ++d)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) sh_o[w - step][d * 4 + i][lane] = o[d][i];
+            for (int i = 0; i < NR * ND * 4; ++i) sh_o[w - step][i][lane] = o[i / (ND * 4)][i / 4 % ND][i % 4];
         __syncthreads();
         if (w < step)
 #pragma unroll
-            for (int d = 0; d < ND; ++d)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o[d][i] += sh_o[w][d * 4 + i][lane];
+            for (int i = 0; i < NR * ND * 4; ++i) o[i / (ND * 4)][i / 4 % ND][i % 4] += sh_o[w][i][lane];
         __syncthreads();
     }
-    if (w != 0 || r >= a.rows) return;
-    const int64_t row = (int64_t)bh * a.rows + r;
-    if (a.splits > 1) {
-        const int64_t at = blockIdx.y * a.rows_all + row;
-        if (g4 == 0) { a.stat[2 * at] = mt; a.stat[2 * at + 1] = lt; }
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-            if (16 * d < a.D) *reinterpret_cast<f32x4*>(a.part + at * a.D + 16 * d + 4 * g4) = o[d];
-        return;
-    }
-    const float rl = lt == 0.0f ? 0.0f : kSumScale / lt;
+    if (w != 0) return;
     using E = Elem<DT>;
-    auto* out = reinterpret_cast<typename E::S*>(a.out) + (((int64_t)b * a.Tq + t) * a.H * a.G + hq) * a.D + 4 * g4;
 #pragma unroll
-    for (int d = 0; d < ND; ++d)
-        if (16 * d < a.D)
+    for (int n = 0; n < NR; ++n) {
+        const int r = r0 + 16 * n + n16, t = r / a.G, hq = h * a.G + r % a.G;
+        if (r >= a.rows) continue;
+        const int64_t row = (int64_t)bh * a.rows + r;
+        if (a.splits > 1) {
+            const int64_t at = blockIdx.y * a.rows_all + row;
+            if (g4 == 0) { a.stat[2 * at] = mt[n]; a.stat[2 * at + 1] = lt[n]; }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) out[16 * d + i] = E::from_f(o[d][i] * rl);
+            for (int d = 0; d < ND; ++d)
+                if (16 * d < a.D) *reinterpret_cast<f32x4*>(a.part + at * a.D + 16 * d + 4 * g4) = o[n][d];
+        } else {
+            const float rl = lt[n] == 0.0f ? 0.0f : kSumScale / lt[n];
+            auto* out =
+                reinterpret_cast<typename E::S*>(a.out) + (((int64_t)b * a.Tq + t) * a.H * a.G + hq) * a.D + 4 * g4;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+                if (16 * d < a.D)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) out[16 * d + i] = E::from_f(o[n][d][i] * rl);
+        }
+    }
 }
 
-// One wave a row: the splits' sums joined in order.
 template <int DT>
-__global__ __launch_bounds__(64) void kv_join_kernel(KvAttnArgs a) {
+__global__ __launch_bounds__(kJoinThreads) void kv_join_kernel(KvAttnArgs a) {
     using E = Elem<DT>;
     const int64_t row = blockIdx.x, bh = row / a.rows;
     const int r = (int)(row - bh * a.rows), t = r / a.G, hq = (int)(bh % a.H) * a.G + r % a.G;
-    float mt = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) mt = fmaxf(mt, a.stat[2 * (s * a.rows_all + row)]);
-    const float ref = mt == -INFINITY ? 0.0f : mt;
-    float lt = 0.0f;
-    const int d = threadIdx.x * 4;
-    f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s = 0; s < a.splits; ++s) {
-        const int64_t at = s * a.rows_all + row;
-        const float f = __builtin_amdgcn_exp2f(a.stat[2 * at] - ref);
-        lt += a.stat[2 * at + 1] * f;
-        if (d < a.D) o += *reinterpret_cast<const f32x4*>(a.part + at * a.D + d) * f;
-    }
-    if (d >= a.D) return;
-    const float rl = lt == 0.0f ? 0.0f : kSumScale / lt;
-    auto* out = reinterpret_cast<typename E::S*>(a.out) +
-                (((bh / a.H) * a.Tq + t) * a.H * a.G + hq) * a.D + d;
+    const Joined j = join_row(a.part, a.stat, a.rows_all, row, a.splits, a.D);
+    if (j.d < 0) return;
+    const float rl = j.l == 0.0f ? 0.0f : kSumScale / j.l;
+    auto* out = reinterpret_cast<typename E::S*>(a.out) + (((bh / a.H) * a.Tq + t) * a.H * a.G + hq) * a.D + j.d;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) out[i] = E::from_f(o[i] * rl);
+    for (int i = 0; i < 4; ++i) out[i] = E::from_f(j.o[i] * rl);
+}
+
+// How a call is laid out: 16-row pieces a wave takes, workgroups of 8 waves or 4,
+// workgroups that share a set of rows.
+struct Plan {
+    int nr, waves, row_tiles, splits;
+};
+Plan plan(int64_t BH, int64_t rows, int64_t D, int64_t blocks) {
+    Plan p;
+    // Two pieces a wave spare reading and converting the codes again (16 sequences of
+    // 40 rows: 66 -> 64 us); four leave one wave a SIMD (87 us).
+    p.nr = rows <= 16 || D > 128 ? 1 : 2;
+    p.row_tiles = (int)((rows + 16 * p.nr - 1) / (16 * p.nr));
+    const int64_t groups = BH * p.row_tiles;
+    // Few rows and at most 16 blocks: one workgroup of 8 waves, for a second launch
+    // that joins splits costs more than it saves (1 x 300 tokens 9.0 us, split 11.3).
+    p.waves = groups < 256 && blocks <= 16 && p.nr == 1 && D <= 128 ? 8 : 4;
+    // Splits: two workgroups a CU, or 128 blocks each at the most, which evens out
+    // sequences of unequal length (64 sequences to 16383 tokens: 2048 workgroups
+    // 280 us, 1024 298; 1 x 131072: 512 workgroups 50 us, 1024 55).
+    int64_t s = (512 + groups - 1) / (groups > 0 ? groups : 1), by_length = (blocks + 127) / 128;
+    s = s > by_length ? s : by_length;
+    s = s < blocks / 4 ? s : blocks / 4;
+    s = s < kMaxSplits ? s : kMaxSplits;
+    p.splits = p.waves == 8 || s < 1 ? 1 : (int)s;
+    return p;
+}
+
+template <int DT, int NC>
+void launch_kernel(const KvAttnArgs& a, const Plan& p, int64_t B, hipStream_t st) {
+    const dim3 grid((unsigned)(B * a.H * a.row_tiles), (unsigned)a.splits);
+    if constexpr (NC <= 2) {
+        if (p.waves == 8) {
+            kv_attention_kernel<DT, NC, 1, 8><<<grid, 512, 0, st>>>(a);
+            return;
+        }
+        if (p.nr == 2) {
+            kv_attention_kernel<DT, NC, 2, 4><<<grid, 256, 0, st>>>(a);
+            return;
+        }
+    }
+    kv_attention_kernel<DT, NC, 1, 4><<<grid, 256, 0, st>>>(a);
 }
 
 template <int DT>
-void launch_attention(const KvAttnArgs& a, int64_t B, hipStream_t st) {
-    const dim3 grid((unsigned)(B * a.H * a.row_tiles), (unsigned)a.splits);
+void launch_attention(const KvAttnArgs& a, const Plan& p, int64_t B, hipStream_t st) {
     switch ((a.D + 63) / 64) {
-        case 1: kv_attention_kernel<DT, 1><<<grid, 64 * kWaves, 0, st>>>(a); break;
-        case 2: kv_attention_kernel<DT, 2><<<grid, 64 * kWaves, 0, st>>>(a); break;
-        case 3: kv_attention_kernel<DT, 3><<<grid, 64 * kWaves, 0, st>>>(a); break;
-        default: kv_attention_kernel<DT, 4><<<grid, 64 * kWaves, 0, st>>>(a); break;
+        case 1: launch_kernel<DT, 1>(a, p, B, st); break;
+        case 2: launch_kernel<DT, 2>(a, p, B, st); break;
+        case 3: launch_kernel<DT, 3>(a, p, B, st); break;
+        default: launch_kernel<DT, 4>(a, p, B, st); break;
     }
-    if (a.splits > 1) kv_join_kernel<DT><<<(unsigned)a.rows_all, 64, 0, st>>>(a);
-}
-
-// Workgroups that share one set of rows: enough to give the chip's 256 CUs
-// four each, as long as a wave keeps two blocks.
-int split_count(int64_t groups, int64_t blocks) {
-    int64_t s = (1024 + groups - 1) / (groups > 0 ? groups : 1);
-    const int64_t most = blocks / (2 * kWaves);
-    s = s < most ? s : most;
-    return s < 1 ? 1 : (int)s;
+    if (a.splits > 1) kv_join_kernel<DT><<<(unsigned)a.rows_all, kJoinThreads, 0, st>>>(a);
 }
 
 }  // namespace
@@ -316,7 +379,7 @@ using namespace axs6;
 
 extern "C" int64_t axs6_kv_attention_workspace(int64_t B, int64_t Tq, int64_t Hq, int64_t H, int64_t D, int64_t blocks) {
     if (B <= 0 || Tq <= 0 || H <= 0 || Hq <= 0 || Hq % H || D <= 0 || blocks <= 0) return 0;
-    const int64_t rows = Tq * (Hq / H), s = split_count(B * H * ((rows + 15) / 16), blocks);
+    const int64_t rows = Tq * (Hq / H), s = plan(B * H, rows, D, blocks).splits;
     return s == 1 ? 0 : s * B * H * rows * (D + 2) * (int64_t)sizeof(float);
 }
 
@@ -348,8 +411,8 @@ extern "C" int axs6_kv_attention(const void* q, int32_t dtype, int64_t B, int64_
         a.qvec = a.qvec && q_strides[i] % vl == 0;
     }
     a.H = (int)H; a.G = (int)(Hq / H); a.Tq = (int)Tq; a.D = (int)D; a.nb = (int)blocks; a.rows = (int)rows;
-    a.row_tiles = (int)((rows + 15) / 16); a.rows_all = B * H * rows; a.scale = scale;
-    a.splits = split_count(B * H * a.row_tiles, blocks);
+    const Plan p = plan(B * H, rows, D, blocks);
+    a.row_tiles = p.row_tiles; a.rows_all = B * H * rows; a.scale = scale; a.splits = p.splits;
     if (a.splits > 1) {
         const int64_t need = axs6_kv_attention_workspace(B, Tq, Hq, H, D, blocks);
         if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16)
@@ -359,8 +422,8 @@ extern "C" int axs6_kv_attention(const void* q, int32_t dtype, int64_t B, int64_
         a.stat = a.part + a.splits * a.rows_all * D;
     }
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == AXS6_F32) launch_attention<AXS6_F32>(a, B, st);
-    else if (dtype == AXS6_BF16) launch_attention<AXS6_BF16>(a, B, st);
-    else launch_attention<AXS6_F16>(a, B, st);
+    if (dtype == AXS6_F32) launch_attention<AXS6_F32>(a, p, B, st);
+    else if (dtype == AXS6_BF16) launch_attention<AXS6_BF16>(a, p, B, st);
+    else launch_attention<AXS6_F16>(a, p, B, st);
     return check_launch(fn);
 }

@@ -128,7 +128,7 @@ def test_zeros_extremes_and_bad_values():
 @pytest.mark.parametrize("B,Tq,Hq,H,D,lengths", [
     (1, 1, 1, 1, 16, [1]), (2, 1, 8, 2, 64, [31, 33]), (3, 1, 8, 1, 128, [0, 300, 64]), (2, 5, 4, 2, 80, [5, 129]),
     (1, 1, 32, 4, 96, [777]), (2, 3, 6, 2, 256, [2, 1000]), (1, 40, 3, 1, 192, [100]), (4, 2, 2, 1, 112, [1, 2, 3, 4]),
-    (1, 1, 4, 1, 128, [9000]),
+    (1, 1, 4, 1, 128, [9000]), (2, 5, 16, 4, 128, [700, 5]), (1, 3, 8, 2, 64, [5000]), (40, 1, 28, 7, 64, list(range(1, 241, 6))),
 ])
 def test_attention(B, Tq, Hq, H, D, lengths, dtype):
     from axs.unified import axs_cache_attention_unified
