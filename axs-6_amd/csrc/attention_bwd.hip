@@ -158,6 +158,7 @@ __global__ __launch_bounds__(kThr, (DqShape<DT, DC>::kOccupancy)) void attn_dq_k
     f32x16 dq[DC / 32];
 #pragma unroll
     for (int d = 0; d < DC / 32; ++d) dq[d] = zero16();
+    const bool rows_here = q0 + 32 * w < a.Tq;
     const int w_last = q0 + 32 * w + 31 < a.Tq ? q0 + 32 * w + 31 : a.Tq - 1;   // the wave's last row and its keys
     const int w_keys = a.causal && w_last + off + 1 < a.Tk ? w_last + off + 1 : a.Tk;
     for (int t = first; t < tiles; ++t) {
@@ -170,8 +171,8 @@ __global__ __launch_bounds__(kThr, (DqShape<DT, DC>::kOccupancy)) void attn_dq_k
         }
         const char *ks = kt[t & 1], *vs = vt[t & 1];
         const int k0 = t * KEYS;
-        bool any = true;
-        if constexpr (MASK == kKeyMask) any = __any(!(term[t & 1][lane & (KEYS - 1)] == -INFINITY));
+        bool any = rows_here;
+        if constexpr (MASK == kKeyMask) any = any && __any(!(term[t & 1][lane & (KEYS - 1)] == -INFINITY));
         if (any) {
 #pragma unroll
             for (int j = 0; j < NK; ++j) {

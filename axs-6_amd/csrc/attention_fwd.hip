@@ -137,6 +137,7 @@ attn_fwd_kernel(AttnArgs a) {
     float m = -INFINITY, l = 0.0f;   // the reference that scores are taken from; the sum of exponentials
     const float c = a.scale * kLog2e;
 
+    const bool rows_here = q0 + 32 * w < a.Tq;   // the others only help to load
     const int w_last = q0 + 32 * w + 31 < a.Tq ? q0 + 32 * w + 31 : a.Tq - 1;   // the wave's last row and its keys
     const int w_keys = a.causal && w_last + off + 1 < a.Tk ? w_last + off + 1 : a.Tk;
     for (int t = first; t < tiles; ++t) {
@@ -153,7 +154,7 @@ attn_fwd_kernel(AttnArgs a) {
         // none of the wave's rows sees; in the 16-bit types those branches cost more
         // than they save (1 x 16384 forward 985 -> 1019 us).
         const int live = DT == AXS6_F32 && t >= free_tiles ? (w_keys - k0 + 31) >> 5 : NK;
-        bool any = DT != AXS6_F32 || live > 0;
+        bool any = rows_here && (DT != AXS6_F32 || live > 0);
         if constexpr (MASK == kKeyMask) {
             float f = term[t & 1][lane];
             if constexpr (S::kKeys > 64) f = fmaxf(f, term[t & 1][lane + 64]);
