@@ -89,12 +89,13 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     }
 }
 
-// Rows of DC values (a multiple of 32) at a pitch of 64 or 128 values; the
+// Rows of DC values (a multiple of 16) at a pitch of 64 or 128 values; the
 // 16-byte chunk c of a row lies in slot c ^ key(row).  gfx950's LDS serves 256
 // bytes at once: the key spreads a fragment's 16 rows over all of them, and
 // the four rows (16-bit) or two rows (float32) of a column read as well.
 template <int DT, int DC>
 struct Tile {
+    static_assert(DC % 16 == 0 && DC <= 128, "a multiple of a product's depth");
     static constexpr int kBytes = kElemBytes<DT>;
     static constexpr int kPitch = (DC <= 64 ? 64 : 128) * kBytes;
     static constexpr int kChunks = DC * kBytes / 16;    // of a row
@@ -129,11 +130,11 @@ struct Tile {
         return a;
     }
 
-    // Results over a tile's columns: DC / 32 of them.  Row r of result d is
+    // Results over a tile's columns: DC / 32 of them, rounded up.  Row r of result d is
     // column 32 d + r of the tile in the 16-bit types.  In float32 a lane reads
     // the columns of several results at once: column 4 r + d of four, 2 r + d of
     // the first two, 64 + r of the third of three.
-    static constexpr int kResults = DC / 32;
+    static constexpr int kResults = (DC + 31) / 32;
 
     // o += (the 32 rows from row0)^T p, p a result whose rows are these rows; pf: p
     // in fragments (16-bit types).
@@ -339,13 +340,13 @@ __device__ __forceinline__ void mask_terms(const AttnArgs& a, const char* row, i
 }
 
 // The scores s of 32 keys from k0 (rows of the result) against the lane's
-// query, in units of log2, with the mask; `edge`: keys at or past limit are
-// not seen.  term: the keys' terms in LDS (by key).
+// query: with the mask, in units of log2, unless it is `plain` here; `edge`: keys
+// at or past limit are not seen.  term: the keys' terms in LDS (by key).
 template <int MASK>
 __device__ __forceinline__ void apply_mask(const AttnArgs& a, f32x16& s, float c, int k0, const float* term,
-                                           const char* row, bool edge, int limit, int lane) {
+                                           const char* row, bool plain, bool edge, int limit, int lane) {
     const int h4 = 4 * (lane >> 5);
-    if constexpr (MASK != kNoMask) {
+    if (MASK != kNoMask && !plain) {
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             float f[4];
@@ -356,7 +357,7 @@ __device__ __forceinline__ void apply_mask(const AttnArgs& a, f32x16& s, float c
                 mask_terms(a, row, k0 + 8 * g + h4, f);
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[4 * g + e] = f[e] == -INFINITY ? -INFINITY : __builtin_fmaf(s[4 * g + e], c, f[e]);
+            for (int e = 0; e < 4; ++e) s[4 * g + e] = __builtin_fmaf(s[4 * g + e], c, f[e]);
         }
     }
     if (edge)
@@ -367,8 +368,8 @@ __device__ __forceinline__ void apply_mask(const AttnArgs& a, f32x16& s, float c
 
 // ---- rows again -------------------------------------------------------------
 // A key that a query does not see has no part in its results, whatever key and
-// value hold there.  The products over a tile's rows give it a weight of 0, which
-// an infinity or NaN turns into NaN; so a result that is not finite is made
+// value hold there.  An infinity or NaN there turns the mask's -inf and the weight of 0 in the
+// products over a tile's rows into NaN; so a result that is not finite is made
 // again from the pairs that see each other alone, one pair at a time by one wave.
 // Where those give a NaN everywhere there is nothing more to find.
 

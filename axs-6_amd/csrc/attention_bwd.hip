@@ -155,9 +155,9 @@ __global__ __launch_bounds__(kThr, (DqShape<DT, DC>::kOccupancy)) void attn_dq_k
     }
     const float lse = a.lse[row], c = a.scale * kLog2e;
 
-    f32x16 dq[DC / 32];
+    f32x16 dq[T::kResults];
 #pragma unroll
-    for (int d = 0; d < DC / 32; ++d) dq[d] = zero16();
+    for (int d = 0; d < T::kResults; ++d) dq[d] = zero16();
     const bool rows_here = q0 + 32 * w < a.Tq;
     const int w_last = q0 + 32 * w + 31 < a.Tq ? q0 + 32 * w + 31 : a.Tq - 1;   // the wave's last row and its keys
     const int w_keys = a.causal && w_last + off + 1 < a.Tk ? w_last + off + 1 : a.Tk;
@@ -172,7 +172,13 @@ __global__ __launch_bounds__(kThr, (DqShape<DT, DC>::kOccupancy)) void attn_dq_k
         const char *ks = kt[t & 1], *vs = vt[t & 1];
         const int k0 = t * KEYS;
         bool any = rows_here;
-        if constexpr (MASK == kKeyMask) any = any && __any(!(term[t & 1][lane & (KEYS - 1)] == -INFINITY));
+        bool plain = MASK == kNoMask;
+        if constexpr (MASK == kKeyMask) {
+            const float f = term[t & 1][lane & (KEYS - 1)];
+            any = any && __any(!(f == -INFINITY));
+            plain = __all(f == 0.0f);
+        }
+        const float cs = plain ? c : 1.0f;
         if (any) {
 #pragma unroll
             for (int j = 0; j < NK; ++j) {
@@ -182,12 +188,11 @@ __global__ __launch_bounds__(kThr, (DqShape<DT, DC>::kOccupancy)) void attn_dq_k
                 for (int i = 0; i < T::kSteps; ++i) s = mma<DT>(T::rows(ks, 32 * j, i, lane), qf[i], s);
 #pragma unroll
                 for (int i = 0; i < T::kSteps; ++i) dp = mma<DT>(T::rows(vs, 32 * j, i, lane), gf[i], dp);
-                apply_mask<MASK>(a, s, c, k0 + 32 * j, &term[t & 1][MASK == kKeyMask ? 32 * j : 0], mrow,
+                apply_mask<MASK>(a, s, c, k0 + 32 * j, &term[t & 1][MASK == kKeyMask ? 32 * j : 0], mrow, plain,
                                  t >= free_tiles, limit, lane);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const float x = MASK == kNoMask ? __builtin_fmaf(s[i], c, -lse) : s[i] - lse;
-                    s[i] = __builtin_amdgcn_exp2f(x) * (dp[i] - delta);
+                    s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], cs, -lse)) * (dp[i] - delta);
                 }
                 u32x4 pf[2];
                 fragments<DT>(s, pf);
@@ -278,9 +283,9 @@ __global__ __launch_bounds__(kThr, (DkvShape<DT, DC>::kOccupancy)) void attn_dkv
     u32x4 kf[T::kSteps], vf[VL ? 1 : T::kSteps];
     load_rows<DT, DC>(kf, a.k, b * a.ks[0] + kr * a.ks[1] + h * a.ks[2], a.D, lane);
     if constexpr (!VL) load_rows<DT, DC>(vf, a.v, b * a.vs[0] + kr * a.vs[1] + h * a.vs[2], a.D, lane);
-    f32x16 dk[DC / 32], dv[DC / 32];
+    f32x16 dk[T::kResults], dv[T::kResults];
 #pragma unroll
-    for (int d = 0; d < DC / 32; ++d) { dk[d] = zero16(); dv[d] = zero16(); }
+    for (int d = 0; d < T::kResults; ++d) { dk[d] = zero16(); dv[d] = zero16(); }
     const float c = a.scale * kLog2e;
     float term = 0.0f;   // the mask's of the lane's key
     for (int t = first; t < tiles; ++t) {
@@ -315,14 +320,10 @@ __global__ __launch_bounds__(kThr, (DkvShape<DT, DC>::kOccupancy)) void attn_dkv
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int i = 4 * g + e, q = i_now + 8 * g + 4 * (lane >> 5) + e;
-                    float x;
-                    if constexpr (MASK == kNoMask) {
-                        x = __builtin_fmaf(s[i], c, -ls[e]);
-                    } else {
-                        const float f = MASK == kKeyMask ? term
-                                                         : mask_term(a, mask_row(a, b, hq_now, q < a.Tq ? q : a.Tq - 1), kr);
-                        x = f == -INFINITY ? f : __builtin_fmaf(s[i], c, f) - ls[e];
-                    }
+                    float f = term;   // by key: the lane's
+                    if constexpr (MASK == kFullMask)
+                        f = mask_term(a, mask_row(a, b, hq_now, q < a.Tq ? q : a.Tq - 1), kr);
+                    float x = __builtin_fmaf(s[i], c, MASK == kNoMask ? -ls[e] : f - ls[e]);
                     if (edge) x = kr <= q + off ? x : -INFINITY;
                     s[i] = __builtin_amdgcn_exp2f(x);
                     dp[i] = s[i] * (dp[i] - ds[e]);
@@ -398,6 +399,7 @@ void pick(const AttnArgs& a, hipStream_t st) {
 template <int DT>
 void dispatch(const AttnArgs& a, hipStream_t st) {
     if (a.D <= 64) pick<DT, 64>(a, st);
+    else if (a.D <= 80) pick<DT, 80>(a, st);
     else if (a.D <= 96) pick<DT, 96>(a, st);
     else pick<DT, 128>(a, st);
 }

@@ -131,9 +131,9 @@ attn_fwd_kernel(AttnArgs a) {
     const char* mrow = MASK == kFullMask ? mask_row(a, b, hq, qr) : nullptr;
     u32x4 qf[T::kSteps];
     load_rows<DT, DC>(qf, a.q, b * a.qs[0] + qr * a.qs[1] + hq * a.qs[2], a.D, lane);
-    f32x16 o[DC / 32];
+    f32x16 o[T::kResults];
 #pragma unroll
-    for (int d = 0; d < DC / 32; ++d) o[d] = zero16();
+    for (int d = 0; d < T::kResults; ++d) o[d] = zero16();
     float m = -INFINITY, l = 0.0f;   // the reference that scores are taken from; the sum of exponentials
     const float c = a.scale * kLog2e;
 
@@ -155,11 +155,13 @@ attn_fwd_kernel(AttnArgs a) {
         // than they save (1 x 16384 forward 985 -> 1019 us).
         const int live = DT == AXS6_F32 && t >= free_tiles ? (w_keys - k0 + 31) >> 5 : NK;
         bool any = rows_here && (DT != AXS6_F32 || live > 0);
+        bool plain = MASK == kNoMask;   // the mask adds nothing to any of the tile's scores
         if constexpr (MASK == kKeyMask) {
-            float f = term[t & 1][lane];
-            if constexpr (S::kKeys > 64) f = fmaxf(f, term[t & 1][lane + 64]);
-            any = any && __any(!(f == -INFINITY));
+            const float f = term[t & 1][lane], g = S::kKeys > 64 ? term[t & 1][lane + S::kKeys - 64] : f;
+            any = any && __any(!(f == -INFINITY && g == -INFINITY));
+            plain = __all(f == 0.0f && g == 0.0f);
         }
+        const float cs = plain ? c : 1.0f;   // what takes the scores to units of log2
         if (any) {
             f32x16 s[NK];
 #pragma unroll
@@ -172,20 +174,20 @@ attn_fwd_kernel(AttnArgs a) {
             float mx = -INFINITY;
 #pragma unroll
             for (int j = 0; j < NK; ++j)
-                apply_mask<MASK>(a, s[j], c, k0 + 32 * j, &term[t & 1][MASK == kKeyMask ? 32 * j : 0], mrow, t >= free_tiles,
-                                 limit, lane);
+                apply_mask<MASK>(a, s[j], c, k0 + 32 * j, &term[t & 1][MASK == kKeyMask ? 32 * j : 0], mrow, plain,
+                                 t >= free_tiles, limit, lane);
 #pragma unroll
             for (int j = 0; j < NK; ++j)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[j][i]);
-            if constexpr (MASK == kNoMask) mx *= c;
+            mx *= cs;
             mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
             if (__any(mx > m + kSlack)) {   // m is -inf until the row sees a key
                 const float mn = fmaxf(m, mx), alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn));
                 m = mn;
                 l *= alpha;
 #pragma unroll
-                for (int d = 0; d < DC / 32; ++d) o[d] *= alpha;
+                for (int d = 0; d < T::kResults; ++d) o[d] *= alpha;
             }
             const float ref = m == -INFINITY ? 0.0f : m;
             u32x4 pf[NK][2];
@@ -193,7 +195,7 @@ attn_fwd_kernel(AttnArgs a) {
             for (int j = 0; j < NK; ++j) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    s[j][i] = __builtin_amdgcn_exp2f(MASK == kNoMask ? __builtin_fmaf(s[j][i], c, -ref) : s[j][i] - ref);
+                    s[j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][i], cs, -ref));
                 fragments<DT>(s[j], pf[j]);
                 if constexpr (DT == AXS6_F32) {
 #pragma unroll
@@ -209,7 +211,7 @@ attn_fwd_kernel(AttnArgs a) {
                     if (j < live) T::accumulate(vs, 32 * j, s[j], pf[j], o, lane);
             } else {
 #pragma unroll
-                for (int d = 0; d < DC / 32; ++d)
+                for (int d = 0; d < T::kResults; ++d)
 #pragma unroll
                     for (int j = 0; j < 2 * NK; ++j)
                         o[d] = mma<DT>(T::col_fragment(vs, 16 * j, d, lane), pf[j / 2][j % 2], o[d]);
@@ -276,6 +278,7 @@ void pick(const AttnArgs& a, hipStream_t st) {
 template <int DT>
 void dispatch(const AttnArgs& a, hipStream_t st) {
     if (a.D <= 64) pick<DT, 64>(a, st);
+    else if (a.D <= 80) pick<DT, 80>(a, st);
     else if (a.D <= 96) pick<DT, 96>(a, st);
     else pick<DT, 128>(a, st);
 }
