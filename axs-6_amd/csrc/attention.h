@@ -366,6 +366,26 @@ __device__ __forceinline__ void apply_mask(const AttnArgs& a, f32x16& s, float c
             s[i] = k0 + 8 * (i >> 2) + h4 + (i & 3) < limit ? s[i] : -INFINITY;
 }
 
+// Adds the second group's results to the first's: the four waves of each group
+// hold the same rows.  ex: 4 * N * 16 * 64 floats of LDS that nobody uses; every
+// wave of the workgroup calls it.
+template <int N>
+__device__ __forceinline__ void add_groups(f32x16 (&c)[N], float* ex, int group, int w, int lane) {
+    __syncthreads();
+    ex += w * (N * 16) * 64 + lane;
+    if (group == 1)
+#pragma unroll
+        for (int d = 0; d < N; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) ex[(16 * d + i) * 64] = c[d][i];
+    __syncthreads();
+    if (group == 0)
+#pragma unroll
+        for (int d = 0; d < N; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) c[d][i] += ex[(16 * d + i) * 64];
+}
+
 // ---- rows again -------------------------------------------------------------
 // A key that a query does not see has no part in its results, whatever key and
 // value hold there.  An infinity or NaN there turns the mask's -inf and the weight of 0 in the

@@ -70,25 +70,37 @@ __device__ void forward_row(const AttnArgs& a, int b, int hq, int q, int k0, int
         a.lse[((int64_t)b * a.Hq + hq) * a.Tq + q] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
+// The forms of the kernel: four waves; eight that hold twice the queries; two
+// groups of four that hold the same queries and take every second tile of keys,
+// for 16-bit problems of at most a workgroup a CU, which would leave half the
+// waves out (2 x 1024, 16 heads of 128, causal: 28 -> 24 us; in float32, where
+// the matrix cores take their time with either, 64 x 128 gets 15 -> 18).
+enum Form { kFour, kEight, kPaired };
+
 // Queries and keys of a workgroup's tile.
-template <int DT, int DC, bool LARGE> struct FwdShape {
-    static constexpr int kWaves = LARGE ? 8 : 4;
-    static constexpr int kKeys = DT == AXS6_F32 ? 64 : LARGE || DC <= 64 ? 128 : 64;
-    static constexpr int kQ = 32 * kWaves, kThreads = 64 * kWaves;
+template <int DT, int DC, int FORM> struct FwdShape {
+    static constexpr int kWaves = FORM == kEight ? 8 : 4;   // of a group
+    static constexpr int kGroups = FORM == kPaired ? 2 : 1;
+    static constexpr int kKeys = DT == AXS6_F32 ? 64 : FORM == kEight || DC <= 64 ? 128 : 64;
+    static constexpr int kQ = 32 * kWaves, kThreads = 64 * kWaves * kGroups;
     // two waves a SIMD, of which one computes softmax while the other multiplies
     static constexpr int kOccupancy = DT == AXS6_F32 ? 1 : 2;
 };
 
-template <int DT, int DC, int MASK, bool LARGE>
-__global__ __launch_bounds__((FwdShape<DT, DC, LARGE>::kThreads), (FwdShape<DT, DC, LARGE>::kOccupancy)) void
+template <int DT, int DC, int MASK, int FORM>
+__global__ __launch_bounds__((FwdShape<DT, DC, FORM>::kThreads), (FwdShape<DT, DC, FORM>::kOccupancy)) void
 attn_fwd_kernel(AttnArgs a) {
     using T = Tile<DT, DC>;
-    using S = FwdShape<DT, DC, LARGE>;
-    constexpr int NK = S::kKeys / 32, W = S::kWaves;
-    __shared__ __attribute__((aligned(1024))) char kt[2][S::kKeys * T::kPitch];
-    __shared__ __attribute__((aligned(1024))) char vt[2][S::kKeys * T::kPitch];
-    __shared__ __attribute__((aligned(16))) float term[2][MASK == kKeyMask ? S::kKeys : 1];
-    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    using S = FwdShape<DT, DC, FORM>;
+    constexpr int NK = S::kKeys / 32, W = S::kWaves, GROUPS = S::kGroups;
+    // keys, then values; of each group two buffers
+    __shared__ __attribute__((aligned(1024))) char kv[2][GROUPS][2][S::kKeys * T::kPitch];
+    __shared__ __attribute__((aligned(16))) float terms[GROUPS][2][MASK == kKeyMask ? S::kKeys : 1];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int w = wave % W, group = wave / W, tid = threadIdx.x % (64 * W);
+    auto& kt = kv[0][group];
+    auto& vt = kv[1][group];
+    auto& term = terms[group];
     const int q_tiles = (a.Tq + S::kQ - 1) / S::kQ;
     int bh, piece;
     work_item(blockIdx.x, a.B * a.Hq, q_tiles * a.splits, false, bh, piece);
@@ -113,17 +125,18 @@ attn_fwd_kernel(AttnArgs a) {
     Direct<DT, DC, S::kKeys, W> dk, dv;
     dk.init(a.ks[1], a.D, lane, w);
     dv.init(a.vs[1], a.D, lane, w);
-    // the mask's term of key threadIdx.x of tile t
+    // the mask's term of key tid of tile t
     auto key_term = [&](int t) {
-        const int key = t * S::kKeys + threadIdx.x;
-        return threadIdx.x < S::kKeys && key < a.Tk ? mask_term(a, mask_row(a, b, hq, 0), key) : -INFINITY;
+        const int key = t * S::kKeys + tid;
+        return tid < S::kKeys && key < a.Tk ? mask_term(a, mask_row(a, b, hq, 0), key) : -INFINITY;
     };
-    if (first < tiles) {
-        dk.load(kt[first & 1], kb, first * S::kKeys, a.Tk, a.D, w);
-        dv.load(vt[first & 1], vb, first * S::kKeys, a.Tk, a.D, w);
+    if (first + group < tiles) {
+        const int t = first + group;
+        dk.load(kt[0], kb, t * S::kKeys, a.Tk, a.D, w);
+        dv.load(vt[0], vb, t * S::kKeys, a.Tk, a.D, w);
         if constexpr (MASK == kKeyMask) {
-            const float f = key_term(first);
-            if (threadIdx.x < S::kKeys) term[first & 1][threadIdx.x] = f;
+            const float f = key_term(t);
+            if (tid < S::kKeys) term[0][tid] = f;
         }
     }
     const int q = q0 + 32 * w + (lane & 31), qr = q < a.Tq ? q : a.Tq - 1;
@@ -140,24 +153,25 @@ attn_fwd_kernel(AttnArgs a) {
     const bool rows_here = q0 + 32 * w < a.Tq;   // the others only help to load
     const int w_last = q0 + 32 * w + 31 < a.Tq ? q0 + 32 * w + 31 : a.Tq - 1;   // the wave's last row and its keys
     const int w_keys = a.causal && w_last + off + 1 < a.Tk ? w_last + off + 1 : a.Tk;
-    for (int t = first; t < tiles; ++t) {
+    int buf = 0;
+    for (int t = first + group; t - group < tiles; t += GROUPS, buf ^= 1) {
         tile_barrier();   // tile t is there, and nobody reads the other buffers any more
         float next_term = 0.0f;
-        if (t + 1 < tiles) {
-            dk.load(kt[(t + 1) & 1], kb, (t + 1) * S::kKeys, a.Tk, a.D, w);
-            dv.load(vt[(t + 1) & 1], vb, (t + 1) * S::kKeys, a.Tk, a.D, w);
-            if constexpr (MASK == kKeyMask) next_term = key_term(t + 1);
+        if (t + GROUPS < tiles) {
+            dk.load(kt[buf ^ 1], kb, (t + GROUPS) * S::kKeys, a.Tk, a.D, w);
+            dv.load(vt[buf ^ 1], vb, (t + GROUPS) * S::kKeys, a.Tk, a.D, w);
+            if constexpr (MASK == kKeyMask) next_term = key_term(t + GROUPS);
         }
-        const char *ks = kt[t & 1], *vs = vt[t & 1];
+        const char *ks = kt[buf], *vs = vt[buf];
         const int k0 = t * S::kKeys;
         // A tile that the mask hides is passed over, and in float32 the 32 keys that
         // none of the wave's rows sees; in the 16-bit types those branches cost more
         // than they save (1 x 16384 forward 985 -> 1019 us).
         const int live = DT == AXS6_F32 && t >= free_tiles ? (w_keys - k0 + 31) >> 5 : NK;
-        bool any = rows_here && (DT != AXS6_F32 || live > 0);
+        bool any = rows_here && (GROUPS == 1 || t < tiles) && (DT != AXS6_F32 || live > 0);
         bool plain = MASK == kNoMask;   // the mask adds nothing to any of the tile's scores
         if constexpr (MASK == kKeyMask) {
-            const float f = term[t & 1][lane], g = S::kKeys > 64 ? term[t & 1][lane + S::kKeys - 64] : f;
+            const float f = term[buf][lane & (S::kKeys - 1)], g = S::kKeys > 64 ? term[buf][lane + S::kKeys - 64] : f;
             any = any && __any(!(f == -INFINITY && g == -INFINITY));
             plain = __all(f == 0.0f && g == 0.0f);
         }
@@ -174,7 +188,7 @@ attn_fwd_kernel(AttnArgs a) {
             float mx = -INFINITY;
 #pragma unroll
             for (int j = 0; j < NK; ++j)
-                apply_mask<MASK>(a, s[j], c, k0 + 32 * j, &term[t & 1][MASK == kKeyMask ? 32 * j : 0], mrow, plain,
+                apply_mask<MASK>(a, s[j], c, k0 + 32 * j, &term[buf][MASK == kKeyMask ? 32 * j : 0], mrow, plain,
                                  t >= free_tiles, limit, lane);
 #pragma unroll
             for (int j = 0; j < NK; ++j)
@@ -218,9 +232,22 @@ attn_fwd_kernel(AttnArgs a) {
             }
         }
         if constexpr (MASK == kKeyMask)
-            if (threadIdx.x < S::kKeys) term[(t + 1) & 1][threadIdx.x] = next_term;
+            if (tid < S::kKeys) term[buf ^ 1][tid] = next_term;
     }
     l += __shfl_xor(l, 32, 64);
+    if constexpr (GROUPS == 2) {   // one reference for both groups, then their sums
+        __shared__ float other[2][2][W][32];
+        if (lane < 32) { other[0][group][w][lane] = m; other[1][group][w][lane] = l; }
+        __syncthreads();
+        const float mo = other[0][group ^ 1][w][lane & 31], lo = other[1][group ^ 1][w][lane & 31];
+        const float mn = fmaxf(m, mo), ref = mn == -INFINITY ? 0.0f : mn, f = __builtin_amdgcn_exp2f(m - ref);
+        l = l * f + lo * __builtin_amdgcn_exp2f(mo - ref);
+        m = mn;
+#pragma unroll
+        for (int d = 0; d < T::kResults; ++d) o[d] *= f;
+        add_groups(o, reinterpret_cast<float*>(kv), group, w, lane);
+        if (group == 1) return;
+    }
     const bool bad = not_finite(o);
     if (q < a.Tq) {
         if (a.splits > 1) {
@@ -254,25 +281,29 @@ __global__ __launch_bounds__(kJoinThreads) void attn_join_kernel(AttnArgs a) {
     for (int i = 0; i < 4; ++i) out[i] = E::from_f(j.o[i] * rl);
 }
 
-template <int DT, int DC, int MASK, bool LARGE>
+template <int DT, int DC, int MASK, int FORM>
 void launch(const AttnArgs& a, hipStream_t st) {
-    using S = FwdShape<DT, DC, LARGE>;
+    using S = FwdShape<DT, DC, FORM>;
     const unsigned grid = (unsigned)((a.Tq + S::kQ - 1) / S::kQ * a.B * a.Hq * a.splits);
-    attn_fwd_kernel<DT, DC, MASK, LARGE><<<grid, S::kThreads, 0, st>>>(a);
+    attn_fwd_kernel<DT, DC, MASK, FORM><<<grid, S::kThreads, 0, st>>>(a);
     if (a.splits > 1) attn_join_kernel<DT><<<(unsigned)(a.B * a.Hq * a.Tq), kJoinThreads, 0, st>>>(a);
 }
 
 template <int DT, int DC>
 void pick(const AttnArgs& a, hipStream_t st) {
-    if (a.mask && a.ms[2] == 0) return launch<DT, DC, kKeyMask, false>(a, st);
-    if (a.mask) return launch<DT, DC, kFullMask, false>(a, st);
+    if constexpr (DT != AXS6_F32) {
+        if ((int64_t)((a.Tq + 127) / 128) * a.B * a.Hq * a.splits <= 256 && (!a.mask || a.ms[2] == 0) &&
+            a.Tk / a.splits > FwdShape<DT, DC, kPaired>::kKeys)
+            return a.mask ? launch<DT, DC, kKeyMask, kPaired>(a, st) : launch<DT, DC, kNoMask, kPaired>(a, st);
+    }
+    if (a.mask) return a.ms[2] == 0 ? launch<DT, DC, kKeyMask, kFour>(a, st) : launch<DT, DC, kFullMask, kFour>(a, st);
     if constexpr (DT != AXS6_F32 && DC > 64) {
         // 256 queries a workgroup and 128 keys a tile from two workgroups a CU on:
         // fewer barriers (1 x 16384, 16 heads of 128, causal 990 us against 1063,
         // 2 x 4096 x 32 heads 333 against 327, without the mask 526 against 562)
-        if ((int64_t)((a.Tq + 255) / 256) * a.B * a.Hq >= 512) return launch<DT, DC, kNoMask, true>(a, st);
+        if ((int64_t)((a.Tq + 255) / 256) * a.B * a.Hq >= 512) return launch<DT, DC, kNoMask, kEight>(a, st);
     }
-    launch<DT, DC, kNoMask, false>(a, st);
+    launch<DT, DC, kNoMask, kFour>(a, st);
 }
 
 template <int DT>

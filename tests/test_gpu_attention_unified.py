@@ -76,13 +76,13 @@ def test_split_axes(shape, causal, dtype):
 
 
 @pytest.mark.parametrize("dtype", ref.DTYPES)
-def test_many_workgroups(dtype):
-    """The form of large problems: 256 queries a workgroup."""
-    from axs.unified import axs_attention_unified
-
-    q, k, v, _ = _inputs(8, 300, 280, 32, 4, 72, dtype)
+@pytest.mark.parametrize("D", [64, 72, 96, 128])
+def test_many_workgroups(D, dtype):
+    """The forms of larger problems: one group of waves a workgroup, and in the forward 256 queries a workgroup."""
     for causal in (False, True):
-        assert ref.rel(axs_attention_unified(q, k, v, causal=causal), ref.attention(q, k, v, causal=causal)) <= _bounds(dtype)[0]
+        _check(*_inputs(5, 190, 200, 32, 32, D, dtype), causal=causal)
+    mask = torch.arange(200) < torch.tensor([[200], [50], [128], [1], [0]])
+    _check(*_inputs(5, 190, 200, 32, 32, D, dtype), mask[:, None, None].to(DEV))
 
 
 @pytest.mark.parametrize("dtype", ref.DTYPES)
