@@ -352,10 +352,13 @@ __global__ __launch_bounds__(kThr, (DkvShape<DT, DC>::kOccupancy)) void attn_dkv
         dkv_row<DT>(a, b, h, k0 + 32 * w + __builtin_ctzll(rows), first, tiles, q_first, per_head, split, lane);
 }
 
-// Sums of the splits in order, four values a thread.
+// Sums of the splits in order, four values a thread; of two results, one after
+// the other in part, in one launch.
 template <int DT>
-__global__ __launch_bounds__(256) void attn_sum_kernel(const float* part, int splits, int64_t n, void* out) {
+__global__ __launch_bounds__(256) void attn_sum_kernel(const float* part, int splits, int64_t n, void* out0, void* out1) {
     using E = Elem<DT>;
+    void* out = blockIdx.y ? out1 : out0;
+    part += blockIdx.y * splits * n;
     const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
     if (i >= n) return;
     float4 x = *reinterpret_cast<const float4*>(part + i);
@@ -369,23 +372,20 @@ __global__ __launch_bounds__(256) void attn_sum_kernel(const float* part, int sp
 }
 
 template <int DT>
-void sum_splits(const float* part, int splits, int64_t n, void* out, hipStream_t st) {
-    attn_sum_kernel<DT><<<(unsigned)((n / 4 + 255) / 256), 256, 0, st>>>(part, splits, n, out);
+void sum_splits(const float* part, int splits, int64_t n, void* out0, void* out1, hipStream_t st) {
+    attn_sum_kernel<DT><<<dim3((unsigned)((n / 4 + 255) / 256), out1 ? 2 : 1), 256, 0, st>>>(part, splits, n, out0, out1);
 }
 
 template <int DT, int DC, int MASK>
 void launch(const AttnArgs& a, hipStream_t st) {
     if (a.Tq) {
         attn_dq_kernel<DT, DC, MASK><<<(unsigned)((a.Tq + kHeld - 1) / kHeld * a.B * a.Hq * a.splits), kThr, 0, st>>>(a);
-        if (a.splits > 1) sum_splits<DT>(a.part, a.splits, (int64_t)a.B * a.Tq * a.Hq * a.D, a.dq, st);
+        if (a.splits > 1) sum_splits<DT>(a.part, a.splits, (int64_t)a.B * a.Tq * a.Hq * a.D, a.dq, nullptr, st);
     }
     if (a.Tk) {
         attn_dkv_kernel<DT, DC, MASK><<<(unsigned)((a.Tk + kHeld - 1) / kHeld * a.B * a.H * a.splits_kv), kThr, 0, st>>>(a);
-        if (a.splits_kv > 1) {
-            const int64_t n = (int64_t)a.B * a.Tk * a.H * a.D;
-            sum_splits<DT>(a.part_kv, a.splits_kv, n, a.dk, st);
-            sum_splits<DT>(a.part_kv + a.splits_kv * n, a.splits_kv, n, a.dv, st);
-        }
+        if (a.splits_kv > 1)
+            sum_splits<DT>(a.part_kv, a.splits_kv, (int64_t)a.B * a.Tk * a.H * a.D, a.dk, a.dv, st);
     }
 }
 

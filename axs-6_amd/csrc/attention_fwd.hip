@@ -267,13 +267,20 @@ attn_fwd_kernel(AttnArgs a) {
                         tiles * S::kKeys < a.Tk ? tiles * S::kKeys : a.Tk, split, lane);
 }
 
-template <int DT>
+// FEW: at most kFewSplits, a thread four values; else a workgroup a row.
+template <int DT, bool FEW>
 __global__ __launch_bounds__(kJoinThreads) void attn_join_kernel(AttnArgs a) {
     using E = Elem<DT>;
-    const int64_t row = blockIdx.x, bh = row / a.Tq;
-    const int q = (int)(row - bh * a.Tq);
-    const Joined j = join_row(a.part, a.stat, (int64_t)a.B * a.Hq * a.Tq, row, a.splits, a.D);
+    const int64_t rows = (int64_t)a.B * a.Hq * a.Tq;
+    int64_t row = blockIdx.x;
+    Joined j;
+    if constexpr (FEW)
+        j = join_few(a.part, a.stat, rows, (int64_t)blockIdx.x * kJoinThreads + threadIdx.x, a.splits, a.D, row);
+    else
+        j = join_row(a.part, a.stat, rows, row, a.splits, a.D);
     if (j.d < 0) return;
+    const int64_t bh = row / a.Tq;
+    const int q = (int)(row - bh * a.Tq);
     if (a.lse && j.d == 0) a.lse[row] = j.l == 0.0f ? INFINITY : j.m + __builtin_amdgcn_logf(j.l);
     const float rl = j.l == 0.0f ? 0.0f : 1.0f / j.l;
     auto* out = reinterpret_cast<typename E::S*>(a.o) + (((bh / a.Hq) * a.Tq + q) * a.Hq + bh % a.Hq) * a.D + j.d;
@@ -281,12 +288,22 @@ __global__ __launch_bounds__(kJoinThreads) void attn_join_kernel(AttnArgs a) {
     for (int i = 0; i < 4; ++i) out[i] = E::from_f(j.o[i] * rl);
 }
 
+template <int DT>
+void join(const AttnArgs& a, hipStream_t st) {
+    const int64_t rows = (int64_t)a.B * a.Hq * a.Tq;
+    if (a.splits == 1) return;
+    if (!join_by_value(rows, a.splits))
+        attn_join_kernel<DT, false><<<(unsigned)rows, kJoinThreads, 0, st>>>(a);
+    else
+        attn_join_kernel<DT, true><<<(unsigned)((rows * (a.D / 4) + kJoinThreads - 1) / kJoinThreads), kJoinThreads, 0, st>>>(a);
+}
+
 template <int DT, int DC, int MASK, int FORM>
 void launch(const AttnArgs& a, hipStream_t st) {
     using S = FwdShape<DT, DC, FORM>;
     const unsigned grid = (unsigned)((a.Tq + S::kQ - 1) / S::kQ * a.B * a.Hq * a.splits);
     attn_fwd_kernel<DT, DC, MASK, FORM><<<grid, S::kThreads, 0, st>>>(a);
-    if (a.splits > 1) attn_join_kernel<DT><<<(unsigned)(a.B * a.Hq * a.Tq), kJoinThreads, 0, st>>>(a);
+    join<DT>(a, st);
 }
 
 template <int DT, int DC>

@@ -306,13 +306,19 @@ __global__ __launch_bounds__(64 * WAVES) void kv_attention_kernel(KvAttnArgs a) 
     }
 }
 
-template <int DT>
+// FEW: at most kFewSplits, a thread four values; else a workgroup a row.
+template <int DT, bool FEW>
 __global__ __launch_bounds__(kJoinThreads) void kv_join_kernel(KvAttnArgs a) {
     using E = Elem<DT>;
-    const int64_t row = blockIdx.x, bh = row / a.rows;
-    const int r = (int)(row - bh * a.rows), t = r / a.G, hq = (int)(bh % a.H) * a.G + r % a.G;
-    const Joined j = join_row(a.part, a.stat, a.rows_all, row, a.splits, a.D);
+    int64_t row = blockIdx.x;
+    Joined j;
+    if constexpr (FEW)
+        j = join_few(a.part, a.stat, a.rows_all, (int64_t)blockIdx.x * kJoinThreads + threadIdx.x, a.splits, a.D, row);
+    else
+        j = join_row(a.part, a.stat, a.rows_all, row, a.splits, a.D);
     if (j.d < 0) return;
+    const int64_t bh = row / a.rows;
+    const int r = (int)(row - bh * a.rows), t = r / a.G, hq = (int)(bh % a.H) * a.G + r % a.G;
     const float rl = j.l == 0.0f ? 0.0f : kSumScale / j.l;
     auto* out = reinterpret_cast<typename E::S*>(a.out) + (((bh / a.H) * a.Tq + t) * a.H * a.G + hq) * a.D + j.d;
 #pragma unroll
@@ -369,7 +375,11 @@ void launch_attention(const KvAttnArgs& a, const Plan& p, int64_t B, hipStream_t
         case 3: launch_kernel<DT, 3>(a, p, B, st); break;
         default: launch_kernel<DT, 4>(a, p, B, st); break;
     }
-    if (a.splits > 1) kv_join_kernel<DT><<<(unsigned)a.rows_all, kJoinThreads, 0, st>>>(a);
+    if (a.splits == 1) return;
+    if (!join_by_value(a.rows_all, a.splits))
+        kv_join_kernel<DT, false><<<(unsigned)a.rows_all, kJoinThreads, 0, st>>>(a);
+    else
+        kv_join_kernel<DT, true><<<(unsigned)((a.rows_all * (a.D / 4) + kJoinThreads - 1) / kJoinThreads), kJoinThreads, 0, st>>>(a);
 }
 
 }  // namespace
