@@ -98,7 +98,7 @@ __global__ __launch_bounds__(kThr, (DqShape<DT, DC>::kOccupancy)) void attn_dq_k
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int q_tiles = (a.Tq + kHeld - 1) / kHeld;
     int bh, piece;
-    work_item(blockIdx.x, a.B * a.Hq, q_tiles * a.splits, false, bh, piece);
+    work_item(blockIdx.x, a.B * a.Hq, q_tiles * a.splits, a.causal, bh, piece);
     const int b = bh / a.Hq, hq = bh % a.Hq, h = hq / a.G, split = piece % a.splits;
     const int q0 = (q_tiles - 1 - piece / a.splits) * kHeld;
     const int off = a.Tk - a.Tq;

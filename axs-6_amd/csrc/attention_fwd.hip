@@ -103,7 +103,7 @@ attn_fwd_kernel(AttnArgs a) {
     auto& term = terms[group];
     const int q_tiles = (a.Tq + S::kQ - 1) / S::kQ;
     int bh, piece;
-    work_item(blockIdx.x, a.B * a.Hq, q_tiles * a.splits, false, bh, piece);
+    work_item(blockIdx.x, a.B * a.Hq, q_tiles * a.splits, a.causal, bh, piece);
     const int b = bh / a.Hq, hq = bh % a.Hq, h = hq / a.G, split = piece % a.splits;
     const int q0 = (q_tiles - 1 - piece / a.splits) * S::kQ;   // a causal mask's longest rows first
     const int off = a.Tk - a.Tq;
