@@ -263,9 +263,9 @@ __global__ __launch_bounds__(kThr, (DkvShape<DT, DC>::kOccupancy)) void attn_dkv
     // head and first query of the tile on its way
     int hq = h * a.G + (per_head ? first / per_head : 0), i0 = q_first + (per_head ? first % per_head : 0) * kWalk;
     float sl = 0.0f, sd = 0.0f;
-    auto load = [&](int buf) {
-        lq.load(qt[buf], reinterpret_cast<const char*>(a.q) + (b * a.qs[0] + hq * a.qs[2]) * T::kBytes, i0, a.Tq, a.D, w);
-        lg.load(gt[buf], reinterpret_cast<const char*>(a.dout) + (b * a.gs[0] + hq * a.gs[2]) * T::kBytes, i0, a.Tq, a.D, w);
+    auto load = [&](char* qn, char* gn) {
+        lq.load(qn, reinterpret_cast<const char*>(a.q) + (b * a.qs[0] + hq * a.qs[2]) * T::kBytes, i0, a.Tq, a.D, w);
+        lg.load(gn, reinterpret_cast<const char*>(a.dout) + (b * a.gs[0] + hq * a.gs[2]) * T::kBytes, i0, a.Tq, a.D, w);
         if (threadIdx.x < kWalk) {
             const int i = i0 + threadIdx.x;
             const int64_t row = ((int64_t)b * a.Hq + hq) * a.Tq + i;
@@ -277,7 +277,7 @@ __global__ __launch_bounds__(kThr, (DkvShape<DT, DC>::kOccupancy)) void attn_dkv
         if (threadIdx.x < kWalk) { lt[buf][threadIdx.x] = sl; dt[buf][threadIdx.x] = sd; }
     };
     if (first < tiles) {
-        load(first & 1);
+        load(qt[first & 1], gt[first & 1]);
         store(first & 1);
     }
     u32x4 kf[T::kSteps], vf[VL ? 1 : T::kSteps];
@@ -288,15 +288,16 @@ __global__ __launch_bounds__(kThr, (DkvShape<DT, DC>::kOccupancy)) void attn_dkv
     for (int d = 0; d < T::kResults; ++d) { dk[d] = zero16(); dv[d] = zero16(); }
     const float c = a.scale * kLog2e;
     float term = 0.0f;   // the mask's of the lane's key
-    for (int t = first; t < tiles; ++t) {
-        tile_barrier();
+    // The tile's buffers and the next one's are told apart by the parameters: the
+    // compiler would else wait for the next tile before it reads this one.
+    auto step = [&](int t, const char* __restrict__ qs, const char* __restrict__ gs, char* __restrict__ qn,
+                    char* __restrict__ gn) __attribute__((always_inline)) {
         const int hq_now = hq, i_now = i0;
         if constexpr (MASK == kKeyMask)
             if (t == first || i_now == q_first) term = mask_term(a, mask_row(a, b, hq_now, 0), kr);
         i0 += kWalk;
         if (i0 >= a.Tq) { i0 = q_first; ++hq; }
-        if (t + 1 < tiles) load((t + 1) & 1);
-        const char *qs = qt[t & 1], *gs = gt[t & 1];
+        if (t + 1 < tiles) load(qn, gn);
         // none of the tile's queries sees the wave's keys: they are before them, or the mask hides them
         bool any = !a.causal || i_now + kWalk - 1 + off >= k0 + 32 * w;
         if constexpr (MASK == kKeyMask) any = any && __any(!(term == -INFINITY));
@@ -336,6 +337,10 @@ __global__ __launch_bounds__(kThr, (DkvShape<DT, DC>::kOccupancy)) void attn_dkv
             T::accumulate(qs, 0, dp, df, dk, lane);
         }
         if (t + 1 < tiles) store((t + 1) & 1);
+    };
+    for (int t = first; t < tiles; ++t) {
+        tile_barrier();
+        step(t, qt[t & 1], gt[t & 1], qt[(t + 1) & 1], gt[(t + 1) & 1]);
     }
     const bool bad = not_finite(dk) || not_finite(dv);
     if (key < a.Tk) {
