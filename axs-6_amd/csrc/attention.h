@@ -9,7 +9,7 @@
 // a result (probabilities, their gradients) is the next product's operand
 // without leaving its registers.
 //   16-bit types: 32x32x16, columns by transposing LDS reads of 4 rows;
-//   float32: 32x32x2, columns by plain 4-byte reads.
+//   float32: 32x32x2, columns by 4-byte reads, those of all the row's results at once.
 #pragma once
 
 #include <math.h>

@@ -16,13 +16,13 @@
 // barrier a tile.  Two waves a SIMD (at most 256 registers each) let one
 // multiply while the other exponentiates: 1 x 16384, 16 heads of 128, causal,
 // bf16: 1816 us with one, 1063 with two (2179 through registers with two
-// barriers), 998 with 128 keys a tile and 256 queries a workgroup, 1102
-// TFLOP/s, where a bf16 matrix product of 8192^3 reaches 1139 on this card.
+// barriers), 985 to 1018 with 128 keys a tile and 256 queries a workgroup,
+// 1080 to 1116 TFLOP/s, where a bf16 matrix product of 8192^3 reaches 1139 on this card.
 // The row's reference is only raised when a score passes it by 2^8, so the
 // output is hardly ever rescaled; the sum is taken of the probabilities as they
 // are rounded for the product.
 // Few rows against many keys: the keys are split over workgroups, whose sums a
-// second launch joins (4 x 4 queries of 16 heads, 8000 keys: 165 -> 41 us).
+// second launch joins (4 x 4 queries of 16 heads, 8000 keys: 165 -> 31 us).
 #include "attention.h"
 #include "split_join.h"
 

@@ -13,6 +13,11 @@
 // exponentials in one pass), the backward reads them and writes the gradient
 // once; the K entries of a row are gathered from cache.  All sums are float32
 // in a fixed order; the gradient is rounded once.
+// The gradient could only be written by the forward if its factor from above
+// were known there, or by a second rounding: so three passes, 6 bytes a logit.
+// Measured: 8192 x 128000 bf16, both directions, 1205 us, 5.2 TB/s over the three
+// passes (two read 2.1 GB, one writes it); 509 x 1000 float32 63 us, of which the
+// caller's backward call is nearly all.
 #include <math.h>
 
 #include "axs6_internal.h"
@@ -169,7 +174,8 @@ template <int DT, bool VEC>
 __global__ __launch_bounds__(kDistillThreads) void distill_backward_kernel(DistillArgs a) {
     using E = Elem<DT>;
     __shared__ float red[kDistillThreads / 64];
-    const int64_t r = blockIdx.x;
+    // the last rows first: the forward's last ones may still be in the 256 MB cache
+    const int64_t r = gridDim.x - 1 - blockIdx.x;
     constexpr int W = VEC ? E::V : 1;
     auto* dz = reinterpret_cast<typename E::S*>(a.dz) + r * a.V;
     const float w = a.weights ? a.weights[r] : 1.0f;

@@ -13,6 +13,10 @@
 // Bound by HBM: each value is read once and written once.  A thread keeps the
 // cosines and sines of its place in the head in registers and walks over
 // heads of one token, so the table is read once a token and not once a head.
+// Measured, bf16, 40 heads of 128: 2 x 4096 tokens 28 us, 6.0 TB/s (two
+// thirds from the last cache), interleaved 34; 4 x 4095 forward and backward
+// 276 us, 4.9 TB/s, a copy's rate from memory; one token 7 us, of which the launch
+// is nearly all.
 #include "axs6_internal.h"
 #include "nf5_device.h"
 
@@ -32,20 +36,37 @@ struct RotaryArgs {
     float sign;
 };
 
-// V elements from p; one 16-byte access where V is a whole vector.
+// V elements from p: one access of 16 bytes, or of 8 (four 16-bit values), or one
+// value.
 template <int DT, int V>
 __device__ __forceinline__ void get(const void* p, int64_t i, float* f) {
     using E = Elem<DT>;
     const auto* q = reinterpret_cast<const typename E::S*>(p) + i;
-    if constexpr (V == 1) f[0] = E::to_f(q[0]);
-    else E::unpack(*reinterpret_cast<const u32x4*>(q), f);
+    if constexpr (V == 1) {
+        f[0] = E::to_f(q[0]);
+    } else if constexpr (V == E::V) {
+        E::unpack(*reinterpret_cast<const u32x4*>(q), f);
+    } else {
+        const uint2 w = *reinterpret_cast<const uint2*>(q);
+        float x[8];
+        E::unpack(u32x4{w.x, w.y, 0, 0}, x);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = x[j];
+    }
 }
 template <int DT, int V>
 __device__ __forceinline__ void put(void* p, int64_t i, const float* f) {
     using E = Elem<DT>;
     auto* q = reinterpret_cast<typename E::S*>(p) + i;
-    if constexpr (V == 1) q[0] = E::from_f(f[0]);
-    else *reinterpret_cast<u32x4*>(q) = E::pack(f);
+    if constexpr (V == 1) {
+        q[0] = E::from_f(f[0]);
+    } else if constexpr (V == E::V) {
+        *reinterpret_cast<u32x4*>(q) = E::pack(f);
+    } else {
+        const float x[8] = {f[0], f[1], f[2], f[3]};
+        const u32x4 w = E::pack(x);
+        *reinterpret_cast<uint2*>(q) = make_uint2(w.x, w.y);
+    }
 }
 
 // A unit is two vectors of V elements of a head: at d and d + R/2 in the half
@@ -147,8 +168,7 @@ __global__ void rotary_kernel(RotaryArgs a) {
 constexpr int kRotaryThreads = 256;
 
 template <int DT, bool INTER>
-void launch(RotaryArgs a, bool vec, hipStream_t st) {
-    const int v = vec ? Elem<DT>::V : 1;
+void launch(RotaryArgs a, int v, hipStream_t st) {
     a.units = INTER ? (a.D + 2 * v - 1) / (2 * v) : a.R / 2 / v + (a.D - a.R + 2 * v - 1) / (2 * v);
     const int most = kRotaryThreads / a.units;   // heads that a workgroup holds at once
     // up to 8 heads a thread where there are tokens enough to fill the chip without more threads
@@ -163,7 +183,8 @@ void launch(RotaryArgs a, bool vec, hipStream_t st) {
     const int threads = (a.units * a.hslots * a.tpb + 63) / 64 * 64;
     const dim3 grid((unsigned)((a.tokens + a.tpb - 1) / a.tpb),
                     (unsigned)((a.H + a.hslots * a.iters - 1) / (a.hslots * a.iters)));
-    if (vec) rotary_kernel<DT, Elem<DT>::V, INTER><<<grid, threads, 0, st>>>(a);
+    if (v == Elem<DT>::V) rotary_kernel<DT, Elem<DT>::V, INTER><<<grid, threads, 0, st>>>(a);
+    else if (v == 4) rotary_kernel<DT, 4, INTER><<<grid, threads, 0, st>>>(a);
     else rotary_kernel<DT, 1, INTER><<<grid, threads, 0, st>>>(a);
 }
 
@@ -193,30 +214,35 @@ extern "C" int axs6_rotary(const void* q, const void* k, void* q_out, void* k_ou
     if ((Hq && (!q_out || !q_strides)) || (Hkv && (!k_out || !k_strides)) || (R && !table) || table_rows < 0 ||
         (R && table_rows == 0))
         return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: null output, strides or table", fn);
-    const int64_t es = dtype == AXS6_F32 ? 4 : 2, v = 16 / es;
-    // whole 16-byte vectors, none of which crosses a boundary of the layout
-    bool vec = D % v == 0 && R % v == 0 && (interleaved || (R / 2) % v == 0) && (uintptr_t)table % 16 == 0;
+    const int64_t es = dtype == AXS6_F32 ? 4 : 2;
     const void* ptrs[] = {q, q_out, k, k_out};
-    for (const void* p : ptrs) {
+    for (const void* p : ptrs)
         if ((uintptr_t)p % es) return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: pointer not element-aligned", fn);
-        vec = vec && (uintptr_t)p % 16 == 0;
-    }
     RotaryArgs a{};
     a.q = q; a.k = k; a.qo = q_out; a.ko = k_out; a.table = table; a.positions = positions;
     a.tokens = B * T; a.T = T; a.table_rows = table_rows;
     for (int i = 0; i < 3; ++i) {
         a.qs[i] = Hq ? q_strides[i] : 0;
         a.ks[i] = Hkv ? k_strides[i] : 0;
-        vec = vec && a.qs[i] % v == 0 && a.ks[i] % v == 0;
+    }
+    // The longest whole aligned vectors, none of which crosses a boundary of the
+    // layout: 16 bytes; in 16 bits 8 (2 x 4096 tokens, 40 heads of 80, the first 40
+    // values rotated in halves of 20: 20 us, by single values 44); a value.
+    int v = (int)(16 / es);
+    for (; v > 1; v = v == 8 ? 4 : 1) {
+        bool whole = D % v == 0 && R % v == 0 && (interleaved || R / 2 % v == 0) && (uintptr_t)table % 16 == 0;
+        for (const void* p : ptrs) whole = whole && (uintptr_t)p % (v * es) == 0;
+        for (int i = 0; i < 3; ++i) whole = whole && a.qs[i] % v == 0 && a.ks[i] % v == 0;
+        if (whole) break;
     }
     a.pos_b = pos_stride_b; a.pos_t = pos_stride_t;
     a.Hq = (int)Hq; a.H = (int)(Hq + Hkv); a.D = (int)D; a.R = (int)R;
     a.sign = inverse ? -1.0f : 1.0f;
     hipStream_t st = (hipStream_t)stream;
     switch (dtype) {
-        case AXS6_F32: interleaved ? launch<AXS6_F32, true>(a, vec, st) : launch<AXS6_F32, false>(a, vec, st); break;
-        case AXS6_BF16: interleaved ? launch<AXS6_BF16, true>(a, vec, st) : launch<AXS6_BF16, false>(a, vec, st); break;
-        default: interleaved ? launch<AXS6_F16, true>(a, vec, st) : launch<AXS6_F16, false>(a, vec, st); break;
+        case AXS6_F32: interleaved ? launch<AXS6_F32, true>(a, v, st) : launch<AXS6_F32, false>(a, v, st); break;
+        case AXS6_BF16: interleaved ? launch<AXS6_BF16, true>(a, v, st) : launch<AXS6_BF16, false>(a, v, st); break;
+        default: interleaved ? launch<AXS6_F16, true>(a, v, st) : launch<AXS6_F16, false>(a, v, st); break;
     }
     return check_launch(fn);
 }

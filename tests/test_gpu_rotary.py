@@ -22,7 +22,7 @@ def _bound(dt):
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("B,T,Hq,Hkv,D,R", [
     (1, 1, 1, 1, 2, 2), (2, 1, 32, 8, 128, 128), (3, 37, 4, 2, 64, 32), (1, 5, 3, 1, 7, 4), (2, 9, 5, 5, 80, 80),
-    (1, 300, 6, 2, 96, 48), (2, 17, 4, 4, 40, 8), (1, 3, 2, 1, 512, 512), (2, 4, 2, 2, 33, 0), (5, 129, 8, 2, 128, 16),
+    (1, 300, 6, 2, 96, 48), (2, 17, 4, 4, 40, 8), (1, 3, 2, 1, 512, 512), (2, 4, 2, 2, 33, 0), (5, 129, 8, 2, 128, 16), (2, 31, 5, 1, 80, 40), (1, 50, 2, 2, 36, 24),
 ])
 def test_rotation_and_gradient(B, T, Hq, Hkv, D, R, interleaved, dtype):
     from axs.unified import axs_rotary_unified, rotary_table
