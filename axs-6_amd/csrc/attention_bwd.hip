@@ -15,6 +15,13 @@
 // launch adds (1 x 16384, 2 key heads for 16, bf16: 9072 -> 3824 us for both
 // launches; 2 x 4096, 8 for 32: 1511 -> 1127, now 1064, of which dq 450: the 7
 // products' 9.6e11 operations at 904 TFLOP/s, 79% of a bf16 product of 8192^3).
+// A head of up to 64 values whose queries and keys are at most 128 is one
+// workgroup's: the second launch then makes dq too, from ds by way of LDS, 5
+// products instead of 7 and one launch instead of two.  64 x 128, 4 heads, causal:
+// float32 61 -> 43 us, bf16 20 either way; 512 x 128: 496 -> 325, 93 -> 89; 64 x 32
+// queries of 77 keys, 8 heads: 67 -> 37, 16 -> 13.  (Larger heads' keys and scores
+// leave no room for a second workgroup on the CU, or for the first.)  In float32 what
+// is left is the wave's own chain: its 640 products of 64 cycles are 17 us of the 43.
 #include "attention.h"
 
 namespace axs6 {
@@ -224,11 +231,47 @@ template <int DT, int DC> struct DkvShape {
     static constexpr int kOccupancy = DT == AXS6_F32 ? 1 : 2;
 };
 
-// dk and dv of 128 keys of one key head.
-template <int DT, int DC, int MASK>
+// ds of a head's 128 queries and the 128 keys held, in the type, a query's keys
+// one after another: the waves that made it hold keys, those that take it hold queries.
+template <int DT>
+struct Scores {
+    using S = typename Elem<DT>::S;
+    static constexpr int kPitch = kHeld + 16 / (int)sizeof(S);   // 16 bytes more: rows start at all banks
+    // the 32 queries from q0 and the lane's key; df: ds in fragments (16-bit types)
+    __device__ static void put(S* p, int q0, int key, const f32x16& ds, const u32x4 (&df)[2], int lane) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            S* x = p + (q0 + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3)) * kPitch + key;
+            if constexpr (DT == AXS6_F32) *x = ds[i];
+            else *reinterpret_cast<uint16_t*>(x) = (uint16_t)(df[i >> 3][(i & 7) >> 1] >> (16 * (i & 1)));
+        }
+    }
+    // the lane's query and the 32 keys from k0, as a result whose rows are the keys
+    __device__ static void get(const S* p, int q, int k0, f32x16& ds, u32x4 (&df)[2], int lane) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const S* x = p + q * kPitch + k0 + 8 * g + 4 * (lane >> 5);
+            if constexpr (DT == AXS6_F32) {
+                const float4 v = *reinterpret_cast<const float4*>(x);
+                ds[4 * g] = v.x; ds[4 * g + 1] = v.y; ds[4 * g + 2] = v.z; ds[4 * g + 3] = v.w;
+            } else {
+                const uint2 v = *reinterpret_cast<const uint2*>(x);
+                df[g >> 1][2 * (g & 1)] = v.x;
+                df[g >> 1][2 * (g & 1) + 1] = v.y;
+            }
+        }
+    }
+};
+
+// dk and dv of 128 keys of one key head.  WHOLE: there are no more keys and no more
+// than 128 queries, and dq is made here too.
+template <int DT, int DC, int MASK, bool WHOLE>
 __global__ __launch_bounds__(kThr, (DkvShape<DT, DC>::kOccupancy)) void attn_dkv_kernel(AttnArgs a) {
     using T = Tile<DT, DC>;
+    using S = Scores<DT>;
     constexpr bool VL = DkvShape<DT, DC>::kVInLds;
+    __shared__ __attribute__((aligned(1024))) char kt[WHOLE ? kHeld * T::kPitch : 16];
+    __shared__ __attribute__((aligned(16))) typename S::S scores[WHOLE ? kHeld * S::kPitch : 4];
     __shared__ __attribute__((aligned(1024))) char qt[2][kWalk * T::kPitch];
     __shared__ __attribute__((aligned(1024))) char gt[2][kWalk * T::kPitch];
     __shared__ __attribute__((aligned(1024))) char vt[VL ? kHeld * T::kPitch : 16];
@@ -261,9 +304,18 @@ __global__ __launch_bounds__(kThr, (DkvShape<DT, DC>::kOccupancy)) void attn_dkv
         lv.init(a.vs[1], a.D, lane, w);
         lv.load(vt, vb, k0, a.Tk, a.D, w);
     }
+    if constexpr (WHOLE) {
+        Direct<DT, DC, kHeld, kWaves> lk;
+        lk.init(a.ks[1], a.D, lane, w);
+        lk.load(kt, reinterpret_cast<const char*>(a.k) + (b * a.ks[0] + h * a.ks[2]) * T::kBytes, 0, a.Tk, a.D, w);
+    }
     // head and first query of the tile on its way
     int hq = h * a.G + (per_head ? first / per_head : 0), i0 = q_first + (per_head ? first % per_head : 0) * kWalk;
     float sl = 0.0f, sd = 0.0f;
+    // WHOLE: out and dout of the tile's rows, eight threads a row, for its delta
+    constexpr int N = DC / 8 / T::kVals;
+    u32x4 xo[N], xg[N];
+    int64_t row_on_way = -1;
     auto load = [&](char* qn, char* gn) {
         lq.load(qn, reinterpret_cast<const char*>(a.q) + (b * a.qs[0] + hq * a.qs[2]) * T::kBytes, i0, a.Tq, a.D, w);
         lg.load(gn, reinterpret_cast<const char*>(a.dout) + (b * a.gs[0] + hq * a.gs[2]) * T::kBytes, i0, a.Tq, a.D, w);
@@ -271,11 +323,45 @@ __global__ __launch_bounds__(kThr, (DkvShape<DT, DC>::kOccupancy)) void attn_dkv
             const int i = i0 + threadIdx.x;
             const int64_t row = ((int64_t)b * a.Hq + hq) * a.Tq + i;
             sl = i < a.Tq ? a.lse[row] : INFINITY;   // rows past the end have no probabilities
-            sd = i < a.Tq ? a.delta[row] : 0.0f;
+            if constexpr (!WHOLE) sd = i < a.Tq ? a.delta[row] : 0.0f;
+        }
+        if constexpr (WHOLE) {
+            const int i = i0 + (threadIdx.x >> 3), d = (threadIdx.x & 7) * (DC / 8);
+            row_on_way = i < a.Tq ? ((int64_t)b * a.Hq + hq) * a.Tq + i : -1;
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                xo[e] = xg[e] = u32x4{0, 0, 0, 0};
+                if (i < a.Tq && d + e * T::kVals < a.D) {
+                    xo[e] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(a.out) +
+                                                            (b * a.os[0] + i * a.os[1] + hq * a.os[2] + d + e * T::kVals) * T::kBytes);
+                    xg[e] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(a.dout) +
+                                                            (b * a.gs[0] + i * a.gs[1] + hq * a.gs[2] + d + e * T::kVals) * T::kBytes);
+                }
+            }
         }
     };
     auto store = [&](int buf) {
-        if (threadIdx.x < kWalk) { lt[buf][threadIdx.x] = sl; dt[buf][threadIdx.x] = sd; }
+        if (threadIdx.x < kWalk) {
+            lt[buf][threadIdx.x] = sl;
+            if constexpr (!WHOLE) dt[buf][threadIdx.x] = sd;
+        }
+        if constexpr (WHOLE) {
+            float delta = 0.0f;
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                float x[T::kVals], y[T::kVals];
+                Elem<DT>::unpack(xo[e], x);
+                Elem<DT>::unpack(xg[e], y);
+#pragma unroll
+                for (int i = 0; i < T::kVals; ++i) delta += x[i] * y[i];
+            }
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) delta += __shfl_xor(delta, o, 64);
+            if ((threadIdx.x & 7) == 0) {
+                dt[buf][threadIdx.x >> 3] = delta;
+                if (row_on_way >= 0) a.delta[row_on_way] = delta;   // for rows made again
+            }
+        }
     };
     if (first < tiles) {
         load(qt[first & 1], gt[first & 1]);
@@ -336,12 +422,45 @@ __global__ __launch_bounds__(kThr, (DkvShape<DT, DC>::kOccupancy)) void attn_dkv
             fragments<DT>(dp, df);
             T::accumulate(gs, 0, s, pf, dv, lane);
             T::accumulate(qs, 0, dp, df, dk, lane);
+            if constexpr (WHOLE) S::put(scores, i_now, key, dp, df, lane);
+        } else if constexpr (WHOLE) {
+            const u32x4 none[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+            S::put(scores, i_now, key, zero16(), none, lane);
         }
         if (t + 1 < tiles) store((t + 1) & 1);
     };
+    // WHOLE: dq of a head when its last tile is done; a wave takes 32 queries
+    auto queries = [&](int head) {
+        __syncthreads();
+        const int q0 = 32 * w, q = q0 + (lane & 31);
+        const int q_last = q0 + 31 < a.Tq ? q0 + 31 : a.Tq - 1;
+        if (q0 >= a.Tq) return;
+        f32x16 dq[T::kResults];
+#pragma unroll
+        for (int d = 0; d < T::kResults; ++d) dq[d] = zero16();
+        const int keys = a.causal && q_last + off + 1 < a.Tk ? q_last + off + 1 : a.Tk;
+        if (q0 >= q_first)   // those before see no key
+            for (int j = 0; j < keys; j += 32) {
+                f32x16 ds;
+                u32x4 df[2];
+                S::get(scores, q, j, ds, df, lane);
+                T::accumulate(kt, j, ds, df, dq, lane);
+            }
+        const bool bad = not_finite(dq);
+        if (q < a.Tq)
+            T::template store<DT>(a.dq, (((int64_t)b * a.Tq + q) * a.Hq + head) * a.D, dq, a.scale, a.D, lane);
+        for (uint64_t rows = __ballot(bad && lane < 32 && q < a.Tq); rows; rows &= rows - 1) {
+            const int r = q0 + __builtin_ctzll(rows);
+            const int64_t row = ((int64_t)b * a.Hq + head) * a.Tq + r;
+            dq_row<DT>(a, b, head, r, 0, a.Tk, 0, a.lse[row], a.delta[row], lane);
+        }
+    };
     for (int t = first; t < tiles; ++t) {
         tile_barrier();
+        const int head = hq;
         step(t, qt[t & 1], gt[t & 1], qt[(t + 1) & 1], gt[(t + 1) & 1]);
+        if constexpr (WHOLE)
+            if (hq != head) queries(head);
     }
     const bool bad = not_finite(dk) || not_finite(dv);
     if (key < a.Tk) {
@@ -384,12 +503,18 @@ void sum_splits(const float* part, int splits, int64_t n, void* out0, void* out1
 
 template <int DT, int DC, int MASK>
 void launch(const AttnArgs& a, hipStream_t st) {
+    if constexpr (DC == 64) {
+        if (a.Tq && a.Tk && a.Tq <= kHeld && a.Tk <= kHeld && a.splits_kv == 1) {
+            attn_dkv_kernel<DT, DC, MASK, true><<<(unsigned)(a.B * a.H), kThr, 0, st>>>(a);
+            return;
+        }
+    }
     if (a.Tq) {
         attn_dq_kernel<DT, DC, MASK><<<(unsigned)((a.Tq + kHeld - 1) / kHeld * a.B * a.Hq * a.splits), kThr, 0, st>>>(a);
         if (a.splits > 1) sum_splits<DT>(a.part, a.splits, (int64_t)a.B * a.Tq * a.Hq * a.D, a.dq, nullptr, st);
     }
     if (a.Tk) {
-        attn_dkv_kernel<DT, DC, MASK><<<(unsigned)((a.Tk + kHeld - 1) / kHeld * a.B * a.H * a.splits_kv), kThr, 0, st>>>(a);
+        attn_dkv_kernel<DT, DC, MASK, false><<<(unsigned)((a.Tk + kHeld - 1) / kHeld * a.B * a.H * a.splits_kv), kThr, 0, st>>>(a);
         if (a.splits_kv > 1)
             sum_splits<DT>(a.part_kv, a.splits_kv, (int64_t)a.B * a.Tk * a.H * a.D, a.dk, a.dv, st);
     }

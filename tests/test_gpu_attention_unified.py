@@ -86,6 +86,36 @@ def test_many_workgroups(D, dtype):
 
 
 @pytest.mark.parametrize("dtype", ref.DTYPES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("shape", [(2, 128, 128, 4, 2, 64), (1, 127, 128, 3, 3, 64), (3, 128, 40, 2, 2, 64), (2, 97, 128, 8, 2, 48),
+                                   (1, 129, 128, 2, 2, 64), (1, 128, 129, 2, 1, 64), (1, 33, 1, 2, 2, 32), (2, 160, 150, 2, 1, 64)])
+def test_sequences_of_one_workgroup(shape, causal, dtype):
+    """All of a head's tokens in one workgroup, which then makes all three gradients, and just past that: no mask, one
+    by key, one by pair, and bad values where a causal mask or the mask hides them."""
+    B, Tq, Tk, Hq, H, D = shape
+    q, k, v, go = _inputs(*shape, dtype)
+    _check(q, k, v, go, causal=causal)
+    g = torch.Generator().manual_seed(2)
+    by_key = (torch.rand(B, 1, 1, Tk, generator=g) < 0.6).to(DEV)
+    by_key[0, ..., 32:64] = False
+    _check(q, k, v, go, by_key, causal)
+    by_pair = (torch.randn(B, Hq, Tq, Tk, generator=g) * 2).masked_fill(torch.rand(B, Hq, Tq, Tk, generator=g) < 0.3, -math.inf)
+    _check(q, k, v, go, by_pair.to(DEV), causal)
+    hidden = ~by_key[:, 0, 0].to(DEV)
+    _, want = _check(q, k, v, go, by_key, causal)
+    k[hidden] = math.nan
+    v[hidden] = math.inf
+    from axs.unified import axs_attention_unified
+    qq, kk, vv = (x.detach().requires_grad_(True) for x in (q, k, v))
+    got = torch.autograd.grad(axs_attention_unified(qq, kk, vv, by_key, causal), (qq, kk, vv), go)
+    fwd, bwd = _bounds(dtype)
+    for x, y, name in zip(got, want, "qkv"):
+        if name != "q":     # rows of hidden keys: 0
+            assert not x[hidden].any()
+        assert ref.rel(x, y) <= 2 * bwd or float(y.double().norm()) == 0.0 == float(x.double().norm()), name
+
+
+@pytest.mark.parametrize("dtype", ref.DTYPES)
 @pytest.mark.parametrize("D", [1, 3, 33, 72, 127])
 def test_odd_heads(D, dtype):
     _check(*_inputs(1, 70, 70, 2, 1, D, dtype), causal=True)
