@@ -29,8 +29,6 @@ namespace {
 
 constexpr int kWaves = 4, kThr = 64 * kWaves, kHeld = 32 * kWaves;
 
-constexpr int kWalk = 32;   // queries of a tile that the held keys walk over
-
 // dq of a query from the keys k0 .. k1 - 1 that it sees, one by one.
 template <int DT>
 __device__ void dq_row(const AttnArgs& a, int b, int hq, int q, int k0, int k1, int split, float lse, float delta,
@@ -57,7 +55,7 @@ __device__ void dq_row(const AttnArgs& a, int b, int hq, int q, int k0, int k1, 
 
 // dk and dv of a key from the queries of the group's tiles first .. tiles - 1
 // that see it, one by one.
-template <int DT>
+template <int DT, int kWalk>
 __device__ void dkv_row(const AttnArgs& a, int b, int h, int key, int first, int tiles, int q_first, int per_head,
                         int split, int lane) {
     const float c = a.scale * kLog2e;
@@ -224,11 +222,17 @@ __global__ __launch_bounds__(kThr, (DqShape<DT, DC>::kOccupancy)) void attn_dq_k
     }
 }
 
-template <int DT, int DC> struct DkvShape {
+template <int DT, int DC, int MASK, bool WHOLE> struct DkvShape {
     // the values held stay in LDS where their fragments would leave a wave more
     // than half of a SIMD's registers
     static constexpr bool kVInLds = DC > 96;
-    static constexpr int kOccupancy = DT == AXS6_F32 ? 1 : 2;
+    // three waves a SIMD where 168 registers are enough (8 x 777, 12 heads of 64, a mask by
+    // key: 127 -> 103 us for both launches)
+    static constexpr int kOccupancy = DT == AXS6_F32 ? 1 : DC <= 64 && MASK != kFullMask && !WHOLE ? 3 : 2;
+    // Queries of a tile that the held keys walk over: 64 for half the barriers, where
+    // they and two waves fit (8 x 777, 12 heads of 80: 156 -> 148 us for both launches; 8 x 2048, 16
+    // heads of 96: 843 -> 826; heads of 64, with two waves then for three, 95 -> 112)
+    static constexpr int kWalk = DT != AXS6_F32 && DC > 64 && DC <= 96 && MASK != kFullMask ? 64 : 32;
 };
 
 // ds of a head's 128 queries and the 128 keys held, in the type, a query's keys
@@ -266,10 +270,11 @@ struct Scores {
 // dk and dv of 128 keys of one key head.  WHOLE: there are no more keys and no more
 // than 128 queries, and dq is made here too.
 template <int DT, int DC, int MASK, bool WHOLE>
-__global__ __launch_bounds__(kThr, (DkvShape<DT, DC>::kOccupancy)) void attn_dkv_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kThr, (DkvShape<DT, DC, MASK, WHOLE>::kOccupancy)) void attn_dkv_kernel(AttnArgs a) {
     using T = Tile<DT, DC>;
     using S = Scores<DT>;
-    constexpr bool VL = DkvShape<DT, DC>::kVInLds;
+    constexpr bool VL = DkvShape<DT, DC, MASK, WHOLE>::kVInLds;
+    constexpr int kWalk = DkvShape<DT, DC, MASK, WHOLE>::kWalk;
     __shared__ __attribute__((aligned(1024))) char kt[WHOLE ? kHeld * T::kPitch : 16];
     __shared__ __attribute__((aligned(16))) typename S::S scores[WHOLE ? kHeld * S::kPitch : 4];
     __shared__ __attribute__((aligned(1024))) char qt[2][kWalk * T::kPitch];
@@ -385,47 +390,52 @@ __global__ __launch_bounds__(kThr, (DkvShape<DT, DC>::kOccupancy)) void attn_dkv
         i0 += kWalk;
         if (i0 >= a.Tq) { i0 = q_first; ++hq; }
         if (t + 1 < tiles) load(qn, gn);
-        // none of the tile's queries sees the wave's keys: they are before them, or the mask hides them
-        bool any = !a.causal || i_now + kWalk - 1 + off >= k0 + 32 * w;
-        if constexpr (MASK == kKeyMask) any = any && __any(!(term == -INFINITY));
-        if (any) {
-            f32x16 s = zero16(), dp = zero16();
 #pragma unroll
-            for (int i = 0; i < T::kSteps; ++i) s = mma<DT>(T::rows(qs, 0, i, lane), kf[i], s);
+        for (int j = 0; j < kWalk / 32; ++j) {
+            const int i_sub = i_now + 32 * j;
+            if (j && i_sub >= a.Tq) break;
+            // none of the 32 queries sees the wave's keys: they are before them, or the mask hides them
+            bool any = !a.causal || i_sub + 31 + off >= k0 + 32 * w;
+            if constexpr (MASK == kKeyMask) any = any && __any(!(term == -INFINITY));
+            if (any) {
+                f32x16 s = zero16(), dp = zero16();
 #pragma unroll
-            for (int i = 0; i < T::kSteps; ++i) {
-                u32x4 v;
-                if constexpr (VL) v = T::rows(vt, 32 * w, i, lane);
-                else v = vf[i];
-                dp = mma<DT>(T::rows(gs, 0, i, lane), v, dp);
-            }
-            const bool edge = i_now < free_q;
+                for (int i = 0; i < T::kSteps; ++i) s = mma<DT>(T::rows(qs, 32 * j, i, lane), kf[i], s);
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const float4 lse = *reinterpret_cast<const float4*>(&lt[t & 1][8 * g + 4 * (lane >> 5)]);
-                const float4 del = *reinterpret_cast<const float4*>(&dt[t & 1][8 * g + 4 * (lane >> 5)]);
-                const float ls[4] = {lse.x, lse.y, lse.z, lse.w}, ds[4] = {del.x, del.y, del.z, del.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int i = 4 * g + e, q = i_now + 8 * g + 4 * (lane >> 5) + e;
-                    float f = term;   // by key: the lane's
-                    if constexpr (MASK == kFullMask)
-                        f = mask_term(a, mask_row(a, b, hq_now, q < a.Tq ? q : a.Tq - 1), kr);
-                    float x = __builtin_fmaf(s[i], c, MASK == kNoMask ? -ls[e] : f - ls[e]);
-                    if (edge) x = kr <= q + off ? x : -INFINITY;
-                    s[i] = __builtin_amdgcn_exp2f(x);
-                    dp[i] = s[i] * (dp[i] - ds[e]);
+                for (int i = 0; i < T::kSteps; ++i) {
+                    u32x4 v;
+                    if constexpr (VL) v = T::rows(vt, 32 * w, i, lane);
+                    else v = vf[i];
+                    dp = mma<DT>(T::rows(gs, 32 * j, i, lane), v, dp);
                 }
+                const bool edge = i_sub < free_q;
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const float4 lse = *reinterpret_cast<const float4*>(&lt[t & 1][32 * j + 8 * g + 4 * (lane >> 5)]);
+                    const float4 del = *reinterpret_cast<const float4*>(&dt[t & 1][32 * j + 8 * g + 4 * (lane >> 5)]);
+                    const float ls[4] = {lse.x, lse.y, lse.z, lse.w}, ds[4] = {del.x, del.y, del.z, del.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int i = 4 * g + e, q = i_sub + 8 * g + 4 * (lane >> 5) + e;
+                        float f = term;   // by key: the lane's
+                        if constexpr (MASK == kFullMask)
+                            f = mask_term(a, mask_row(a, b, hq_now, q < a.Tq ? q : a.Tq - 1), kr);
+                        float x = __builtin_fmaf(s[i], c, MASK == kNoMask ? -ls[e] : f - ls[e]);
+                        if (edge) x = kr <= q + off ? x : -INFINITY;
+                        s[i] = __builtin_amdgcn_exp2f(x);
+                        dp[i] = s[i] * (dp[i] - ds[e]);
+                    }
+                }
+                u32x4 pf[2], df[2];
+                fragments<DT>(s, pf);
+                fragments<DT>(dp, df);
+                T::accumulate(gs, 32 * j, s, pf, dv, lane);
+                T::accumulate(qs, 32 * j, dp, df, dk, lane);
+                if constexpr (WHOLE) S::put(scores, i_sub, key, dp, df, lane);
+            } else if constexpr (WHOLE) {
+                const u32x4 none[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+                S::put(scores, i_sub, key, zero16(), none, lane);
             }
-            u32x4 pf[2], df[2];
-            fragments<DT>(s, pf);
-            fragments<DT>(dp, df);
-            T::accumulate(gs, 0, s, pf, dv, lane);
-            T::accumulate(qs, 0, dp, df, dk, lane);
-            if constexpr (WHOLE) S::put(scores, i_now, key, dp, df, lane);
-        } else if constexpr (WHOLE) {
-            const u32x4 none[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-            S::put(scores, i_now, key, zero16(), none, lane);
         }
         if (t + 1 < tiles) store((t + 1) & 1);
     };
@@ -474,7 +484,7 @@ __global__ __launch_bounds__(kThr, (DkvShape<DT, DC>::kOccupancy)) void attn_dkv
         }
     }
     for (uint64_t rows = __ballot(bad && lane < 32 && key < a.Tk); rows; rows &= rows - 1)
-        dkv_row<DT>(a, b, h, k0 + 32 * w + __builtin_ctzll(rows), first, tiles, q_first, per_head, split, lane);
+        dkv_row<DT, kWalk>(a, b, h, k0 + 32 * w + __builtin_ctzll(rows), first, tiles, q_first, per_head, split, lane);
 }
 
 // Sums of the splits in order, four values a thread; of two results, one after
