@@ -169,7 +169,8 @@ struct ReadArgs {
 };
 
 // One workgroup a (sequence, head, block, keys or values) of the tokens from
-// first[b] on; places outside the cache give 0.
+// first[b] on; places outside the cache give 0 and nothing is read for them (a cache
+// without blocks has no memory).
 __global__ __launch_bounds__(kAppendThreads) void kv_read_kernel(ReadArgs a) {
     __shared__ int8_t tile[kMaxHead * (kKvBlock + 4)];
     const int b = blockIdx.x / a.H, h = blockIdx.x % a.H, z = blockIdx.z, D = a.D;
@@ -178,10 +179,10 @@ __global__ __launch_bounds__(kAppendThreads) void kv_read_kernel(ReadArgs a) {
     const int64_t blk = (first >= 0 ? first / kKvBlock : -((-first + kKvBlock - 1) / kKvBlock)) + blockIdx.y;
     if (blk * kKvBlock >= first + a.count) return;
     const bool inside = blk >= 0 && blk < a.nb;
-    const int64_t cell = ((int64_t)b * a.H + h) * a.nb + (inside ? blk : 0);
-    const int8_t* codes = a.codes[z] + cell * kKvBlock * D;
+    const int64_t cell = ((int64_t)b * a.H + h) * a.nb + blk;
+    const int8_t* codes = inside ? a.codes[z] + cell * kKvBlock * D : nullptr;
     const float scale = inside ? a.scales[z][cell] : 0.0f;
-    if (z == 1) {
+    if (z == 1 && inside) {
         for (int c = threadIdx.x; c < D * (kKvBlock / 4); c += kAppendThreads) {
             const int d = c / (kKvBlock / 4), t = c % (kKvBlock / 4) * 4;
             *reinterpret_cast<uint32_t*>(tile + d * (kKvBlock + 4) + t) =
@@ -193,15 +194,15 @@ __global__ __launch_bounds__(kAppendThreads) void kv_read_kernel(ReadArgs a) {
         const int t = c / (D / 4), d = c % (D / 4) * 4;
         const int64_t i = blk * kKvBlock + t - first;   // place in the output
         if (i < 0 || i >= a.count) continue;
-        uint32_t w = 0;
-        if (z == 0) {
-            w = *reinterpret_cast<const uint32_t*>(codes + t * D + d);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) w |= (uint32_t)(uint8_t)tile[(d + j) * (kKvBlock + 4) + t] << (8 * j);
-        }
         float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (inside) {
+            uint32_t w = 0;
+            if (z == 0) {
+                w = *reinterpret_cast<const uint32_t*>(codes + t * D + d);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w |= (uint32_t)(uint8_t)tile[(d + j) * (kKvBlock + 4) + t] << (8 * j);
+            }
             f.x = scale * (float)(int8_t)w;
             f.y = scale * (float)(int8_t)(w >> 8);
             f.z = scale * (float)(int8_t)(w >> 16);

@@ -224,3 +224,30 @@ def test_refusals():
                 lambda: axs_cache_read_unified(c, n, -1), lambda: axs_cache_read_unified(c, n[:1], 1)):
         with pytest.raises(RuntimeError):
             bad()
+
+
+def test_a_cache_without_blocks():
+    """Reading gives 0, appending drops everything, attention sees nothing."""
+    from axs.unified import AXSKVCacheUnified, axs_cache_append_unified, axs_cache_attention_unified, axs_cache_read_unified
+
+    cache = AXSKVCacheUnified.empty(2, 2, 32, 0, torch.float32, DEV)
+    x = torch.ones(2, 3, 2, 32, device=DEV)
+    n = torch.tensor([0, 5], device=DEV)
+    axs_cache_append_unified(cache, x, x, n)
+    for count in (1, 40):
+        for y in axs_cache_read_unified(cache, n - 2, count):
+            assert y.shape == (2, count, 2, 32) and not y.any()
+    assert not axs_cache_attention_unified(x, cache, n).any()
+
+
+def test_reading_outside_the_blocks():
+    from axs.unified import axs_cache_read_unified
+
+    cache, k, v = _filled(1, 64, 2, 32, torch.float32)
+    for first, count in ((-100, 90), (64, 33), (1000, 5), (-3, 70)):
+        for x, y in zip((k, v), axs_cache_read_unified(cache, torch.tensor([first], device=DEV), count)):
+            want = torch.zeros(count, 2, 32)
+            lo, hi = max(first, 0), min(first + count, 64)
+            if lo < hi:
+                want[lo - first:hi - first] = ref.cache_values(x[0])[lo:hi]
+            assert torch.equal(y[0].cpu(), want)
