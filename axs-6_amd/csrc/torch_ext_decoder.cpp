@@ -401,7 +401,7 @@ struct DistillFunction : public torch::autograd::Function<DistillFunction> {
         d["reduction"] = reduction;
         d["shape"] = logits.sizes().vec();
         if (reduction) return loss;
-        if (has_weights) rows.mul_(w);
+        if (has_weights) rows.mul_(w.view({N}));
         return rows.view(logits.sizes().slice(0, logits.dim() - 1));
     }
 

@@ -139,3 +139,22 @@ def test_refusals():
             bad()
     with pytest.raises(ValueError):
         f(z, v, i, 1.0, None, "average")
+
+
+@pytest.mark.parametrize("dtype", ref.DTYPES)
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("batch", [(), (6,), (2, 3), (1, 6), (2, 1, 3)])
+def test_batch_dims_and_reductions(batch, reduction, dtype):
+    from axs.unified import axs_distillation_loss_unified
+
+    z, values, idx, w = _case(max(1, math.prod(batch)), 100, 4, dtype)
+    w[0] = 0.5
+    z = z.detach().view(*batch, 100).requires_grad_(True)
+    values, idx, w = values.view(*batch, 4), idx.view(*batch, 4), w.view(batch)
+    loss = axs_distillation_loss_unified(z, values, idx, 2.0, w, reduction)
+    assert loss.shape == (batch if reduction == "none" else ())
+    grad, = torch.autograd.grad(loss.sum(), z)
+    want, dz = ref.distill(z, values, idx, 2.0, w, reduction)
+    want = want.view(loss.shape)
+    assert float((loss.detach().double().cpu() - want).abs().max()) <= 2e-5 * float(want.abs().max()) + 3e-6 * 4 * 12
+    assert grad.shape == z.shape and ref.rel(grad.reshape(-1, 100), dz) <= _bound(dtype)
