@@ -223,8 +223,10 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* p, int64
 typedef __attribute__((address_space(3))) void lds_void;
 
 // A tile of R rows straight from memory into LDS (16 bytes a lane, 1 KB a wave
-// and instruction, in slot order): rows past the last and values past D arrive
-// as zeros.  The caller waits on vmcnt and a barrier.
+// and instruction, in slot order): values past D arrive as zeros, and so do rows
+// past the last one where rows lie a row's bytes apart or more; of rows that overlap
+// (an expanded dim) some are real values, so what multiplies them has to be 0.  The
+// caller waits on vmcnt and a barrier.
 template <int DT, int DC, int R, int WAVES>
 struct Direct {
     using T = Tile<DT, DC>;

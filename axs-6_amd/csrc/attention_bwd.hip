@@ -431,7 +431,14 @@ __global__ __launch_bounds__(kThr, (DkvShape<DT, DC, MASK, WHOLE>::kOccupancy)) 
                 fragments<DT>(dp, df);
                 T::accumulate(gs, 32 * j, s, pf, dv, lane);
                 T::accumulate(qs, 32 * j, dp, df, dk, lane);
-                if constexpr (WHOLE) S::put(scores, i_sub, key, dp, df, lane);
+                if constexpr (WHOLE) {
+                    if (key >= a.Tk) {   // a copy of the last key, which dq must not add again
+                        const u32x4 none[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+                        S::put(scores, i_sub, key, zero16(), none, lane);
+                    } else {
+                        S::put(scores, i_sub, key, dp, df, lane);
+                    }
+                }
             } else if constexpr (WHOLE) {
                 const u32x4 none[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
                 S::put(scores, i_sub, key, zero16(), none, lane);

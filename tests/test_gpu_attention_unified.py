@@ -346,3 +346,18 @@ def test_refusals():
                 lambda: f(*[torch.zeros(1, 4, 1, 136, device=DEV)] * 3)):
         with pytest.raises(RuntimeError):
             bad()
+
+
+@pytest.mark.parametrize("dtype", ref.DTYPES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("Tq,Tk", [(40, 33), (70, 40), (128, 127), (130, 40)])
+def test_tokens_that_overlap_in_memory(Tq, Tk, causal, dtype):
+    """Keys and values expanded over the tokens (one token's memory for all), and rows that overlap."""
+    B, H, D = 2, 2, 64
+    q, k, v, go = _inputs(B, Tq, Tk, H, H, D, dtype)
+    _check(q, k[:, :1].expand(-1, Tk, -1, -1), v, go, causal=causal)
+    # q, k: the same keys give every score of a row the same value, so tell them apart by overlapping windows
+    step = 16
+    mem = torch.randn(B, H, Tk * step + D, generator=torch.Generator().manual_seed(4)).to(DEV, dtype)
+    near = mem.as_strided((B, Tk, H, D), (mem.stride(0), step, mem.stride(1), 1))
+    _check(q, near, near, go, causal=causal)
