@@ -60,8 +60,9 @@ def rotary_table(
         def turns(n: float) -> float:   # the index whose frequency turns n times
             return rotary_dim * math.log(original_positions / (2 * math.pi * n)) / (2 * math.log(base))
 
-        low, high = max(math.floor(turns(32.0)), 0), min(math.ceil(turns(1.0)), max(rotary_dim // 2 - 1, 0))
-        ramp = ((i - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)
+        # high may lie past the last index: no frequency is then divided in full
+        low, high = max(math.floor(turns(32.0)), 0), math.ceil(turns(1.0))
+        ramp = torch.where(i >= high, 1.0, ((i - low) / max(high - low, 1)).clamp(0.0, 1.0))
         inv = inv / factor * ramp + inv * (1.0 - ramp)
         gain = 0.1 * math.log(factor) + 1.0
     angle = torch.arange(max_positions, dtype=torch.float64)[:, None] * inv

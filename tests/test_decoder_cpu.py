@@ -108,3 +108,26 @@ def test_c_entries_check_their_arguments():
     dis = [p, 0, 100, 4, 100, p, p, 8, 1.0, None, p, p, 0, p, p, None]
     for change, rc in (({"a10": None}, 1), ({"a11": None}, 1), ({"a14": None}, 1), ({"a3": 0}, 0)):
         assert call(L.axs6_distill_backward, dis, **change) == rc, change
+
+
+@pytest.mark.parametrize("rotary_dim,original,base", [(128, 4096, 1e4), (128, 131072, 1e4), (128, 65536, 1e4), (64, 32768, 1e6),
+                                                      (80, 300, 1e4), (32, 6, 1e4), (128, 2, 1e4)])
+def test_rotary_table_by_parts(rotary_dim, original, base):
+    """By wavelength: 32 turns or more within the original positions stay, one at most is divided by the factor, a
+    linear ramp over the index between, also where that ends past the last index."""
+    from axs.unified import rotary_table
+
+    factor, n = 4.0, rotary_dim // 2
+    t = rotary_table(rotary_dim, 2, base=base, scaling="parts", factor=factor, original_positions=original).double()
+    got = torch.atan2(t[1, n:], t[1, :n])               # the frequencies: angles of position 1
+    i = torch.arange(n, dtype=torch.float64)
+    whole = base ** (-i / n)
+    turns = whole * original / (2 * math.pi)
+    kept = 1 - (got / whole - 1 / factor) / (1 - 1 / factor)    # 0: as it was, 1: divided in full
+    assert kept[turns <= 1].sub(1).abs().le(1e-5).all() and kept[turns >= 32].abs().le(1e-5).all()
+    # between: a line over the index from the last that stays to the first that is divided in full
+    at = lambda k: n * math.log(original / (2 * math.pi * k)) / math.log(base)
+    low, high = max(math.floor(at(32)), 0), math.ceil(at(1))
+    between = (i > low) & (i < high)
+    assert (kept - (i - low) / max(high - low, 1))[between].abs().le(1e-5).all()
+    assert not ((kept > 1 - 1e-5) & (turns > 1) & (i < high)).any()
