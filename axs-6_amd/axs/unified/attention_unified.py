@@ -75,12 +75,19 @@ class AXSCausalSelfAttentionUnified(nn.Module):
         self.out_proj = AXSLinearUnified(embed_dim, embed_dim, bias=bias, block_size=block_size)
 
     def _heads(self, x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """Queries, keys and values: one grouped linear where the three projections are
+        quantized ones of the same settings, else one by one -- also when a projection
+        has hooks, which see only calls of the module itself."""
         p = (self.q_proj, self.k_proj, self.v_proj)
-        if any(m._warmup_active or m._forward_hooks or m._forward_pre_hooks for m in p):
-            y = tuple(m(x) for m in p)
+        grouped = (all(type(m) is AXSLinearUnified for m in p)
+                   and not any(m._warmup_active or m._forward_hooks or m._forward_pre_hooks for m in p)
+                   and len({(m.block_size, m.quantize_input, m.quantize_grad) for m in p}) == 1)
+        if grouped:
+            m = p[0]
+            y = axs_linear_group_unified(x, [l.weight for l in p], [l.bias for l in p], m.block_size,
+                                         m.quantize_input, m.quantize_grad)
         else:
-            y = axs_linear_group_unified(x, [m.weight for m in p], [m.bias for m in p], self.block_size,
-                                         self.q_proj.quantize_input, self.q_proj.quantize_grad)
+            y = tuple(m(x) for m in p)
         B, T = x.shape[:2]
         return tuple(t.reshape(B, T, -1, self.head_dim) for t in y)
 

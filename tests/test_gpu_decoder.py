@@ -75,3 +75,61 @@ def test_example_learns_and_answers():
     top = whole.topk(2, -1).values
     sure = top[..., 0] - top[..., 1] > 0.1 * whole.std()
     assert torch.equal(whole.argmax(-1)[sure], out[:, 24:][sure])
+
+
+@pytest.mark.parametrize("setting", [{"quantize_input": False}, {"quantize_grad": False}, {"block_size": 16}])
+@pytest.mark.parametrize("which", ["q_proj", "k_proj", "v_proj"])
+def test_each_projection_keeps_its_settings(which, setting):
+    """Settings of one projection, or a projection of another type, hold in forward, backward and decode."""
+    import axs.unified as axu
+
+    torch.manual_seed(0)
+    m = axu.AXSCausalSelfAttentionUnified(128, 4, 2).to(DEV)
+    for name, value in setting.items():
+        setattr(getattr(m, which), name, value)
+    _is_its_parts(m)
+
+
+@pytest.mark.parametrize("which", ["q_proj", "k_proj", "v_proj"])
+def test_projections_of_another_type(which):
+    import axs.unified as axu
+
+    torch.manual_seed(0)
+    m = axu.AXSCausalSelfAttentionUnified(128, 4, 2).to(DEV)
+    p = getattr(m, which)
+    setattr(m, which, torch.nn.Linear(p.in_features, p.out_features).to(DEV))
+    _is_its_parts(m)
+    m = axu.AXSCausalSelfAttentionUnified(128, 4, 2, block_size=16).to(DEV)
+    _is_its_parts(m, gradients=False)    # grouped: rounded by other random numbers
+
+
+def _is_its_parts(m, gradients=True):
+    import axs.unified as axu
+
+    table = axu.rotary_table(32, 64, device=DEV)
+    x = torch.randn(2, 40, 128, device=DEV, requires_grad=True)
+    go = torch.randn(2, 40, 128, device=DEV)
+
+    def heads():
+        return (p(x).unflatten(-1, (-1, 32)) for p in (m.q_proj, m.k_proj, m.v_proj))
+
+    y = m(x, table)
+    params = list(m.parameters())
+    torch.manual_seed(5)    # of the gradients' stochastic rounding
+    got = torch.autograd.grad(y, [x, *params], go)
+    q, k, v = heads()
+    q, k = axu.axs_rotary_unified(q, k, table)
+    parts = m.out_proj(axu.axs_attention_unified(q, k, v, causal=True).flatten(2))
+    assert torch.equal(y, parts)
+    torch.manual_seed(5)
+    for a, b in zip(got, torch.autograd.grad(parts, [x, *params], go)):
+        assert not gradients or ref.rel(a, b) <= 1e-5
+    with torch.no_grad():
+        cache, other = (m.new_cache(2, 40, device=DEV) for _ in range(2))
+        starts = torch.zeros(2, dtype=torch.int64, device=DEV)
+        out = m.decode(x, table, cache, starts)
+        q, k, v = heads()
+        q, k = axu.axs_rotary_unified(q, k, table)
+        axu.axs_cache_append_unified(other, k, v, starts)
+        want = m.out_proj(axu.axs_cache_attention_unified(q, other, starts + 40).flatten(2))
+    assert torch.equal(out, want)
