@@ -25,7 +25,8 @@ struct AttnArgs {
     const void *q, *k, *v, *out, *dout;
     void *o, *dq, *dk, *dv;            // contiguous (B, T, H, D)
     int64_t qs[3], ks[3], vs[3], os[3], gs[3];   // strides of batch, token, head (q, k, v, out, dout)
-    float *lse, *delta;                // (B, Hq, Tq); lse in units of log2, +inf where a row sees nothing
+    float2* stats;                     // (B, Hq, Tq): row_stats
+    float* delta;                      // (B, Hq, Tq)
     // Splits of the walked axis and their partial results: of the forward each
     // row's sums, maximum and sum; of the backward dq, and dk and dv.
     int splits, splits_kv;
@@ -311,8 +312,22 @@ __device__ __forceinline__ void load_rows(u32x4 (&f)[N], const void* base, int64
 }
 
 // How a mask is read: not at all; by key (the same for all queries of a head: a
-// tile's terms lie in LDS); by query and key.
-enum MaskKind { kNoMask, kKeyMask, kFullMask };
+// tile's terms lie in LDS); by query and key.  The backward tells masks by key that add
+// values from those that only hide: a row's maximum may then be of any size.
+enum MaskKind { kNoMask, kKeyMask, kFullMask, kKeyAdd };
+constexpr bool by_key(int mask) { return mask == kKeyMask || mask == kKeyAdd; }
+constexpr bool adds(int mask) { return mask == kFullMask || mask == kKeyAdd; }
+
+// What a row's probabilities are made from again: p = exp2((x - y) - z), x the score in
+// units of log2, for y = m + log2 l and z = 0, or y = m and z = log2 l where float32 has
+// no place for log2 l beside m (the keys of a row all carry -1e9, which leaves m there).
+// 64: log2 l is then off by 2^-19 at the most, 1.3e-6 of a probability.  A row that sees
+// nothing has y = +inf.
+__device__ __forceinline__ float2 row_stats(float m, float l) {
+    const float s = __builtin_amdgcn_logf(l);
+    if (l == 0.0f) return make_float2(INFINITY, 0.0f);
+    return fabsf(m) < 64.0f ? make_float2(m + s, 0.0f) : make_float2(m, s);
+}
 
 // What the mask adds to a score in units of log2: -inf where the query does not
 // see the key.  An added value below -1e38 counts as that: times log2(e) it
@@ -352,7 +367,7 @@ __device__ __forceinline__ void apply_mask(const AttnArgs& a, f32x16& s, float c
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             float f[4];
-            if constexpr (MASK == kKeyMask) {
+            if constexpr (by_key(MASK)) {
                 const float4 t = *reinterpret_cast<const float4*>(term + 8 * g + h4);
                 f[0] = t.x; f[1] = t.y; f[2] = t.z; f[3] = t.w;
             } else {

@@ -1,7 +1,7 @@
 // Attention backward: the gradients of queries, keys and values from the
-// output's, with the probabilities made again from each row's lse.
+// output's, with the probabilities made again from each row's maximum m and sum l.
 //
-//   p_ij = exp(x_ij - lse_i),  dv_j = sum_i p_ij do_i,
+//   p_ij = exp(x_ij - m_i - log l_i),  dv_j = sum_i p_ij do_i,
 //   ds_ij = p_ij (do_i . v_j - delta_i),  delta_i = sum_j p_ij do_i . v_j = do_i . o_i,
 //   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i  (over the group's heads).
 //
@@ -31,7 +31,7 @@ constexpr int kWaves = 4, kThr = 64 * kWaves, kHeld = 32 * kWaves;
 
 // dq of a query from the keys k0 .. k1 - 1 that it sees, one by one.
 template <int DT>
-__device__ void dq_row(const AttnArgs& a, int b, int hq, int q, int k0, int k1, int split, float lse, float delta,
+__device__ void dq_row(const AttnArgs& a, int b, int hq, int q, int k0, int k1, int split, float2 st, float delta,
                        int lane) {
     const int h = hq / a.G;
     const float c = a.scale * kLog2e;
@@ -43,7 +43,7 @@ __device__ void dq_row(const AttnArgs& a, int b, int hq, int q, int k0, int k1, 
         if (f == -INFINITY) continue;
         const Two kv = load_two<DT>(a.k, b * a.ks[0] + key * a.ks[1] + h * a.ks[2], a.D, lane);
         const Two vv = load_two<DT>(a.v, b * a.vs[0] + key * a.vs[1] + h * a.vs[2], a.D, lane);
-        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(dot(qv, kv), c, f) - lse);
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(dot(qv, kv), c, f) - st.x - st.y);
         const float ds = p * (dot(gv, vv) - delta);
         r = {r.x + ds * kv.x, r.y + ds * kv.y};
     }
@@ -70,7 +70,8 @@ __device__ void dkv_row(const AttnArgs& a, int b, int h, int key, int first, int
             const int64_t row = ((int64_t)b * a.Hq + hq) * a.Tq + q;
             const Two qv = load_two<DT>(a.q, b * a.qs[0] + q * a.qs[1] + hq * a.qs[2], a.D, lane);
             const Two gv = load_two<DT>(a.dout, b * a.gs[0] + q * a.gs[1] + hq * a.gs[2], a.D, lane);
-            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(dot(qv, kv), c, f) - a.lse[row]);
+            const float2 st = a.stats[row];
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(dot(qv, kv), c, f) - st.x - st.y);
             const float ds = p * (dot(gv, vv) - a.delta[row]);
             rk = {rk.x + ds * qv.x, rk.y + ds * qv.y};
             rv = {rv.x + p * gv.x, rv.y + p * gv.y};
@@ -100,7 +101,7 @@ __global__ __launch_bounds__(kThr, (DqShape<DT, DC>::kOccupancy)) void attn_dq_k
     constexpr int KEYS = DqShape<DT, DC>::kKeys, NK = KEYS / 32;
     __shared__ __attribute__((aligned(1024))) char kt[2][KEYS * T::kPitch];
     __shared__ __attribute__((aligned(1024))) char vt[2][KEYS * T::kPitch];
-    __shared__ __attribute__((aligned(16))) float term[2][MASK == kKeyMask ? KEYS : 1];
+    __shared__ __attribute__((aligned(16))) float term[2][by_key(MASK) ? KEYS : 1];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int q_tiles = (a.Tq + kHeld - 1) / kHeld;
     int bh, piece;
@@ -132,7 +133,7 @@ __global__ __launch_bounds__(kThr, (DqShape<DT, DC>::kOccupancy)) void attn_dq_k
     if (first < tiles) {
         dk.load(kt[first & 1], kb, first * KEYS, a.Tk, a.D, w);
         dv.load(vt[first & 1], vb, first * KEYS, a.Tk, a.D, w);
-        if constexpr (MASK == kKeyMask) {
+        if constexpr (by_key(MASK)) {
             const float f = key_term(first);
             if (threadIdx.x < KEYS) term[first & 1][threadIdx.x] = f;
         }
@@ -159,7 +160,9 @@ __global__ __launch_bounds__(kThr, (DqShape<DT, DC>::kOccupancy)) void attn_dq_k
         delta += __shfl_xor(delta, 32, 64);
         if (lane < 32 && q < a.Tq && split == 0) a.delta[row] = delta;
     }
-    const float lse = a.lse[row], c = a.scale * kLog2e;
+    const float2 st = a.stats[row];
+    const float lse = adds(MASK) ? st.x : st.x + st.y, c = a.scale * kLog2e;
+    const bool apart = adds(MASK) && __any(st.y != 0.0f);
 
     f32x16 dq[T::kResults];
 #pragma unroll
@@ -173,13 +176,13 @@ __global__ __launch_bounds__(kThr, (DqShape<DT, DC>::kOccupancy)) void attn_dq_k
         if (t + 1 < tiles) {
             dk.load(kt[(t + 1) & 1], kb, (t + 1) * KEYS, a.Tk, a.D, w);
             dv.load(vt[(t + 1) & 1], vb, (t + 1) * KEYS, a.Tk, a.D, w);
-            if constexpr (MASK == kKeyMask) next_term = key_term(t + 1);
+            if constexpr (by_key(MASK)) next_term = key_term(t + 1);
         }
         const char *ks = kt[t & 1], *vs = vt[t & 1];
         const int k0 = t * KEYS;
         bool any = rows_here;
         bool plain = MASK == kNoMask;
-        if constexpr (MASK == kKeyMask) {
+        if constexpr (by_key(MASK)) {
             const float f = term[t & 1][lane & (KEYS - 1)];
             any = any && __any(!(f == -INFINITY));
             plain = __all(f == 0.0f);
@@ -194,18 +197,25 @@ __global__ __launch_bounds__(kThr, (DqShape<DT, DC>::kOccupancy)) void attn_dq_k
                 for (int i = 0; i < T::kSteps; ++i) s = mma<DT>(T::rows(ks, 32 * j, i, lane), qf[i], s);
 #pragma unroll
                 for (int i = 0; i < T::kSteps; ++i) dp = mma<DT>(T::rows(vs, 32 * j, i, lane), gf[i], dp);
-                apply_mask<MASK>(a, s, c, k0 + 32 * j, &term[t & 1][MASK == kKeyMask ? 32 * j : 0], mrow, plain,
+                apply_mask<MASK>(a, s, c, k0 + 32 * j, &term[t & 1][by_key(MASK) ? 32 * j : 0], mrow, plain,
                                  t >= free_tiles, limit, lane);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], cs, -lse)) * (dp[i] - delta);
+                    s[i] = __builtin_fmaf(s[i], cs, -lse);
+                }
+                if (apart)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[i] -= st.y;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    s[i] = __builtin_amdgcn_exp2f(s[i]) * (dp[i] - delta);
                 }
                 u32x4 pf[2];
                 fragments<DT>(s, pf);
                 T::accumulate(ks, 32 * j, s, pf, dq, lane);
             }
         }
-        if constexpr (MASK == kKeyMask)
+        if constexpr (by_key(MASK))
             if (threadIdx.x < KEYS) term[(t + 1) & 1][threadIdx.x] = next_term;
     }
     const bool bad = not_finite(dq);
@@ -218,7 +228,7 @@ __global__ __launch_bounds__(kThr, (DqShape<DT, DC>::kOccupancy)) void attn_dq_k
     for (uint64_t rows = __ballot(bad && lane < 32 && q < a.Tq); rows; rows &= rows - 1) {
         const int r = __builtin_ctzll(rows);
         dq_row<DT>(a, b, hq, q0 + 32 * w + r, first * KEYS, tiles * KEYS < a.Tk ? tiles * KEYS : a.Tk, split,
-                   __shfl(lse, r, 64), __shfl(delta, r, 64), lane);
+                   make_float2(__shfl(st.x, r, 64), __shfl(st.y, r, 64)), __shfl(delta, r, 64), lane);
     }
 }
 
@@ -281,6 +291,9 @@ __global__ __launch_bounds__(kThr, (DkvShape<DT, DC, MASK, WHOLE>::kOccupancy)) 
     __shared__ __attribute__((aligned(1024))) char gt[2][kWalk * T::kPitch];
     __shared__ __attribute__((aligned(1024))) char vt[VL ? kHeld * T::kPitch : 16];
     __shared__ __attribute__((aligned(16))) float lt[2][kWalk], dt[2][kWalk];
+    // the rows' second numbers, and whether one of them is not 0
+    __shared__ __attribute__((aligned(16))) float rt[2][adds(MASK) ? kWalk : 4];
+    __shared__ int rest[2];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int k_tiles = (a.Tk + kHeld - 1) / kHeld;
     int bh, piece;
@@ -316,7 +329,7 @@ __global__ __launch_bounds__(kThr, (DkvShape<DT, DC, MASK, WHOLE>::kOccupancy)) 
     }
     // head and first query of the tile on its way
     int hq = h * a.G + (per_head ? first / per_head : 0), i0 = q_first + (per_head ? first % per_head : 0) * kWalk;
-    float sl = 0.0f, sd = 0.0f;
+    float sl = 0.0f, sr = 0.0f, sd = 0.0f;
     // WHOLE: out and dout of the tile's rows, eight threads a row, for its delta
     constexpr int N = DC / 8 / T::kVals;
     u32x4 xo[N], xg[N];
@@ -327,7 +340,9 @@ __global__ __launch_bounds__(kThr, (DkvShape<DT, DC, MASK, WHOLE>::kOccupancy)) 
         if (threadIdx.x < kWalk) {
             const int i = i0 + threadIdx.x;
             const int64_t row = ((int64_t)b * a.Hq + hq) * a.Tq + i;
-            sl = i < a.Tq ? a.lse[row] : INFINITY;   // rows past the end have no probabilities
+            const float2 st = i < a.Tq ? a.stats[row] : make_float2(INFINITY, 0.0f);   // rows past the end have no probabilities
+            sl = adds(MASK) ? st.x : st.x + st.y;
+            sr = st.y;
             if constexpr (!WHOLE) sd = i < a.Tq ? a.delta[row] : 0.0f;
         }
         if constexpr (WHOLE) {
@@ -348,6 +363,11 @@ __global__ __launch_bounds__(kThr, (DkvShape<DT, DC, MASK, WHOLE>::kOccupancy)) 
     auto store = [&](int buf) {
         if (threadIdx.x < kWalk) {
             lt[buf][threadIdx.x] = sl;
+            if constexpr (adds(MASK)) {
+                rt[buf][threadIdx.x] = sr;
+                const bool some = __any(sr != 0.0f);
+                if (threadIdx.x == 0) rest[buf] = some;
+            }
             if constexpr (!WHOLE) dt[buf][threadIdx.x] = sd;
         }
         if constexpr (WHOLE) {
@@ -372,6 +392,9 @@ __global__ __launch_bounds__(kThr, (DkvShape<DT, DC, MASK, WHOLE>::kOccupancy)) 
         load(qt[first & 1], gt[first & 1]);
         store(first & 1);
     }
+    if constexpr (WHOLE)   // lanes past the last key hold a copy of it, which dq must not add again
+        if (key >= a.Tk)
+            for (int i = lane >> 5; i < kHeld; i += 2) scores[i * S::kPitch + key - k0] = typename S::S(0);
     u32x4 kf[T::kSteps], vf[VL ? 1 : T::kSteps];
     load_rows<DT, DC>(kf, a.k, b * a.ks[0] + kr * a.ks[1] + h * a.ks[2], a.D, lane);
     if constexpr (!VL) load_rows<DT, DC>(vf, a.v, b * a.vs[0] + kr * a.vs[1] + h * a.vs[2], a.D, lane);
@@ -385,7 +408,7 @@ __global__ __launch_bounds__(kThr, (DkvShape<DT, DC, MASK, WHOLE>::kOccupancy)) 
     auto step = [&](int t, const char* __restrict__ qs, const char* __restrict__ gs, char* __restrict__ qn,
                     char* __restrict__ gn) __attribute__((always_inline)) {
         const int hq_now = hq, i_now = i0;
-        if constexpr (MASK == kKeyMask)
+        if constexpr (by_key(MASK))
             if (t == first || i_now == q_first) term = mask_term(a, mask_row(a, b, hq_now, 0), kr);
         i0 += kWalk;
         if (i0 >= a.Tq) { i0 = q_first; ++hq; }
@@ -396,7 +419,7 @@ __global__ __launch_bounds__(kThr, (DkvShape<DT, DC, MASK, WHOLE>::kOccupancy)) 
             if (j && i_sub >= a.Tq) break;
             // none of the 32 queries sees the wave's keys: they are before them, or the mask hides them
             bool any = !a.causal || i_sub + 31 + off >= k0 + 32 * w;
-            if constexpr (MASK == kKeyMask) any = any && __any(!(term == -INFINITY));
+            if constexpr (by_key(MASK)) any = any && __any(!(term == -INFINITY));
             if (any) {
                 f32x16 s = zero16(), dp = zero16();
 #pragma unroll
@@ -409,18 +432,29 @@ __global__ __launch_bounds__(kThr, (DkvShape<DT, DC, MASK, WHOLE>::kOccupancy)) 
                     dp = mma<DT>(T::rows(gs, 32 * j, i, lane), v, dp);
                 }
                 const bool edge = i_sub < free_q;
+                const int sub = 32 * j + 4 * (lane >> 5);
+                // the rows' second numbers: for a full mask where one is not 0 (always: 8 x 1024 x 1024
+                // scores of 128 values 330 -> 403 us), by key always (where one is not 0, which
+                // takes registers of the whole loop: 8 x 777, 12 heads of 64 109 -> 120 us)
+                const bool apart = MASK == kFullMask && __builtin_amdgcn_readfirstlane(rest[t & 1]);
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    const float4 lse = *reinterpret_cast<const float4*>(&lt[t & 1][32 * j + 8 * g + 4 * (lane >> 5)]);
-                    const float4 del = *reinterpret_cast<const float4*>(&dt[t & 1][32 * j + 8 * g + 4 * (lane >> 5)]);
+                    const float4 lse = *reinterpret_cast<const float4*>(&lt[t & 1][sub + 8 * g]);
+                    const float4 del = *reinterpret_cast<const float4*>(&dt[t & 1][sub + 8 * g]);
                     const float ls[4] = {lse.x, lse.y, lse.z, lse.w}, ds[4] = {del.x, del.y, del.z, del.w};
+                    float4 second = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if constexpr (MASK == kKeyAdd) second = *reinterpret_cast<const float4*>(&rt[t & 1][sub + 8 * g]);
+                    const float rs[4] = {second.x, second.y, second.z, second.w};
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int i = 4 * g + e, q = i_sub + 8 * g + 4 * (lane >> 5) + e;
                         float f = term;   // by key: the lane's
                         if constexpr (MASK == kFullMask)
                             f = mask_term(a, mask_row(a, b, hq_now, q < a.Tq ? q : a.Tq - 1), kr);
-                        float x = __builtin_fmaf(s[i], c, MASK == kNoMask ? -ls[e] : f - ls[e]);
+                        float x = __builtin_fmaf(s[i], c, adds(MASK) ? f : MASK == kNoMask ? -ls[e] : f - ls[e]);
+                        if constexpr (adds(MASK)) x -= ls[e];
+                        if constexpr (MASK == kKeyAdd) x -= rs[e];
+                        if (apart) x -= rt[t & 1][sub + 8 * g + e];
                         if (edge) x = kr <= q + off ? x : -INFINITY;
                         s[i] = __builtin_amdgcn_exp2f(x);
                         dp[i] = s[i] * (dp[i] - ds[e]);
@@ -431,14 +465,8 @@ __global__ __launch_bounds__(kThr, (DkvShape<DT, DC, MASK, WHOLE>::kOccupancy)) 
                 fragments<DT>(dp, df);
                 T::accumulate(gs, 32 * j, s, pf, dv, lane);
                 T::accumulate(qs, 32 * j, dp, df, dk, lane);
-                if constexpr (WHOLE) {
-                    if (key >= a.Tk) {   // a copy of the last key, which dq must not add again
-                        const u32x4 none[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-                        S::put(scores, i_sub, key, zero16(), none, lane);
-                    } else {
-                        S::put(scores, i_sub, key, dp, df, lane);
-                    }
-                }
+                if constexpr (WHOLE)
+                    if (key < a.Tk) S::put(scores, i_sub, key, dp, df, lane);
             } else if constexpr (WHOLE) {
                 const u32x4 none[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
                 S::put(scores, i_sub, key, zero16(), none, lane);
@@ -469,7 +497,7 @@ __global__ __launch_bounds__(kThr, (DkvShape<DT, DC, MASK, WHOLE>::kOccupancy)) 
         for (uint64_t rows = __ballot(bad && lane < 32 && q < a.Tq); rows; rows &= rows - 1) {
             const int r = q0 + __builtin_ctzll(rows);
             const int64_t row = ((int64_t)b * a.Hq + head) * a.Tq + r;
-            dq_row<DT>(a, b, head, r, 0, a.Tk, 0, a.lse[row], a.delta[row], lane);
+            dq_row<DT>(a, b, head, r, 0, a.Tk, 0, a.stats[row], a.delta[row], lane);
         }
     };
     for (int t = first; t < tiles; ++t) {
@@ -540,7 +568,7 @@ void launch(const AttnArgs& a, hipStream_t st) {
 template <int DT, int DC>
 void pick(const AttnArgs& a, hipStream_t st) {
     if (!a.mask) launch<DT, DC, kNoMask>(a, st);
-    else if (a.ms[2] == 0) launch<DT, DC, kKeyMask>(a, st);
+    else if (a.ms[2] == 0) a.mask_type < 0 ? launch<DT, DC, kKeyMask>(a, st) : launch<DT, DC, kKeyAdd>(a, st);
     else launch<DT, DC, kFullMask>(a, st);
 }
 

@@ -4,8 +4,8 @@
 // With x_ij = scale q_i . k_j (and the mask), one pass over the keys keeps a
 // row's running maximum m and sum l = sum_j exp(x_ij - m) and rescales the
 // output when m grows; at the end o = sum_j exp(x_ij - m) v_j / l and
-// lse = m + log l, the one number a row's probabilities are made from again in
-// the backward.  A row that sees no key gives 0.
+// m and log l, from which the backward makes a row's probabilities again.  A row that
+// sees no key gives 0.
 //
 // Bound by the matrix cores (4 D operations a pair) and the exponentials
 // beside them.  A wave holds 32 queries in registers; S^T = K q^T puts a
@@ -66,8 +66,7 @@ __device__ void forward_row(const AttnArgs& a, int b, int hq, int q, int k0, int
     }
     const float rl = l == 0.0f ? 0.0f : 1.0f / l;
     store_two<DT>(a.o, (((int64_t)b * a.Tq + q) * a.Hq + hq) * a.D, {o.x * rl, o.y * rl}, a.D, lane);
-    if (a.lse && lane == 0)
-        a.lse[((int64_t)b * a.Hq + hq) * a.Tq + q] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
+    if (a.stats && lane == 0) a.stats[((int64_t)b * a.Hq + hq) * a.Tq + q] = row_stats(m, l);
 }
 
 // The forms of the kernel: four waves; eight that hold twice the queries; two
@@ -258,8 +257,7 @@ attn_fwd_kernel(AttnArgs a) {
             const float rl = l == 0.0f ? 0.0f : 1.0f / l;
             const int64_t row = (((int64_t)b * a.Tq + q) * a.Hq + hq) * a.D;
             T::template store<DT>(a.o, row, o, rl, a.D, lane);
-            if (a.lse && lane < 32)
-                a.lse[((int64_t)b * a.Hq + hq) * a.Tq + q] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
+            if (a.stats && lane < 32) a.stats[((int64_t)b * a.Hq + hq) * a.Tq + q] = row_stats(m, l);
         }
     }
     for (uint64_t rows = __ballot(bad && lane < 32 && q < a.Tq); rows; rows &= rows - 1)
@@ -281,7 +279,7 @@ __global__ __launch_bounds__(kJoinThreads) void attn_join_kernel(AttnArgs a) {
     if (j.d < 0) return;
     const int64_t bh = row / a.Tq;
     const int q = (int)(row - bh * a.Tq);
-    if (a.lse && j.d == 0) a.lse[row] = j.l == 0.0f ? INFINITY : j.m + __builtin_amdgcn_logf(j.l);
+    if (a.stats && j.d == 0) a.stats[row] = row_stats(j.m, j.l);
     const float rl = j.l == 0.0f ? 0.0f : 1.0f / j.l;
     auto* out = reinterpret_cast<typename E::S*>(a.o) + (((bh / a.Hq) * a.Tq + q) * a.Hq + bh % a.Hq) * a.D + j.d;
 #pragma unroll
@@ -427,7 +425,7 @@ extern "C" int axs6_attention_forward(const void* q, const void* k, const void* 
                                       int64_t Tk, int64_t Hq, int64_t H, int64_t D, const int64_t* q_strides,
                                       const int64_t* k_strides, const int64_t* v_strides, const void* mask,
                                       int32_t mask_type, const int64_t* mask_strides, int32_t causal, float scale,
-                                      void* out, float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
+                                      void* out, float* stats, void* workspace, int64_t workspace_bytes, void* stream) {
     const char* fn = "axs6_attention_forward";
     AttnArgs a{};
     int rc = fill(fn, a, dtype, B, Tq, Tk, Hq, H, D, mask, mask_type, mask_strides, causal, scale);
@@ -437,7 +435,8 @@ extern "C" int axs6_attention_forward(const void* q, const void* k, const void* 
     if (Tk && ((rc = operand(fn, "k", k, k_strides, dtype, a.ks)) || (rc = operand(fn, "v", v, v_strides, dtype, a.vs))))
         return rc;
     if (!out || (uintptr_t)out % 16) return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: output null or not aligned", fn);
-    a.q = q; a.k = k; a.v = v; a.o = out; a.lse = lse;
+    if ((uintptr_t)stats % 8) return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: stats not aligned to 8 bytes", fn);
+    a.q = q; a.k = k; a.v = v; a.o = out; a.stats = reinterpret_cast<float2*>(stats);
     a.splits = forward_splits(B, Tq, Tk, Hq);
     const int64_t need = axs6_attention_forward_workspace(B, Tq, Tk, Hq, D);
     if ((rc = scratch(fn, workspace, workspace_bytes, need))) return rc;
@@ -451,7 +450,7 @@ extern "C" int axs6_attention_forward(const void* q, const void* k, const void* 
 }
 
 extern "C" int axs6_attention_backward(const void* dout, const void* q, const void* k, const void* v, const void* out,
-                                       const float* lse, int32_t dtype, int64_t B, int64_t Tq, int64_t Tk, int64_t Hq,
+                                       const float* stats, int32_t dtype, int64_t B, int64_t Tq, int64_t Tk, int64_t Hq,
                                        int64_t H, int64_t D, const int64_t* dout_strides, const int64_t* q_strides,
                                        const int64_t* k_strides, const int64_t* v_strides, const void* mask,
                                        int32_t mask_type, const int64_t* mask_strides, int32_t causal, float scale,
@@ -469,11 +468,13 @@ extern "C" int axs6_attention_backward(const void* dout, const void* q, const vo
         return rc;
     if (Tk && ((rc = operand(fn, "k", k, k_strides, dtype, a.ks)) || (rc = operand(fn, "v", v, v_strides, dtype, a.vs))))
         return rc;
-    if ((Tq && (!lse || !delta || !dq)) || (Tk && (!dk || !dv)))
-        return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: null lse, delta or gradient", fn);
+    if ((Tq && (!stats || !delta || !dq)) || (Tk && (!dk || !dv)))
+        return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: null stats, delta or gradient", fn);
+    if ((uintptr_t)stats % 8) return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: stats not aligned to 8 bytes", fn);
     if ((uintptr_t)dq % 16 || (uintptr_t)dk % 16 || (uintptr_t)dv % 16)
         return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: gradients not aligned to 16 bytes", fn);
-    a.q = q; a.k = k; a.v = v; a.out = out; a.dout = dout; a.lse = const_cast<float*>(lse); a.delta = delta;
+    a.q = q; a.k = k; a.v = v; a.out = out; a.dout = dout; a.delta = delta;
+    a.stats = reinterpret_cast<float2*>(const_cast<float*>(stats));
     a.dq = dq; a.dk = dk; a.dv = dv;
     a.splits = forward_splits(B, Tq, Tk, Hq);
     a.splits_kv = key_splits(B, Tq, Tk, Hq, H, causal);

@@ -182,20 +182,20 @@ Mask mask_of(const at::Tensor& t, int64_t B, int64_t Hq, int64_t Tq, int64_t Tk)
     return m;
 }
 
-// The kernels' out and lse of operands of whole vectors.
+// The kernels' out and, for the backward, row statistics of operands of whole vectors.
 std::pair<at::Tensor, at::Tensor> attention_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-                                                const at::Tensor& mask, bool causal, double scale, bool lse) {
+                                                const at::Tensor& mask, bool causal, double scale, bool stats) {
     const int64_t B = q.size(0), Tq = q.size(1), Hq = q.size(2), D = q.size(3), Tk = k.size(1), H = k.size(2);
     const Mask m = mask_of(mask, B, Hq, Tq, Tk);
     at::Tensor out = at::empty({B, Tq, Hq, D}, q.options());
-    at::Tensor l = lse ? at::empty({B, Hq, Tq}, q.options().dtype(at::kFloat)) : at::Tensor();
+    at::Tensor st = stats ? at::empty({B, Hq, Tq, 2}, q.options().dtype(at::kFloat)) : at::Tensor();
     const at::Tensor ws = workspace(axs6_attention_forward_workspace(B, Tq, Tk, Hq, D), q);
     check_rc(axs6_attention_forward(q.data_ptr(), k.data_ptr(), v.data_ptr(), dtype_code(q.scalar_type()), B, Tq, Tk, Hq,
                                     H, D, q.strides().data(), k.strides().data(), v.strides().data(), m.data(), m.type,
                                     m.strides, causal, (float)scale, out.data_ptr(),
-                                    lse ? l.data_ptr<float>() : nullptr, data_of(ws), size_of(ws), stream_of(q)),
+                                    stats ? st.data_ptr<float>() : nullptr, data_of(ws), size_of(ws), stream_of(q)),
              "axs6_attention_forward");
-    return {out, l};
+    return {out, st};
 }
 
 struct AttentionFunction : public torch::autograd::Function<AttentionFunction> {
@@ -203,8 +203,8 @@ struct AttentionFunction : public torch::autograd::Function<AttentionFunction> {
                               const at::Tensor& mask, bool has_mask, bool causal, double scale) {
         c10::DeviceGuard guard(q.device());
         const at::Tensor qv = vectors(q), kv = vectors(k), vv = vectors(v), m = has_mask ? mask : at::Tensor();
-        auto [out, lse] = attention_fwd(qv, kv, vv, m, causal, scale, true);
-        ctx->save_for_backward({qv, kv, vv, out, lse, m});
+        auto [out, stats] = attention_fwd(qv, kv, vv, m, causal, scale, true);
+        ctx->save_for_backward({qv, kv, vv, out, stats, m});
         auto& d = ctx->saved_data;
         d["causal"] = causal;
         d["scale"] = scale;
@@ -217,18 +217,18 @@ struct AttentionFunction : public torch::autograd::Function<AttentionFunction> {
         if (!grads[0].defined()) return r;
         const auto s = ctx->get_saved_variables();
         auto& d = ctx->saved_data;
-        const at::Tensor &q = s[0], &k = s[1], &v = s[2], &out = s[3], &lse = s[4];
+        const at::Tensor &q = s[0], &k = s[1], &v = s[2], &out = s[3], &stats = s[4];
         const int64_t B = q.size(0), Tq = q.size(1), Hq = q.size(2), D = q.size(3), Tk = k.size(1), H = k.size(2);
         const int64_t D0 = d["D"].toInt();
         c10::DeviceGuard guard(q.device());
         const at::Tensor g = vectors(grads[0].to(q.scalar_type()));
         const Mask m = mask_of(s[5], B, Hq, Tq, Tk);
         at::Tensor dq = at::empty({B, Tq, Hq, D}, q.options()), dk = at::empty({B, Tk, H, D}, q.options());
-        at::Tensor dv = at::empty({B, Tk, H, D}, q.options()), delta = at::empty_like(lse);
+        at::Tensor dv = at::empty({B, Tk, H, D}, q.options()), delta = at::empty({B, Hq, Tq}, stats.options());
         const bool causal = d["causal"].toBool();
         const at::Tensor ws = workspace(axs6_attention_backward_workspace(B, Tq, Tk, Hq, H, D, causal), q);
         check_rc(axs6_attention_backward(
-                     g.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr<float>(),
+                     g.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), stats.data_ptr<float>(),
                      dtype_code(q.scalar_type()), B, Tq, Tk, Hq, H, D, g.strides().data(), q.strides().data(),
                      k.strides().data(), v.strides().data(), m.data(), m.type, m.strides, causal,
                      (float)d["scale"].toDouble(), delta.data_ptr<float>(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),

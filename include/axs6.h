@@ -409,9 +409,10 @@ int axs6_rotary(const void* q, const void* k, void* q_out, void* k_out, int32_t 
  *   head, query, key) in elements, 0 for a broadcast dim;
  *   a query that sees no key gives 0, and no gradient.
  * D <= AXS6_ATTENTION_MAX_HEAD, token strides below AXS6_ATTENTION_MAX_TOKEN_STRIDE, D, every stride and pointer whole 16-byte vectors, a
- * head's values adjacent; out and the gradients contiguous.  lse (B, Hq, Tq)
- * floats is written by the forward (may be NULL there) and read by the
- * backward, which overwrites delta (B, Hq, Tq) floats.  Products run on the
+ * head's values adjacent; out and the gradients contiguous.  stats (B, Hq, Tq, 2)
+ * floats, aligned to 8 bytes, is written by the forward (may be NULL there) and
+ * read by the backward: y, z of which a probability is exp2((x - y) - z), x the score
+ * in units of log2 (y = +inf for a query that sees no key).  The backward overwrites delta (B, Hq, Tq) floats.  Products run on the
  * matrix cores in the operands' type with float32 sums; no atomics, fixed
  * orders.  scale positive and finite.  Each direction needs its query's bytes
  * of workspace, 16-byte aligned (0: none): partial sums where few workgroups
@@ -422,12 +423,12 @@ int64_t axs6_attention_forward_workspace(int64_t B, int64_t Tq, int64_t Tk, int6
 int axs6_attention_forward(const void* q, const void* k, const void* v, int32_t dtype, int64_t B, int64_t Tq,
                            int64_t Tk, int64_t Hq, int64_t Hkv, int64_t D, const int64_t* q_strides,
                            const int64_t* k_strides, const int64_t* v_strides, const void* mask, int32_t mask_type,
-                           const int64_t* mask_strides, int32_t causal, float scale, void* out, float* lse,
+                           const int64_t* mask_strides, int32_t causal, float scale, void* out, float* stats,
                            void* workspace, int64_t workspace_bytes, void* stream);
 int64_t axs6_attention_backward_workspace(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hkv, int64_t D,
                                           int32_t causal);
 int axs6_attention_backward(const void* dout, const void* q, const void* k, const void* v, const void* out,
-                            const float* lse, int32_t dtype, int64_t B, int64_t Tq, int64_t Tk, int64_t Hq,
+                            const float* stats, int32_t dtype, int64_t B, int64_t Tq, int64_t Tk, int64_t Hq,
                             int64_t Hkv, int64_t D, const int64_t* dout_strides, const int64_t* q_strides,
                             const int64_t* k_strides, const int64_t* v_strides, const void* mask, int32_t mask_type,
                             const int64_t* mask_strides, int32_t causal, float scale, float* delta, void* dq,

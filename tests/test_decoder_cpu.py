@@ -131,3 +131,12 @@ def test_rotary_table_by_parts(rotary_dim, original, base):
     between = (i > low) & (i < high)
     assert (kept - (i - low) / max(high - low, 1))[between].abs().le(1e-5).all()
     assert not ((kept > 1 - 1e-5) & (turns > 1) & (i < high)).any()
+
+
+def test_row_statistics_are_aligned():
+    L = _lib.lib()
+    st = ctypes.cast(_i64(256, 64, 64, 1), ctypes.c_void_p)
+    p, half = 4096, 4100
+    assert L.axs6_attention_forward(p, p, p, 0, 1, 4, 4, 2, 1, 64, st, st, st, None, 0, None, 0, 0.1, p, half, None, 0, None) == 1
+    assert L.axs6_attention_backward(p, p, p, p, p, half, 0, 1, 4, 4, 2, 1, 64, st, st, st, st, None, 0, None, 0, 0.1, p, p, p,
+                                     p, p, 1 << 20, None) == 1

@@ -361,3 +361,50 @@ def test_tokens_that_overlap_in_memory(Tq, Tk, causal, dtype):
     mem = torch.randn(B, H, Tk * step + D, generator=torch.Generator().manual_seed(4)).to(DEV, dtype)
     near = mem.as_strided((B, Tk, H, D), (mem.stride(0), step, mem.stride(1), 1))
     _check(q, near, near, go, causal=causal)
+
+
+def _low_rows(B, Hq, Tq, Tk, by_key, low):
+    """An additive mask whose row 3 (by key: every row of sequence 1) carries `low` on all keys, and which of the
+    (B, Tq) rows those are."""
+    add = torch.zeros(B, 1, 1 if by_key else Tq, Tk)
+    rows = torch.zeros(B, Tq, dtype=torch.bool)
+    if by_key:
+        add[1], rows[1] = low, True
+    else:
+        add[:, :, 3], rows[:, 3] = low, True
+    return add, rows
+
+
+@pytest.mark.parametrize("dtype", ref.DTYPES)
+@pytest.mark.parametrize("low", [-1e9, torch.finfo(torch.float32).min])
+@pytest.mark.parametrize("by_key", [False, True])
+@pytest.mark.parametrize("B,Tq,Tk,Hq,H,D", [(2, 70, 100, 2, 1, 64), (2, 70, 100, 2, 1, 128), (2, 300, 200, 2, 2, 64),
+                                            (2, 6, 2100, 2, 2, 64), (2, 700, 100, 4, 1, 96)])
+def test_gradients_of_rows_of_large_finite_mask_values(B, Tq, Tk, Hq, H, D, by_key, low, dtype):
+    """Beside such a value the scores vanish: the row's keys have equal probabilities, forward and backward.  The
+    operands' sizes: one workgroup a head, several, the keys split, the queries split."""
+    from axs.unified import axs_attention_unified
+
+    q, k, v, go = _inputs(B, Tq, Tk, Hq, H, D, dtype)
+    add, rows = _low_rows(B, Hq, Tq, Tk, by_key, low)
+    xs = [x.requires_grad_(True) for x in (q, k, v)]
+    out = axs_attention_unified(*xs, add.to(DEV))
+    got = (out.detach(), *torch.autograd.grad(out, xs, go))
+    q, k, v, go = (x.detach().double().cpu() for x in (q, k, v, go))
+    want = [torch.zeros_like(x) for x in (q, q, k, v)]
+    for b in range(B):
+        for h in range(Hq):
+            g, scale = h // (Hq // H), 1 / math.sqrt(D)
+            x = q[b, :, h] @ k[b, :, g].T * scale
+            p = torch.softmax(torch.where(rows[b, :, None], 0.0, x), -1)
+            dp = go[b, :, h] @ v[b, :, g].T
+            ds = p * (dp - (p * dp).sum(-1, keepdim=True)) * scale
+            for i, y in enumerate((p @ v[b, :, g], ds @ k[b, :, g])):
+                want[i][b, :, h] = y
+            want[2][b, :, g] += ds.T @ q[b, :, h]
+            want[3][b, :, g] += p.T @ go[b, :, h]
+    fwd, bwd = _bounds(dtype)
+    for i, (x, y) in enumerate(zip(got, want)):
+        assert ref.rel(x, y) <= (bwd if i else fwd), "o dq dk dv".split()[i]
+        if i < 2:    # the rows by themselves
+            assert ref.rel(x[rows.to(DEV)], y[rows]) <= (bwd if i else fwd), "o dq".split()[i]
