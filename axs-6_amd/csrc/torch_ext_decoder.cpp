@@ -45,9 +45,19 @@ at::Tensor vectors(const at::Tensor& t) {
     const int64_t v = vec_multiple(t.scalar_type()), d = t.size(3), pad = (v - d % v) % v;
     if (pad) return at::constant_pad_nd(t, {0, pad});
     if (t.numel() == 0) return t;
-    const bool ok = t.stride(3) == 1 && t.stride(1) < AXS6_ATTENTION_MAX_TOKEN_STRIDE && t.stride(0) % v == 0 && t.stride(1) % v == 0 && t.stride(2) % v == 0;
-    if (!ok) return t.contiguous();
-    return aligned(t) ? t : t.clone(at::MemoryFormat::Contiguous);
+    // a dim of one element is never walked: its stride may be anything, and the kernels get d
+    bool ok = t.stride(3) == 1, same = true;
+    std::vector<int64_t> strides = t.strides().vec();
+    for (int i = 0; i < 3; ++i) {
+        if (t.size(i) == 1) {
+            same = same && strides[i] % v == 0 && strides[i] < AXS6_ATTENTION_MAX_TOKEN_STRIDE;
+            strides[i] = d;
+        }
+        ok = ok && strides[i] % v == 0;
+    }
+    if (!ok || strides[1] >= AXS6_ATTENTION_MAX_TOKEN_STRIDE) return t.contiguous();
+    if (!aligned(t)) return t.clone(at::MemoryFormat::Contiguous);
+    return same ? t : t.as_strided(t.sizes(), strides);
 }
 
 at::Tensor int64s(const at::Tensor& t, at::IntArrayRef shape, const at::Tensor& like, const char* fn, const char* name) {

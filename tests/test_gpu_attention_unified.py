@@ -408,3 +408,22 @@ def test_gradients_of_rows_of_large_finite_mask_values(B, Tq, Tk, Hq, H, D, by_k
         assert ref.rel(x, y) <= (bwd if i else fwd), "o dq dk dv".split()[i]
         if i < 2:    # the rows by themselves
             assert ref.rel(x[rows.to(DEV)], y[rows]) <= (bwd if i else fwd), "o dq".split()[i]
+
+
+@pytest.mark.parametrize("dtype", ref.DTYPES)
+def test_one_sequence_or_token_of_an_unaligned_batch(dtype):
+    """A dim of one element may have any stride: it is never walked."""
+    q, k, v, go = _inputs(1, 1, 5, 2, 2, 64, dtype)
+    want, grads = _check(q, k, v, go)
+
+    def odd(x, dim):    # x with a stride of 1 along a dim of one element
+        strides = list(x.stride())
+        strides[dim] = 1
+        return x.as_strided(x.shape, strides)
+
+    for qq, kk, vv, gg in ((odd(q, 0), odd(k, 0), odd(v, 0), odd(go, 0)), (odd(q, 1), k, v, odd(go, 1))):
+        out, got = _check(qq, kk, vv, gg)
+        assert torch.equal(out, want) and all(torch.equal(x, y) for x, y in zip(got, grads))
+    batch = torch.randn(2, 5 * 2 * 64 + 1, generator=torch.Generator().manual_seed(1)).to(DEV, dtype)
+    one = batch[:, :-1].unflatten(-1, (5, 2, 64))[:1]
+    _check(q, one, one, go)
