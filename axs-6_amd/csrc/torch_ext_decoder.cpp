@@ -19,7 +19,11 @@ using OptTensor = std::optional<at::Tensor>;
 
 bool given(const OptTensor& t) { return t && t->defined(); }
 
-bool records(const at::Tensor& t) { return t.defined() && t.requires_grad(); }
+// Whether a call on t goes through its autograd node: for a gradient, or for a forward-mode
+// tangent, which the node refuses (there is no such derivative) and no call may drop.
+bool records(const at::Tensor& t) {
+    return t.defined() && ((at::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(0).defined());
+}
 
 void check_dtype(const at::Tensor& t, const char* fn, const char* name) {
     TORCH_CHECK(dtype_code(t.scalar_type()) >= 0, fn, ": ", name, " has dtype ", t.scalar_type(),
@@ -162,7 +166,7 @@ py::object rotary(const at::Tensor& q, const OptTensor& k, const at::Tensor& tab
     } else {
         TORCH_CHECK(T <= tab.size(0), fn, ": ", T, " tokens for a table of ", tab.size(0), " positions");
     }
-    if (at::GradMode::is_enabled() && (records(q) || (given(k) && records(*k)))) {
+    if (records(q) || (given(k) && records(*k))) {
         // absent tensors travel as empty ones: the node records every argument's device
         const at::Tensor none = at::empty({0}, q.options());
         variable_list r = RotaryFunction::apply(q, given(k) ? *k : none, tab, pos.defined() ? pos : none, interleaved,
@@ -280,7 +284,7 @@ at::Tensor attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor&
                     Tk, ")");
     }
     const at::Tensor m = given(mask) ? *mask : at::Tensor();
-    if (at::GradMode::is_enabled() && (records(q) || records(k) || records(v)))
+    if (records(q) || records(k) || records(v))
         return AttentionFunction::apply(q, k, v, m.defined() ? m : at::empty({0}, q.options()), m.defined(), causal, s);
     c10::DeviceGuard guard(q.device());
     at::Tensor out = attention_fwd(vectors(q), vectors(k), vectors(v), m, causal, s, false).first;

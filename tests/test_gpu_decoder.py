@@ -133,3 +133,25 @@ def _is_its_parts(m, gradients=True):
         axu.axs_cache_append_unified(other, k, v, starts)
         want = m.out_proj(axu.axs_cache_attention_unified(q, other, starts + 40).flatten(2))
     assert torch.equal(out, want)
+
+
+def test_forward_mode_tangents_raise():
+    """The operators have no forward-mode derivative: a tangent raises, as in the linear, and is never dropped."""
+    import torch.autograd.forward_ad as fwd
+    from axs.unified import axs_attention_unified, axs_distillation_loss_unified, axs_rotary_unified, rotary_table
+
+    x = torch.randn(1, 8, 2, 16, device=DEV)
+    table = rotary_table(16, 8, device=DEV)
+    z, t, i = torch.randn(4, 10, device=DEV), torch.randn(4, 2, device=DEV), torch.zeros(4, 2, dtype=torch.int64, device=DEV)
+    with fwd.dual_level():
+        d = fwd.make_dual(x, torch.ones_like(x))
+        for call in (lambda: axs_rotary_unified(d, x, table), lambda: axs_rotary_unified(x, d, table),
+                     lambda: axs_rotary_unified(d, None, table), lambda: axs_attention_unified(d, x, x),
+                     lambda: axs_attention_unified(x, d, x), lambda: axs_attention_unified(x, x, d),
+                     lambda: axs_distillation_loss_unified(fwd.make_dual(z, torch.ones_like(z)), t, i)):
+            with pytest.raises(RuntimeError, match="jvp"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="jvp"):
+                call()
+        # without a tangent nothing changes
+        assert axs_rotary_unified(x, x, table)[0].shape == x.shape and axs_attention_unified(x, x, x).shape == x.shape
