@@ -327,6 +327,7 @@ __global__ __launch_bounds__(kJoinThreads) void kv_join_kernel(KvAttnArgs a) {
 
 // How a call is laid out: 16-row pieces a wave takes, workgroups of 8 waves or 4,
 // workgroups that share a set of rows.
+constexpr int64_t kMaxPartial = (int64_t)64 << 20;   // bytes of partial sums that splits by length may take
 struct Plan {
     int nr, waves, row_tiles, splits;
 };
@@ -344,6 +345,12 @@ Plan plan(int64_t BH, int64_t rows, int64_t D, int64_t blocks) {
     // sequences of unequal length (64 sequences to 16383 tokens: 2048 workgroups
     // 280 us, 1024 298; 1 x 131072: 512 workgroups 50 us, 1024 55).
     int64_t s = (512 + groups - 1) / (groups > 0 ? groups : 1), by_length = (blocks + 127) / 128;
+    // The capacity is known here, the lengths are not: splits by it cost a prompt, whose rows
+    // are many, most where it is short.  Their partial sums stay within 64 MiB, which
+    // generation does not reach (1 x 4096 tokens, 32 heads on 8 of 128, a cache of 16384: 693 us
+    // and 260 MiB of partial sums, now 453 and none).
+    const int64_t bytes = BH * rows * (D + 2) * (int64_t)sizeof(float), most = kMaxPartial / (bytes > 0 ? bytes : 1);
+    by_length = by_length < most ? by_length : most;
     s = s > by_length ? s : by_length;
     s = s < blocks / 4 ? s : blocks / 4;
     s = s < kMaxSplits ? s : kMaxSplits;

@@ -140,3 +140,13 @@ def test_row_statistics_are_aligned():
     assert L.axs6_attention_forward(p, p, p, 0, 1, 4, 4, 2, 1, 64, st, st, st, None, 0, None, 0, 0.1, p, half, None, 0, None) == 1
     assert L.axs6_attention_backward(p, p, p, p, p, half, 0, 1, 4, 4, 2, 1, 64, st, st, st, st, None, 0, None, 0, 0.1, p, p, p,
                                      p, p, 1 << 20, None) == 1
+
+
+@pytest.mark.parametrize("B,Tq,Hq,H,D", [(1, 4096, 32, 8, 128), (1, 16384, 32, 8, 128), (4, 512, 32, 8, 128), (1, 100, 8, 1, 256),
+                                         (64, 1, 64, 8, 128), (1, 1, 32, 8, 128), (8, 5, 64, 8, 128), (1, 1 << 20, 8, 8, 64)])
+@pytest.mark.parametrize("capacity", [512, 16384, 131072, 1 << 20])
+def test_cache_attention_workspace_stays_small(B, Tq, Hq, H, D, capacity):
+    """Partial sums of a long prompt do not grow with the cache's capacity."""
+    rows = B * Tq * Hq * (D + 2) * 4        # bytes of one split's
+    need = _lib.lib().axs6_kv_attention_workspace(B, Tq, Hq, H, D, capacity // 32)
+    assert need % rows == 0 and need <= 64 << 20
