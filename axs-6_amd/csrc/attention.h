@@ -27,6 +27,7 @@ struct AttnArgs {
     int64_t qs[3], ks[3], vs[3], os[3], gs[3];   // strides of batch, token, head (q, k, v, out, dout)
     float2* stats;                     // (B, Hq, Tq): row_stats
     float* delta;                      // (B, Hq, Tq)
+    float2* bounds;                    // (B, Hq, Tq / 32 rounded up): 32 queries' largest |do| and |delta| (float16)
     // Splits of the walked axis and their partial results: of the forward each
     // row's sums, maximum and sum; of the backward dq, and dk and dv.
     int splits, splits_kv;

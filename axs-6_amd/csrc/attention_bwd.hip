@@ -29,6 +29,46 @@ namespace {
 
 constexpr int kWaves = 4, kThr = 64 * kWaves, kHeld = 32 * kWaves;
 
+// float16 has 2^-14 as its smallest normal value and 65504 as its largest: probabilities
+// and score gradients go into their products times a power of two, which costs nothing
+// inside the loops and is undone with the results' factors.
+//  * dq: a query's score gradients times 2^4 / |do_i| (the power of two below), which
+//    p 2^-18 keeps normal beside values of 1, and values of norm 4096 in range.
+//  * dk, dv: both times 2^e, e in 0 .. 15 and as large as leaves ds_ij, at most
+//    p (|do_i| |v_j| + |delta_i|), below 2^15 for the keys held and all queries of the
+//    group; the first launch leaves their largest |do| and |delta|.  e goes into the rows' y.
+//    (A scale that follows the largest ds so far: 2 x 4096, 32 heads on 8, 1065 -> 1420 us.)
+//  * Up to 128 keys (the form of one workgroup a head): as they are, p is large enough.
+// 4096 keys, do of 1e-4: dq off by 5e-2 without, 7e-3, its own rounding, with.
+// A larger ds still overflows, and its rows are made again.  The other types have
+// float32's range and no scale.
+__device__ __forceinline__ float row_scale(float norm2) {
+    return norm2 > 0.0f && norm2 < INFINITY ? ldexpf(1.0f, 4 - (__builtin_amdgcn_frexp_expf(norm2) >> 1)) : 1.0f;
+}
+__device__ __forceinline__ float finite_or_0(float x) { return fabsf(x) < INFINITY ? x : 0.0f; }
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) x = fmaxf(x, __shfl_xor(x, o, 64));
+    return x;
+}
+__device__ __forceinline__ int64_t bound_at(const AttnArgs& a, int b, int hq, int q) {
+    return ((int64_t)b * a.Hq + hq) * ((a.Tq + 31) >> 5) + (q >> 5);
+}
+// |x|^2 of rows in fragments, the lane's row is l % 32
+template <int DT, int N>
+__device__ __forceinline__ float norm2(const u32x4 (&f)[N]) {
+    constexpr int V = 16 / kElemBytes<DT>;
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        float x[V];
+        Elem<DT>::unpack(f[i], x);
+#pragma unroll
+        for (int j = 0; j < V; ++j) s += x[j] * x[j];
+    }
+    return s + __shfl_xor(s, 32, 64);
+}
+
 // dq of a query from the keys k0 .. k1 - 1 that it sees, one by one.
 template <int DT>
 __device__ void dq_row(const AttnArgs& a, int b, int hq, int q, int k0, int k1, int split, float2 st, float delta,
@@ -167,6 +207,15 @@ __global__ __launch_bounds__(kThr, (DqShape<DT, DC>::kOccupancy)) void attn_dq_k
     f32x16 dq[T::kResults];
 #pragma unroll
     for (int d = 0; d < T::kResults; ++d) dq[d] = zero16();
+    float rs = 1.0f;   // the scale of the row's score gradients
+    if constexpr (DT == AXS6_F16) {
+        const float g2 = norm2<DT>(gf);
+        rs = row_scale(g2);
+        const bool here = lane < 32 && q < a.Tq;
+        const float g = sqrtf(wave_max(here ? finite_or_0(g2) : 0.0f)), d = wave_max(here ? fabsf(finite_or_0(delta)) : 0.0f);
+        if (lane == 0 && q < a.Tq && split == 0) a.bounds[bound_at(a, b, hq, q)] = make_float2(g, d);
+    }
+    const float delta_s = delta * rs;
     const bool rows_here = q0 + 32 * w < a.Tq;
     const int w_last = q0 + 32 * w + 31 < a.Tq ? q0 + 32 * w + 31 : a.Tq - 1;   // the wave's last row and its keys
     const int w_keys = a.causal && w_last + off + 1 < a.Tk ? w_last + off + 1 : a.Tk;
@@ -208,7 +257,7 @@ __global__ __launch_bounds__(kThr, (DqShape<DT, DC>::kOccupancy)) void attn_dq_k
                     for (int i = 0; i < 16; ++i) s[i] -= st.y;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    s[i] = __builtin_amdgcn_exp2f(s[i]) * (dp[i] - delta);
+                    s[i] = __builtin_amdgcn_exp2f(s[i]) * (DT == AXS6_F16 ? __builtin_fmaf(dp[i], rs, -delta_s) : dp[i] - delta);
                 }
                 u32x4 pf[2];
                 fragments<DT>(s, pf);
@@ -222,8 +271,8 @@ __global__ __launch_bounds__(kThr, (DqShape<DT, DC>::kOccupancy)) void attn_dq_k
     const int64_t out = (((int64_t)b * a.Tq + qr) * a.Hq + hq) * a.D;
     if (q < a.Tq) {
         float* part = a.part + split * ((int64_t)a.B * a.Tq * a.Hq * a.D);
-        if (a.splits > 1) T::template store<AXS6_F32>(part, out, dq, a.scale, a.D, lane);
-        else T::template store<DT>(a.dq, out, dq, a.scale, a.D, lane);
+        if (a.splits > 1) T::template store<AXS6_F32>(part, out, dq, a.scale / rs, a.D, lane);
+        else T::template store<DT>(a.dq, out, dq, a.scale / rs, a.D, lane);
     }
     for (uint64_t rows = __ballot(bad && lane < 32 && q < a.Tq); rows; rows &= rows - 1) {
         const int r = __builtin_ctzll(rows);
@@ -294,6 +343,8 @@ __global__ __launch_bounds__(kThr, (DkvShape<DT, DC, MASK, WHOLE>::kOccupancy)) 
     // the rows' second numbers, and whether one of them is not 0
     __shared__ __attribute__((aligned(16))) float rt[2][adds(MASK) ? kWalk : 4];
     __shared__ int rest[2];
+    constexpr bool kScaled = DT == AXS6_F16 && !WHOLE;
+    __shared__ float4 largest[kScaled ? kWaves : 1];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int k_tiles = (a.Tk + kHeld - 1) / kHeld;
     int bh, piece;
@@ -330,6 +381,7 @@ __global__ __launch_bounds__(kThr, (DkvShape<DT, DC, MASK, WHOLE>::kOccupancy)) 
     // head and first query of the tile on its way
     int hq = h * a.G + (per_head ? first / per_head : 0), i0 = q_first + (per_head ? first % per_head : 0) * kWalk;
     float sl = 0.0f, sr = 0.0f, sd = 0.0f;
+    float e = 0.0f;   // probabilities and score gradients are 2^e of themselves
     // WHOLE: out and dout of the tile's rows, eight threads a row, for its delta
     constexpr int N = DC / 8 / T::kVals;
     u32x4 xo[N], xg[N];
@@ -361,6 +413,11 @@ __global__ __launch_bounds__(kThr, (DkvShape<DT, DC, MASK, WHOLE>::kOccupancy)) 
         }
     };
     auto store = [&](int buf) {
+        if constexpr (kScaled) {
+            // see row_stats: a large y has no place for e
+            if (adds(MASK) && fabsf(sl) >= 128.0f && sl != INFINITY) sr -= e;
+            else sl -= e;
+        }
         if (threadIdx.x < kWalk) {
             lt[buf][threadIdx.x] = sl;
             if constexpr (adds(MASK)) {
@@ -389,7 +446,36 @@ __global__ __launch_bounds__(kThr, (DkvShape<DT, DC, MASK, WHOLE>::kOccupancy)) 
         }
     };
     if (first < tiles) {
-        load(qt[first & 1], gt[first & 1]);
+        if constexpr (kScaled) {
+            // the largest |v| held, |do| and |delta| of the group's queries: on their way before the tiles
+            const int n = (a.Tq + 31) >> 5, from = q_first >> 5, all = (n - from) * a.G;
+            auto bound = [&](int i) {
+                return i < all ? a.bounds[bound_at(a, b, h * a.G + i / (n - from), (from + i % (n - from)) * 32)]
+                               : make_float2(0.0f, 0.0f);
+            };
+            u32x4 rows[T::kSteps];
+            load_rows<DT, DC>(rows, a.v, b * a.vs[0] + kr * a.vs[1] + h * a.vs[2], a.D, lane);
+            const float2 x = bound(threadIdx.x);
+            load(qt[first & 1], gt[first & 1]);
+            float3 m = make_float3(finite_or_0(norm2<DT>(rows)), x.x, x.y);
+            for (int i = threadIdx.x + kThr; i < all; i += kThr) {
+                const float2 y = bound(i);
+                m.y = fmaxf(m.y, y.x);
+                m.z = fmaxf(m.z, y.y);
+            }
+            m = make_float3(wave_max(m.x), wave_max(m.y), wave_max(m.z));
+            if (lane == 0) largest[w] = make_float4(m.x, m.y, m.z, 0.0f);
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < kWaves; ++i) {
+                const float4 x = largest[i];
+                m = make_float3(fmaxf(m.x, x.x), fmaxf(m.y, x.y), fmaxf(m.z, x.z));
+            }
+            e = (float)(15 - __builtin_amdgcn_frexp_expf(m.y * sqrtf(m.x) + m.z));
+            e = fminf(fmaxf(e, 0.0f), 15.0f);
+        } else {
+            load(qt[first & 1], gt[first & 1]);
+        }
         store(first & 1);
     }
     if constexpr (WHOLE)   // lanes past the last key hold a copy of it, which dq must not add again
@@ -508,14 +594,15 @@ __global__ __launch_bounds__(kThr, (DkvShape<DT, DC, MASK, WHOLE>::kOccupancy)) 
             if (hq != head) queries(head);
     }
     const bool bad = not_finite(dk) || not_finite(dv);
+    const float fv = kScaled ? ldexpf(1.0f, -(int)e) : 1.0f, fk = a.scale * fv;
     if (key < a.Tk) {
         const int64_t out = (((int64_t)b * a.Tk + key) * a.H + h) * a.D, all = (int64_t)a.B * a.Tk * a.H * a.D;
         if (a.splits_kv > 1) {
-            T::template store<AXS6_F32>(a.part_kv + split * all, out, dk, a.scale, a.D, lane);
-            T::template store<AXS6_F32>(a.part_kv + (a.splits_kv + split) * all, out, dv, 1.0f, a.D, lane);
+            T::template store<AXS6_F32>(a.part_kv + split * all, out, dk, fk, a.D, lane);
+            T::template store<AXS6_F32>(a.part_kv + (a.splits_kv + split) * all, out, dv, fv, a.D, lane);
         } else {
-            T::template store<DT>(a.dk, out, dk, a.scale, a.D, lane);
-            T::template store<DT>(a.dv, out, dv, 1.0f, a.D, lane);
+            T::template store<DT>(a.dk, out, dk, fk, a.D, lane);
+            T::template store<DT>(a.dv, out, dv, fv, a.D, lane);
         }
     }
     for (uint64_t rows = __ballot(bad && lane < 32 && key < a.Tk); rows; rows &= rows - 1)

@@ -418,7 +418,8 @@ extern "C" int64_t axs6_attention_backward_workspace(int64_t B, int64_t Tq, int6
                                                      int32_t causal) {
     if (B <= 0 || Tq <= 0 || Tk <= 0 || Hq <= 0 || H <= 0 || D <= 0) return 0;
     const int64_t s = forward_splits(B, Tq, Tk, Hq), kv = key_splits(B, Tq, Tk, Hq, H, causal);
-    return ((s == 1 ? 0 : s * B * Tq * Hq * D) + (kv == 1 ? 0 : 2 * kv * B * Tk * H * D)) * (int64_t)sizeof(float);
+    return ((s == 1 ? 0 : s * B * Tq * Hq * D) + (kv == 1 ? 0 : 2 * kv * B * Tk * H * D)) * (int64_t)sizeof(float) +
+           B * Hq * ((Tq + 31) / 32) * (int64_t)sizeof(float2);
 }
 
 extern "C" int axs6_attention_forward(const void* q, const void* k, const void* v, int32_t dtype, int64_t B, int64_t Tq,
@@ -482,6 +483,7 @@ extern "C" int axs6_attention_backward(const void* dout, const void* q, const vo
         return rc;
     a.part = reinterpret_cast<float*>(workspace);
     a.part_kv = a.part + (a.splits == 1 ? 0 : a.splits * B * Tq * Hq * D);
+    a.bounds = reinterpret_cast<float2*>(a.part_kv + (a.splits_kv == 1 ? 0 : 2 * a.splits_kv * B * Tk * H * D));
     attention_backward(a, dtype, (hipStream_t)stream);
     return check_launch(fn);
 }

@@ -238,15 +238,19 @@ struct AttentionFunction : public torch::autograd::Function<AttentionFunction> {
         const at::Tensor g = vectors(grads[0].to(q.scalar_type()));
         const Mask m = mask_of(s[5], B, Hq, Tq, Tk);
         at::Tensor dq = at::empty({B, Tq, Hq, D}, q.options()), dk = at::empty({B, Tk, H, D}, q.options());
-        at::Tensor dv = at::empty({B, Tk, H, D}, q.options()), delta = at::empty({B, Hq, Tq}, stats.options());
+        at::Tensor dv = at::empty({B, Tk, H, D}, q.options());
         const bool causal = d["causal"].toBool();
-        const at::Tensor ws = workspace(axs6_attention_backward_workspace(B, Tq, Tk, Hq, H, D, causal), q);
+        // delta, then the workspace (whole 16 bytes each)
+        const int64_t rows = (B * Hq * Tq + 3) / 4 * 4;
+        const int64_t bytes = axs6_attention_backward_workspace(B, Tq, Tk, Hq, H, D, causal);
+        const at::Tensor scratch = at::empty({rows + bytes / 4}, stats.options());
+        float* delta = scratch.data_ptr<float>();
         check_rc(axs6_attention_backward(
                      g.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), stats.data_ptr<float>(),
                      dtype_code(q.scalar_type()), B, Tq, Tk, Hq, H, D, g.strides().data(), q.strides().data(),
                      k.strides().data(), v.strides().data(), m.data(), m.type, m.strides, causal,
-                     (float)d["scale"].toDouble(), delta.data_ptr<float>(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                     data_of(ws), size_of(ws), stream_of(q)),
+                     (float)d["scale"].toDouble(), delta, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                     delta + rows, bytes, stream_of(q)),
                  "axs6_attention_backward");
         const at::Tensor got[3] = {dq, dk, dv};
         for (int i = 0; i < 3; ++i)

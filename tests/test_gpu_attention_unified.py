@@ -427,3 +427,36 @@ def test_one_sequence_or_token_of_an_unaligned_batch(dtype):
     batch = torch.randn(2, 5 * 2 * 64 + 1, generator=torch.Generator().manual_seed(1)).to(DEV, dtype)
     one = batch[:, :-1].unflatten(-1, (5, 2, 64))[:1]
     _check(q, one, one, go)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("Tq,Tk,D", [(1024, 1024, 64), (4096, 4096, 64), (128, 128, 64), (300, 2048, 80), (600, 600, 128)])
+@pytest.mark.parametrize("size", [1.0, 1e-3, 1e-4])
+def test_small_float16_gradients(size, Tq, Tk, D, causal):
+    """float16 gradients from small ones of the output: the error is that of the products' operands, 3 u of the
+    gradient, and the result's own rounding, half a step of float16 (2^-24 below 2^-14)."""
+    from axs.unified import axs_attention_unified
+
+    q, k, v, go = _inputs(1, Tq, Tk, 1, 1, D, torch.float16)
+    go = (go.float() * size).half()
+    xs = [x.requires_grad_(True) for x in (q, k, v)]
+    got = torch.autograd.grad(axs_attention_unified(*xs, causal=causal), xs, go)
+    for name, x, y in zip("qkv", got, ref.attention(q, k, v, go, causal=causal)[1:]):
+        error = float((x.double().cpu() - y).norm())
+        assert error <= 3 * ref.U[torch.float16] * float(y.norm()) + 2.0 ** -25 * math.sqrt(y.numel()), name
+
+
+def test_float16_gradients_of_large_ones_and_of_long_rows():
+    """Score gradients past float16's largest value behind small keys and queries; probabilities far below its
+    smallest normal one."""
+    from axs.unified import axs_attention_unified
+
+    for Tq, Tk, D in ((100, 8, 64), (200, 9, 64), (130, 140, 128)):
+        q, k, v, go = _inputs(1, Tq, Tk, 2, 1, D, torch.float16)
+        _check(q * 0.01, k * 0.01, v * 300, go * 300)
+    q, k, v, go = _inputs(1, 48, 200000, 1, 1, 32, torch.float16)
+    xs = [x.requires_grad_(True) for x in (q, k, v)]
+    got = torch.autograd.grad(axs_attention_unified(*xs), xs, go)
+    for name, x, y in zip("qkv", got, ref.attention(q, k, v, go)[1:]):
+        error = float((x.double().cpu() - y).norm())
+        assert error <= 3 * ref.U[torch.float16] * float(y.norm()) + 2.0 ** -25 * math.sqrt(y.numel()), name
