@@ -62,16 +62,20 @@ struct KvAttnArgs {
 };
 
 // Eight int8 codes as f16: with the sign bit flipped a byte u is code + 128,
-// and the f16 with the bits 0x6400 | u is 1024 + u.
+// and the f16 with the bits 0x6400 | u is 1024 + u.  SMALL: times 2^-20 (bits 0x1400 | u),
+// 1 / kSumScale, where a block's scale times that might itself be too small for float32.
+template <bool SMALL>
 __device__ __forceinline__ f16x8 codes_f16(uint32_t a, uint32_t b) {
+    constexpr uint32_t kHigh = SMALL ? 0x14141414u : 0x64646464u;
     union { uint32_t w[4]; f16x2 h[4]; f16x8 v; } r;
     a ^= 0x80808080u;
     b ^= 0x80808080u;
-    r.w[0] = __builtin_amdgcn_perm(0x64646464u, a, 0x04010400u);
-    r.w[1] = __builtin_amdgcn_perm(0x64646464u, a, 0x04030402u);
-    r.w[2] = __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u);
-    r.w[3] = __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u);
-    const f16x2 bias = {(_Float16)1152.0f, (_Float16)1152.0f};
+    r.w[0] = __builtin_amdgcn_perm(kHigh, a, 0x04010400u);
+    r.w[1] = __builtin_amdgcn_perm(kHigh, a, 0x04030402u);
+    r.w[2] = __builtin_amdgcn_perm(kHigh, b, 0x04010400u);
+    r.w[3] = __builtin_amdgcn_perm(kHigh, b, 0x04030402u);
+    constexpr float kBias = SMALL ? 1152.0f / kSumScale : 1152.0f;
+    const f16x2 bias = {(_Float16)kBias, (_Float16)kBias};
 #pragma unroll
     for (int i = 0; i < 4; ++i) r.h[i] = r.h[i] - bias;
     return r.v;
@@ -186,7 +190,7 @@ __global__ __launch_bounds__(64 * WAVES) void kv_attention_kernel(KvAttnArgs a) 
     for (int blk = b0 + w; blk < b1; blk += WAVES) {
         const int64_t cell = cell0 + blk;
         if (blk != b0 + w) load_block<NC>(kr, vr, a, cell, n16, g4);   // the first came before the queries
-        const float ks = a.ks[cell], vs = a.vs[cell] * (1.0f / (kProbScale * kSumScale));
+        const float ks = a.ks[cell], vs = a.vs[cell] * (1.0f / kProbScale);   // the codes bring 1 / kSumScale
         f32x4 s[NR][2];
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt) {
@@ -194,7 +198,7 @@ __global__ __launch_bounds__(64 * WAVES) void kv_attention_kernel(KvAttnArgs a) 
             for (int n = 0; n < NR; ++n) s[n][tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
-                const f16x8 k0 = codes_f16(kr[tt][c].x, kr[tt][c].y), k1 = codes_f16(kr[tt][c].z, kr[tt][c].w);
+                const f16x8 k0 = codes_f16<false>(kr[tt][c].x, kr[tt][c].y), k1 = codes_f16<false>(kr[tt][c].z, kr[tt][c].w);
 #pragma unroll
                 for (int n = 0; n < NR; ++n)
 #pragma unroll
@@ -234,7 +238,7 @@ __global__ __launch_bounds__(64 * WAVES) void kv_attention_kernel(KvAttnArgs a) 
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
             if (16 * d >= a.D) continue;
-            const f16x8 vf = codes_f16(vr[d].x, vr[d].y);
+            const f16x8 vf = codes_f16<true>(vr[d].x, vr[d].y);
 #pragma unroll
             for (int n = 0; n < NR; ++n) {
                 f32x4 y = f32x4{0.0f, 0.0f, 0.0f, 0.0f};

@@ -251,3 +251,20 @@ def test_reading_outside_the_blocks():
             if lo < hi:
                 want[lo - first:hi - first] = ref.cache_values(x[0])[lo:hi]
             assert torch.equal(y[0].cpu(), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("size", [1e30, 1e-20, 1e-26, 1e-28, 1e-30])
+def test_values_of_any_size(size, dtype):
+    """Sums over large values stay finite and those over small ones keep their digits."""
+    from axs.unified import axs_cache_attention_unified, axs_cache_append_unified, AXSKVCacheUnified
+
+    for Tq, n in ((1, 300), (3, 9000)):
+        cache = AXSKVCacheUnified.empty(1, 2, 64, n, dtype, DEV)
+        k, v = _tokens(1, n, 2, 64, dtype)
+        v = (v.float() * size).to(dtype)
+        axs_cache_append_unified(cache, k, v, torch.zeros(1, dtype=torch.int64, device=DEV))
+        q = torch.randn(1, Tq, 8, 64, generator=torch.Generator().manual_seed(7)).to(DEV, dtype)
+        out = axs_cache_attention_unified(q, cache, torch.tensor([n], device=DEV))
+        want = ref.attention(q, ref.cache_values(k[0])[None], ref.cache_values(v[0])[None], causal=True)
+        assert ref.rel(out.double() / size, want / size) <= _bound(dtype), (n, Tq)
