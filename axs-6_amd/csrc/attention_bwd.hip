@@ -32,8 +32,8 @@ constexpr int kWaves = 4, kThr = 64 * kWaves, kHeld = 32 * kWaves;
 // float16 has 2^-14 as its smallest normal value and 65504 as its largest: probabilities
 // and score gradients go into their products times a power of two, which costs nothing
 // inside the loops and is undone with the results' factors.
-//  * dq: a query's score gradients times 2^4 / |do_i| (the power of two below), which
-//    p 2^-18 keeps normal beside values of 1, and values of norm 4096 in range.
+//  * dq: a query's score gradients times 2^3 / |do_i| (the power of two above it): ds is
+//    normal down to p = 2^-17 beside values of 1, and in range for values of norm 4000.
 //  * dk, dv: both times 2^e, e in 0 .. 15 and as large as leaves ds_ij, at most
 //    p (|do_i| |v_j| + |delta_i|), below 2^15 for the keys held and all queries of the
 //    group; the first launch leaves their largest |do| and |delta|.  e goes into the rows' y.
@@ -43,7 +43,7 @@ constexpr int kWaves = 4, kThr = 64 * kWaves, kHeld = 32 * kWaves;
 // A larger ds still overflows, and its rows are made again.  The other types have
 // float32's range and no scale.
 __device__ __forceinline__ float row_scale(float norm2) {
-    return norm2 > 0.0f && norm2 < INFINITY ? ldexpf(1.0f, 4 - (__builtin_amdgcn_frexp_expf(norm2) >> 1)) : 1.0f;
+    return norm2 > 0.0f && norm2 < INFINITY ? ldexpf(1.0f, 3 - ((__builtin_amdgcn_frexp_expf(norm2) + 1) >> 1)) : 1.0f;
 }
 __device__ __forceinline__ float finite_or_0(float x) { return fabsf(x) < INFINITY ? x : 0.0f; }
 __device__ __forceinline__ float wave_max(float x) {
