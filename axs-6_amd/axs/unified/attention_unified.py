@@ -37,7 +37,10 @@ def axs_attention_unified(
     pass ``x.transpose(1, 2)``).  ``causal``: query i sees keys j <= i + Tk - Tq.
     ``mask`` broadcasts to (B, Hq, Tq, Tk): bool, True where a query sees a key, or
     values added to the scores, -inf where it does not; no gradient.  A query that
-    sees no key gives 0.  ``scale`` is 1 / sqrt(D) if None.
+    sees no key gives 0.  ``scale`` is 1 / sqrt(D) if None, else positive.
+
+    A result that is not finite is made again pair by pair (places that a query does not
+    see have no part in it), which takes much longer.
 
     Scores, softmax and sums are float32; for 16-bit operands the probabilities
     (and, in the backward, their gradients) are rounded to the operands' type for

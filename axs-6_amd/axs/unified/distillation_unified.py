@@ -28,7 +28,8 @@ def axs_distillation_loss_unified(
     0 is left out, one at or past V makes its row NaN; ``weights`` (*) per row, a row of
     weight 0 is not read.  ``"mean"`` is the weighted mean (0 where the weights sum to
     0), ``"sum"`` the weighted sum, ``"none"`` the weighted rows.  float32 result; the
-    gradient T w (q - p), for the student's logits alone, is rounded once to their type.
+    gradient T w (q - p), for the student's logits alone, is rounded once to their type;
+    its time grows with K^2, since classes may repeat: K is meant to be some hundreds.
     """
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be 'mean', 'sum' or 'none', got {reduction!r}")

@@ -55,8 +55,11 @@ def axs_cache_append_unified(cache: AXSKVCacheUnified, k: torch.Tensor, v: torch
     """``k`` and ``v`` (B, n, heads, D) become tokens ``starts[b]`` .. ``starts[b] + n - 1``
     of sequence b; tokens from there on are forgotten.  ``starts`` (B) int64 or int32
     is read on the device: tokens past the cache's end are dropped, and all of a
-    sequence whose start lies outside it.  A start inside a block needs the call
-    before to have ended there (the block's earlier tokens come from the tail)."""
+    sequence whose start lies outside it.  A start past its block's
+    first token needs the call before to have ended inside the same block, there or
+    later: the block's earlier tokens come from the tail, which holds those of the last,
+    partial block alone.  To go back further, append again from the first token of the
+    block that this leads to."""
     _lib.ext().kv_append(*cache, k, v, starts)
 
 
@@ -75,5 +78,6 @@ def axs_cache_attention_unified(
     """Attention of ``q`` (B, Tq, Hq, D), the last Tq of the ``lengths[b]`` tokens that the
     cache holds of sequence b, over them -> (B, Tq, Hq, D) of q's dtype.  Query t sees
     keys j <= lengths[b] - Tq + t (none: 0); Hq is a multiple of the cache's heads.
-    ``lengths`` (B) int64 or int32 is read on the device.  No gradient."""
+    ``lengths`` (B) int64 or int32 is read on the device.  ``scale`` is 1 / sqrt(D) if
+    None, else any finite number.  No gradient."""
     return _lib.ext().kv_attention(q, *cache, lengths, scale)

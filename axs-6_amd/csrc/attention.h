@@ -409,7 +409,10 @@ __device__ __forceinline__ void add_groups(f32x16 (&c)[N], float* ex, int group,
 // value hold there.  An infinity or NaN there turns the mask's -inf and the weight of 0 in the
 // products over a tile's rows into NaN; so a result that is not finite is made
 // again from the pairs that see each other alone, one pair at a time by one wave.
-// Where those give a NaN everywhere there is nothing more to find.
+// Where those give a NaN everywhere there is nothing more to find.  That is slow, and an
+// infinity that is seen costs it too: 1 x 1024, 8 heads on 2 of 64, 16 bit, forward and
+// backward 0.12 ms, with one infinity in dout 4.6, in one value 9.5; a wave's 32 rows go
+// over all their pairs, so the time grows with the length (and the group's heads).
 
 // Whether any of the results of the lane's column is not finite.
 template <int N>

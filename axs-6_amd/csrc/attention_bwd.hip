@@ -13,15 +13,15 @@
 // Under a causal mask the first keys are seen by far more queries than the
 // last: their queries are split over workgroups, whose float32 sums a third
 // launch adds (1 x 16384, 2 key heads for 16, bf16: 9072 -> 3824 us for both
-// launches; 2 x 4096, 8 for 32: 1511 -> 1127, now 1064, of which dq 450: the 7
-// products' 9.6e11 operations at 904 TFLOP/s, 79% of a bf16 product of 8192^3).
+// launches; 2 x 4096, 8 for 32: 1511 -> 1127, now 1020, of which dq 391: the 7
+// products' 9.6e11 operations at 943 TFLOP/s, 83% of a bf16 product of 8192^3).
 // A head of up to 64 values whose queries and keys are at most 128 is one
 // workgroup's: the second launch then makes dq too, from ds by way of LDS, 5
 // products instead of 7 and one launch instead of two.  64 x 128, 4 heads, causal:
-// float32 61 -> 43 us, bf16 20 either way; 512 x 128: 496 -> 325, 93 -> 89; 64 x 32
-// queries of 77 keys, 8 heads: 67 -> 37, 16 -> 13.  (Larger heads' keys and scores
+// float32 61 -> 44 us, bf16 20 either way; 512 x 128: float32 431 -> 338, bf16 97 -> 101,
+// float16 102 -> 98; 64 x 32 queries of 77 keys, 8 heads: 67 -> 37, bf16 16 -> 13.  (Larger heads' keys and scores
 // leave no room for a second workgroup on the CU, or for the first.)  In float32 what
-// is left is the wave's own chain: its 640 products of 64 cycles are 17 us of the 43.
+// is left is the wave's own chain: its 640 products of 64 cycles are 17 us of the 44.
 #include "attention.h"
 
 namespace axs6 {

@@ -13,6 +13,10 @@
 // exponentials in one pass), the backward reads them and writes the gradient
 // once; the K entries of a row are gathered from cache.  All sums are float32
 // in a fixed order; the gradient is rounded once.
+// A class may stand in several entries: the backward compares a row's entries with each
+// other, K^2 of them, which is nothing for a teacher's top logits and much for whole
+// vocabularies (2048 x 32000 bf16, the backward: K = 64 75 us, 512 317, 2048
+// 4.0 ms; 256 x 32000, K = 32000: 193 ms).
 // The gradient could only be written by the forward if its factor from above
 // were known there, or by a second rounding: so three passes, 6 bytes a logit.
 // Measured: 8192 x 128000 bf16, both directions, 1206 us, 5.2 TB/s over the three

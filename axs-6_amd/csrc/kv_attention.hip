@@ -25,7 +25,9 @@
 // attention: 1 x 16384 tokens, 8 key heads for 32, 48 us against 15).
 // Measured: 64 sequences of 4096 to 16383 tokens, 8 key heads of 128 for 64,
 // 290 us, 4.6 TB/s (a copy of 4 GiB runs at 4.7 on this card); one of 131072
-// 55 us; one of 300, where launches and latency count, 8.7 us.  Holding the next
+// 55 us; one of 300, where launches and latency count, 8.7 us.  A prompt's workgroups
+// each read and convert all the blocks before them again: 1024 tokens, 8 key heads of
+// 128 for 32, 58 us, 4096 453 us.  Holding the next
 // block's codes on their way costs registers and with them waves: 64 x 2048
 // tokens 22.8 -> 25.7 us.
 #include <math.h>

@@ -444,13 +444,15 @@ int axs6_attention_backward(const void* dout, const void* q, const void* k, cons
  * `dtype`, the raw values of the block that is not full yet.
  * append: k, v (B, n, H, D) (strides as above) become tokens starts[b].. of
  *   sequence b; tokens past the capacity are dropped, and all of a sequence whose
- *   start lies outside the cache; a start inside a block takes the block's earlier
- *   tokens from the tail.
+ *   start lies outside the cache; a start past its block's first token takes the
+ *   block's earlier tokens from the tail, so the call before has to have ended inside
+ *   the same block, there or later.
  * read: tokens first[b] .. first[b] + count - 1 as float32 (B, count, H, D), code
  *   times scale; 0 outside the cache.
  * attention: q (B, Tq, Hq, D), the last Tq of the lengths[b] tokens of sequence b;
  *   query t sees keys j <= lengths[b] - Tq + t (none: 0); out (B, Tq, Hq, D)
- *   contiguous.  Needs axs6_kv_attention_workspace(...) bytes, 16-byte aligned.
+ *   contiguous; scale any finite number.  Needs axs6_kv_attention_workspace(...)
+ *   bytes, 16-byte aligned.
  * D a multiple of 16 up to AXS6_KV_MAX_HEAD; codes and tails 16-byte aligned;
  * starts, first and lengths are read on the device. */
 #define AXS6_KV_BLOCK 32
@@ -477,7 +479,8 @@ int axs6_kv_attention(const void* q, int32_t dtype, int64_t B, int64_t Tq, int64
  * weights NULL: all 1; a row of weight 0 is not read.  An index at or past V
  * gives the row NaN.  rows: N floats, stats: 2 N floats kept for the backward,
  * loss and norm: one float each (loss may be NULL).  The backward writes
- * dlogits (N, V) contiguous: T w_r (q - sum of p over an index) times grad_out
+ * dlogits (N, V) contiguous, in time that grows with K^2 (a class may repeat; K is
+ * meant to be some hundreds): T w_r (q - sum of p over an index) times grad_out
  * (one float, or N with grad_rows) and norm[0] (NULL: 1). */
 int axs6_distill_forward(const void* logits, int32_t dtype, int64_t ld, int64_t N, int64_t V, const float* values,
                          const int64_t* indices, int64_t K, float temperature, const float* weights, int32_t mean,
