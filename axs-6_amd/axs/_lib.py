@@ -91,6 +91,13 @@ _SIGNATURES: dict[str, list] = {
     "axs6_kv_attention_workspace": [_i64, _i64, _i64, _i64, _i64, _i64],
     "axs6_kv_attention": [_vp, _i32, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp,
                           ctypes.c_float, _vp, _vp, _i64, _vp],
+    "axs6_kv_copy": [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _vp,
+                     _vp, _vp, _vp, _vp, _vp],
+    "axs6_kv_shared_attention_workspace": [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64],
+    "axs6_kv_shared_attention": [_vp, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp,
+                                 _vp, _vp, _vp, _i64, _vp, ctypes.c_float, _vp, _vp, _i64, _vp],
+    "axs6_beam_select_workspace": [_i64, _i64, _i64, _i32],
+    "axs6_beam_select": [_vp, _i32, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp],
     "axs6_distill_forward": [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _i64, ctypes.c_float, _vp, _i32, _vp, _vp, _vp,
                              _vp, _vp],
     "axs6_distill_backward": [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _i64, ctypes.c_float, _vp, _vp, _vp, _i32, _vp,
@@ -103,6 +110,7 @@ _RESTYPES = {"axs6_linear_padded_k": _i64, "axs6_nf5_linear_backward_workspace":
              "axs6_nf5_fused_linear_split_workspace": _i64, "axs6_nf5_linear_infer_workspace": _i64,
              "axs6_nf5_linear_infer_stacked_workspace": _i64,
              "axs6_layer_norm_backward_workspace": _i64, "axs6_kv_attention_workspace": _i64,
+             "axs6_kv_shared_attention_workspace": _i64, "axs6_beam_select_workspace": _i64,
              "axs6_attention_forward_workspace": _i64, "axs6_attention_backward_workspace": _i64}
 
 

@@ -26,6 +26,7 @@ from axs.unified.backend import (
     get_backend,
     set_backend,
 )
+from axs.unified.beam_unified import axs_beam_select_unified
 from axs.unified.distillation_unified import axs_distillation_loss_unified
 from axs.unified.functional_unified import (
     axs_linear_group_unified,
@@ -38,7 +39,9 @@ from axs.unified.kv_cache_unified import (
     AXSKVCacheUnified,
     axs_cache_append_unified,
     axs_cache_attention_unified,
+    axs_cache_copy_unified,
     axs_cache_read_unified,
+    axs_cache_shared_attention_unified,
 )
 from axs.unified.mixed_precision import (
     AXSLinearMixedPrecision,
@@ -120,5 +123,8 @@ __all__ = [
     "axs_cache_append_unified",
     "axs_cache_read_unified",
     "axs_cache_attention_unified",
+    "axs_cache_copy_unified",
+    "axs_cache_shared_attention_unified",
+    "axs_beam_select_unified",
     "axs_distillation_loss_unified",
 ]

@@ -81,3 +81,44 @@ def axs_cache_attention_unified(
     ``lengths`` (B) int64 or int32 is read on the device.  ``scale`` is 1 / sqrt(D) if
     None, else any finite number.  No gradient."""
     return _lib.ext().kv_attention(q, *cache, lengths, scale)
+
+
+def axs_cache_shared_attention_unified(
+    q: torch.Tensor,
+    prefix: AXSKVCacheUnified,
+    prefix_lengths: torch.Tensor,
+    cache: AXSKVCacheUnified,
+    lengths: torch.Tensor,
+    scale: float | None = None,
+) -> torch.Tensor:
+    """Attention of sequences that share a prefix, whose codes are read once for all of them:
+    of the B sequences of ``q`` (B, Tq, Hq, D), B a multiple of the P that ``prefix`` holds, number
+    b continues prefix ``b // (B / P)``.  Its tokens are the ``prefix_lengths[b // (B / P)]`` of that
+    prefix and then the ``lengths[b]`` of its own that ``cache`` holds, and ``q`` its last Tq:
+    query t sees the keys at places j <= prefix + own - Tq + t of them (none: 0).
+    -> (B, Tq, Hq, D) of q's dtype, that of both caches' tails.  ``prefix_lengths`` (P) and
+    ``lengths`` (B), int64 or int32, are read on the device.  ``scale`` as in
+    :func:`axs_cache_attention_unified`.  No gradient."""
+    return _lib.ext().kv_shared_attention(q, *prefix, prefix_lengths, *cache, lengths, scale)
+
+
+def axs_cache_copy_unified(
+    cache: AXSKVCacheUnified,
+    sources: torch.Tensor,
+    lengths: torch.Tensor,
+    target: AXSKVCacheUnified | None = None,
+) -> None:
+    """Sequence i of ``target`` becomes sequence ``sources[i]`` of ``cache``; ``target`` None:
+    of the cache itself, in place, whatever the order of the sources.
+
+    ``sources`` (target's sequences), or (G, n) for G groups: then its numbers count within the
+    group's sequences of the cache, as the parents of :func:`axs_beam_select_unified` do.  One that
+    is none of them (-1, say) leaves its sequence as it was.  ``lengths`` (cache's sequences):
+    the tokens that each holds; whole blocks are copied and the raw rows of the partial one, and what
+    lies behind them is left as it was.  Tokens past the end of either cache are dropped.  Both are int64
+    or int32 and read on the device.  A target of its own has the cache's heads and dtype and
+    shares no memory with it; its number of sequences and its capacity are its own.
+
+    Reorder beams: ``sources=parents``.  Fork a prompt: one source for several sequences.  Close
+    up a batch: the live sequences' numbers, then -1.  In place a group has up to 4096 sequences."""
+    _lib.ext().kv_copy(*cache, sources, lengths, *(cache if target is None else target))

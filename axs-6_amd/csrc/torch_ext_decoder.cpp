@@ -385,6 +385,121 @@ at::Tensor kv_attention(const at::Tensor& q, const at::Tensor& k_codes, const at
     return out;
 }
 
+// Sequence i of the target becomes sequence sources[i] of the cache; (groups, sequences): of its group.
+void kv_copy(const at::Tensor& k_codes, const at::Tensor& k_scales, const at::Tensor& v_codes, const at::Tensor& v_scales,
+             const at::Tensor& k_tail, const at::Tensor& v_tail, const at::Tensor& sources, const at::Tensor& lengths,
+             const at::Tensor& to_k_codes, const at::Tensor& to_k_scales, const at::Tensor& to_v_codes,
+             const at::Tensor& to_v_scales, const at::Tensor& to_k_tail, const at::Tensor& to_v_tail) {
+    const char* fn = "axs_cache_copy_unified";
+    const Cache c = cache_of(k_codes, k_scales, v_codes, v_scales, k_tail, v_tail, fn);
+    const Cache t = cache_of(to_k_codes, to_k_scales, to_v_codes, to_v_scales, to_k_tail, to_v_tail, fn);
+    TORCH_CHECK(t.H == c.H && t.D == c.D && t.kt.scalar_type() == c.kt.scalar_type() && t.kc.device() == c.kc.device(), fn,
+                ": a target of ", t.H, " heads of ", t.D, ", ", t.kt.scalar_type(), " on ", t.kc.device(), " for a cache of ",
+                c.H, " heads of ", c.D, ", ", c.kt.scalar_type(), " on ", c.kc.device());
+    TORCH_CHECK(sources.dim() == 1 || sources.dim() == 2, fn, ": sources must be (sequences) or (groups, sequences), got ",
+                sources.sizes());
+    const int64_t groups = sources.dim() == 2 ? sources.size(0) : 1, each = sources.size(-1);
+    TORCH_CHECK(groups * each == t.B && (groups ? c.B % groups == 0 : c.B == 0), fn, ": sources ", sources.sizes(), " for ",
+                t.B, " target sequences and a cache of ", c.B);
+    const at::Tensor s = int64s(sources, sources.sizes(), c.kc, fn, "sources"),
+                     n = int64s(lengths, {c.B}, c.kc, fn, "lengths");
+    if (groups == 0) return;
+    c10::DeviceGuard guard(c.kc.device());
+    check_rc(axs6_kv_copy(c.kc.data_ptr(), c.ks.data_ptr<float>(), c.vc.data_ptr(), c.vs.data_ptr<float>(), c.kt.data_ptr(),
+                          c.vt.data_ptr(), dtype_code(c.kt.scalar_type()), groups, c.B / groups, each, c.H, c.D, c.nb,
+                          s.data_ptr<int64_t>(), n.data_ptr<int64_t>(), t.nb, t.kc.data_ptr(), t.ks.data_ptr<float>(),
+                          t.vc.data_ptr(), t.vs.data_ptr<float>(), t.kt.data_ptr(), t.vt.data_ptr(), stream_of(c.kc)),
+             "axs6_kv_copy");
+}
+
+at::Tensor kv_shared_attention(const at::Tensor& q, const at::Tensor& pk_codes, const at::Tensor& pk_scales,
+                               const at::Tensor& pv_codes, const at::Tensor& pv_scales, const at::Tensor& pk_tail,
+                               const at::Tensor& pv_tail, const at::Tensor& prefix_lengths, const at::Tensor& k_codes,
+                               const at::Tensor& k_scales, const at::Tensor& v_codes, const at::Tensor& v_scales,
+                               const at::Tensor& k_tail, const at::Tensor& v_tail, const at::Tensor& lengths,
+                               std::optional<double> scale) {
+    const char* fn = "axs_cache_shared_attention_unified";
+    const Cache p = cache_of(pk_codes, pk_scales, pv_codes, pv_scales, pk_tail, pv_tail, fn);
+    const Cache c = cache_of(k_codes, k_scales, v_codes, v_scales, k_tail, v_tail, fn);
+    check_like(q, c.kt, 4, fn, "q");
+    check_like(p.kt, c.kt, 4, fn, "the prefix's tail");
+    const int64_t Tq = q.size(1), Hq = q.size(2);
+    TORCH_CHECK(p.H == c.H && p.D == c.D && (p.B ? c.B % p.B == 0 : c.B == 0), fn, ": a prefix of ", p.B, " sequences, ", p.H,
+                " heads of ", p.D, " for a cache of ", c.B, " sequences, ", c.H, " heads of ", c.D);
+    TORCH_CHECK(q.size(0) == c.B && q.size(3) == c.D && (c.H ? Hq % c.H == 0 : Hq == 0), fn, ": q ", q.sizes(),
+                " for a cache of ", c.B, " sequences, ", c.H, " heads of ", c.D);
+    const double s = scale ? *scale : 1.0 / std::sqrt((double)c.D);
+    TORCH_CHECK(std::isfinite((float)s), fn, ": the scale must be finite, got ", s);
+    const at::Tensor np = int64s(prefix_lengths, {p.B}, q, fn, "prefix_lengths"), n = int64s(lengths, {c.B}, q, fn, "lengths"),
+                     qp = packed_last(q);
+    c10::DeviceGuard guard(q.device());
+    at::Tensor out = at::empty({c.B, Tq, Hq, c.D}, q.options());
+    if (out.numel() == 0) return out;
+    if (p.nb == 0) {   // no prefix: the sequences' own tokens are all
+        if (c.nb == 0) return out.zero_();
+        const at::Tensor ws = workspace(axs6_kv_attention_workspace(c.B, Tq, Hq, c.H, c.D, c.nb), q);
+        check_rc(axs6_kv_attention(qp.data_ptr(), dtype_code(q.scalar_type()), c.B, Tq, Hq, c.H, c.D, qp.strides().data(),
+                                   c.kc.data_ptr(), c.ks.data_ptr<float>(), c.vc.data_ptr(), c.vs.data_ptr<float>(), c.nb,
+                                   n.data_ptr<int64_t>(), (float)s, out.data_ptr(), data_of(ws), size_of(ws), stream_of(q)),
+                 "axs6_kv_attention");
+        return out;
+    }
+    const at::Tensor ws = workspace(
+        axs6_kv_shared_attention_workspace(p.B, c.B / p.B, Tq, Hq, c.H, c.D, p.nb, c.nb), q);
+    check_rc(axs6_kv_shared_attention(qp.data_ptr(), dtype_code(q.scalar_type()), p.B, c.B / p.B, Tq, Hq, c.H, c.D,
+                                      qp.strides().data(), p.kc.data_ptr(), p.ks.data_ptr<float>(), p.vc.data_ptr(),
+                                      p.vs.data_ptr<float>(), p.nb, np.data_ptr<int64_t>(), c.kc.data_ptr(),
+                                      c.ks.data_ptr<float>(), c.vc.data_ptr(), c.vs.data_ptr<float>(), c.nb,
+                                      n.data_ptr<int64_t>(), (float)s, out.data_ptr(), data_of(ws), size_of(ws),
+                                      stream_of(q)),
+             "axs6_kv_shared_attention");
+    return out;
+}
+
+// ---- beam search's selection --------------------------------------------------------------
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> beam_select(const at::Tensor& logits, const at::Tensor& scores,
+                                                           const OptTensor& finished, std::optional<int64_t> end,
+                                                           std::optional<int64_t> count) {
+    const char* fn = "axs_beam_select_unified";
+    require_device(logits, fn);
+    check_dtype(logits, fn, "logits");
+    TORCH_CHECK(logits.dim() == 3 && logits.size(1) >= 1 && logits.size(2) >= 1, fn,
+                ": logits must be (sequences, beams, classes), got ", logits.sizes());
+    const int64_t G = logits.size(0), W = logits.size(1), V = logits.size(2), C = count ? *count : W;
+    require_device(scores, fn);
+    TORCH_CHECK(scores.device() == logits.device() && scores.sizes() == logits.sizes().slice(0, 2), fn,
+                ": scores must be of shape ", logits.sizes().slice(0, 2), " on ", logits.device(), ", got ", scores.sizes(),
+                " on ", scores.device());
+    TORCH_CHECK(scores.scalar_type() == at::kFloat, fn, ": scores must be float32, got ", scores.scalar_type());
+    TORCH_CHECK(W <= AXS6_BEAM_MAX_BEAMS && C >= 1 && C <= AXS6_BEAM_MAX_COUNT, fn, ": 1 to ", AXS6_BEAM_MAX_COUNT,
+                " continuations of at most ", AXS6_BEAM_MAX_BEAMS, " beams, got ", C, " of ", W);
+    TORCH_CHECK(!records(logits) && !records(scores), fn, ": a choice has no gradient; detach logits and scores");
+    at::Tensor f;
+    if (given(finished)) {
+        require_device(*finished, fn);
+        TORCH_CHECK(finished->device() == logits.device() && finished->sizes() == scores.sizes() &&
+                        finished->scalar_type() == at::kBool,
+                    fn, ": finished must be bool of shape ", scores.sizes(), " on ", logits.device(), ", got ",
+                    finished->scalar_type(), " ", finished->sizes(), " on ", finished->device());
+        TORCH_CHECK(end, fn, ": finished needs end, the token that ends a sequence");
+        f = finished->contiguous();
+    }
+    TORCH_CHECK(!end || (*end >= 0 && *end < V), fn, ": end must be a class below ", V, ", got ", end ? *end : 0);
+    c10::DeviceGuard guard(logits.device());
+    const at::Tensor z = packed_last(logits), c = scores.contiguous();
+    at::Tensor top = at::empty({G, C}, scores.options()), parents = at::empty({G, C}, scores.options().dtype(at::kLong)),
+               tokens = at::empty_like(parents);
+    if (G == 0) return {top, parents, tokens};
+    const at::Tensor ws = workspace(axs6_beam_select_workspace(G, W, V, dtype_code(z.scalar_type())), z);
+    check_rc(axs6_beam_select(z.data_ptr(), dtype_code(z.scalar_type()), G, W, V, z.stride(0), z.stride(1),
+                              c.data_ptr<float>(), f.defined() ? reinterpret_cast<const uint8_t*>(f.data_ptr<bool>()) : nullptr,
+                              end ? *end : 0, C, top.data_ptr<float>(), parents.data_ptr<int64_t>(),
+                              tokens.data_ptr<int64_t>(), data_of(ws), size_of(ws), stream_of(z)),
+             "axs6_beam_select");
+    return {top, parents, tokens};
+}
+
 // ---- distillation ---------------------------------------------------------------------------
 
 // Reductions: 0 each row's loss, 1 the weighted mean, 2 the weighted sum.
@@ -491,6 +606,17 @@ void register_decoder(py::module& m) {
     m.def("kv_attention", &kv_attention, "attention of the newest tokens over the 8-bit cache", py::arg("q"),
           py::arg("k_codes"), py::arg("k_scales"), py::arg("v_codes"), py::arg("v_scales"), py::arg("k_tail"),
           py::arg("v_tail"), py::arg("lengths"), py::arg("scale"));
+    m.def("kv_copy", &kv_copy, "sequences of the 8-bit cache copied, in place or into another one", py::arg("k_codes"),
+          py::arg("k_scales"), py::arg("v_codes"), py::arg("v_scales"), py::arg("k_tail"), py::arg("v_tail"),
+          py::arg("sources"), py::arg("lengths"), py::arg("to_k_codes"), py::arg("to_k_scales"), py::arg("to_v_codes"),
+          py::arg("to_v_scales"), py::arg("to_k_tail"), py::arg("to_v_tail"));
+    m.def("kv_shared_attention", &kv_shared_attention, "attention of the newest tokens over a shared prefix and their own cache",
+          py::arg("q"), py::arg("pk_codes"), py::arg("pk_scales"), py::arg("pv_codes"), py::arg("pv_scales"),
+          py::arg("pk_tail"), py::arg("pv_tail"), py::arg("prefix_lengths"), py::arg("k_codes"), py::arg("k_scales"),
+          py::arg("v_codes"), py::arg("v_scales"), py::arg("k_tail"), py::arg("v_tail"), py::arg("lengths"),
+          py::arg("scale"));
+    m.def("beam_select", &beam_select, "the best continuations of each sequence's beams", py::arg("logits"), py::arg("scores"),
+          py::arg("finished"), py::arg("end"), py::arg("count"));
     m.def("distill", &distill, "distillation loss against a teacher's top logits (autograd node)", py::arg("logits"),
           py::arg("values"), py::arg("indices"), py::arg("temperature"), py::arg("weights"), py::arg("reduction"));
 }

@@ -470,6 +470,53 @@ int axs6_kv_attention(const void* q, int32_t dtype, int64_t B, int64_t Tq, int64
                       const float* v_scales, int64_t blocks, const int64_t* lengths, float scale, void* out,
                       void* workspace, int64_t workspace_bytes, void* stream);
 
+/* Sequences copied: target sequence i of group g (targets each) becomes the cache's
+ * sequence sources[g * targets + i] of that group (sequences each), its first
+ * lengths[] tokens (one for each of the cache's groups * sequences, clamped to both
+ * capacities): whole blocks' codes and scales, and the raw rows of a partial one.  A
+ * source outside 0 .. sequences - 1 leaves its target as it was, and so does all that
+ * lies behind the copied tokens.  The outputs are a cache of the same heads and dtype,
+ * or the cache itself (every pointer the same): then all of a group is read before it
+ * is written, and a group has at most AXS6_KV_COPY_MAX_IN_PLACE sequences. */
+#define AXS6_KV_COPY_MAX_IN_PLACE 4096
+int axs6_kv_copy(const void* k_codes, const float* k_scales, const void* v_codes, const float* v_scales,
+                 const void* k_tail, const void* v_tail, int32_t dtype, int64_t groups, int64_t sequences,
+                 int64_t targets, int64_t H, int64_t D, int64_t blocks, const int64_t* sources, const int64_t* lengths,
+                 int64_t target_blocks, void* k_codes_out, float* k_scales_out, void* v_codes_out, float* v_scales_out,
+                 void* k_tail_out, void* v_tail_out, void* stream);
+/* Attention of P * W sequences, of which W in a row share a prefix: sequence b holds
+ * the prefix_lengths[b / W] tokens of the first cache's sequence b / W and then the
+ * lengths[b] tokens of its own in the second; q (P * W, Tq, Hq, D) are its last Tq.
+ * Query t sees the keys at places j <= prefix + own - Tq + t (none: 0).  As
+ * axs6_kv_attention otherwise; blocks may be 0, prefix_blocks not. */
+int64_t axs6_kv_shared_attention_workspace(int64_t P, int64_t W, int64_t Tq, int64_t Hq, int64_t H, int64_t D,
+                                           int64_t prefix_blocks, int64_t blocks);
+int axs6_kv_shared_attention(const void* q, int32_t dtype, int64_t P, int64_t W, int64_t Tq, int64_t Hq, int64_t H,
+                             int64_t D, const int64_t* q_strides, const void* prefix_k_codes,
+                             const float* prefix_k_scales, const void* prefix_v_codes, const float* prefix_v_scales,
+                             int64_t prefix_blocks, const int64_t* prefix_lengths, const void* k_codes,
+                             const float* k_scales, const void* v_codes, const float* v_scales, int64_t blocks,
+                             const int64_t* lengths, float scale, void* out, void* workspace, int64_t workspace_bytes,
+                             void* stream);
+
+/* ---- beam search's selection ------------------------------------------------------
+ * Of the W beams of each of G sequences, with logits (G, W, V) (ld_sequence and ld_beam
+ * elements apart, a row's adjacent) and scores (G, W), the `count` best continuations:
+ *   score of (w, j) = scores[w] + logits[w][j] - log sum_j exp(logits[w][j]),
+ * the largest first, equal ones in the order of w V + j.  finished (may be NULL): bytes,
+ * nonzero where a beam has ended; it offers (w, end) with its own score, its logits are
+ * not read.  A logit of -inf is no candidate, nor is any of a beam of score -inf, whose
+ * logits are not read.  Slots without a candidate: score -inf, parent and token 0.  A NaN or +inf that
+ * counts: the sequence's scores NaN, parents and tokens 0.  Sums in float64; scores
+ * rounded once to float32.  Outputs (G, count). */
+#define AXS6_BEAM_MAX_COUNT 128
+#define AXS6_BEAM_MAX_BEAMS 1024   /* of a sequence; of all 65535 */
+int64_t axs6_beam_select_workspace(int64_t G, int64_t W, int64_t V, int32_t dtype);
+int axs6_beam_select(const void* logits, int32_t dtype, int64_t G, int64_t W, int64_t V, int64_t ld_sequence,
+                     int64_t ld_beam, const float* scores, const uint8_t* finished, int64_t end, int64_t count,
+                     float* out_scores, int64_t* parents, int64_t* tokens, void* workspace, int64_t workspace_bytes,
+                     void* stream);
+
 /* ---- distillation ----------------------------------------------------------------
  * Loss of student logits (N, V) (rows ld apart) against a teacher's top K logits
  * of each row (values, indices (N, K); an index below 0 leaves its entry out):
