@@ -93,7 +93,7 @@ _SIGNATURES: dict[str, list] = {
                           ctypes.c_float, _vp, _vp, _i64, _vp],
     "axs6_kv_copy": [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _vp,
                      _vp, _vp, _vp, _vp, _vp],
-    "axs6_kv_shared_attention_workspace": [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64],
+    "axs6_kv_shared_attention_workspace": [_i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64],
     "axs6_kv_shared_attention": [_vp, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp,
                                  _vp, _vp, _vp, _i64, _vp, ctypes.c_float, _vp, _vp, _i64, _vp],
     "axs6_beam_select_workspace": [_i64, _i64, _i64, _i32],

@@ -32,24 +32,11 @@
 // tokens 22.8 -> 25.7 us.
 #include <math.h>
 
-#include <type_traits>
-
-#include "axs6_internal.h"
-#include "kv_cache.h"
-#include "nf5_device.h"
+#include "kv_attention.h"
 #include "split_join.h"
 
 namespace axs6 {
 namespace {
-
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kProbScale = 16384.0f;   // 2^14
-constexpr float kSumScale = 1048576.0f;  // 2^20: sums are held as 2^-20 of themselves, so that values near
-                                         // float32's largest, summed before they are divided, stay finite
 
 struct KvAttnArgs {
     const void* q;
@@ -63,55 +50,7 @@ struct KvAttnArgs {
     int H, G, Tq, D, nb, rows, row_tiles, splits;
     int qvec;
     float scale;
-    // a prefix that W sequences share: the sequences' own lengths and blocks.  The prefix's
-    // rows are those of all W, (sequence, token, head)
-    const int64_t* own_lengths;
-    int W, own_nb;
-    int split0, splits_all;   // of the row's splits, the first of this launch, and their number
 };
-
-__device__ __forceinline__ int64_t clamp_length(int64_t n, int nb) {
-    const int64_t cap = (int64_t)nb * kKvBlock;
-    return n < 0 ? 0 : n > cap ? cap : n;
-}
-
-// Eight int8 codes as f16: with the sign bit flipped a byte u is code + 128,
-// and the f16 with the bits 0x6400 | u is 1024 + u.  SMALL: times 2^-20 (bits 0x1400 | u),
-// 1 / kSumScale, where a block's scale times that might itself be too small for float32.
-template <bool SMALL>
-__device__ __forceinline__ f16x8 codes_f16(uint32_t a, uint32_t b) {
-    constexpr uint32_t kHigh = SMALL ? 0x14141414u : 0x64646464u;
-    union { uint32_t w[4]; f16x2 h[4]; f16x8 v; } r;
-    a ^= 0x80808080u;
-    b ^= 0x80808080u;
-    r.w[0] = __builtin_amdgcn_perm(kHigh, a, 0x04010400u);
-    r.w[1] = __builtin_amdgcn_perm(kHigh, a, 0x04030402u);
-    r.w[2] = __builtin_amdgcn_perm(kHigh, b, 0x04010400u);
-    r.w[3] = __builtin_amdgcn_perm(kHigh, b, 0x04030402u);
-    constexpr float kBias = SMALL ? 1152.0f / kSumScale : 1152.0f;
-    const f16x2 bias = {(_Float16)kBias, (_Float16)kBias};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r.h[i] = r.h[i] - bias;
-    return r.v;
-}
-
-__device__ __forceinline__ f32x4 mma(f16x8 a, f16x8 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-}
-
-// Sixteen values of a query from element i.
-template <int DT>
-__device__ __forceinline__ void load16(const void* p, int64_t i, bool vec, float* f) {
-    using E = Elem<DT>;
-    const auto* q = reinterpret_cast<const typename E::S*>(p) + i;
-    if (vec) {
-#pragma unroll
-        for (int j = 0; j < 16; j += E::V) E::unpack(*reinterpret_cast<const u32x4*>(q + j), f + j);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) f[j] = E::to_f(q[j]);
-    }
-}
 
 // A block's codes as a lane takes them.
 template <int NC>
@@ -138,8 +77,7 @@ __device__ __forceinline__ void load_block(u32x4 (&k)[2][NC], uint2 (&v)[NC * 4]
 // NC: 64-value pieces of a head.  NR: 16-row pieces of queries that a wave takes
 // against each block.  WAVES: of a workgroup, each of which takes every WAVES-th
 // block of its range.
-// PREFIX: the cache's sequence is the prefix of W sequences, whose rows all attend over it.
-template <int DT, int NC, int NR, int WAVES, bool PREFIX>
+template <int DT, int NC, int NR, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void kv_attention_kernel(KvAttnArgs a) {
     constexpr int TERMS = DT == AXS6_F32 ? 2 : 1;
     constexpr int ND = NC * 4;   // 16-value pieces of a head
@@ -147,10 +85,11 @@ __global__ __launch_bounds__(64 * WAVES) void kv_attention_kernel(KvAttnArgs a) 
     __shared__ float sh_m[WAVES][NR * 16], sh_l[WAVES][NR * 16];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n16 = lane & 15, g4 = lane >> 4;
     const int rt = blockIdx.x % a.row_tiles, bh = blockIdx.x / a.row_tiles, h = bh % a.H, b = bh / a.H;
-    const int64_t len = clamp_length(a.lengths[b], a.nb);
+    const int64_t cap = (int64_t)a.nb * kKvBlock;
+    int64_t len = a.lengths[b];
+    len = len < 0 ? 0 : len > cap ? cap : len;
     const int r0 = rt * NR * 16, r_top = r0 + NR * 16 < a.rows ? r0 + NR * 16 - 1 : a.rows - 1;
-    const int per_seq = a.Tq * a.G;   // rows of a sequence
-    const int keys = PREFIX ? (int)len : (int)(len - a.Tq) + r_top / a.G + 1;
+    const int keys = (int)(len - a.Tq) + r_top / a.G + 1;
     const int blocks = keys <= 0 ? 0 : (keys + kKvBlock - 1) / kKvBlock;
     const int per = (blocks + a.splits - 1) / a.splits;
     const int b0 = blockIdx.y * per, b1 = b0 + per < blocks ? b0 + per : blocks;
@@ -165,27 +104,15 @@ __global__ __launch_bounds__(64 * WAVES) void kv_attention_kernel(KvAttnArgs a) 
     int last[NR];   // the last key that the lane's row sees
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
-        int r = r0 + 16 * n + n16;
-        r = r < a.rows ? r : a.rows - 1;
-        int64_t seq = b;
-        if constexpr (PREFIX) {
-            seq = (int64_t)b * a.W + r / per_seq;
-            r %= per_seq;
-        }
-        const int t = r / a.G, hq = h * a.G + r % a.G;
+        const int r = r0 + 16 * n + n16, rr = r < a.rows ? r : a.rows - 1, t = rr / a.G, hq = h * a.G + rr % a.G;
         last[n] = (int)(len - a.Tq) + t;
-        // the places of a sequence's own tokens follow the prefix's
-        if constexpr (PREFIX) {
-            const int64_t to = last[n] + clamp_length(a.own_lengths[seq], a.own_nb);
-            last[n] = (int)(to < len ? to : len - 1);
-        }
         float f[NC][16], amax = 0.0f;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
 #pragma unroll
             for (int j = 0; j < 16; ++j) f[c][j] = 0.0f;
             if (64 * c + 16 * g4 < a.D)
-                load16<DT>(a.q, seq * a.qs[0] + t * a.qs[1] + hq * a.qs[2] + 64 * c + 16 * g4, a.qvec, f[c]);
+                load16<DT>(a.q, b * a.qs[0] + t * a.qs[1] + hq * a.qs[2] + 64 * c + 16 * g4, a.qvec, f[c]);
 #pragma unroll
             for (int j = 0; j < 16; ++j) amax = fmaxf(amax, fabsf(f[c][j]));
         }
@@ -316,10 +243,9 @@ __global__ __launch_bounds__(64 * WAVES) void kv_attention_kernel(KvAttnArgs a) 
     for (int n = 0; n < NR; ++n) {
         const int r = r0 + 16 * n + n16, t = r / a.G, hq = h * a.G + r % a.G;
         if (r >= a.rows) continue;
-        int64_t row = (int64_t)bh * a.rows + r;
-        if constexpr (PREFIX) row = (((int64_t)b * a.W + r / per_seq) * a.H + h) * per_seq + r % per_seq;
-        if (PREFIX || a.splits_all > 1) {
-            const int64_t at = (a.split0 + blockIdx.y) * a.rows_all + row;
+        const int64_t row = (int64_t)bh * a.rows + r;
+        if (a.splits > 1) {
+            const int64_t at = blockIdx.y * a.rows_all + row;
             if (g4 == 0) { a.stat[2 * at] = mt[n]; a.stat[2 * at + 1] = lt[n]; }
 #pragma unroll
             for (int d = 0; d < ND; ++d)
@@ -344,9 +270,9 @@ __global__ __launch_bounds__(kJoinThreads) void kv_join_kernel(KvAttnArgs a) {
     int64_t row = blockIdx.x;
     Joined j;
     if constexpr (FEW)
-        j = join_few(a.part, a.stat, a.rows_all, (int64_t)blockIdx.x * kJoinThreads + threadIdx.x, a.splits_all, a.D, row);
+        j = join_few(a.part, a.stat, a.rows_all, (int64_t)blockIdx.x * kJoinThreads + threadIdx.x, a.splits, a.D, row);
     else
-        j = join_row(a.part, a.stat, a.rows_all, row, a.splits_all, a.D);
+        j = join_row(a.part, a.stat, a.rows_all, row, a.splits, a.D);
     if (j.d < 0) return;
     const int64_t bh = row / a.rows;
     const int r = (int)(row - bh * a.rows), t = r / a.G, hq = (int)(bh % a.H) * a.G + r % a.G;
@@ -389,62 +315,35 @@ Plan plan(int64_t BH, int64_t rows, int64_t D, int64_t blocks) {
     return p;
 }
 
-template <int DT, int NC, bool PREFIX>
+template <int DT, int NC>
 void launch_kernel(const KvAttnArgs& a, const Plan& p, int64_t B, hipStream_t st) {
     const dim3 grid((unsigned)(B * a.H * a.row_tiles), (unsigned)a.splits);
     if constexpr (NC <= 2) {
         if (p.waves == 8) {
-            kv_attention_kernel<DT, NC, 1, 8, PREFIX><<<grid, 512, 0, st>>>(a);
+            kv_attention_kernel<DT, NC, 1, 8><<<grid, 512, 0, st>>>(a);
             return;
         }
         if (p.nr == 2) {
-            kv_attention_kernel<DT, NC, 2, 4, PREFIX><<<grid, 256, 0, st>>>(a);
+            kv_attention_kernel<DT, NC, 2, 4><<<grid, 256, 0, st>>>(a);
             return;
         }
     }
-    kv_attention_kernel<DT, NC, 1, 4, PREFIX><<<grid, 256, 0, st>>>(a);
-}
-
-template <int DT, bool PREFIX>
-void launch_part(const KvAttnArgs& a, const Plan& p, int64_t B, hipStream_t st) {
-    switch ((a.D + 63) / 64) {
-        case 1: launch_kernel<DT, 1, PREFIX>(a, p, B, st); break;
-        case 2: launch_kernel<DT, 2, PREFIX>(a, p, B, st); break;
-        case 3: launch_kernel<DT, 3, PREFIX>(a, p, B, st); break;
-        default: launch_kernel<DT, 4, PREFIX>(a, p, B, st); break;
-    }
+    kv_attention_kernel<DT, NC, 1, 4><<<grid, 256, 0, st>>>(a);
 }
 
 template <int DT>
-void launch_join(const KvAttnArgs& a, hipStream_t st) {
-    if (!join_by_value(a.rows_all, a.splits_all))
+void launch_attention(const KvAttnArgs& a, const Plan& p, int64_t B, hipStream_t st) {
+    switch ((a.D + 63) / 64) {
+        case 1: launch_kernel<DT, 1>(a, p, B, st); break;
+        case 2: launch_kernel<DT, 2>(a, p, B, st); break;
+        case 3: launch_kernel<DT, 3>(a, p, B, st); break;
+        default: launch_kernel<DT, 4>(a, p, B, st); break;
+    }
+    if (a.splits == 1) return;
+    if (!join_by_value(a.rows_all, a.splits))
         kv_join_kernel<DT, false><<<(unsigned)a.rows_all, kJoinThreads, 0, st>>>(a);
     else
         kv_join_kernel<DT, true><<<(unsigned)((a.rows_all * (a.D / 4) + kJoinThreads - 1) / kJoinThreads), kJoinThreads, 0, st>>>(a);
-}
-
-// Calls f with the dtype code as a constant.
-template <class F>
-void by_dtype(int dtype, F f) {
-    if (dtype == AXS6_F32) f(std::integral_constant<int, AXS6_F32>{});
-    else if (dtype == AXS6_BF16) f(std::integral_constant<int, AXS6_BF16>{});
-    else f(std::integral_constant<int, AXS6_F16>{});
-}
-
-// A prefix and what follows it: each launch leaves partial sums, which are joined; at most
-// half of a row's splits each.
-Plan half_splits(Plan p) {
-    if (p.splits > kMaxSplits / 2) p.splits = kMaxSplits / 2;
-    return p;
-}
-Plan prefix_plan(int64_t P, int64_t W, int64_t H, int64_t rows, int64_t D, int64_t blocks) {
-    return half_splits(plan(P * H, W * rows, D, blocks));
-}
-Plan own_plan(int64_t B, int64_t H, int64_t rows, int64_t D, int64_t blocks) {
-    return half_splits(plan(B * H, rows, D, blocks));
-}
-int64_t shared_splits(int64_t P, int64_t W, int64_t H, int64_t rows, int64_t D, int64_t prefix_blocks, int64_t blocks) {
-    return prefix_plan(P, W, H, rows, D, prefix_blocks).splits + (blocks ? own_plan(P * W, H, rows, D, blocks).splits : 0);
 }
 
 }  // namespace
@@ -487,7 +386,7 @@ extern "C" int axs6_kv_attention(const void* q, int32_t dtype, int64_t B, int64_
     }
     a.H = (int)H; a.G = (int)(Hq / H); a.Tq = (int)Tq; a.D = (int)D; a.nb = (int)blocks; a.rows = (int)rows;
     const Plan p = plan(B * H, rows, D, blocks);
-    a.row_tiles = p.row_tiles; a.rows_all = B * H * rows; a.scale = scale; a.splits = a.splits_all = p.splits;
+    a.row_tiles = p.row_tiles; a.rows_all = B * H * rows; a.scale = scale; a.splits = p.splits;
     if (a.splits > 1) {
         const int64_t need = axs6_kv_attention_workspace(B, Tq, Hq, H, D, blocks);
         if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16)
@@ -497,81 +396,8 @@ extern "C" int axs6_kv_attention(const void* q, int32_t dtype, int64_t B, int64_
         a.stat = a.part + a.splits * a.rows_all * D;
     }
     hipStream_t st = (hipStream_t)stream;
-    by_dtype(dtype, [&](auto dt) {
-        launch_part<decltype(dt)::value, false>(a, p, B, st);
-        if (a.splits > 1) launch_join<decltype(dt)::value>(a, st);
-    });
-    return check_launch(fn);
-}
-
-extern "C" int64_t axs6_kv_shared_attention_workspace(int64_t P, int64_t W, int64_t Tq, int64_t Hq, int64_t H, int64_t D,
-                                                      int64_t prefix_blocks, int64_t blocks) {
-    if (P <= 0 || W <= 0 || Tq <= 0 || H <= 0 || Hq <= 0 || Hq % H || D <= 0 || prefix_blocks <= 0) return 0;
-    const int64_t rows = Tq * (Hq / H);
-    return shared_splits(P, W, H, rows, D, prefix_blocks, blocks) * P * W * H * rows * (D + 2) * (int64_t)sizeof(float);
-}
-
-extern "C" int axs6_kv_shared_attention(const void* q, int32_t dtype, int64_t P, int64_t W, int64_t Tq, int64_t Hq,
-                                        int64_t H, int64_t D, const int64_t* q_strides, const void* pk_codes,
-                                        const float* pk_scales, const void* pv_codes, const float* pv_scales,
-                                        int64_t prefix_blocks, const int64_t* prefix_lengths, const void* k_codes,
-                                        const float* k_scales, const void* v_codes, const float* v_scales, int64_t blocks,
-                                        const int64_t* lengths, float scale, void* out, void* workspace,
-                                        int64_t workspace_bytes, void* stream) {
-    const char* fn = "axs6_kv_shared_attention";
-    if (!valid_dtype(dtype)) return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: unknown dtype code %d", fn, dtype);
-    constexpr int64_t kMost = ((int64_t)1 << 31) - 1;
-    if (P < 0 || W < 0 || P > kMost || W > kMost || P * W > kMost)
-        return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: bad number of sequences", fn);
-    int rc = check_cache(fn, P, H, D, prefix_blocks, pk_codes, pk_scales, pv_codes, pv_scales);
-    if (rc) return rc;
-    const int64_t B = P * W;
-    rc = check_cache(fn, B, H, D, blocks, k_codes, k_scales, v_codes, v_scales);
-    if (rc) return rc;
-    if (Tq < 0 || Hq < 0 || (H > 0 && Hq % H))
-        return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: %lld query heads for %lld key heads", fn, (long long)Hq, (long long)H);
-    if (!isfinite(scale)) return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: the scale must be finite", fn);
-    if (B * Tq * Hq == 0) return AXS6_OK;
-    if (H == 0 || prefix_blocks == 0) return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: an empty prefix", fn);
-    if (!q || !q_strides || !prefix_lengths || !lengths || !out)
-        return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: null operand", fn);
-    const int64_t es = dtype == AXS6_F32 ? 4 : 2, vl = 16 / es, rows = Tq * (Hq / H);
-    if (rows > (1 << 24) || W * rows > (1 << 24) || B * H * rows > kMost)
-        return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: dimension too large", fn);
-    if ((uintptr_t)q % es || (uintptr_t)out % es)
-        return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: pointer not element-aligned", fn);
-    const int64_t need = axs6_kv_shared_attention_workspace(P, W, Tq, Hq, H, D, prefix_blocks, blocks);
-    if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16)
-        return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: a 16-byte aligned workspace of %lld bytes required, got %lld", fn,
-                    (long long)need, (long long)workspace_bytes);
-    KvAttnArgs a{};
-    a.q = q; a.out = out; a.scale = scale;
-    a.qvec = (uintptr_t)q % 16 == 0;
-    for (int i = 0; i < 3; ++i) {
-        a.qs[i] = q_strides[i];
-        a.qvec = a.qvec && q_strides[i] % vl == 0;
-    }
-    a.H = (int)H; a.G = (int)(Hq / H); a.Tq = (int)Tq; a.D = (int)D; a.rows_all = B * H * rows;
-    a.own_lengths = lengths; a.own_nb = (int)blocks; a.W = (int)W;
-    a.splits_all = (int)shared_splits(P, W, H, rows, D, prefix_blocks, blocks);
-    a.part = reinterpret_cast<float*>(workspace);
-    a.stat = a.part + a.splits_all * a.rows_all * D;
-    // the prefix
-    KvAttnArgs s = a;
-    s.kc = reinterpret_cast<const int8_t*>(pk_codes); s.vc = reinterpret_cast<const int8_t*>(pv_codes);
-    s.ks = pk_scales; s.vs = pv_scales; s.lengths = prefix_lengths; s.nb = (int)prefix_blocks; s.rows = (int)(W * rows);
-    const Plan ps = prefix_plan(P, W, H, rows, D, prefix_blocks);
-    s.row_tiles = ps.row_tiles; s.splits = ps.splits;
-    // the sequences' own tokens
-    a.kc = reinterpret_cast<const int8_t*>(k_codes); a.vc = reinterpret_cast<const int8_t*>(v_codes);
-    a.ks = k_scales; a.vs = v_scales; a.lengths = lengths; a.nb = (int)blocks; a.rows = (int)rows;
-    const Plan po = own_plan(B, H, rows, D, blocks);
-    a.row_tiles = po.row_tiles; a.splits = po.splits; a.split0 = ps.splits;
-    hipStream_t st = (hipStream_t)stream;
-    by_dtype(dtype, [&](auto dt) {
-        launch_part<decltype(dt)::value, true>(s, ps, P, st);
-        if (blocks) launch_part<decltype(dt)::value, false>(a, po, B, st);
-        launch_join<decltype(dt)::value>(a, st);
-    });
+    if (dtype == AXS6_F32) launch_attention<AXS6_F32>(a, p, B, st);
+    else if (dtype == AXS6_BF16) launch_attention<AXS6_BF16>(a, p, B, st);
+    else launch_attention<AXS6_F16>(a, p, B, st);
     return check_launch(fn);
 }

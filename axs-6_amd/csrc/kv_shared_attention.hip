@@ -1,0 +1,671 @@
+// Attention of sequences that share a prefix, over the 8-bit cache.
+//
+// W sequences in a row continue one prefix.  Sequence b's tokens are the prefix's n_p and
+// then the n_b of its own cache; query t (of Tq) stands at place n_p + n_b - Tq + t and
+// sees the places up to its own:
+//   x_j = scale * ks * (q . kc_j),  o = sum_j softmax(x)_j vs * vc_j
+// over the keys of both caches (codes kc, vc, a block's scales ks, vs).  The prefix is read
+// once for the rows of all W sequences, W Tq G of a key head.
+//
+// One launch for both, in which a workgroup takes up to 64 rows against a piece of the prefix,
+// or a sequence's rows against its own blocks (those are bound by HBM, the prefix's with
+// many rows by the matrix cores and the softmax: side by side each hides the other), and
+// leaves maximum, sum and D sums a row; a second launch joins a row's pieces.  The prefixes'
+// pieces are cut from all the blocks that they hold, so that workgroups have equal work
+// whatever the lengths, which only the device knows.
+//
+// A wave holds 16 or 32 rows in registers and takes every fourth block of its workgroup's; codes
+// come straight from memory into a ring of blocks in LDS that is the wave's own, so no
+// barrier stands in the loop.  Products as in the cache attention (S^T = K q^T by
+// 16x16x32 f16 instructions in which codes are exact, probabilities stay in their lanes).
+// A block's value scale goes into its probabilities' exponent, which counts from a reference of its own; the
+// references move only when a score passes them by kSlack, and between that the sums stay where the products add
+// to them.  Probabilities go in as f16 times 2^11 (float32: two terms), 11 bits down to 2^-25 of the largest.
+#include "kv_attention.h"
+
+namespace axs6 {
+namespace {
+
+typedef __attribute__((address_space(3))) void lds_void;
+
+constexpr int kSharedWaves = 4, kSharedThreads = 64 * kSharedWaves;
+constexpr float kSlack = 4.0f;          // in units of log2
+constexpr int kWeightLog2 = 11;         // probabilities go in times 2^11; with 2^kSlack still an f16
+constexpr int kSumLog2 = 20;            // kSumScale
+constexpr int kMaxEven = 64;            // prefixes whose blocks are shared out evenly
+
+struct SharedArgs {
+    const void* q;
+    int64_t qs[3];                      // batch, token, head, in elements
+    const int8_t *kc[2], *vc[2];        // the prefixes, the sequences' own
+    const float *ks[2], *vs[2];
+    const int64_t* lengths[2];
+    void* out;                          // (B, Tq, Hq, D) contiguous
+    float* part[2];                     // of each piece, head and row D sums; then (maximum, sum)
+    float* stat[2];
+    int P, W, H, G, Tq, D, qvec;
+    int nb[2];                          // blocks
+    int rows[2], row_tiles[2];          // of a head: W Tq G, Tq G
+    int pieces[2];                      // of all prefixes; of each sequence
+    int even;                           // whether the prefixes' pieces are cut from all their blocks
+    int units, prefix_groups;           // (piece, head) of the prefixes; workgroups that take them
+    float scale;
+};
+
+__device__ __forceinline__ int clamp_length(int64_t n, int nb) {
+    const int64_t cap = (int64_t)nb * kKvBlock;
+    return (int)(n < 0 ? 0 : n > cap ? cap : n);
+}
+__device__ __forceinline__ float uniform(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
+}
+__device__ __forceinline__ float lane_value(float x, int lane) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), lane));
+}
+__device__ __forceinline__ int blocks_of(int n) { return (n + kKvBlock - 1) / kKvBlock; }
+
+// The pieces of the prefixes.  Even: lane p < P <= 64 has prefix p; every piece is of `size`
+// blocks but each prefix's last, size the smallest with which all pieces suffice.  Else a
+// prefix has pieces / P of them.
+struct Pieces {
+    int blocks, size, first, count;   // the lane's prefix: blocks, of a piece, first piece, pieces
+};
+__device__ __forceinline__ Pieces even_pieces(const SharedArgs& a, int lane) {
+    Pieces c;
+    c.blocks = lane < a.P ? blocks_of(clamp_length(a.lengths[0][lane], a.nb[0])) : 0;
+    int total = c.blocks;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) total += __shfl_xor(total, o, 64);
+    const int spare = a.pieces[0] - a.P + 1;   // a prefix's last piece may be short: P - 1 pieces more
+    c.size = (total + spare - 1) / spare;
+    c.size = c.size < 1 ? 1 : c.size;
+    c.count = (c.blocks + c.size - 1) / c.size;
+    c.first = c.count;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int x = __shfl_up(c.first, o, 64);
+        if (lane >= o) c.first += x;
+    }
+    c.first -= c.count;
+    return c;
+}
+
+// A head of up to 16 ND values in LDS: a block's key codes, 32 rows of kRow 16-byte pieces, and its value codes, 16 ND
+// rows of two.
+template <int ND> constexpr int kRow = ND <= 4 ? 4 : ND <= 8 ? 8 : 16;
+template <int ND> constexpr int kKeyBytes = kKvBlock * kRow<ND> * 16;
+template <int ND> constexpr int kSlotBytes = kKeyBytes<ND> + ND * 512;
+// A wave's blocks in LDS, that it computes on and those on their way; the instructions that fetch one; waves a SIMD.
+template <int ND> constexpr int kSlots = 2;
+template <int ND> constexpr int kFetches = kRow<ND> / 2 + ND / 2;
+template <int ND> constexpr int kOccupancy = ND <= 8 ? 2 : 1;
+template <int ND> constexpr int kRingBytes = kSlots<ND> * kSlotBytes<ND>;
+
+// Waits until at most `ahead` blocks (ahead <= MOST, uniform) are still on their way.
+template <int MOST, int FETCHES>
+__device__ __forceinline__ void wait_blocks(int ahead) {
+    if constexpr (MOST == 0) {
+        __builtin_amdgcn_s_waitcnt(0x0070 | (0xf << 8));   // vmcnt(0)
+    } else {
+        constexpr int N = MOST * FETCHES;
+        static_assert(N < 64, "vmcnt's range");
+        if (ahead >= MOST) __builtin_amdgcn_s_waitcnt((N & 0xf) | ((N >> 4) << 14) | (0x7 << 4) | (0xf << 8));
+        else wait_blocks<MOST - 1, FETCHES>(ahead);
+    }
+}
+
+// Piece j of key row r lies in place j ^ key_turn(r): the 16 rows that a fragment reads at one piece, 8 a + 4 tt + b, fall
+// on all banks.  Of r = 64 i / kRow + lane / kRow it is key_turn(64 i / kRow) ^ key_turn(lane / kRow).
+template <int ND> __device__ __forceinline__ constexpr int key_turn(int r) {
+    constexpr int L = kRow<ND> == 4 ? 0 : kRow<ND> == 8 ? 1 : 2;
+    return ((r >> 3) & 3) << L | (r & 3) >> (2 - L);
+}
+
+// A block's codes on their way to the wave's slot, 1 KB an instruction; what lies past the head's values arrives as
+// zeros.  The two halves of a value's row change places in rows 8 .. 15 of 16.
+template <int ND>
+__device__ __forceinline__ void fetch_block(char* slot, const int8_t* kc, const int8_t* vc, int64_t cell, int D, int lane) {
+#if defined(__HIP_DEVICE_COMPILE__)   // the host pass knows no 16-byte form and would drop the kernel's stub
+    const int bytes = kKvBlock * D;
+    const auto kr = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(kc + cell * bytes), 0, bytes, 0x00020000);
+    const auto vr = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(vc + cell * bytes), 0, bytes, 0x00020000);
+    asm("" : "+v"(lane));   // the places are made again each time: as values kept over the loop they would cost registers
+    const int row = lane / kRow<ND>, turned = lane % kRow<ND> ^ key_turn<ND>(row), at = row * D;
+#pragma unroll
+    for (int i = 0; i < kRow<ND> / 2; ++i) {
+        const int j16 = (turned ^ key_turn<ND>(64 * i / kRow<ND>)) * 16;
+        const int off = ND % 4 == 0 && D == 16 * kRow<ND> ? at + j16 : j16 < D ? at + j16 : bytes;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (lds_void*)(slot + i * 1024), 16, off, 64 * i / kRow<ND> * D, 0, 0);
+    }
+    const int half = (lane ^ ((lane >> 4) & 1)) * 16;
+#pragma unroll
+    for (int i = 0; i < ND / 2; ++i)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lds_void*)(slot + kKeyBytes<ND> + i * 1024), 16, half, i * 1024, 0, 0);
+#endif
+}
+
+// Up to 16 NR rows of one key head against blocks [b0, b1) of sequence `set` of a cache: S 0, a
+// prefix (rows of all its W sequences), or 1, a sequence's own.
+template <int DT, int ND, int NR, int S>
+__device__ __forceinline__ void attend(const SharedArgs& a, char* ring, int set, int h, int rt, int b0, int b1,
+                                       int64_t row0) {
+    constexpr int TERMS = DT == AXS6_F32 ? 2 : 1;
+    constexpr int NC = (ND + 3) / 4;   // 64-value pieces of a key's row
+    static_assert(2 * NR * ND * 4 * 256 <= kSharedWaves * kRingBytes<ND>, "the waves' sums fit the rings");
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n16 = lane & 15, g4 = lane >> 4;
+    const int len = clamp_length(a.lengths[S][set], a.nb[S]);
+    const int64_t cell0 = ((int64_t)set * a.H + h) * a.nb[S];
+    const int per_seq = a.Tq * a.G, r0 = rt * NR * 16;
+    char* my_ring = ring + wave * kRingBytes<ND>;
+    // the scales of the wave's next 64 blocks, one a lane; then the first blocks
+    float ks64, vs64;
+    auto load_scales = [&](int blk) {
+        const int mine = blk + lane * kSharedWaves;
+        ks64 = mine < b1 ? a.ks[S][cell0 + mine] : 0.0f;
+        vs64 = mine < b1 ? a.vs[S][cell0 + mine] : 0.0f;
+    };
+    load_scales(b0 + wave);
+#pragma unroll
+    for (int i = 0; i < kSlots<ND> - 1; ++i) {
+        const int blk = b0 + wave + i * kSharedWaves;
+        if (blk < b1) fetch_block<ND>(my_ring + i * kSlotBytes<ND>, a.kc[S], a.vc[S], cell0 + blk, a.D, lane);
+    }
+
+    // the rows' queries, scaled, in the products' order: piece c, value 16 g4 + j
+    f16x8 qf[NR][TERMS][NC][2];
+    float rs[NR];
+    int last[NR];   // the last key that the lane's row sees
+    int whole = len;   // keys that all the wave's rows see
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+        int r = r0 + 16 * n + n16;
+        r = r < a.rows[S] ? r : a.rows[S] - 1;
+        const int seq = S ? set : set * a.W + r / per_seq;
+        r = S ? r : r % per_seq;
+        const int t = r / a.G, hq = h * a.G + r % a.G;
+        last[n] = len - a.Tq + t;
+        if constexpr (S == 0) {   // the sequence's own tokens follow the prefix's
+            const int64_t to = (int64_t)last[n] + clamp_length(a.lengths[1][seq], a.nb[1]);
+            last[n] = (int)(to < len ? to : len - 1);
+        }
+        whole = last[n] + 1 < whole ? last[n] + 1 : whole;
+        float f[NC][16], amax = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) f[c][j] = 0.0f;
+            if (64 * c + 16 * g4 < a.D)
+                load16<DT>(a.q, (int64_t)seq * a.qs[0] + t * a.qs[1] + hq * a.qs[2] + 64 * c + 16 * g4, a.qvec, f[c]);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) amax = fmaxf(amax, fabsf(f[c][j]));
+        }
+        amax = fmaxf(amax, __shfl_xor(amax, 16, 64));
+        amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
+        const int e = amax > 0.0f && isfinite(amax) ? ilogbf(amax) - 7 : 0;
+        const float sign = a.scale < 0.0f ? -1.0f : 1.0f;   // the largest product is then the largest score
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const float x = ldexpf(sign * f[c][j], -e);
+                const _Float16 hi = (_Float16)x;
+                qf[n][0][c][j >> 3][j & 7] = hi;
+                if constexpr (TERMS == 2) qf[n][1][c][j >> 3][j & 7] = (_Float16)(x - (float)hi);
+            }
+        rs[n] = ldexpf(fabsf(a.scale) * kLog2e, e);
+    }
+    // value scales count from the largest one's power of two
+    float largest = 0.0f;
+    for (int i = b0 + lane; i < b1; i += 64) largest = fmaxf(largest, a.vs[S][cell0 + i]);
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+        largest = fmaxf(largest, __shfl_xor(largest, o, 64));
+        const int x = __shfl_xor(whole, o, 64);
+        whole = x < whole ? x : whole;
+    }
+    const int unit = __builtin_amdgcn_readfirstlane(largest > 0.0f ? ilogbf(largest) : 0);
+    whole = __builtin_amdgcn_readfirstlane(whole);
+
+    // l counts from the maximum m, o from the maximum w of x + log2(value scale)
+    f32x4 o[NR][ND];
+    float m[NR], w[NR], l[NR];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[n][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        m[n] = w[n] = -INFINITY;
+        l[n] = 0.0f;
+    }
+    // fragments: key row 8 (n16 / 4) + 4 tt + n16 % 4, piece 4 c + g4; value row 16 d + n16, keys 8 g4 .. 8 g4 + 7
+    const int key_row = 8 * (n16 >> 2) + (n16 & 3);
+    const int key_at = (key_row * kRow<ND> + (g4 ^ key_turn<ND>(key_row))) * 16;
+    const int value_at = kKeyBytes<ND> + (n16 * 2 + ((g4 >> 1) ^ (n16 >> 3))) * 16 + (g4 & 1) * 8;
+    asm volatile("" : "+v"(ks64), "+v"(vs64));   // they are here
+    int step = 0, at = 0;   // the slot of the block
+    for (int blk = b0 + wave; blk < b1; blk += kSharedWaves, ++step) {
+        // the block is there
+        asm volatile("" ::: "memory");
+        wait_blocks<kSlots<ND> - 2, kFetches<ND>>((b1 - 1 - blk) / kSharedWaves);
+        asm volatile("" ::: "memory");
+        if (step % 64 == 0 && step) {
+            load_scales(blk);
+            asm volatile("" : "+v"(ks64), "+v"(vs64));
+        }
+        const float ks = lane_value(ks64, step % 64), vs = lane_value(vs64, step % 64);
+        const char* slot = my_ring + at * kSlotBytes<ND>;
+        // the slot of the block before is free: all reads of it have come back, for its products are done
+        const int next = blk + (kSlots<ND> - 1) * kSharedWaves, free_at = at == 0 ? kSlots<ND> - 1 : at - 1;
+        if (next < b1) fetch_block<ND>(my_ring + free_at * kSlotBytes<ND>, a.kc[S], a.vc[S], cell0 + next, a.D, lane);
+        at = at + 1 == kSlots<ND> ? 0 : at + 1;
+        // Codes are read a step ahead, and the steps stand apart (sched_barrier): else the compiler, with all reads
+        // first, wants more registers than there are.
+        f32x4 s[NR][2];
+        auto key_codes = [&](int i) {
+            return *reinterpret_cast<const u32x4*>(slot + (key_at ^ i / 2 * 64) + i % 2 * 4 * kRow<ND> * 16);
+        };
+        auto value_codes = [&](int d) { return *reinterpret_cast<const uint2*>(slot + value_at + d * 512); };
+#pragma unroll
+        for (int n = 0; n < NR; ++n) s[n][0] = s[n][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        u32x4 k = key_codes(0);
+#pragma unroll
+        for (int i = 0; i < 2 * NC; ++i) {   // both 16-key halves in turn: products that do not wait for each other
+            const u32x4 next = key_codes(i + 1 < 2 * NC ? i + 1 : i);
+            const f16x8 k0 = codes_f16<false>(k.x, k.y), k1 = codes_f16<false>(k.z, k.w);
+#pragma unroll
+            for (int n = 0; n < NR; ++n)
+#pragma unroll
+                for (int u = 0; u < TERMS; ++u) s[n][i % 2] = mma(k0, qf[n][u][i / 2][0], s[n][i % 2]);
+#pragma unroll
+            for (int n = 0; n < NR; ++n)
+#pragma unroll
+                for (int u = 0; u < TERMS; ++u) s[n][i % 2] = mma(k1, qf[n][u][i / 2][1], s[n][i % 2]);
+            k = next;
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        uint2 v = value_codes(0);
+        f16x8 pf[NR][TERMS];
+        float c[NR], lv[NR];   // what takes the products to units of log2; log2 of the value scale
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+            c[n] = rs[n] * ks;
+            c[n] = c[n] == 0.0f ? 1e-30f : c[n];   // so that it leaves -inf what it is
+            lv[n] = __builtin_amdgcn_logf(ldexpf(vs, -unit));
+        }
+        if ((blk + 1) * kKvBlock > whole) {
+#pragma unroll
+            for (int n = 0; n < NR; ++n) {
+                if (blk * kKvBlock > last[n]) { c[n] = 1.0f; lv[n] = 0.0f; }   // a row that sees none of it, whatever its scales
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (blk * kKvBlock + 8 * g4 + j > last[n]) s[n][j >> 2][j & 3] = -INFINITY;
+            }
+        }
+        float top[NR];
+        bool passed = false;
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+            top[n] = s[n][0][0];
+#pragma unroll
+            for (int j = 1; j < 8; ++j) top[n] = fmaxf(top[n], s[n][j >> 2][j & 3]);
+            top[n] *= c[n];
+            passed = passed || top[n] > m[n] + kSlack || top[n] + lv[n] > w[n] + kSlack;
+        }
+        if (__any(passed)) {
+#pragma unroll
+            for (int n = 0; n < NR; ++n) {
+                float mx = fmaxf(top[n], __shfl_xor(top[n], 16, 64));
+                mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+                const float mn = fmaxf(m[n], mx), wn = fmaxf(w[n], mx + lv[n]);
+                l[n] *= __builtin_amdgcn_exp2f(m[n] - (mn == -INFINITY ? 0.0f : mn));
+                const float alpha = __builtin_amdgcn_exp2f(w[n] - (wn == -INFINITY ? 0.0f : wn));
+                m[n] = mn;
+                w[n] = wn;
+#pragma unroll
+                for (int d = 0; d < ND; ++d) o[n][d] *= alpha;
+            }
+        }
+        // exponentials with the value scale in them; l's are the same ones but for a factor, where that is not too far off
+        bool far = false;
+        float back[NR];
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+            const float ref = w[n] == -INFINITY ? 0.0f : w[n], from = m[n] == -INFINITY ? 0.0f : m[n];
+            const float shift = lv[n] - ref, to_l = -from - shift;
+            far = far || !(fabsf(to_l) < 60.0f);
+            back[n] = __builtin_amdgcn_exp2f(to_l - kWeightLog2);
+            float sum = 0.0f, y[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                y[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][j >> 2][j & 3], c[n], shift + kWeightLog2));
+                sum += y[j];
+                pf[n][0][j] = (_Float16)y[j];
+                if constexpr (TERMS == 2) pf[n][1][j] = (_Float16)(y[j] - (float)pf[n][0][j]);
+            }
+            back[n] *= sum;
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (__any(far)) {
+#pragma unroll
+            for (int n = 0; n < NR; ++n) {
+                const float from = m[n] == -INFINITY ? 0.0f : m[n];
+                back[n] = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) back[n] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][j >> 2][j & 3], c[n], -from));
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NR; ++n) l[n] += back[n];
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+            const uint2 next = value_codes(d + 1 < ND ? d + 1 : d);
+            const f16x8 vf = codes_f16<false>(v.x, v.y);
+#pragma unroll
+            for (int n = 0; n < NR; ++n)
+#pragma unroll
+                for (int u = 0; u < TERMS; ++u) o[n][d] = mma(vf, pf[n][u], o[n][d]);
+            v = next;
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    // join the waves: the four lanes of a row, then the upper half of the waves into the lower
+    auto stats_of = [&](int i) { return reinterpret_cast<float2*>(ring + i * kRingBytes<ND>); };
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+        l[n] += __shfl_xor(l[n], 16, 64);
+        l[n] += __shfl_xor(l[n], 32, 64);
+        if (g4 == 0) stats_of(wave)[16 * n + n16] = make_float2(m[n], l[n]);
+    }
+    __syncthreads();
+    auto* sums = reinterpret_cast<float(*)[NR * ND * 4][64]>(ring);
+    float lt[NR], mt[NR];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+        float2 st[kSharedWaves];
+        mt[n] = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kSharedWaves; ++i) {
+            st[i] = stats_of(i)[16 * n + n16];
+            mt[n] = fmaxf(mt[n], st[i].x);
+        }
+        const float ref = mt[n] == -INFINITY ? 0.0f : mt[n];
+        lt[n] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kSharedWaves; ++i)
+            lt[n] += st[i].y * __builtin_amdgcn_exp2f(st[i].x - ref);
+        // from w to the maximum, in one step: a power of two, and 1 / kSumScale, which keeps sums of the largest values
+        // finite, with it (w is -inf where a row saw nothing or values of 0)
+        const float by = w[n] == -INFINITY ? 0.0f : w[n] - ref, whole_by = floorf(by), f = __builtin_amdgcn_exp2f(by - whole_by);
+        const int e = (int)whole_by + unit - kWeightLog2 - kSumLog2;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[n][d][i] = ldexpf(o[n][d][i] * f, e);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int step = kSharedWaves / 2; step >= 1; step >>= 1) {
+        if (wave >= step && wave < 2 * step)
+#pragma unroll
+            for (int i = 0; i < NR * ND * 4; ++i) sums[wave - step][i][lane] = o[i / (ND * 4)][i / 4 % ND][i % 4];
+        __syncthreads();
+        if (wave < step)
+#pragma unroll
+            for (int i = 0; i < NR * ND * 4; ++i) o[i / (ND * 4)][i / 4 % ND][i % 4] += sums[wave][i][lane];
+        __syncthreads();
+    }
+    if (wave != 0) return;
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+        const int r = r0 + 16 * n + n16;
+        if (r >= a.rows[S]) continue;
+        const int64_t at = row0 + r;
+        if (g4 == 0) *reinterpret_cast<float2*>(a.stat[S] + 2 * at) = make_float2(mt[n], lt[n]);
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+            if (16 * d < a.D) *reinterpret_cast<f32x4*>(a.part[S] + at * a.D + 16 * d + 4 * g4) = o[n][d];
+    }
+}
+
+// NP, NO: 16-row pieces of a workgroup's rows, of a prefix and of a sequence's own.
+template <int DT, int ND, int NP, int NO>
+__global__ __launch_bounds__(kSharedThreads, kOccupancy<ND>) void kv_shared_kernel(SharedArgs a) {
+    // The kernel's only LDS variable: beside a second one the compiler waits for all loads into LDS before any read of it.
+    __shared__ __attribute__((aligned(1024))) char ring[kSharedWaves * kRingBytes<ND>];
+    const int lane = threadIdx.x & 63;
+    if ((int)blockIdx.x < a.prefix_groups) {
+        // consecutive workgroups go round the 8 XCDs: the row tiles of a piece stay on one, whose
+        // L2 then has its codes
+        const int i = blockIdx.x >> 3, unit = i / a.row_tiles[0] * 8 + (blockIdx.x & 7), rt = i % a.row_tiles[0];
+        if (unit >= a.units) return;
+        const int piece = unit / a.H, h = unit % a.H;
+        int p, b0, b1;
+        if (a.even) {
+            const Pieces c = even_pieces(a, lane);
+            const uint64_t mine = __ballot(piece >= c.first && piece < c.first + c.count);
+            if (!mine) return;
+            p = __builtin_ctzll(mine);
+            b0 = (piece - __shfl(c.first, p, 64)) * c.size;
+            const int blocks = __shfl(c.blocks, p, 64);
+            b1 = b0 + c.size < blocks ? b0 + c.size : blocks;
+        } else {
+            const int each = a.pieces[0] / a.P;
+            p = piece / each;
+            const int blocks = blocks_of(clamp_length(a.lengths[0][p], a.nb[0])), size = (blocks + each - 1) / each;
+            b0 = piece % each * size;
+            b1 = b0 + size < blocks ? b0 + size : blocks;
+        }
+        attend<DT, ND, NP, 0>(a, ring, __builtin_amdgcn_readfirstlane(p), h, rt, __builtin_amdgcn_readfirstlane(b0),
+                              __builtin_amdgcn_readfirstlane(b1), (int64_t)unit * a.rows[0]);
+    } else {
+        const int i = blockIdx.x - a.prefix_groups, piece = i % a.pieces[1], j = i / a.pieces[1];
+        const int rt = j % a.row_tiles[1], bh = j / a.row_tiles[1], b = bh / a.H, h = bh % a.H;
+        const int len = clamp_length(a.lengths[1][b], a.nb[1]), blocks = blocks_of(len);
+        const int size = (blocks + a.pieces[1] - 1) / a.pieces[1], b0 = piece * size;
+        attend<DT, ND, NO, 1>(a, ring, b, h, rt, b0, b0 + size < blocks ? b0 + size : blocks,
+                              ((int64_t)piece * a.P * a.W * a.H + bh) * a.rows[1]);
+    }
+}
+
+constexpr int kJoinSize = 256;
+
+// GROUPS groups of D / 4 threads a row, which take every GROUPS-th of its pieces.
+template <int DT, bool MANY>
+__global__ __launch_bounds__(kJoinSize) void kv_shared_join_kernel(SharedArgs a) {
+    using E = Elem<DT>;
+    __shared__ int first_of[kMaxEven], count_of[kMaxEven];
+    __shared__ float sh_m[kJoinSize], sh_l[kJoinSize];
+    __shared__ f32x4 sh_o[kJoinSize];
+    const int t = threadIdx.x, lanes = a.D / 4, groups = MANY ? kJoinSize / lanes : 1;
+    if (a.even) {
+        if (t < 64) {
+            const Pieces c = even_pieces(a, t);
+            if (t < kMaxEven) { first_of[t] = c.first; count_of[t] = c.count; }
+        }
+        __syncthreads();
+    }
+    const int64_t rows = (int64_t)a.P * a.W * a.H * a.rows[1];
+    const int64_t i = MANY ? (int64_t)t : (int64_t)blockIdx.x * kJoinSize + t;
+    const int64_t row = MANY ? (int64_t)blockIdx.x : i / lanes;
+    const int g = MANY ? t / lanes : 0, d = (int)(MANY ? t % lanes : i % lanes) * 4;
+    const bool here = row < rows && g < groups;
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -INFINITY, l = 0.0f;
+    int64_t bh = 0;
+    int r = 0;
+    if (here) {
+        bh = row / a.rows[1];
+        r = (int)(row - bh * a.rows[1]);
+        const int b = (int)(bh / a.H), h = (int)(bh % a.H), p = b / a.W;
+        const int each = a.even ? 0 : a.pieces[0] / a.P;
+        const int first = a.even ? first_of[p] : p * each, count = a.even ? count_of[p] : each;
+        const int64_t of_prefix = (int64_t)h * a.rows[0] + (int64_t)(b - p * a.W) * a.rows[1] + r;
+        const int pieces = count + a.pieces[1];
+        auto add = [&](int s) {
+            const int S = s < count ? 0 : 1;
+            const int64_t at = S == 0 ? (int64_t)(first + s) * a.H * a.rows[0] + of_prefix
+                                      : (s - count) * rows + row;
+            const float2 st = *reinterpret_cast<const float2*>(a.stat[S] + 2 * at);
+            const f32x4 x = *reinterpret_cast<const f32x4*>(a.part[S] + at * a.D + d);
+            const float mn = fmaxf(m, st.x), ref = mn == -INFINITY ? 0.0f : mn;
+            const float f = __builtin_amdgcn_exp2f(m - ref), fx = __builtin_amdgcn_exp2f(st.x - ref);
+            o = o * f + x * fx;
+            l = l * f + st.y * fx;
+            m = mn;
+        };
+#pragma unroll 4
+        for (int s = g; s < pieces; s += groups) add(s);
+    }
+    if constexpr (MANY) {
+        sh_m[t] = m;
+        sh_l[t] = l;
+        sh_o[t] = o;
+        __syncthreads();
+        if (!here || g != 0) return;
+        float top = m;
+        for (int j = 1; j < groups; ++j) top = fmaxf(top, sh_m[j * lanes + t]);
+        const float ref = top == -INFINITY ? 0.0f : top, f = __builtin_amdgcn_exp2f(m - ref);
+        o *= f;
+        l *= f;
+        for (int j = 1; j < groups; ++j) {
+            const float fj = __builtin_amdgcn_exp2f(sh_m[j * lanes + t] - ref);
+            o += sh_o[j * lanes + t] * fj;
+            l += sh_l[j * lanes + t] * fj;
+        }
+    } else if (!here) {
+        return;
+    }
+    const float rl = l == 0.0f ? 0.0f : kSumScale / l;
+    const int64_t b = bh / a.H;
+    const int q = r / a.G, hq = (int)(bh % a.H) * a.G + r % a.G;
+    auto* out = reinterpret_cast<typename E::S*>(a.out) + ((b * a.Tq + q) * a.H * a.G + hq) * a.D + d;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) out[j] = E::from_f(o[j] * rl);
+}
+
+constexpr int kMostRows = 2;   // 16-row pieces
+
+// How a call is laid out.
+struct SharedPlan {
+    int np, no, even;
+    int64_t pieces[2], row_tiles[2];
+};
+SharedPlan shared_plan(int dtype, int64_t P, int64_t W, int64_t H, int64_t rows, int64_t D, int64_t prefix_blocks,
+                       int64_t blocks) {
+    SharedPlan p;
+    p.np = D > 128 && dtype == AXS6_F32 ? 1 : kMostRows;
+    p.no = D > 128 || rows <= 16 ? 1 : 2;
+    p.row_tiles[0] = (W * rows + 16 * p.np - 1) / (16 * p.np);
+    p.row_tiles[1] = (rows + 16 * p.no - 1) / (16 * p.no);
+    // two workgroups a CU, and at least 8 blocks each
+    const int64_t most = 512;
+    const int64_t groups = H * p.row_tiles[0];
+    int64_t n = (most + groups - 1) / groups;
+    n = n < P * ((prefix_blocks + 7) / 8) ? n : P * ((prefix_blocks + 7) / 8);
+    p.even = P <= kMaxEven;
+    if (p.even) p.pieces[0] = n + P - 1;
+    else p.pieces[0] = P * ((n + P - 1) / P);
+    const int64_t own = P * W * H * p.row_tiles[1];
+    n = (most + own - 1) / own;
+    n = n < (blocks + 7) / 8 ? n : (blocks + 7) / 8;
+    p.pieces[1] = n;
+    return p;
+}
+
+template <int DT, int ND>
+void launch_shared(const SharedArgs& a, const SharedPlan& p, unsigned grid, hipStream_t st) {
+    if constexpr (ND > 8) {
+        kv_shared_kernel<DT, ND, DT == AXS6_F32 ? 1 : 2, 1><<<grid, kSharedThreads, 0, st>>>(a);
+    } else {
+        if (p.no == 1) kv_shared_kernel<DT, ND, kMostRows, 1><<<grid, kSharedThreads, 0, st>>>(a);
+        else kv_shared_kernel<DT, ND, kMostRows, 2><<<grid, kSharedThreads, 0, st>>>(a);
+    }
+}
+
+}  // namespace
+}  // namespace axs6
+
+using namespace axs6;
+
+extern "C" int64_t axs6_kv_shared_attention_workspace(int32_t dtype, int64_t P, int64_t W, int64_t Tq, int64_t Hq, int64_t H,
+                                                      int64_t D, int64_t prefix_blocks, int64_t blocks) {
+    if (!valid_dtype(dtype) || P <= 0 || W <= 0 || Tq <= 0 || H <= 0 || Hq <= 0 || Hq % H || D <= 0 || prefix_blocks <= 0 ||
+        blocks < 0)
+        return 0;
+    const int64_t rows = Tq * (Hq / H);
+    const SharedPlan p = shared_plan(dtype, P, W, H, rows, D, prefix_blocks, blocks);
+    return (p.pieces[0] + p.pieces[1] * P) * W * H * rows * (D + 2) * (int64_t)sizeof(float);
+}
+
+extern "C" int axs6_kv_shared_attention(const void* q, int32_t dtype, int64_t P, int64_t W, int64_t Tq, int64_t Hq,
+                                        int64_t H, int64_t D, const int64_t* q_strides, const void* pk_codes,
+                                        const float* pk_scales, const void* pv_codes, const float* pv_scales,
+                                        int64_t prefix_blocks, const int64_t* prefix_lengths, const void* k_codes,
+                                        const float* k_scales, const void* v_codes, const float* v_scales, int64_t blocks,
+                                        const int64_t* lengths, float scale, void* out, void* workspace,
+                                        int64_t workspace_bytes, void* stream) {
+    const char* fn = "axs6_kv_shared_attention";
+    if (!valid_dtype(dtype)) return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: unknown dtype code %d", fn, dtype);
+    constexpr int64_t kMost = ((int64_t)1 << 31) - 1;
+    if (P < 0 || W < 0 || P > kMost || W > kMost || P * W > kMost)
+        return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: bad number of sequences", fn);
+    int rc = check_cache(fn, P, H, D, prefix_blocks, pk_codes, pk_scales, pv_codes, pv_scales);
+    if (rc) return rc;
+    const int64_t B = P * W;
+    rc = check_cache(fn, B, H, D, blocks, k_codes, k_scales, v_codes, v_scales);
+    if (rc) return rc;
+    if (Tq < 0 || Hq < 0 || (H > 0 && Hq % H))
+        return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: %lld query heads for %lld key heads", fn, (long long)Hq, (long long)H);
+    if (!isfinite(scale)) return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: the scale must be finite", fn);
+    if (B * Tq * Hq == 0) return AXS6_OK;
+    if (H == 0 || prefix_blocks == 0) return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: an empty prefix", fn);
+    if (!q || !q_strides || !prefix_lengths || !lengths || !out)
+        return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: null operand", fn);
+    const int64_t es = dtype == AXS6_F32 ? 4 : 2, vl = 16 / es, rows = Tq * (Hq / H);
+    if (Tq > (1 << 24) || Hq / H > (1 << 24) || rows > (1 << 24) || W * rows > (1 << 24) || B * H * rows > kMost / 64)
+        return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: dimension too large", fn);
+    if ((uintptr_t)q % es || (uintptr_t)out % es)
+        return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: pointer not element-aligned", fn);
+    const int64_t need = axs6_kv_shared_attention_workspace(dtype, P, W, Tq, Hq, H, D, prefix_blocks, blocks);
+    if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16)
+        return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: a 16-byte aligned workspace of %lld bytes required, got %lld", fn,
+                    (long long)need, (long long)workspace_bytes);
+    const SharedPlan p = shared_plan(dtype, P, W, H, rows, D, prefix_blocks, blocks);
+    SharedArgs a{};
+    a.q = q; a.out = out; a.scale = scale;
+    a.qvec = (uintptr_t)q % 16 == 0;
+    for (int i = 0; i < 3; ++i) {
+        a.qs[i] = q_strides[i];
+        a.qvec = a.qvec && q_strides[i] % vl == 0;
+    }
+    a.kc[0] = reinterpret_cast<const int8_t*>(pk_codes); a.vc[0] = reinterpret_cast<const int8_t*>(pv_codes);
+    a.ks[0] = pk_scales; a.vs[0] = pv_scales; a.lengths[0] = prefix_lengths; a.nb[0] = (int)prefix_blocks;
+    a.kc[1] = reinterpret_cast<const int8_t*>(k_codes); a.vc[1] = reinterpret_cast<const int8_t*>(v_codes);
+    a.ks[1] = k_scales; a.vs[1] = v_scales; a.lengths[1] = lengths; a.nb[1] = (int)blocks;
+    a.P = (int)P; a.W = (int)W; a.H = (int)H; a.G = (int)(Hq / H); a.Tq = (int)Tq; a.D = (int)D;
+    a.rows[0] = (int)(W * rows); a.rows[1] = (int)rows;
+    for (int i = 0; i < 2; ++i) { a.row_tiles[i] = (int)p.row_tiles[i]; a.pieces[i] = (int)p.pieces[i]; }
+    a.even = p.even;
+    const int64_t units = p.pieces[0] * H, prefix_groups = (units + 7) / 8 * 8 * p.row_tiles[0];
+    const int64_t grid = prefix_groups + B * H * p.row_tiles[1] * p.pieces[1];
+    if (grid > kMost) return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: dimension too large", fn);
+    a.units = (int)units;
+    a.prefix_groups = (int)prefix_groups;
+    const int64_t rows0 = (int64_t)p.pieces[0] * H * a.rows[0], rows1 = (int64_t)p.pieces[1] * B * H * rows;
+    a.part[0] = reinterpret_cast<float*>(workspace);
+    a.part[1] = a.part[0] + rows0 * D;
+    a.stat[0] = a.part[1] + rows1 * D;
+    a.stat[1] = a.stat[0] + rows0 * 2;
+    hipStream_t st = (hipStream_t)stream;
+    by_dtype(dtype, [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        if (D <= 64) launch_shared<DT, 4>(a, p, (unsigned)grid, st);
+        else if (D <= 96) launch_shared<DT, 6>(a, p, (unsigned)grid, st);
+        else if (D <= 128) launch_shared<DT, 8>(a, p, (unsigned)grid, st);
+        else if (D <= 192) launch_shared<DT, 12>(a, p, (unsigned)grid, st);
+        else launch_shared<DT, 16>(a, p, (unsigned)grid, st);
+        const int64_t all = B * H * rows, lanes = D / 4;
+        if (all < 1024) kv_shared_join_kernel<DT, true><<<(unsigned)all, kJoinSize, 0, st>>>(a);
+        else kv_shared_join_kernel<DT, false><<<(unsigned)((all * lanes + kJoinSize - 1) / kJoinSize), kJoinSize, 0, st>>>(a);
+    });
+    return check_launch(fn);
+}

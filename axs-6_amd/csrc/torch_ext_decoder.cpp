@@ -445,7 +445,7 @@ at::Tensor kv_shared_attention(const at::Tensor& q, const at::Tensor& pk_codes, 
         return out;
     }
     const at::Tensor ws = workspace(
-        axs6_kv_shared_attention_workspace(p.B, c.B / p.B, Tq, Hq, c.H, c.D, p.nb, c.nb), q);
+        axs6_kv_shared_attention_workspace(dtype_code(q.scalar_type()), p.B, c.B / p.B, Tq, Hq, c.H, c.D, p.nb, c.nb), q);
     check_rc(axs6_kv_shared_attention(qp.data_ptr(), dtype_code(q.scalar_type()), p.B, c.B / p.B, Tq, Hq, c.H, c.D,
                                       qp.strides().data(), p.kc.data_ptr(), p.ks.data_ptr<float>(), p.vc.data_ptr(),
                                       p.vs.data_ptr<float>(), p.nb, np.data_ptr<int64_t>(), c.kc.data_ptr(),

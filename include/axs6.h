@@ -489,8 +489,8 @@ int axs6_kv_copy(const void* k_codes, const float* k_scales, const void* v_codes
  * lengths[b] tokens of its own in the second; q (P * W, Tq, Hq, D) are its last Tq.
  * Query t sees the keys at places j <= prefix + own - Tq + t (none: 0).  As
  * axs6_kv_attention otherwise; blocks may be 0, prefix_blocks not. */
-int64_t axs6_kv_shared_attention_workspace(int64_t P, int64_t W, int64_t Tq, int64_t Hq, int64_t H, int64_t D,
-                                           int64_t prefix_blocks, int64_t blocks);
+int64_t axs6_kv_shared_attention_workspace(int32_t dtype, int64_t P, int64_t W, int64_t Tq, int64_t Hq, int64_t H,
+                                           int64_t D, int64_t prefix_blocks, int64_t blocks);
 int axs6_kv_shared_attention(const void* q, int32_t dtype, int64_t P, int64_t W, int64_t Tq, int64_t Hq, int64_t H,
                              int64_t D, const int64_t* q_strides, const void* prefix_k_codes,
                              const float* prefix_k_scales, const void* prefix_v_codes, const float* prefix_v_scales,

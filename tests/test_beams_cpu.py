@@ -69,7 +69,7 @@ def test_copy_checks_its_arguments():
 def test_shared_attention_checks_its_arguments():
     L = _lib.lib()
     p, st = 4096, _i64(256, 64, 64)
-    need = L.axs6_kv_shared_attention_workspace(2, 3, 1, 4, 2, 64, 8, 2)
+    need = L.axs6_kv_shared_attention_workspace(0, 2, 3, 1, 4, 2, 64, 8, 2)
     assert need > 0
     good = [p, 0, 2, 3, 1, 4, 2, 64, st, p, p, p, p, 8, p, p, p, p, p, 2, p, 0.1, p, p, need, None]
     for change, rc in (({"a1": 3}, 1), ({"a2": -1}, 1), ({"a3": -1}, 1), ({"a5": 3}, 1), ({"a7": 40}, 2), ({"a9": None}, 1),
@@ -77,5 +77,5 @@ def test_shared_attention_checks_its_arguments():
                        ({"a22": None}, 1), ({"a23": None}, 1), ({"a23": 4104}, 1), ({"a24": need - 1}, 1), ({"a0": 4097}, 1),
                        ({"a4": 1 << 25, "a24": 1 << 50}, 1), ({"a2": 1 << 20, "a3": 1 << 20}, 1), ({"a4": 0}, 0), ({"a2": 0}, 0)):
         assert _call(L.axs6_kv_shared_attention, good, **change) == rc, change
-    assert L.axs6_kv_shared_attention_workspace(0, 3, 1, 4, 2, 64, 8, 2) == 0
-    assert L.axs6_kv_shared_attention_workspace(2, 3, 1, 4, 2, 64, 0, 2) == 0
+    assert L.axs6_kv_shared_attention_workspace(0, 0, 3, 1, 4, 2, 64, 8, 2) == 0
+    assert L.axs6_kv_shared_attention_workspace(0, 2, 3, 1, 4, 2, 64, 0, 2) == 0
