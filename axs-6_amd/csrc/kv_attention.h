@@ -46,17 +46,17 @@ __device__ __forceinline__ f32x4 mma(f16x8 a, f16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// Sixteen values of a query from element i.
-template <int DT>
-__device__ __forceinline__ void load16(const void* p, int64_t i, bool vec, float* f) {
+// N values of a query from element i.
+template <int DT, int N>
+__device__ __forceinline__ void load_values(const void* p, int64_t i, bool vec, float* f) {
     using E = Elem<DT>;
     const auto* q = reinterpret_cast<const typename E::S*>(p) + i;
     if (vec) {
 #pragma unroll
-        for (int j = 0; j < 16; j += E::V) E::unpack(*reinterpret_cast<const u32x4*>(q + j), f + j);
+        for (int j = 0; j < N; j += E::V) E::unpack(*reinterpret_cast<const u32x4*>(q + j), f + j);
     } else {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) f[j] = E::to_f(q[j]);
+        for (int j = 0; j < N; ++j) f[j] = E::to_f(q[j]);
     }
 }
 

@@ -112,7 +112,7 @@ __global__ __launch_bounds__(64 * WAVES) void kv_attention_kernel(KvAttnArgs a) 
 #pragma unroll
             for (int j = 0; j < 16; ++j) f[c][j] = 0.0f;
             if (64 * c + 16 * g4 < a.D)
-                load16<DT>(a.q, b * a.qs[0] + t * a.qs[1] + hq * a.qs[2] + 64 * c + 16 * g4, a.qvec, f[c]);
+                load_values<DT, 16>(a.q, b * a.qs[0] + t * a.qs[1] + hq * a.qs[2] + 64 * c + 16 * g4, a.qvec, f[c]);
 #pragma unroll
             for (int j = 0; j < 16; ++j) amax = fmaxf(amax, fabsf(f[c][j]));
         }

@@ -7,20 +7,20 @@
 // over the keys of both caches (codes kc, vc, a block's scales ks, vs).  The prefix is read
 // once for the rows of all W sequences, W Tq G of a key head.
 //
-// One launch for both, in which a workgroup takes up to 64 rows against a piece of the prefix,
+// One launch for both, in which a workgroup takes 64 rows against a piece of the prefix,
 // or a sequence's rows against its own blocks (those are bound by HBM, the prefix's with
 // many rows by the matrix cores and the softmax: side by side each hides the other), and
 // leaves maximum, sum and D sums a row; a second launch joins a row's pieces.  The prefixes'
 // pieces are cut from all the blocks that they hold, so that workgroups have equal work
 // whatever the lengths, which only the device knows.
 //
-// A wave holds 16 or 32 rows in registers and takes every fourth block of its workgroup's; codes
-// come straight from memory into a ring of blocks in LDS that is the wave's own, so no
-// barrier stands in the loop.  Products as in the cache attention (S^T = K q^T by
-// 16x16x32 f16 instructions in which codes are exact, probabilities stay in their lanes).
-// A block's value scale goes into its probabilities' exponent, which counts from a reference of its own; the
-// references move only when a score passes them by kSlack, and between that the sums stay where the products add
-// to them.  Probabilities go in as f16 times 2^11 (float32: two terms), 11 bits down to 2^-25 of the largest.
+// Products as in the cache attention (S^T = K q^T by 16x16x32 f16 instructions in which codes are exact, probabilities
+// stay in their lanes).  A block's value scale goes into its probabilities' exponent, which counts from a reference of
+// its own; the references move only when a score passes them by kSlack, and between that the sums stay where the products
+// add to them.  Probabilities go in as f16 times 2^11 (float32: two terms), 11 bits down to 2^-25 of the largest.
+// Turning codes into f16 costs as much as a block's softmax for 32 rows: a prefix's workgroup does it once for its four
+// waves' 64 rows, into LDS; rows of one sequence are few, and there each wave has blocks of its own, whose codes come
+// straight from memory into LDS.
 #include "kv_attention.h"
 
 namespace axs6 {
@@ -55,9 +55,6 @@ struct SharedArgs {
 __device__ __forceinline__ int clamp_length(int64_t n, int nb) {
     const int64_t cap = (int64_t)nb * kKvBlock;
     return (int)(n < 0 ? 0 : n > cap ? cap : n);
-}
-__device__ __forceinline__ float uniform(float x) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
 }
 __device__ __forceinline__ float lane_value(float x, int lane) {
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), lane));
@@ -95,11 +92,7 @@ __device__ __forceinline__ Pieces even_pieces(const SharedArgs& a, int lane) {
 template <int ND> constexpr int kRow = ND <= 4 ? 4 : ND <= 8 ? 8 : 16;
 template <int ND> constexpr int kKeyBytes = kKvBlock * kRow<ND> * 16;
 template <int ND> constexpr int kSlotBytes = kKeyBytes<ND> + ND * 512;
-// A wave's blocks in LDS, that it computes on and those on their way; the instructions that fetch one; waves a SIMD.
-template <int ND> constexpr int kSlots = 2;
-template <int ND> constexpr int kFetches = kRow<ND> / 2 + ND / 2;
-template <int ND> constexpr int kOccupancy = ND <= 8 ? 2 : 1;
-template <int ND> constexpr int kRingBytes = kSlots<ND> * kSlotBytes<ND>;
+template <int ND> constexpr int kFetches = kRow<ND> / 2 + ND / 2;   // the instructions that fetch a block
 
 // Waits until at most `ahead` blocks (ahead <= MOST, uniform) are still on their way.
 template <int MOST, int FETCHES>
@@ -144,146 +137,88 @@ __device__ __forceinline__ void fetch_block(char* slot, const int8_t* kc, const 
 #endif
 }
 
-// Up to 16 NR rows of one key head against blocks [b0, b1) of sequence `set` of a cache: S 0, a
-// prefix (rows of all its W sequences), or 1, a sequence's own.
+// A wave's 16 NR rows (a lane has row 16 n + lane % 16) of a key head's: queries, what they see, and what attention
+// leaves of the blocks so far.  l counts from the maximum m, o from the maximum w of x + log2(value scale) + unit.
+// S 0: rows of all sequences of a prefix, 1: of one sequence.
 template <int DT, int ND, int NR, int S>
-__device__ __forceinline__ void attend(const SharedArgs& a, char* ring, int set, int h, int rt, int b0, int b1,
-                                       int64_t row0) {
-    constexpr int TERMS = DT == AXS6_F32 ? 2 : 1;
-    constexpr int NC = (ND + 3) / 4;   // 64-value pieces of a key's row
-    static_assert(2 * NR * ND * 4 * 256 <= kSharedWaves * kRingBytes<ND>, "the waves' sums fit the rings");
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n16 = lane & 15, g4 = lane >> 4;
-    const int len = clamp_length(a.lengths[S][set], a.nb[S]);
-    const int64_t cell0 = ((int64_t)set * a.H + h) * a.nb[S];
-    const int per_seq = a.Tq * a.G, r0 = rt * NR * 16;
-    char* my_ring = ring + wave * kRingBytes<ND>;
-    // the scales of the wave's next 64 blocks, one a lane; then the first blocks
-    float ks64, vs64;
-    auto load_scales = [&](int blk) {
-        const int mine = blk + lane * kSharedWaves;
-        ks64 = mine < b1 ? a.ks[S][cell0 + mine] : 0.0f;
-        vs64 = mine < b1 ? a.vs[S][cell0 + mine] : 0.0f;
-    };
-    load_scales(b0 + wave);
-#pragma unroll
-    for (int i = 0; i < kSlots<ND> - 1; ++i) {
-        const int blk = b0 + wave + i * kSharedWaves;
-        if (blk < b1) fetch_block<ND>(my_ring + i * kSlotBytes<ND>, a.kc[S], a.vc[S], cell0 + blk, a.D, lane);
-    }
-
-    // the rows' queries, scaled, in the products' order: piece c, value 16 g4 + j
+struct Rows {
+    static constexpr int TERMS = DT == AXS6_F32 ? 2 : 1;
+    static constexpr int NC = (ND + 3) / 4;   // 64-value pieces of a head
     f16x8 qf[NR][TERMS][NC][2];
     float rs[NR];
     int last[NR];   // the last key that the lane's row sees
-    int whole = len;   // keys that all the wave's rows see
-#pragma unroll
-    for (int n = 0; n < NR; ++n) {
-        int r = r0 + 16 * n + n16;
-        r = r < a.rows[S] ? r : a.rows[S] - 1;
-        const int seq = S ? set : set * a.W + r / per_seq;
-        r = S ? r : r % per_seq;
-        const int t = r / a.G, hq = h * a.G + r % a.G;
-        last[n] = len - a.Tq + t;
-        if constexpr (S == 0) {   // the sequence's own tokens follow the prefix's
-            const int64_t to = (int64_t)last[n] + clamp_length(a.lengths[1][seq], a.nb[1]);
-            last[n] = (int)(to < len ? to : len - 1);
-        }
-        whole = last[n] + 1 < whole ? last[n] + 1 : whole;
-        float f[NC][16], amax = 0.0f;
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) f[c][j] = 0.0f;
-            if (64 * c + 16 * g4 < a.D)
-                load16<DT>(a.q, (int64_t)seq * a.qs[0] + t * a.qs[1] + hq * a.qs[2] + 64 * c + 16 * g4, a.qvec, f[c]);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) amax = fmaxf(amax, fabsf(f[c][j]));
-        }
-        amax = fmaxf(amax, __shfl_xor(amax, 16, 64));
-        amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
-        const int e = amax > 0.0f && isfinite(amax) ? ilogbf(amax) - 7 : 0;
-        const float sign = a.scale < 0.0f ? -1.0f : 1.0f;   // the largest product is then the largest score
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const float x = ldexpf(sign * f[c][j], -e);
-                const _Float16 hi = (_Float16)x;
-                qf[n][0][c][j >> 3][j & 7] = hi;
-                if constexpr (TERMS == 2) qf[n][1][c][j >> 3][j & 7] = (_Float16)(x - (float)hi);
-            }
-        rs[n] = ldexpf(fabsf(a.scale) * kLog2e, e);
-    }
-    // value scales count from the largest one's power of two
-    float largest = 0.0f;
-    for (int i = b0 + lane; i < b1; i += 64) largest = fmaxf(largest, a.vs[S][cell0 + i]);
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) {
-        largest = fmaxf(largest, __shfl_xor(largest, o, 64));
-        const int x = __shfl_xor(whole, o, 64);
-        whole = x < whole ? x : whole;
-    }
-    const int unit = __builtin_amdgcn_readfirstlane(largest > 0.0f ? ilogbf(largest) : 0);
-    whole = __builtin_amdgcn_readfirstlane(whole);
-
-    // l counts from the maximum m, o from the maximum w of x + log2(value scale)
+    int whole;      // keys that all the wave's rows see
+    int unit;       // value scales count from 2^unit
     f32x4 o[NR][ND];
     float m[NR], w[NR], l[NR];
+
+    // The queries from row r0 on, scaled to [128, 256): of piece c a lane has values 64 c + 16 g4 + j; HALVES: of both
+    // its halves 8 g4 + j each.  `largest`: the largest value scale, the lanes' own yet.
+    template <bool HALVES>
+    __device__ __forceinline__ void init(const SharedArgs& a, int set, int h, int r0, int len, float largest, int lane) {
+        const int n16 = lane & 15, g4 = lane >> 4, per_seq = a.Tq * a.G;
+        whole = len;
 #pragma unroll
-    for (int n = 0; n < NR; ++n) {
+        for (int n = 0; n < NR; ++n) {
+            int r = r0 + 16 * n + n16;
+            r = r < a.rows[S] ? r : a.rows[S] - 1;
+            const int seq = S ? set : set * a.W + r / per_seq;
+            r = S ? r : r % per_seq;
+            const int t = r / a.G, hq = h * a.G + r % a.G;
+            last[n] = len - a.Tq + t;
+            if constexpr (S == 0) {   // the sequence's own tokens follow the prefix's
+                const int64_t to = (int64_t)last[n] + clamp_length(a.lengths[1][seq], a.nb[1]);
+                last[n] = (int)(to < len ? to : len - 1);
+            }
+            whole = last[n] + 1 < whole ? last[n] + 1 : whole;
+            const int64_t q0 = (int64_t)seq * a.qs[0] + t * a.qs[1] + hq * a.qs[2];
+            float f[NC][16], amax = 0.0f;
 #pragma unroll
-        for (int d = 0; d < ND; ++d) o[n][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        m[n] = w[n] = -INFINITY;
-        l[n] = 0.0f;
+            for (int c = 0; c < NC; ++c) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) f[c][j] = 0.0f;
+                if constexpr (HALVES) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        if (64 * c + 32 * e + 8 * g4 < a.D) load_values<DT, 8>(a.q, q0 + 64 * c + 32 * e + 8 * g4, a.qvec, f[c] + 8 * e);
+                } else {
+                    if (64 * c + 16 * g4 < a.D) load_values<DT, 16>(a.q, q0 + 64 * c + 16 * g4, a.qvec, f[c]);
+                }
+#pragma unroll
+                for (int j = 0; j < 16; ++j) amax = fmaxf(amax, fabsf(f[c][j]));
+            }
+            amax = fmaxf(amax, __shfl_xor(amax, 16, 64));
+            amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
+            const int e = amax > 0.0f && isfinite(amax) ? ilogbf(amax) - 7 : 0;
+            const float sign = a.scale < 0.0f ? -1.0f : 1.0f;   // the largest product is then the largest score
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const float x = ldexpf(sign * f[c][j], -e);
+                    const _Float16 hi = (_Float16)x;
+                    qf[n][0][c][j >> 3][j & 7] = hi;
+                    if constexpr (TERMS == 2) qf[n][1][c][j >> 3][j & 7] = (_Float16)(x - (float)hi);
+                }
+            rs[n] = ldexpf(fabsf(a.scale) * kLog2e, e);
+#pragma unroll
+            for (int d = 0; d < ND; ++d) o[n][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            m[n] = w[n] = -INFINITY;
+            l[n] = 0.0f;
+        }
+#pragma unroll
+        for (int i = 32; i >= 1; i >>= 1) {
+            largest = fmaxf(largest, __shfl_xor(largest, i, 64));
+            const int x = __shfl_xor(whole, i, 64);
+            whole = x < whole ? x : whole;
+        }
+        unit = __builtin_amdgcn_readfirstlane(largest > 0.0f ? ilogbf(largest) : 0);
+        whole = __builtin_amdgcn_readfirstlane(whole);
     }
-    // fragments: key row 8 (n16 / 4) + 4 tt + n16 % 4, piece 4 c + g4; value row 16 d + n16, keys 8 g4 .. 8 g4 + 7
-    const int key_row = 8 * (n16 >> 2) + (n16 & 3);
-    const int key_at = (key_row * kRow<ND> + (g4 ^ key_turn<ND>(key_row))) * 16;
-    const int value_at = kKeyBytes<ND> + (n16 * 2 + ((g4 >> 1) ^ (n16 >> 3))) * 16 + (g4 & 1) * 8;
-    asm volatile("" : "+v"(ks64), "+v"(vs64));   // they are here
-    int step = 0, at = 0;   // the slot of the block
-    for (int blk = b0 + wave; blk < b1; blk += kSharedWaves, ++step) {
-        // the block is there
-        asm volatile("" ::: "memory");
-        wait_blocks<kSlots<ND> - 2, kFetches<ND>>((b1 - 1 - blk) / kSharedWaves);
-        asm volatile("" ::: "memory");
-        if (step % 64 == 0 && step) {
-            load_scales(blk);
-            asm volatile("" : "+v"(ks64), "+v"(vs64));
-        }
-        const float ks = lane_value(ks64, step % 64), vs = lane_value(vs64, step % 64);
-        const char* slot = my_ring + at * kSlotBytes<ND>;
-        // the slot of the block before is free: all reads of it have come back, for its products are done
-        const int next = blk + (kSlots<ND> - 1) * kSharedWaves, free_at = at == 0 ? kSlots<ND> - 1 : at - 1;
-        if (next < b1) fetch_block<ND>(my_ring + free_at * kSlotBytes<ND>, a.kc[S], a.vc[S], cell0 + next, a.D, lane);
-        at = at + 1 == kSlots<ND> ? 0 : at + 1;
-        // Codes are read a step ahead, and the steps stand apart (sched_barrier): else the compiler, with all reads
-        // first, wants more registers than there are.
-        f32x4 s[NR][2];
-        auto key_codes = [&](int i) {
-            return *reinterpret_cast<const u32x4*>(slot + (key_at ^ i / 2 * 64) + i % 2 * 4 * kRow<ND> * 16);
-        };
-        auto value_codes = [&](int d) { return *reinterpret_cast<const uint2*>(slot + value_at + d * 512); };
-#pragma unroll
-        for (int n = 0; n < NR; ++n) s[n][0] = s[n][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        u32x4 k = key_codes(0);
-#pragma unroll
-        for (int i = 0; i < 2 * NC; ++i) {   // both 16-key halves in turn: products that do not wait for each other
-            const u32x4 next = key_codes(i + 1 < 2 * NC ? i + 1 : i);
-            const f16x8 k0 = codes_f16<false>(k.x, k.y), k1 = codes_f16<false>(k.z, k.w);
-#pragma unroll
-            for (int n = 0; n < NR; ++n)
-#pragma unroll
-                for (int u = 0; u < TERMS; ++u) s[n][i % 2] = mma(k0, qf[n][u][i / 2][0], s[n][i % 2]);
-#pragma unroll
-            for (int n = 0; n < NR; ++n)
-#pragma unroll
-                for (int u = 0; u < TERMS; ++u) s[n][i % 2] = mma(k1, qf[n][u][i / 2][1], s[n][i % 2]);
-            k = next;
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        uint2 v = value_codes(0);
-        f16x8 pf[NR][TERMS];
+
+    // Block blk's products s with the queries, of scales ks and vs, to the weights pf of its values.
+    __device__ __forceinline__ void weigh(f32x4 (&s)[NR][2], float ks, float vs, int blk, int lane, f16x8 (&pf)[NR][TERMS]) {
+        const int g4 = lane >> 4;
         float c[NR], lv[NR];   // what takes the products to units of log2; log2 of the value scale
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
@@ -355,26 +290,145 @@ __device__ __forceinline__ void attend(const SharedArgs& a, char* ring, int set,
         }
 #pragma unroll
         for (int n = 0; n < NR; ++n) l[n] += back[n];
+    }
+
+    // l of whole rows.
+    __device__ __forceinline__ void finish() {
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+            l[n] += __shfl_xor(l[n], 16, 64);
+            l[n] += __shfl_xor(l[n], 32, 64);
+        }
+    }
+
+    // The sums of piece n from w to count from ref, in one step: a power of two, and 1 / kSumScale, which keeps sums of the
+    // largest values finite, with it (w is -inf where a row saw nothing or values of 0).
+    __device__ __forceinline__ void rescale(int n, float ref) {
+        const float by = w[n] == -INFINITY ? 0.0f : w[n] - (ref == -INFINITY ? 0.0f : ref), whole_by = floorf(by);
+        const float f = __builtin_amdgcn_exp2f(by - whole_by);
+        const int e = (int)whole_by + unit - kWeightLog2 - kSumLog2;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[n][d][i] = ldexpf(o[n][d][i] * f, e);
+    }
+
+    __device__ __forceinline__ void store(const SharedArgs& a, int n, int r0, int64_t row0, float mt, float lt, int lane) const {
+        const int r = r0 + 16 * n + (lane & 15), g4 = lane >> 4;
+        if (r >= a.rows[S]) return;
+        const int64_t at = row0 + r;
+        if (g4 == 0) *reinterpret_cast<float2*>(a.stat[S] + 2 * at) = make_float2(mt, lt);
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+            if (16 * d < a.D) *reinterpret_cast<f32x4*>(a.part[S] + at * a.D + 16 * d + 4 * g4) = o[n][d];
+    }
+};
+
+// Up to 16 NR rows of one key head against blocks [b0, b1) of sequence `set` of a cache: S 0, a
+// prefix (rows of all its W sequences), or 1, a sequence's own.
+// SLOTS: of the wave's ring, the block that it computes on and those on their way.
+template <int DT, int ND, int NR, int S, int SLOTS>
+__device__ __forceinline__ void attend(const SharedArgs& a, char* ring, int set, int h, int rt, int b0, int b1,
+                                       int64_t row0) {
+    using R = Rows<DT, ND, NR, S>;
+    constexpr int TERMS = R::TERMS, NC = R::NC;
+    constexpr int kRing = SLOTS * kSlotBytes<ND>;
+    static_assert(2 * NR * ND * 4 * 256 <= kSharedWaves * kRing, "the waves' sums fit the rings");
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n16 = lane & 15, g4 = lane >> 4;
+    const int len = clamp_length(a.lengths[S][set], a.nb[S]);
+    const int64_t cell0 = ((int64_t)set * a.H + h) * a.nb[S];
+    const int r0 = rt * NR * 16;
+    char* my_ring = ring + wave * kRing;
+    // the scales of the wave's next 64 blocks, one a lane; then the first blocks
+    float ks64, vs64;
+    auto load_scales = [&](int blk) {
+        const int mine = blk + lane * kSharedWaves;
+        ks64 = mine < b1 ? a.ks[S][cell0 + mine] : 0.0f;
+        vs64 = mine < b1 ? a.vs[S][cell0 + mine] : 0.0f;
+    };
+    load_scales(b0 + wave);
+#pragma unroll
+    for (int i = 0; i < (SLOTS > 1 ? SLOTS - 1 : 1); ++i) {
+        const int blk = b0 + wave + i * kSharedWaves;
+        if (blk < b1) fetch_block<ND>(my_ring + i * kSlotBytes<ND>, a.kc[S], a.vc[S], cell0 + blk, a.D, lane);
+    }
+    R rows;
+    float largest = 0.0f;
+    for (int i = b0 + lane; i < b1; i += 64) largest = fmaxf(largest, a.vs[S][cell0 + i]);
+    rows.template init<false>(a, set, h, r0, len, largest, lane);
+    // fragments: key row 8 (n16 / 4) + 4 tt + n16 % 4, piece 4 c + g4; value row 16 d + n16, keys 8 g4 .. 8 g4 + 7
+    const int key_row = 8 * (n16 >> 2) + (n16 & 3);
+    const int key_at = (key_row * kRow<ND> + (g4 ^ key_turn<ND>(key_row))) * 16;
+    const int value_at = kKeyBytes<ND> + (n16 * 2 + ((g4 >> 1) ^ (n16 >> 3))) * 16 + (g4 & 1) * 8;
+    asm volatile("" : "+v"(ks64), "+v"(vs64));   // they are here
+    int step = 0, at = 0;   // the slot of the block
+    for (int blk = b0 + wave; blk < b1; blk += kSharedWaves, ++step) {
+        // the block is there
+        asm volatile("" ::: "memory");
+        wait_blocks<(SLOTS > 2 ? SLOTS - 2 : 0), kFetches<ND>>((b1 - 1 - blk) / kSharedWaves);
+        asm volatile("" ::: "memory");
+        if (step % 64 == 0 && step) {
+            load_scales(blk);
+            asm volatile("" : "+v"(ks64), "+v"(vs64));
+        }
+        const float ks = lane_value(ks64, step % 64), vs = lane_value(vs64, step % 64);
+        const char* slot = my_ring + at * kSlotBytes<ND>;
+        // the slot of the block before is free: all reads of it have come back, for its products are done
+        if constexpr (SLOTS > 1) {
+            const int next = blk + (SLOTS - 1) * kSharedWaves, free_at = at == 0 ? SLOTS - 1 : at - 1;
+            if (next < b1) fetch_block<ND>(my_ring + free_at * kSlotBytes<ND>, a.kc[S], a.vc[S], cell0 + next, a.D, lane);
+            at = at + 1 == SLOTS ? 0 : at + 1;
+        }
+        // Codes are read a step ahead, and the steps stand apart (sched_barrier): else the compiler, with all reads
+        // first, wants more registers than there are.
+        f32x4 s[NR][2];
+        auto key_codes = [&](int i) {
+            return *reinterpret_cast<const u32x4*>(slot + (key_at ^ i / 2 * 64) + i % 2 * 4 * kRow<ND> * 16);
+        };
+        auto value_codes = [&](int d) { return *reinterpret_cast<const uint2*>(slot + value_at + d * 512); };
+#pragma unroll
+        for (int n = 0; n < NR; ++n) s[n][0] = s[n][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        u32x4 k = key_codes(0);
+#pragma unroll
+        for (int i = 0; i < 2 * NC; ++i) {   // both 16-key halves in turn: products that do not wait for each other
+            const u32x4 next_k = key_codes(i + 1 < 2 * NC ? i + 1 : i);
+            const f16x8 k0 = codes_f16<false>(k.x, k.y), k1 = codes_f16<false>(k.z, k.w);
+#pragma unroll
+            for (int n = 0; n < NR; ++n)
+#pragma unroll
+                for (int u = 0; u < TERMS; ++u) s[n][i % 2] = mma(k0, rows.qf[n][u][i / 2][0], s[n][i % 2]);
+#pragma unroll
+            for (int n = 0; n < NR; ++n)
+#pragma unroll
+                for (int u = 0; u < TERMS; ++u) s[n][i % 2] = mma(k1, rows.qf[n][u][i / 2][1], s[n][i % 2]);
+            k = next_k;
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        uint2 v = value_codes(0);
+        f16x8 pf[NR][TERMS];
+        rows.weigh(s, ks, vs, blk, lane, pf);
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
-            const uint2 next = value_codes(d + 1 < ND ? d + 1 : d);
+            const uint2 next_v = value_codes(d + 1 < ND ? d + 1 : d);
             const f16x8 vf = codes_f16<false>(v.x, v.y);
 #pragma unroll
             for (int n = 0; n < NR; ++n)
 #pragma unroll
-                for (int u = 0; u < TERMS; ++u) o[n][d] = mma(vf, pf[n][u], o[n][d]);
-            v = next;
+                for (int u = 0; u < TERMS; ++u) rows.o[n][d] = mma(vf, pf[n][u], rows.o[n][d]);
+            v = next_v;
             __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (SLOTS == 1) {
+            asm volatile("" ::: "memory");
+            if (blk + kSharedWaves < b1) fetch_block<ND>(my_ring, a.kc[S], a.vc[S], cell0 + blk + kSharedWaves, a.D, lane);
         }
     }
     // join the waves: the four lanes of a row, then the upper half of the waves into the lower
-    auto stats_of = [&](int i) { return reinterpret_cast<float2*>(ring + i * kRingBytes<ND>); };
+    auto stats_of = [&](int i) { return reinterpret_cast<float2*>(ring + i * kRing); };
+    rows.finish();
 #pragma unroll
-    for (int n = 0; n < NR; ++n) {
-        l[n] += __shfl_xor(l[n], 16, 64);
-        l[n] += __shfl_xor(l[n], 32, 64);
-        if (g4 == 0) stats_of(wave)[16 * n + n16] = make_float2(m[n], l[n]);
-    }
+    for (int n = 0; n < NR; ++n)
+        if (g4 == 0) stats_of(wave)[16 * n + n16] = make_float2(rows.m[n], rows.l[n]);
     __syncthreads();
     auto* sums = reinterpret_cast<float(*)[NR * ND * 4][64]>(ring);
     float lt[NR], mt[NR];
@@ -387,50 +441,181 @@ __device__ __forceinline__ void attend(const SharedArgs& a, char* ring, int set,
             st[i] = stats_of(i)[16 * n + n16];
             mt[n] = fmaxf(mt[n], st[i].x);
         }
-        const float ref = mt[n] == -INFINITY ? 0.0f : mt[n];
         lt[n] = 0.0f;
 #pragma unroll
         for (int i = 0; i < kSharedWaves; ++i)
-            lt[n] += st[i].y * __builtin_amdgcn_exp2f(st[i].x - ref);
-        // from w to the maximum, in one step: a power of two, and 1 / kSumScale, which keeps sums of the largest values
-        // finite, with it (w is -inf where a row saw nothing or values of 0)
-        const float by = w[n] == -INFINITY ? 0.0f : w[n] - ref, whole_by = floorf(by), f = __builtin_amdgcn_exp2f(by - whole_by);
-        const int e = (int)whole_by + unit - kWeightLog2 - kSumLog2;
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[n][d][i] = ldexpf(o[n][d][i] * f, e);
+            lt[n] += st[i].y * __builtin_amdgcn_exp2f(st[i].x - (mt[n] == -INFINITY ? 0.0f : mt[n]));
+        rows.rescale(n, mt[n]);
     }
     __syncthreads();
 #pragma unroll
-    for (int step = kSharedWaves / 2; step >= 1; step >>= 1) {
-        if (wave >= step && wave < 2 * step)
+    for (int half = kSharedWaves / 2; half >= 1; half >>= 1) {
+        if (wave >= half && wave < 2 * half)
 #pragma unroll
-            for (int i = 0; i < NR * ND * 4; ++i) sums[wave - step][i][lane] = o[i / (ND * 4)][i / 4 % ND][i % 4];
+            for (int i = 0; i < NR * ND * 4; ++i) sums[wave - half][i][lane] = rows.o[i / (ND * 4)][i / 4 % ND][i % 4];
         __syncthreads();
-        if (wave < step)
+        if (wave < half)
 #pragma unroll
-            for (int i = 0; i < NR * ND * 4; ++i) o[i / (ND * 4)][i / 4 % ND][i % 4] += sums[wave][i][lane];
+            for (int i = 0; i < NR * ND * 4; ++i) rows.o[i / (ND * 4)][i / 4 % ND][i % 4] += sums[wave][i][lane];
         __syncthreads();
     }
     if (wave != 0) return;
 #pragma unroll
-    for (int n = 0; n < NR; ++n) {
-        const int r = r0 + 16 * n + n16;
-        if (r >= a.rows[S]) continue;
-        const int64_t at = row0 + r;
-        if (g4 == 0) *reinterpret_cast<float2*>(a.stat[S] + 2 * at) = make_float2(mt[n], lt[n]);
+    for (int n = 0; n < NR; ++n) rows.store(a, n, r0, row0, mt[n], lt[n], lane);
+}
+
+// The form for many rows of a prefix: each wave has rows of its own, 16 NR of the workgroup's 64 NR, and all take each
+// block.  Its codes are turned into f16 once for all of them, in registers on their way from memory to LDS: one buffer
+// is computed on while the next block's goes into the other, a barrier a block.
+// LDS: key rows of kWideRow 16-byte pieces, piece j of row 8 a + 4 tt + b in place j ^ turn; value rows of 32 keys, piece j of
+// row d in place j ^ value_place: an instruction serves lanes 0 .. 3, 12 .. 15, 20 .. 27 at once, and the like.
+template <int ND> constexpr int kWideRow = ND <= 4 ? 8 : 16;
+template <int ND> constexpr int kWideKeys = kKvBlock * kWideRow<ND> * 16;
+template <int ND> constexpr int kWideBytes = kWideKeys<ND> + ND * 1024;
+template <int ND> __device__ __forceinline__ int wide_turn(int r) {
+    return kWideRow<ND> == 8 ? ((r >> 3) & 3) << 1 | (r & 3) >> 1 : ((r >> 3) & 3) << 2 | (r & 3);
+}
+
+__device__ __forceinline__ int value_place(int d) { return -(d >> 2) & 3; }
+
+// 16 codes of a thread: piece i of 4 D in a block's 2 D of keys and 2 D of values.
+struct WideCodes {
+    u32x4 c[2];
+};
+__device__ __forceinline__ void load_codes(WideCodes& x, const int8_t* kc, const int8_t* vc, int64_t cell, int D) {
+    const int64_t base = cell * kKvBlock * D;
 #pragma unroll
-        for (int d = 0; d < ND; ++d)
-            if (16 * d < a.D) *reinterpret_cast<f32x4*>(a.part[S] + at * a.D + 16 * d + 4 * g4) = o[n][d];
+    for (int e = 0; e < 2; ++e) {
+        const int i = threadIdx.x + e * kSharedThreads;
+        if (i < 4 * D) x.c[e] = *reinterpret_cast<const u32x4*>((i < 2 * D ? kc : vc - 32 * D) + base + i * 16);
+    }
+}
+template <int ND>
+__device__ __forceinline__ void spread_codes(char* tile, const WideCodes& x, const int (&to)[2][2], int D) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        if ((int)threadIdx.x + e * kSharedThreads >= 4 * D) continue;
+        *reinterpret_cast<f16x8*>(tile + to[e][0]) = codes_f16<false>(x.c[e].x, x.c[e].y);
+        *reinterpret_cast<f16x8*>(tile + to[e][1]) = codes_f16<false>(x.c[e].z, x.c[e].w);
     }
 }
 
-// NP, NO: 16-row pieces of a workgroup's rows, of a prefix and of a sequence's own.
-template <int DT, int ND, int NP, int NO>
-__global__ __launch_bounds__(kSharedThreads, kOccupancy<ND>) void kv_shared_kernel(SharedArgs a) {
+template <int DT, int ND, int NR>
+__device__ __forceinline__ void attend_wide(const SharedArgs& a, char* lds, int set, int h, int rt, int b0, int b1, int64_t row0) {
+    using R = Rows<DT, ND, NR, 0>;
+    constexpr int TERMS = R::TERMS, NC = R::NC;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n16 = lane & 15, g4 = lane >> 4;
+    const int len = clamp_length(a.lengths[0][set], a.nb[0]);
+    const int64_t cell0 = ((int64_t)set * a.H + h) * a.nb[0];
+    const int r0 = (rt * kSharedWaves + wave) * NR * 16;
+    const bool rows_here = r0 < a.rows[0];   // the other waves only turn codes
+    // where the thread's codes go: keys, row i / (D / 16), pieces 2 (i % (D / 16)) and the next; values, row i / 2, pieces
+    // 2 (i % 2) and the next
+    int to[2][2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        int i = threadIdx.x + e * kSharedThreads;
+        const bool value = i >= 2 * a.D;
+        i -= value ? 2 * a.D : 0;
+        const int per = value ? 2 : a.D / 16, row = i / per, j = 2 * (i % per);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+            to[e][u] = value ? kWideKeys<ND> + row * 64 + ((j + u) ^ value_place(row)) * 16
+                             : (row * kWideRow<ND> + ((j + u) ^ wide_turn<ND>(row))) * 16;
+    }
+    float ks64, vs64;
+    auto load_scales = [&](int blk) {
+        ks64 = blk + lane < b1 ? a.ks[0][cell0 + blk + lane] : 0.0f;
+        vs64 = blk + lane < b1 ? a.vs[0][cell0 + blk + lane] : 0.0f;
+    };
+    load_scales(b0);
+    WideCodes raw[2];
+    if (b0 < b1) load_codes(raw[0], a.kc[0], a.vc[0], cell0 + b0, a.D);
+    if (b0 + 1 < b1) load_codes(raw[1], a.kc[0], a.vc[0], cell0 + b0 + 1, a.D);
+    // what no code goes to is read all the same (heads of 80): zeros
+    if (16 * ND != a.D)
+        for (int i = threadIdx.x; i < 2 * kWideBytes<ND> / 16; i += kSharedThreads) reinterpret_cast<u32x4*>(lds)[i] = u32x4{0, 0, 0, 0};
+    R rows;
+    float largest = 0.0f;
+    for (int i = b0 + lane; i < b1; i += 64) largest = fmaxf(largest, a.vs[0][cell0 + i]);
+    rows.template init<true>(a, set, h, r0, len, largest, lane);
+    const int key_row = 8 * (n16 >> 2) + (n16 & 3);
+    const int key_at = (key_row * kWideRow<ND> + (g4 ^ wide_turn<ND>(key_row))) * 16;
+    const int value_at = kWideKeys<ND> + n16 * 64 + (g4 ^ value_place(n16)) * 16;
+    __syncthreads();
+    if (b0 < b1) spread_codes<ND>(lds, raw[0], to, a.D);
+    if (b0 + 2 < b1) load_codes(raw[0], a.kc[0], a.vc[0], cell0 + b0 + 2, a.D);
+    // raw[1] holds the next block; raw[0] the one after it, on its way
+    auto body = [&](int blk, int step, const char* tile, char* other, WideCodes& next) {
+        // every wave has written its part of the tile, and read the other one
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0): loads from memory stay on their way
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (step % 64 == 0 && step) load_scales(blk);
+        const float ks = lane_value(ks64, step % 64), vs = lane_value(vs64, step % 64);
+        if (rows_here) {
+            f32x4 s[NR][2];
+#pragma unroll
+            for (int n = 0; n < NR; ++n) s[n][0] = s[n][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            auto key_codes = [&](int i) {
+                return *reinterpret_cast<const f16x8*>(tile + (key_at ^ i / 2 * 64) + i % 2 * 4 * kWideRow<ND> * 16);
+            };
+            auto value_codes = [&](int d) { return *reinterpret_cast<const f16x8*>(tile + value_at + d * 1024); };
+#pragma unroll
+            for (int i = 0; i < 4 * NC; ++i) {
+                if (i / 2 * 2 >= ND) continue;   // past the head
+                const f16x8 k = key_codes(i);
+#pragma unroll
+                for (int n = 0; n < NR; ++n)
+#pragma unroll
+                    for (int u = 0; u < TERMS; ++u) s[n][i % 2] = mma(k, rows.qf[n][u][i / 4][i / 2 % 2], s[n][i % 2]);
+            }
+            f16x8 pf[NR][TERMS];
+            rows.weigh(s, ks, vs, blk, lane, pf);
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                const f16x8 v = value_codes(d);
+#pragma unroll
+                for (int n = 0; n < NR; ++n)
+#pragma unroll
+                    for (int u = 0; u < TERMS; ++u) rows.o[n][d] = mma(v, pf[n][u], rows.o[n][d]);
+            }
+        }
+        if (blk + 1 < b1) spread_codes<ND>(other, next, to, a.D);
+        if (blk + 3 < b1) load_codes(next, a.kc[0], a.vc[0], cell0 + blk + 3, a.D);
+    };
+    for (int blk = b0, step = 0; blk < b1; blk += 2, step += 2) {
+        body(blk, step, lds, lds + kWideBytes<ND>, raw[1]);
+        if (blk + 1 < b1) body(blk + 1, step + 1, lds + kWideBytes<ND>, lds, raw[0]);
+    }
+    if (!rows_here) return;
+    rows.finish();
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+        rows.rescale(n, rows.m[n]);
+        rows.store(a, n, r0, row0, rows.m[n], rows.l[n], lane);
+    }
+}
+
+// NO: 16-row pieces of a sequence's own rows.  A prefix's go 16 to a wave, all four waves' against each block; heads of
+// more than 128 values, whose tiles of f16 would leave one workgroup a CU, take the form with a ring for 16 (float32) or 32.
+template <int DT, int ND, int NO>
+struct SharedForm {
+    static constexpr bool kWide = ND <= 8;
+    static constexpr int kPrefix = kWide ? 4 : DT == AXS6_F32 ? 1 : 2;   // 16-row pieces of a workgroup's
+    static constexpr int kSlots = kWide ? 1 : 2;
+    static constexpr int kRings = kSharedWaves * kSlots * kSlotBytes<ND>, kTiles = 2 * kWideBytes<ND>;
+    static constexpr int kLds = kWide && kTiles > kRings ? kTiles : kRings;
+    // waves a SIMD: as many as the registers allow
+    static constexpr int kOccupancy = !kWide ? 1 : DT == AXS6_F32 ? (NO == 2 ? 2 : 3) : NO == 2 ? 3 : 4;
+};
+
+template <int DT, int ND, int NO>
+__global__ __launch_bounds__(kSharedThreads, (SharedForm<DT, ND, NO>::kOccupancy)) void kv_shared_kernel(SharedArgs a) {
+    using F = SharedForm<DT, ND, NO>;
     // The kernel's only LDS variable: beside a second one the compiler waits for all loads into LDS before any read of it.
-    __shared__ __attribute__((aligned(1024))) char ring[kSharedWaves * kRingBytes<ND>];
+    __shared__ __attribute__((aligned(1024))) char lds[F::kLds];
     const int lane = threadIdx.x & 63;
     if ((int)blockIdx.x < a.prefix_groups) {
         // consecutive workgroups go round the 8 XCDs: the row tiles of a piece stay on one, whose
@@ -454,14 +639,17 @@ __global__ __launch_bounds__(kSharedThreads, kOccupancy<ND>) void kv_shared_kern
             b0 = piece % each * size;
             b1 = b0 + size < blocks ? b0 + size : blocks;
         }
-        attend<DT, ND, NP, 0>(a, ring, __builtin_amdgcn_readfirstlane(p), h, rt, __builtin_amdgcn_readfirstlane(b0),
-                              __builtin_amdgcn_readfirstlane(b1), (int64_t)unit * a.rows[0]);
+        p = __builtin_amdgcn_readfirstlane(p);
+        b0 = __builtin_amdgcn_readfirstlane(b0);
+        b1 = __builtin_amdgcn_readfirstlane(b1);
+        if constexpr (F::kWide) attend_wide<DT, ND, 1>(a, lds, p, h, rt, b0, b1, (int64_t)unit * a.rows[0]);
+        else attend<DT, ND, F::kPrefix, 0, F::kSlots>(a, lds, p, h, rt, b0, b1, (int64_t)unit * a.rows[0]);
     } else {
         const int i = blockIdx.x - a.prefix_groups, piece = i % a.pieces[1], j = i / a.pieces[1];
         const int rt = j % a.row_tiles[1], bh = j / a.row_tiles[1], b = bh / a.H, h = bh % a.H;
         const int len = clamp_length(a.lengths[1][b], a.nb[1]), blocks = blocks_of(len);
         const int size = (blocks + a.pieces[1] - 1) / a.pieces[1], b0 = piece * size;
-        attend<DT, ND, NO, 1>(a, ring, b, h, rt, b0, b0 + size < blocks ? b0 + size : blocks,
+        attend<DT, ND, NO, 1, F::kSlots>(a, lds, b, h, rt, b0, b0 + size < blocks ? b0 + size : blocks,
                               ((int64_t)piece * a.P * a.W * a.H + bh) * a.rows[1]);
     }
 }
@@ -542,7 +730,7 @@ __global__ __launch_bounds__(kJoinSize) void kv_shared_join_kernel(SharedArgs a)
     for (int j = 0; j < 4; ++j) out[j] = E::from_f(o[j] * rl);
 }
 
-constexpr int kMostRows = 2;   // 16-row pieces
+constexpr int kFewest = 2;   // blocks of a piece (4 beams on 300 tokens: 2 12.6 us, 4 14.7, 8 15.8)
 
 // How a call is laid out.
 struct SharedPlan {
@@ -552,33 +740,31 @@ struct SharedPlan {
 SharedPlan shared_plan(int dtype, int64_t P, int64_t W, int64_t H, int64_t rows, int64_t D, int64_t prefix_blocks,
                        int64_t blocks) {
     SharedPlan p;
-    p.np = D > 128 && dtype == AXS6_F32 ? 1 : kMostRows;
+    p.np = D <= 128 ? 4 : dtype == AXS6_F32 ? 1 : 2;
     p.no = D > 128 || rows <= 16 ? 1 : 2;
     p.row_tiles[0] = (W * rows + 16 * p.np - 1) / (16 * p.np);
     p.row_tiles[1] = (rows + 16 * p.no - 1) / (16 * p.no);
-    // two workgroups a CU, and at least 8 blocks each
-    const int64_t most = 512;
-    const int64_t groups = H * p.row_tiles[0];
+    // seven of eight workgroups that the card holds, of some blocks each
+    const int64_t most = 224 * (D > 128 ? 1 : dtype == AXS6_F32 ? (p.no == 2 ? 2 : 3) : p.no == 2 ? 3 : 4);
+    const int64_t groups = H * p.row_tiles[0], some = P * ((prefix_blocks + kFewest - 1) / kFewest);
     int64_t n = (most + groups - 1) / groups;
-    n = n < P * ((prefix_blocks + 7) / 8) ? n : P * ((prefix_blocks + 7) / 8);
+    n = n < some ? n : some;
     p.even = P <= kMaxEven;
-    if (p.even) p.pieces[0] = n + P - 1;
-    else p.pieces[0] = P * ((n + P - 1) / P);
+    p.pieces[0] = p.even ? n + P - 1 : P * ((n + P - 1) / P);
     const int64_t own = P * W * H * p.row_tiles[1];
     n = (most + own - 1) / own;
-    n = n < (blocks + 7) / 8 ? n : (blocks + 7) / 8;
-    p.pieces[1] = n;
+    p.pieces[1] = n < (blocks + kFewest - 1) / kFewest ? n : (blocks + kFewest - 1) / kFewest;
     return p;
 }
 
 template <int DT, int ND>
 void launch_shared(const SharedArgs& a, const SharedPlan& p, unsigned grid, hipStream_t st) {
-    if constexpr (ND > 8) {
-        kv_shared_kernel<DT, ND, DT == AXS6_F32 ? 1 : 2, 1><<<grid, kSharedThreads, 0, st>>>(a);
-    } else {
-        if (p.no == 1) kv_shared_kernel<DT, ND, kMostRows, 1><<<grid, kSharedThreads, 0, st>>>(a);
-        else kv_shared_kernel<DT, ND, kMostRows, 2><<<grid, kSharedThreads, 0, st>>>(a);
-    }
+    if constexpr (ND <= 8)
+        if (p.no == 2) {
+            kv_shared_kernel<DT, ND, 2><<<grid, kSharedThreads, 0, st>>>(a);
+            return;
+        }
+    kv_shared_kernel<DT, ND, 1><<<grid, kSharedThreads, 0, st>>>(a);
 }
 
 }  // namespace
