@@ -96,7 +96,7 @@ _SIGNATURES: dict[str, list] = {
     "axs6_kv_shared_attention_workspace": [_i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64],
     "axs6_kv_shared_attention": [_vp, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp,
                                  _vp, _vp, _vp, _i64, _vp, ctypes.c_float, _vp, _vp, _i64, _vp],
-    "axs6_beam_select_workspace": [_i64, _i64, _i64, _i32],
+    "axs6_beam_select_workspace": [_i64, _i64, _i64, _i64, _i32],
     "axs6_beam_select": [_vp, _i32, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp],
     "axs6_distill_forward": [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _i64, ctypes.c_float, _vp, _i32, _vp, _vp, _vp,
                              _vp, _vp],

@@ -491,7 +491,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> beam_select(const at::Tensor& log
     at::Tensor top = at::empty({G, C}, scores.options()), parents = at::empty({G, C}, scores.options().dtype(at::kLong)),
                tokens = at::empty_like(parents);
     if (G == 0) return {top, parents, tokens};
-    const at::Tensor ws = workspace(axs6_beam_select_workspace(G, W, V, dtype_code(z.scalar_type())), z);
+    const at::Tensor ws = workspace(axs6_beam_select_workspace(G, W, V, C, dtype_code(z.scalar_type())), z);
     check_rc(axs6_beam_select(z.data_ptr(), dtype_code(z.scalar_type()), G, W, V, z.stride(0), z.stride(1),
                               c.data_ptr<float>(), f.defined() ? reinterpret_cast<const uint8_t*>(f.data_ptr<bool>()) : nullptr,
                               end ? *end : 0, C, top.data_ptr<float>(), parents.data_ptr<int64_t>(),

@@ -511,7 +511,7 @@ int axs6_kv_shared_attention(const void* q, int32_t dtype, int64_t P, int64_t W,
  * rounded once to float32.  Outputs (G, count). */
 #define AXS6_BEAM_MAX_COUNT 128
 #define AXS6_BEAM_MAX_BEAMS 1024   /* of a sequence; of all 65535 */
-int64_t axs6_beam_select_workspace(int64_t G, int64_t W, int64_t V, int32_t dtype);
+int64_t axs6_beam_select_workspace(int64_t G, int64_t W, int64_t V, int64_t count, int32_t dtype);
 int axs6_beam_select(const void* logits, int32_t dtype, int64_t G, int64_t W, int64_t V, int64_t ld_sequence,
                      int64_t ld_beam, const float* scores, const uint8_t* finished, int64_t end, int64_t count,
                      float* out_scores, int64_t* parents, int64_t* tokens, void* workspace, int64_t workspace_bytes,

@@ -45,8 +45,8 @@ def test_select_checks_its_arguments():
                        ({"a14": 4104}, 1), ({"a15": 16}, 1), ({"a2": 0}, 0), ({"a2": -1}, 1)):
         assert _call(L.axs6_beam_select, good, **change) == rc, change
         assert rc == 0 or L.axs6_last_error()
-    assert L.axs6_beam_select_workspace(0, 3, 100, 0) == 0 and L.axs6_beam_select_workspace(2, 3, 100, 9) == 0
-    assert 0 < L.axs6_beam_select_workspace(2, 3, 100, 0) < L.axs6_beam_select_workspace(64, 8, 128000, 1) < 1 << 20
+    assert L.axs6_beam_select_workspace(0, 3, 100, 3, 0) == 0 and L.axs6_beam_select_workspace(2, 3, 100, 3, 9) == 0
+    assert 0 < L.axs6_beam_select_workspace(2, 3, 100, 3, 0) < L.axs6_beam_select_workspace(64, 8, 128000, 16, 1) < 1 << 20
 
 
 def test_copy_checks_its_arguments():
