@@ -8,7 +8,25 @@
 // group have in the same places, waits, and writes: no order of the sequences is
 // needed and no second buffer.
 //
-// Bound by HBM: each source is read and each target written once.
+// Bound by HBM: each source is read and each target written once.  Measured: 32 groups of
+// 8 beams, 2047 tokens, 8 heads of 128 (950 MB) in 208 us, 4.6 TB/s; 256 sequences of 375
+// to 1500 tokens closed up, 4 heads of 64 (200 MB), in 43 us, 4.7 TB/s; a prompt of 4001
+// tokens forked 8 ways for 8 groups, 12 heads of 80, in 66 us; four beams of 40 tokens in
+// 5 us, of which the launch and the chain sources - lengths - codes are all.
+//
+// - A head's blocks lie behind one another in both caches, so a piece is one run of 16-byte
+//   places and a thread keeps the same sequences through all its pieces: what remains a
+//   piece is a load, in place a barrier, and a store.  (Finding tensor, sequence and length
+//   anew for each value: 96 us for the 256 sequences.)
+// - A workgroup takes 1024 threads where a group is so large that fewer would leave a
+//   sequence less than a cache line of a piece.  Two of 1024 or eight of 256 fit a CU; calls
+//   of few pieces start just as many workgroups as fit (1 x 134 sequences of 288 tokens:
+//   8.8 us, one workgroup a piece 12.0), long ones four times that, so that the last ones
+//   to end are short (32 x 8 beams: 208 us, as many as fit 238).
+// - Stores pass the L2 by: what a fork reads stays there for its other sequences (95 us
+//   without, for 66; beams 219 for 214, closing up 45 for 43).
+// - Loading the next piece before this one is stored was slower at all sizes (43 to 48 us
+//   for the 256 sequences, 214 to 225 us for the beams): the workgroups beside it do that.
 #include "axs6_internal.h"
 #include "kv_cache.h"
 #include "nf5_device.h"
@@ -31,10 +49,25 @@ struct CopyArgs {
     int in_place;
 };
 
+// A thread's part of every piece: the same place of kItems of the target's sequences.
+struct Item {
+    uint32_t src, dst;         // sequences' heads in the cache and in the target
+    int n;                     // tokens
+};
+
+// In place: all threads' values are here before any place is written.
+template <class T>
+__device__ __forceinline__ void arrived(T (&v)[kItems], int in_place) {
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) asm volatile("" : "+v"(v[k]) : : "memory");
+    if (in_place) __builtin_amdgcn_s_barrier();
+    asm volatile("" : : : "memory");
+}
+
 // One workgroup a (group, head) and every gridDim.y-th piece of its places.
 template <int THREADS>
-__global__ __launch_bounds__(THREADS) void kv_copy_kernel(CopyArgs a) {
-    extern __shared__ int sh[];            // each target's source, or -1, and its length
+__global__ __launch_bounds__(THREADS, 2048 / THREADS) void kv_copy_kernel(CopyArgs a) {
+    extern __shared__ int sh[];            // each target's source, and its length, 0 where nothing is copied
     __shared__ int top;
     int *from = sh, *len = sh + a.W;
     const int g = blockIdx.x / a.H, h = blockIdx.x % a.H;
@@ -47,61 +80,73 @@ __global__ __launch_bounds__(THREADS) void kv_copy_kernel(CopyArgs a) {
         const bool use = p >= 0 && p < a.src_seq && !(a.in_place && p == i);
         int64_t n = use ? a.lengths[g * a.src_seq + p] : 0;
         n = n < 0 ? 0 : n > cap ? cap : n;
-        from[i] = n > 0 ? (int)p : -1;
+        from[i] = use ? (int)p : 0;
         len[i] = (int)n;
         if (n > 0) atomicMax(&top, (int)n);
     }
     __syncthreads();
-    const int cols = 1 << a.cols_log2, blocks = (top + kKvBlock - 1) / kKvBlock;
-    // pieces of the six tensors: 16-byte values of codes and tails, 4-byte ones of scales
-    const int block_vecs = kKvBlock * a.D / 16, row_vecs = a.D * a.es / 16;
-    const int64_t code_pieces = ((int64_t)blocks * block_vecs + cols - 1) >> a.cols_log2;
-    const int scale_pieces = (blocks + cols - 1) >> a.cols_log2, tail_pieces = (kKvBlock * row_vecs + cols - 1) >> a.cols_log2;
-    const int64_t pieces = 2 * (code_pieces + scale_pieces + tail_pieces);
+    const int blocks = (top + kKvBlock - 1) / kKvBlock, block_vecs = kKvBlock * a.D / 16, row_vecs = a.D * a.es / 16;
     if (blocks == 0) return;
-    const int items = a.W << a.cols_log2;
-    for (int64_t piece = blockIdx.y; piece < pieces; piece += gridDim.y) {
-        int z;                       // which tensor
-        int64_t at = piece;          // which piece of it
-        if (at < 2 * code_pieces) { z = at < code_pieces ? 0 : 2; at -= z ? code_pieces : 0; }
-        else if ((at -= 2 * code_pieces) < 2 * scale_pieces) { z = at < scale_pieces ? 1 : 3; at -= z == 3 ? scale_pieces : 0; }
-        else { at -= 2 * scale_pieces; z = at < tail_pieces ? 4 : 5; at -= z == 5 ? tail_pieces : 0; }
-        const int64_t c0 = at << a.cols_log2;
-        const bool scales = z == 1 || z == 3, tail = z >= 4;
-        // values of a sequence's head in the cache and in the target
-        const int64_t per_src = scales ? a.nb_src : tail ? kKvBlock * row_vecs : (int64_t)a.nb_src * block_vecs;
-        const int64_t per_dst = scales ? a.nb_dst : tail ? kKvBlock * row_vecs : (int64_t)a.nb_dst * block_vecs;
+    const int cols = 1 << a.cols_log2, col = threadIdx.x & (cols - 1);
+    Item it[kItems];
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+        const int i = (threadIdx.x + k * THREADS) >> a.cols_log2;
+        const bool in = i < a.W;
+        it[k].n = in ? len[i] : 0;
+        it[k].src = (uint32_t)((g * a.src_seq + (in ? from[i] : 0)) * a.H + h);
+        it[k].dst = (uint32_t)((g * a.dst_seq + w0 + i) * a.H + h);
+    }
+
+    // codes: a head's blocks lie behind one another; pieces of keys and of values take turns
+    const int pieces = 2 * ((blocks * block_vecs + cols - 1) >> a.cols_log2);
+    const uint32_t per_src = (uint32_t)(a.nb_src * block_vecs), per_dst = (uint32_t)(a.nb_dst * block_vecs);
+    auto has = [&](int p, int k) { return (p >> 1 << a.cols_log2) + col < (it[k].n + kKvBlock - 1) / kKvBlock * block_vecs; };
+    const int step = gridDim.y;
+    int p = blockIdx.y;
+    for (; p < pieces; p += step) {
+        const int64_t at = (p >> 1 << a.cols_log2) + col;
+        const u32x4* src = reinterpret_cast<const u32x4*>(a.src[p & 1 ? 2 : 0]) + at;
+        u32x4* dst = reinterpret_cast<u32x4*>(a.dst[p & 1 ? 2 : 0]) + at;
         u32x4 v[kItems];
-        int64_t to[kItems];
 #pragma unroll
         for (int k = 0; k < kItems; ++k) {
-            const int item = threadIdx.x + k * THREADS, i = item >> a.cols_log2;
-            const int64_t c = c0 + (item & (cols - 1));
-            to[k] = -1;
             v[k] = u32x4{0, 0, 0, 0};
-            if (item >= items) continue;
-            const int p = from[i];
-            if (p < 0) continue;
-            const int n = len[i], nb = (n + kKvBlock - 1) / kKvBlock;
-            const int64_t count = scales ? nb : tail ? n % kKvBlock * row_vecs : (int64_t)nb * block_vecs;
-            if (c >= count) continue;
-            to[k] = ((g * a.dst_seq + w0 + i) * a.H + h) * per_dst + c;
-            const int64_t s = ((g * a.src_seq + p) * a.H + h) * per_src + c;
-            if (scales) v[k].x = reinterpret_cast<const uint32_t*>(a.src[z])[s];
-            else v[k] = reinterpret_cast<const u32x4*>(a.src[z])[s];
+            if (has(p, k)) v[k] = src[(uint64_t)it[k].src * per_src];
         }
-        if (a.in_place) {
-            // the values are here before any of them is written over
+        arrived(v, a.in_place);
 #pragma unroll
-            for (int k = 0; k < kItems; ++k) asm volatile("" : "+v"(v[k]));
-            __syncthreads();
-        }
+        for (int k = 0; k < kItems; ++k)
+            if (has(p, k)) __builtin_nontemporal_store(v[k], dst + (uint64_t)it[k].dst * per_dst);
+    }
+
+    // scales and raw rows: more pieces behind those of the codes
+    const int scale_pieces = 2 * ((blocks + cols - 1) >> a.cols_log2), tail_pieces = 2 * ((kKvBlock * row_vecs + cols - 1) >> a.cols_log2);
+    for (p -= pieces; p < scale_pieces; p += step) {
+        const int c = (p >> 1 << a.cols_log2) + col, z = p & 1 ? 3 : 1;
+        uint32_t v[kItems];
 #pragma unroll
         for (int k = 0; k < kItems; ++k) {
-            if (to[k] < 0) continue;
-            if (scales) reinterpret_cast<uint32_t*>(a.dst[z])[to[k]] = v[k].x;
-            else reinterpret_cast<u32x4*>(a.dst[z])[to[k]] = v[k];
+            v[k] = 0;
+            if (c * kKvBlock < it[k].n) v[k] = reinterpret_cast<const uint32_t*>(a.src[z])[(uint64_t)it[k].src * (uint32_t)a.nb_src + c];
         }
+        arrived(v, a.in_place);
+#pragma unroll
+        for (int k = 0; k < kItems; ++k)
+            if (c * kKvBlock < it[k].n) reinterpret_cast<uint32_t*>(a.dst[z])[(uint64_t)it[k].dst * (uint32_t)a.nb_dst + c] = v[k];
+    }
+    for (p -= scale_pieces; p < tail_pieces; p += step) {
+        const int c = (p >> 1 << a.cols_log2) + col, z = p & 1 ? 5 : 4;
+        u32x4 v[kItems];
+#pragma unroll
+        for (int k = 0; k < kItems; ++k) {
+            v[k] = u32x4{0, 0, 0, 0};
+            if (c < it[k].n % kKvBlock * row_vecs) v[k] = reinterpret_cast<const u32x4*>(a.src[z])[(uint64_t)it[k].src * (kKvBlock * row_vecs) + c];
+        }
+        arrived(v, a.in_place);
+#pragma unroll
+        for (int k = 0; k < kItems; ++k)
+            if (c < it[k].n % kKvBlock * row_vecs) reinterpret_cast<u32x4*>(a.dst[z])[(uint64_t)it[k].dst * (kKvBlock * row_vecs) + c] = v[k];
     }
 }
 
@@ -158,13 +203,14 @@ extern "C" int axs6_kv_copy(const void* k_codes, const float* k_scales, const vo
     a.W = (int)(a.in_place || targets < 64 ? targets : 64);
     a.H = (int)H; a.D = (int)D; a.nb_src = (int)blocks; a.nb_dst = (int)target_blocks; a.es = (int)es;
     const int threads = a.W <= 64 ? 256 : 1024;
-    while (a.cols_log2 < 10 && (a.W << (a.cols_log2 + 1)) <= kItems * threads) ++a.cols_log2;
-    const int64_t tiles = (targets + a.W - 1) / a.W;
-    if (tiles > 65535) return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: dimension too large", fn);
-    const int64_t nb = blocks < target_blocks ? blocks : target_blocks;
+    while ((2 << a.cols_log2) <= threads && (a.W << (a.cols_log2 + 1)) <= kItems * threads) ++a.cols_log2;
+    const int64_t tiles = (targets + a.W - 1) / a.W, nb = blocks < target_blocks ? blocks : target_blocks;
+    // a piece's places are counted in 32 bits, and a sequence's head's
+    if (tiles > 65535 || (blocks > target_blocks ? blocks : target_blocks) * (2 * D) >= (int64_t)1 << 30)
+        return fail(AXS6_ERR_INVALID_ARGUMENT, "%s: dimension too large", fn);
     int64_t pieces = (2 * (nb * kKvBlock * D / 16 + nb) >> a.cols_log2) + 4;
-    const int64_t want = (4096 + groups * H * tiles - 1) / (groups * H * tiles);
-    if (pieces > want) pieces = want;
+    const int64_t heads = groups * H * tiles, fit = 512 * 1024 / threads, want = pieces * heads > 12 * fit ? 4 * fit : fit;
+    if (pieces * heads > want) pieces = (want + heads - 1) / heads;
     if (pieces > 65535) pieces = 65535;
     const dim3 grid((unsigned)(groups * H), (unsigned)pieces, (unsigned)tiles);
     const size_t lds = 2 * a.W * sizeof(int);
