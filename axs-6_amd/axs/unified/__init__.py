@@ -10,8 +10,9 @@ HIP kernels, not Triton.  The training pipeline (``AXSTrainingPipelineUnified``,
 ``AmaxEMA``) runs its gradient unscale, overflow check and clipping as one
 fused device pass.  A decoder's operators beyond the reference's -- rotary
 positions, attention without the score matrix, the 8-bit cache and attention
-over it, distillation from a teacher's top logits -- run on HIP kernels of
-their own.  The distributed gradient hooks are not part of this
+over it, beam search (selection, copies of cached sequences, attention over a
+shared prefix), distillation from a teacher's top logits -- run on HIP kernels
+of their own.  The distributed gradient hooks are not part of this
 package (the NF5 gradient codec is, in ``axs.unified.distributed``).
 """
 from axs.unified.attention_unified import AXSCausalSelfAttentionUnified, axs_attention_unified
@@ -26,7 +27,7 @@ from axs.unified.backend import (
     get_backend,
     set_backend,
 )
-from axs.unified.beam_unified import axs_beam_select_unified
+from axs.unified.beam_unified import axs_beam_search_unified, axs_beam_select_unified
 from axs.unified.distillation_unified import axs_distillation_loss_unified
 from axs.unified.functional_unified import (
     axs_linear_group_unified,
@@ -126,5 +127,6 @@ __all__ = [
     "axs_cache_copy_unified",
     "axs_cache_shared_attention_unified",
     "axs_beam_select_unified",
+    "axs_beam_search_unified",
     "axs_distillation_loss_unified",
 ]

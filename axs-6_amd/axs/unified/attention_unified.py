@@ -16,7 +16,12 @@ import torch.nn as nn
 from axs import _lib
 from axs.core import DEFAULT_BLOCK_SIZE
 from axs.unified.functional_unified import axs_linear_group_unified
-from axs.unified.kv_cache_unified import AXSKVCacheUnified, axs_cache_append_unified, axs_cache_attention_unified
+from axs.unified.kv_cache_unified import (
+    AXSKVCacheUnified,
+    axs_cache_append_unified,
+    axs_cache_attention_unified,
+    axs_cache_shared_attention_unified,
+)
 from axs.unified.modules_unified import AXSLinearUnified
 from axs.unified.rotary_unified import axs_rotary_unified
 
@@ -106,13 +111,29 @@ class AXSCausalSelfAttentionUnified(nn.Module):
         """An empty cache of this layer's heads."""
         return AXSKVCacheUnified.empty(batch, self.num_kv_heads, self.head_dim, max_tokens, dtype, device)
 
-    def decode(self, x: torch.Tensor, table: torch.Tensor, cache: AXSKVCacheUnified, starts: torch.Tensor) -> torch.Tensor:
+    def decode(self, x: torch.Tensor, table: torch.Tensor, cache: AXSKVCacheUnified, starts: torch.Tensor,
+               prefix: AXSKVCacheUnified | None = None, prefix_lengths: torch.Tensor | None = None) -> torch.Tensor:
         """``x`` (B, T, embed_dim): tokens ``starts[b]``.. of each sequence, a prompt's
-        or the next one.  They join the cache and attend over it; no gradient."""
+        or the next one.  They join the cache and attend over it; no gradient.
+
+        ``prefix``, a cache of P sequences of ``prefix_lengths`` (P) tokens: sequence b goes on from
+        prefix b // (B / P), its tokens' places counted from the prefix's end, and attends over
+        both (:func:`axs_cache_shared_attention_unified`)."""
+        if (prefix is None) != (prefix_lengths is None):
+            raise ValueError("a prefix and its lengths come together")
         with torch.no_grad():
             q, k, v = self._heads(x)
-            positions = starts[:, None] + torch.arange(x.shape[1], device=x.device)
+            places = starts
+            if prefix is not None:
+                P = prefix_lengths.numel()
+                if P == 0 or x.shape[0] % P:
+                    raise ValueError(f"{x.shape[0]} sequences do not divide among {P} prefixes")
+                places = starts + prefix_lengths.repeat_interleave(x.shape[0] // P, output_size=x.shape[0])
+            positions = places[:, None] + torch.arange(x.shape[1], device=x.device)
             q, k = axs_rotary_unified(q, k, table, positions)
             axs_cache_append_unified(cache, k, v, starts)
-            out = axs_cache_attention_unified(q, cache, starts + x.shape[1])
+            if prefix is None:
+                out = axs_cache_attention_unified(q, cache, starts + x.shape[1])
+            else:
+                out = axs_cache_shared_attention_unified(q, prefix, prefix_lengths, cache, starts + x.shape[1])
             return self.out_proj(out.flatten(2))

@@ -1,13 +1,17 @@
 """Beam search: the choice of the best continuations over beams and vocabulary.
 
 ``axs_beam_select_unified`` scores every continuation of every beam and keeps the best,
-from one reading of the logits.  The reference has no counterpart.
+from one reading of the logits; ``axs_beam_search_unified`` is the loop around it that
+keeps the 8-bit caches in step with the beams.  The reference has no counterpart.
 """
 from __future__ import annotations
+
+from collections.abc import Callable, Sequence
 
 import torch
 
 from axs import _lib
+from axs.unified.kv_cache_unified import AXSKVCacheUnified, axs_cache_copy_unified
 
 
 def axs_beam_select_unified(
@@ -33,3 +37,47 @@ def axs_beam_select_unified(
 
     Sums and comparisons are in float64, the scores are rounded once.  No gradient."""
     return _lib.ext().beam_select(logits, scores, finished, end, count)
+
+
+@torch.no_grad()
+def axs_beam_search_unified(
+    step: Callable[[torch.Tensor, torch.Tensor], torch.Tensor],
+    logits: torch.Tensor,
+    caches: Sequence[AXSKVCacheUnified],
+    beams: int,
+    steps: int,
+    end: int | None = None,
+    starts: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """The ``beams`` (at most 128) best continuations by ``steps`` tokens of each of G prompts:
+    (scores (G, beams) float32, log probabilities; tokens (G, beams, steps) int64), best first.
+
+    ``logits`` (G, V), those of the token after each prompt.  ``caches``, one a layer, hold the
+    G * beams sequences of the beams: their own tokens alone where the prompt is a shared prefix,
+    else the prompts forked (:func:`axs_cache_copy_unified`) and ``starts`` (G * beams), the tokens
+    that each holds (None: 0).  ``step(tokens (G * beams, 1), starts (G * beams))`` appends those
+    tokens to the caches and returns the logits of the next, (G * beams, V) or (G * beams, 1, V);
+    it is called ``steps - 1`` times.  A beam that chose ``end`` goes on as it, at its score.
+    Slots for which there is no candidate have the score -inf."""
+    if beams < 1 or steps < 1:
+        raise ValueError(f"{beams} beams of {steps} steps")
+    G = logits.shape[0]
+    scores, parents, tokens = axs_beam_select_unified(
+        logits[:, None], torch.zeros(G, 1, device=logits.device), count=beams)
+    if starts is None:
+        starts = torch.zeros(G * beams, dtype=torch.int64, device=logits.device)
+    out = tokens[..., None]
+    finished = None if end is None else tokens == end
+    for i in range(1, steps):
+        logits = step(tokens.view(-1, 1), starts)
+        starts = starts + 1
+        scores, parents, tokens = axs_beam_select_unified(
+            logits.reshape(G, beams, -1), scores, finished, end)
+        out = torch.cat([out.gather(1, parents[..., None].expand(-1, -1, i)), tokens[..., None]], -1)
+        if end is not None:
+            finished = finished.gather(1, parents) | (tokens == end)
+        if i + 1 < steps:
+            for cache in caches:
+                axs_cache_copy_unified(cache, parents, starts)
+            starts = starts.view(G, beams).gather(1, parents).flatten()
+    return scores, out

@@ -9,7 +9,8 @@ from the 8-bit cache: the library's decoder operators together.
    NF5, rotary positions and grouped heads; it never sees the data's labels, only
    the teacher's 16 top logits of each token (``axs_distillation_loss_unified``).
 3. The student continues a prompt, token by token, from the 8-bit cache
-   (``AXSCausalSelfAttentionUnified.decode``).
+   (``AXSCausalSelfAttentionUnified.decode``), then with four beams that share
+   the prompt's cache (``axs_beam_search_unified``).
 """
 from __future__ import annotations
 
@@ -73,8 +74,8 @@ class Block(nn.Module):
     def forward(self, x: torch.Tensor, table: torch.Tensor) -> torch.Tensor:
         return self.ffn(x + self.attn(self.n1(x), table))
 
-    def decode(self, x: torch.Tensor, table: torch.Tensor, cache: axu.AXSKVCacheUnified, starts: torch.Tensor) -> torch.Tensor:
-        return self.ffn(x + self.attn.decode(self.n1(x), table, cache, starts))
+    def decode(self, x: torch.Tensor, table: torch.Tensor, cache: axu.AXSKVCacheUnified, starts: torch.Tensor, *prefix) -> torch.Tensor:
+        return self.ffn(x + self.attn.decode(self.n1(x), table, cache, starts, *prefix))
 
 
 class Decoder(nn.Module):
@@ -94,11 +95,13 @@ class Decoder(nn.Module):
         return self.head(self.norm(x))
 
     @torch.no_grad()
-    def logits_from_cache(self, tokens: torch.Tensor, caches: list, starts: torch.Tensor) -> torch.Tensor:
-        """Logits of ``tokens`` (B, T), which follow the ``starts[b]`` tokens that the caches hold."""
+    def logits_from_cache(self, tokens: torch.Tensor, caches: list, starts: torch.Tensor, prefixes: list | None = None,
+                          lengths: torch.Tensor | None = None) -> torch.Tensor:
+        """Logits of ``tokens`` (B, T), which follow the ``starts[b]`` tokens that the caches hold, and those before
+        them of the shared prefixes, if any."""
         x = self.embed(tokens)
-        for b, cache in zip(self.blocks, caches):
-            x = b.decode(x, self.table, cache, starts)
+        for i, (b, cache) in enumerate(zip(self.blocks, caches)):
+            x = b.decode(x, self.table, cache, starts, *(() if prefixes is None else (prefixes[i], lengths)))
         return self.head(self.norm(x))
 
     @torch.no_grad()
@@ -114,6 +117,20 @@ class Decoder(nn.Module):
             new = logits[:, -1:].argmax(-1)
             out.append(new)
         return torch.cat(out, 1)
+
+    @torch.no_grad()
+    def generate_beams(self, prompt: torch.Tensor, count: int, beams: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """The ``beams`` likeliest continuations found of each ``prompt`` (B, T) by ``count`` tokens: their log
+        probabilities (B, beams) and the whole sequences (B, beams, T + count).  A prompt is cached once for all of
+        its beams, which cache their own tokens alone."""
+        B, T = prompt.shape
+        prompts = [b.attn.new_cache(B, T, device=prompt.device) for b in self.blocks]
+        caches = [b.attn.new_cache(B * beams, count, device=prompt.device) for b in self.blocks]
+        lengths = torch.full((B,), T, dtype=torch.int64, device=prompt.device)
+        logits = self.logits_from_cache(prompt, prompts, torch.zeros_like(lengths))[:, -1]
+        scores, tokens = axu.axs_beam_search_unified(
+            lambda new, starts: self.logits_from_cache(new, caches, starts, prompts, lengths), logits, caches, beams, count)
+        return scores, torch.cat([prompt[:, None].expand(-1, beams, -1), tokens], -1)
 
 
 def sequences(c: Config, g: torch.Generator, device: str) -> torch.Tensor:
@@ -165,6 +182,9 @@ def main() -> None:
     got = student.generate(want[:, :16], a.tokens)
     share = float((got[:, 16:] == want[:, 16:]).float().mean())
     print(f"{a.tokens} tokens from the 8-bit cache after 16: {100 * share:.0f}% as the sequences go on")
+    scores, got = student.generate_beams(want[:, :16], a.tokens, 4)
+    share = float((got[:, 0, 16:] == want[:, 16:]).float().mean())
+    print(f"the best of 4 beams: {100 * share:.0f}%, log probability {float(scores[:, 0].mean()):.2f}")
 
 
 if __name__ == "__main__":

@@ -144,6 +144,37 @@ def test_select_refusals():
     assert [x.shape for x in empty] == [(0, 3)] * 3
 
 
+@pytest.mark.parametrize("dtype", ref.DTYPES)
+@pytest.mark.parametrize("G,W,V,count", [(1, 1000, 9000, 5), (2, 600, 9000, 128)])
+def test_select_over_many_segments(G, W, V, count, dtype):
+    """More segments than are looked at in one go, and as many equal ones."""
+    logits = torch.randn(G, W, V, generator=_gen(V)).to(DEV, dtype)
+    scores = -torch.rand(G, W, generator=_gen(W)).to(DEV)
+    _check_select(logits, scores, count=count)
+    # all alike: the first tokens of the first beam
+    got = axs_select(torch.full_like(logits, 0.5), torch.zeros_like(scores), count)
+    assert not got[1].any() and torch.equal(got[2].cpu(), torch.arange(count).expand(G, count))
+
+
+@pytest.mark.parametrize("dtype", ref.DTYPES)
+def test_select_among_many_equal_tokens(dtype):
+    V = 300000
+    logits = torch.zeros(2, 1, V, device=DEV, dtype=dtype)
+    got = axs_select(logits, torch.zeros(2, 1, device=DEV), 128)
+    assert not got[1].any() and torch.equal(got[2].cpu(), torch.arange(128).expand(2, 128))
+    # the best of them at the end, and one of each few hundred
+    logits[0, 0, -200:] = 1
+    logits[1, 0, 5::601] = 1
+    got = axs_select(logits, torch.zeros(2, 1, device=DEV), 128)
+    assert torch.equal(got[2].cpu(), torch.stack([torch.arange(V - 200, V - 72), 5 + 601 * torch.arange(128)]))
+
+
+def axs_select(logits, scores, count):
+    from axs.unified import axs_beam_select_unified
+
+    return axs_beam_select_unified(logits, scores, count=count)
+
+
 # ---- copies ------------------------------------------------------------------------
 
 
@@ -316,6 +347,8 @@ def _bound(dt):
     (3, 8, 1, 8, 1, 96, [700, 33, 2000], [32] * 24), (1, 6, 5, 4, 2, 64, [129], [0, 1, 4, 5, 6, 70]),
     (1, 2, 7, 2, 1, 48, [3], [2, 5]), (2, 40, 1, 4, 1, 256, [200, 900], [9] * 80), (1, 33, 3, 2, 1, 192, [500], [40] * 33),
     (1, 64, 1, 32, 4, 128, [4000], [50] * 64), (1, 3, 1, 4, 2, 128, [9000], [300, 700, 1]), (12, 2, 1, 28, 7, 64, [257] * 12, [8] * 24),
+    (70, 2, 1, 4, 2, 64, [40, 0, 33, 300, 1, 96, 64] * 10, [8, 1] * 70), (65, 20, 1, 2, 1, 112, [77] * 65, [3] * 1300),
+    (5, 9, 2, 8, 2, 144, [0, 700, 31, 33, 64], [2] * 45),
 ])
 def test_shared_attention(P, W, Tq, Hq, H, D, np, n, dtype):
     from axs.unified import axs_cache_shared_attention_unified
@@ -541,3 +574,146 @@ def test_results_repeat():
     for _ in range(3):
         again = axs_beam_select_unified(logits, scores, count=64), axs_cache_shared_attention_unified(q, prefix, np, cache, n)
         assert all(torch.equal(x, y) for x, y in zip(first[0], again[0])) and torch.equal(first[1], again[1])
+
+
+# ---- in the framework's own paths ------------------------------------------------------
+
+
+def _module(seed=0):
+    import axs.unified as axu
+
+    torch.manual_seed(seed)
+    m = axu.AXSCausalSelfAttentionUnified(128, 4, 2).to(DEV).eval()
+    return m, axu.rotary_table(32, 256, device=DEV)
+
+
+@pytest.mark.parametrize("P,W,T", [(1, 4, 1), (3, 2, 1), (2, 3, 5)])
+def test_decode_over_a_prefix(P, W, T):
+    """A module's beams over a shared prompt: its parts, and as though each beam had its prompt's copy."""
+    import axs.unified as axu
+
+    m, table = _module()
+    np = torch.tensor([64, 32, 0][:P], device=DEV)   # whole blocks: both caches hold the same codes and raw rows
+    with torch.no_grad():
+        prompts = torch.randn(P, 64, 128, generator=_gen(1)).to(DEV)
+        prefix = m.new_cache(P, 64, device=DEV)
+        m.decode(prompts, table, prefix, torch.zeros_like(np))
+        cache, parts, whole = m.new_cache(P * W, 40, device=DEV), m.new_cache(P * W, 40, device=DEV), m.new_cache(P * W, 120, device=DEV)
+        for b in range(P):
+            own = m.new_cache(1, 64, device=DEV)
+            if np[b]:
+                m.decode(prompts[b:b + 1, :int(np[b])], table, own, torch.zeros(1, dtype=torch.int64, device=DEV))
+            axu.axs_cache_copy_unified(own, torch.zeros(W, dtype=torch.int64, device=DEV), np[b:b + 1],
+                                       axu.AXSKVCacheUnified(*(x[b * W:(b + 1) * W] for x in whole)))
+        n = torch.zeros(P * W, dtype=torch.int64, device=DEV)
+        long = np.repeat_interleave(W)
+        for i in range(3):
+            x = torch.randn(P * W, T, 128, generator=_gen(10 + i)).to(DEV)
+            out = m.decode(x, table, cache, n, prefix, np)
+            q, k, v = m._heads(x)
+            q, k = axu.axs_rotary_unified(q, k, table, (long + n)[:, None] + torch.arange(T, device=DEV))
+            axu.axs_cache_append_unified(parts, k, v, n)
+            y = axu.axs_cache_shared_attention_unified(q, prefix, np, parts, n + T)
+            assert torch.equal(out, m.out_proj(y.flatten(2)))
+            axu.axs_cache_append_unified(whole, k, v, long + n)
+            want = axu.axs_cache_attention_unified(q, whole, long + n + T)
+            assert ref.rel(y, want) <= 2 * _bound(torch.float32)
+            n += T
+        with pytest.raises(ValueError):
+            m.decode(x, table, cache, n, prefix)
+        with pytest.raises(ValueError):
+            m.decode(x, table, cache, n, None, np)
+        with pytest.raises(ValueError):
+            m.decode(x[1:], table, cache, n[1:], prefix, torch.zeros(4, dtype=torch.int64, device=DEV))
+
+
+class _Reader:
+    """Logits that depend on each token of the history, read back from two caches: ids that the 8-bit codes hold
+    exactly (at most 100 of them, half a step off by less than half)."""
+
+    def __init__(self, G, W, V, starts, seed):
+        from axs.unified import AXSKVCacheUnified, axs_cache_append_unified
+
+        self.table = (2 * torch.randn(1009, V, generator=_gen(seed))).to(DEV)
+        self.caches = [AXSKVCacheUnified.empty(G * W, h, 16, 80, torch.float32, DEV) for h in (1, 3)]
+        self.prompt = torch.randint(0, V, (G, starts), generator=_gen(seed + 1))
+        rows = self.prompt.repeat_interleave(W, 0).to(DEV).float()[..., None, None]
+        for c in self.caches:
+            x = rows.expand(-1, -1, c.k_codes.shape[1], 16).contiguous()
+            axs_cache_append_unified(c, x, x, torch.zeros(G * W, dtype=torch.int64, device=DEV))
+
+    def logits(self, history):
+        h = torch.zeros(history.shape[0], dtype=torch.int64, device=history.device)
+        for t in range(history.shape[1]):
+            h = (31 * h + history[:, t] + 1) % 1009
+        return self.table[h.to(DEV)]
+
+    def __call__(self, tokens, starts):
+        from axs.unified import axs_cache_append_unified, axs_cache_read_unified
+
+        assert len(set(starts.tolist())) == 1
+        n = int(starts[0]) + 1
+        for c in self.caches:
+            x = tokens.float()[..., None, None].expand(-1, -1, c.k_codes.shape[1], 16).contiguous()
+            axs_cache_append_unified(c, x, -x, starts)
+        ids = [axs_cache_read_unified(c, torch.zeros_like(starts), n) for c in self.caches]
+        ids = [(k[..., 0, 3].round().long(), -v[..., -1, 7].round().long()) for k, v in ids]
+        for k, v in ids[1:]:
+            assert torch.equal(k, ids[0][0])
+        return self.logits(ids[0][0])[:, None]
+
+
+@pytest.mark.parametrize("G,W,V,steps,end,starts", [(1, 4, 60, 50, None, 0), (3, 5, 90, 40, 7, 0), (2, 3, 50, 45, 1, 29), (2, 1, 30, 9, 2, 3),
+                                                    (1, 6, 3, 4, 0, 1), (1, 2, 10, 1, 4, 0)])
+def test_beam_search(G, W, V, steps, end, starts):
+    """The loop keeps histories, caches and ends together: the search over plain histories in 64 bits."""
+    from axs.unified import axs_beam_search_unified
+
+    m = _Reader(G, W, V, starts, 30 + V)
+    start = torch.full((G * W,), starts, device=DEV)
+    got = axs_beam_search_unified(m, m.logits(m.prompt), m.caches, W, steps, end, start if starts else None)
+    assert int(start[0]) == starts
+    scores = torch.tensor([0.0] + [-math.inf] * (W - 1)).expand(G, W)
+    history, finished = m.prompt[:, None].expand(G, W, starts), torch.zeros(G, W, dtype=torch.bool)
+    for _ in range(steps):
+        z = m.logits(history.reshape(G * W, -1)).view(G, W, V)
+        scores, parents, tokens = beam_ref.select(z, scores, finished, 0 if end is None else end)
+        scores = scores.float()
+        history = torch.cat([history.gather(1, parents[..., None].expand_as(history)), tokens[..., None]], 2)
+        finished = finished.gather(1, parents) | (tokens == (-1 if end is None else end))
+    assert torch.equal(got[1].cpu(), history[..., starts:])
+    # a rounding and a sum's error a step
+    some = scores.isfinite()
+    assert torch.equal(got[0].cpu() == -math.inf, ~some)
+    bound = steps * beam_ref.select_bound(scores.double(), V)
+    assert ((got[0].cpu() - scores).abs()[some] <= bound[some]).all()
+
+
+def test_beam_search_refusals():
+    from axs.unified import axs_beam_search_unified as search
+
+    z = torch.zeros(2, 9, device=DEV)
+    for beams, steps in ((0, 3), (2, 0)):
+        with pytest.raises(ValueError):
+            search(None, z, [], beams, steps)
+    for bad in (lambda: search(None, z[0], [], 2, 1), lambda: search(None, z, [], 129, 1), lambda: search(lambda t, s: z, z, [], 2, 3)):
+        with pytest.raises((RuntimeError, IndexError)):
+            bad()
+
+
+def test_example_generates_with_beams():
+    import importlib.util
+    import os
+    import sys
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "axs-6_amd", "examples", "distill_decoder.py")
+    spec = importlib.util.spec_from_file_location("distill_decoder_beams", path)
+    ex = sys.modules[spec.name] = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ex)
+    torch.manual_seed(3)
+    m = ex.Decoder(ex.Config(vocab=64, context=64, width=128), True).to(DEV)
+    prompt = torch.randint(0, 64, (3, 21), generator=_gen(4)).to(DEV)
+    scores, tokens = m.generate_beams(prompt, 40, 4)
+    assert scores.shape == (3, 4) and tokens.shape == (3, 4, 61) and scores.isfinite().all()
+    assert (scores[:, 1:] <= scores[:, :-1]).all() and torch.equal(tokens[..., :21], prompt[:, None].expand(3, 4, 21))
+    assert len({tuple(x) for x in tokens.view(12, -1).tolist()}) == 12
