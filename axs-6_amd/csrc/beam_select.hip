@@ -34,6 +34,7 @@ constexpr int kMaxBeams = AXS6_BEAM_MAX_BEAMS, kMaxCount = AXS6_BEAM_MAX_COUNT;
 constexpr int kList = 256;       // items that are ranked by comparing all with all: at most these,
 constexpr int kDirect = 160;     // and from here on a cut pays (the work grows with the square)
 constexpr int kBins = 2048;
+constexpr int kAhead = 4;        // vectors of the chosen segments that a thread has on their way
 constexpr int kHeld = 8;         // items that a thread holds
 static_assert(kMaxCount <= kDirect && kDirect <= kList);
 constexpr float kLog2e = 1.4426950408889634f;
@@ -266,30 +267,28 @@ __global__ __launch_bounds__(kSelThreads) void beam_select_kernel(BeamArgs a) {
         const int sg = v >> a.vecs_log2, w = seg_beam[sg], j = seg_token[sg] + (v & (vecs - 1)) * E::V;
         return w >= 0 && j < a.V ? load_vector<DT>(z0 + w * a.ld_beam, j, a.V) : raw;
     };
-    // its candidates that do
-    auto candidates = [&](int v, u32x4 raw, auto f) {
-        const int sg = v >> a.vecs_log2, w = seg_beam[sg], j = seg_token[sg] + (v & (vecs - 1)) * E::V;
-        if (w < 0) {
-            const uint64_t k = key_of(score[-1 - w]);
-            if ((v & (vecs - 1)) == 0 && k >= least) f(k, (-1 - w) * a.V + (int)a.end);
-            return;
-        }
+    // a bit for each of its values that may be a candidate; of an ended beam's first vector one
+    auto reach = [&](int v, int n, u32x4 raw) {
+        if (v >= n) return 0u;
+        const int sg = v >> a.vecs_log2, w = seg_beam[sg], at = (v & (vecs - 1)) * E::V;
         const float low = seg_low[sg];
         float x[E::V];
         E::unpack(raw, x);
-        float most = x[0];
+        uint32_t bits = 0;
 #pragma unroll
-        for (int e = 1; e < E::V; ++e) most = fmaxf(most, x[e]);
-        if (!(most >= low) || j >= a.V) return;
-#pragma unroll 1
-        for (int e = 0; e < E::V; ++e) {
-            float z = x[0];
+        for (int e = 0; e < E::V; ++e) bits |= (uint32_t)(x[e] >= low && x[e] != -INFINITY) << e;
+        return w < 0 ? (uint32_t)(at == 0) : seg_token[sg] + at < a.V ? bits : 0u;
+    };
+    // value e of it, where it is one
+    auto candidate = [&](int v, int e, u32x4 raw, auto f) {
+        const int sg = v >> a.vecs_log2, w = seg_beam[sg], j = seg_token[sg] + (v & (vecs - 1)) * E::V;
+        float x[E::V];
+        E::unpack(raw, x);
+        float z = x[0];
 #pragma unroll
-            for (int i = 1; i < E::V; ++i) z = e == i ? x[i] : z;
-            if (!(z >= low) || z == -INFINITY) continue;
-            const uint64_t k = key(w, z);
-            if (k >= least) f(k, w * a.V + j + e);
-        }
+        for (int i = 1; i < E::V; ++i) z = e == i ? x[i] : z;
+        const uint64_t k = w < 0 ? key_of(score[-1 - w]) : key(w, z);
+        if (k >= least) f(k, w < 0 ? (-1 - w) * a.V + (int)a.end : w * a.V + j + e);
     };
     auto list = [&](uint64_t k, int id) {
         const int at = atomicAdd(&s.listed, 1);
@@ -333,7 +332,10 @@ __global__ __launch_bounds__(kSelThreads) void beam_select_kernel(BeamArgs a) {
                     int d = 0;
                     bool is = false;
                     if (i < n && turn == kVectors) {
-                        candidates(i, read(i, n), [&](uint64_t x, int) { k = x > k ? x : k; });
+                        const u32x4 raw = read(i, n);
+#pragma unroll 1
+                        for (uint32_t hits = reach(i, n, raw); hits; hits &= hits - 1)
+                            candidate(i, __builtin_ctz(hits), raw, [&](uint64_t x, int) { k = x > k ? x : k; });
                         d = (source[i >> a.vecs_log2] << a.vecs_log2) + (i & (vecs - 1));
                         is = k != 0;
                     } else if (i < n) {
@@ -487,13 +489,22 @@ __global__ __launch_bounds__(kSelThreads) void beam_select_kernel(BeamArgs a) {
         }
         n = chosen << a.vecs_log2;
 #pragma unroll 1
-        for (int v = t; v - lane < n; v += 4 * kSelThreads) {   // four loads at a time
-            u32x4 raw[4];
+        for (int v = t; v - lane < n; v += kAhead * kSelThreads) {
+            u32x4 raw[kAhead];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) raw[i] = read(v + i * kSelThreads, n);
+            for (int i = 0; i < kAhead; ++i) raw[i] = read(v + i * kSelThreads, n);
+            // a bit for each value that may be a candidate: few have one, and the wave goes round as often as the lane with the most
+            uint64_t hits = 0;
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) hits |= (uint64_t)reach(v + i * kSelThreads, n, raw[i]) << (i * E::V);
 #pragma unroll 1
-            for (int i = 0; i < 4 && v + i * kSelThreads < n; ++i)
-                candidates(v + i * kSelThreads, i == 0 ? raw[0] : i == 1 ? raw[1] : i == 2 ? raw[2] : raw[3], list);
+            for (; hits; hits &= hits - 1) {
+                const int at = __builtin_ctzll(hits), i = at / E::V;
+                u32x4 r = raw[0];
+#pragma unroll
+                for (int q = 1; q < kAhead; ++q) r = i == q ? raw[q] : r;
+                candidate(v + i * kSelThreads, at % E::V, r, list);
+            }
         }
         __syncthreads();
         listed = s.listed <= kList;
@@ -521,7 +532,7 @@ BeamPlan beam_plan(int64_t rows, int64_t W, int64_t V, int64_t count, int dtype)
     while (per > kRowWaves && rows * ((p.units + per - 1) / per) < 2048) per /= 2;
     p.chunks = (p.units + per - 1) / per;
     // The choice looks at all segments, 8192 at a time, and at the vectors of those chosen; up to 160 segments spare it
-    // their cut.  Finer segments where that saves a quarter of this work (3 x 48 rows of 50001 31.9 -> 29.6 us), since
+    // their cut.  Finer segments where that saves a quarter of this work (3 x 48 rows of 50001, an eighth), since
     // they cost the first launch some (64 x 8 of 128000 28.8 -> 31.3), and where there are not four times as many as
     // are chosen: with as many, the last one's maximum is low and most logits pass it.
     int64_t least = -1;
