@@ -126,8 +126,9 @@ class AXSCausalSelfAttentionUnified(nn.Module):
             places = starts
             if prefix is not None:
                 P = prefix_lengths.numel()
-                if P == 0 or x.shape[0] % P:
-                    raise ValueError(f"{x.shape[0]} sequences do not divide among {P} prefixes")
+                if P == 0 or x.shape[0] % P or prefix.k_codes.shape[0] != P:
+                    raise ValueError(f"{x.shape[0]} sequences do not divide among {P} prefixes, or a cache of "
+                                     f"{prefix.k_codes.shape[0]} does not hold them")
                 places = starts + prefix_lengths.repeat_interleave(x.shape[0] // P, output_size=x.shape[0])
             positions = places[:, None] + torch.arange(x.shape[1], device=x.device)
             q, k = axs_rotary_unified(q, k, table, positions)

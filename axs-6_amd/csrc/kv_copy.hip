@@ -66,7 +66,7 @@ __device__ __forceinline__ void arrived(T (&v)[kItems], int in_place) {
 
 // One workgroup a (group, head) and every gridDim.y-th piece of its places.
 template <int THREADS>
-__global__ __launch_bounds__(THREADS, 2048 / THREADS) void kv_copy_kernel(CopyArgs a) {
+__global__ __launch_bounds__(THREADS, 8) void kv_copy_kernel(CopyArgs a) {
     extern __shared__ int sh[];            // each target's source, and its length, 0 where nothing is copied
     __shared__ int top;
     int *from = sh, *len = sh + a.W;

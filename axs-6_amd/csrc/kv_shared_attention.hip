@@ -92,20 +92,6 @@ __device__ __forceinline__ Pieces even_pieces(const SharedArgs& a, int lane) {
 template <int ND> constexpr int kRow = ND <= 4 ? 4 : ND <= 8 ? 8 : 16;
 template <int ND> constexpr int kKeyBytes = kKvBlock * kRow<ND> * 16;
 template <int ND> constexpr int kSlotBytes = kKeyBytes<ND> + ND * 512;
-template <int ND> constexpr int kFetches = kRow<ND> / 2 + ND / 2;   // the instructions that fetch a block
-
-// Waits until at most `ahead` blocks (ahead <= MOST, uniform) are still on their way.
-template <int MOST, int FETCHES>
-__device__ __forceinline__ void wait_blocks(int ahead) {
-    if constexpr (MOST == 0) {
-        __builtin_amdgcn_s_waitcnt(0x0070 | (0xf << 8));   // vmcnt(0)
-    } else {
-        constexpr int N = MOST * FETCHES;
-        static_assert(N < 64, "vmcnt's range");
-        if (ahead >= MOST) __builtin_amdgcn_s_waitcnt((N & 0xf) | ((N >> 4) << 14) | (0x7 << 4) | (0xf << 8));
-        else wait_blocks<MOST - 1, FETCHES>(ahead);
-    }
-}
 
 // Piece j of key row r lies in place j ^ key_turn(r): the 16 rows that a fragment reads at one piece, 8 a + 4 tt + b, fall
 // on all banks.  Of r = 64 i / kRow + lane / kRow it is key_turn(64 i / kRow) ^ key_turn(lane / kRow).
@@ -326,7 +312,7 @@ struct Rows {
 
 // Up to 16 NR rows of one key head against blocks [b0, b1) of sequence `set` of a cache: S 0, a
 // prefix (rows of all its W sequences), or 1, a sequence's own.
-// SLOTS: of the wave's ring, the block that it computes on and those on their way.
+// SLOTS: of the wave's ring, 2 (the block that it computes on and the next one on its way) or 1.
 template <int DT, int ND, int NR, int S, int SLOTS>
 __device__ __forceinline__ void attend(const SharedArgs& a, char* ring, int set, int h, int rt, int b0, int b1,
                                        int64_t row0) {
@@ -347,11 +333,7 @@ __device__ __forceinline__ void attend(const SharedArgs& a, char* ring, int set,
         vs64 = mine < b1 ? a.vs[S][cell0 + mine] : 0.0f;
     };
     load_scales(b0 + wave);
-#pragma unroll
-    for (int i = 0; i < (SLOTS > 1 ? SLOTS - 1 : 1); ++i) {
-        const int blk = b0 + wave + i * kSharedWaves;
-        if (blk < b1) fetch_block<ND>(my_ring + i * kSlotBytes<ND>, a.kc[S], a.vc[S], cell0 + blk, a.D, lane);
-    }
+    if (b0 + wave < b1) fetch_block<ND>(my_ring, a.kc[S], a.vc[S], cell0 + b0 + wave, a.D, lane);
     R rows;
     float largest = 0.0f;
     for (int i = b0 + lane; i < b1; i += 64) largest = fmaxf(largest, a.vs[S][cell0 + i]);
@@ -365,7 +347,7 @@ __device__ __forceinline__ void attend(const SharedArgs& a, char* ring, int set,
     for (int blk = b0 + wave; blk < b1; blk += kSharedWaves, ++step) {
         // the block is there
         asm volatile("" ::: "memory");
-        wait_blocks<(SLOTS > 2 ? SLOTS - 2 : 0), kFetches<ND>>((b1 - 1 - blk) / kSharedWaves);
+        __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
         asm volatile("" ::: "memory");
         if (step % 64 == 0 && step) {
             load_scales(blk);
@@ -374,10 +356,9 @@ __device__ __forceinline__ void attend(const SharedArgs& a, char* ring, int set,
         const float ks = lane_value(ks64, step % 64), vs = lane_value(vs64, step % 64);
         const char* slot = my_ring + at * kSlotBytes<ND>;
         // the slot of the block before is free: all reads of it have come back, for its products are done
-        if constexpr (SLOTS > 1) {
-            const int next = blk + (SLOTS - 1) * kSharedWaves, free_at = at == 0 ? SLOTS - 1 : at - 1;
-            if (next < b1) fetch_block<ND>(my_ring + free_at * kSlotBytes<ND>, a.kc[S], a.vc[S], cell0 + next, a.D, lane);
-            at = at + 1 == SLOTS ? 0 : at + 1;
+        if constexpr (SLOTS == 2) {
+            at ^= 1;
+            if (blk + kSharedWaves < b1) fetch_block<ND>(my_ring + at * kSlotBytes<ND>, a.kc[S], a.vc[S], cell0 + blk + kSharedWaves, a.D, lane);
         }
         // Codes are read a step ahead, and the steps stand apart (sched_barrier): else the compiler, with all reads
         // first, wants more registers than there are.
@@ -464,7 +445,7 @@ __device__ __forceinline__ void attend(const SharedArgs& a, char* ring, int set,
     for (int n = 0; n < NR; ++n) rows.store(a, n, r0, row0, mt[n], lt[n], lane);
 }
 
-// The form for many rows of a prefix: each wave has rows of its own, 16 NR of the workgroup's 64 NR, and all take each
+// The form for many rows of a prefix: each wave has 16 rows of its own, and all take each
 // block.  Its codes are turned into f16 once for all of them, in registers on their way from memory to LDS: one buffer
 // is computed on while the next block's goes into the other, a barrier a block.
 // LDS: key rows of kWideRow 16-byte pieces, piece j of row 8 a + 4 tt + b in place j ^ turn; value rows of 32 keys, piece j of
@@ -500,14 +481,14 @@ __device__ __forceinline__ void spread_codes(char* tile, const WideCodes& x, con
     }
 }
 
-template <int DT, int ND, int NR>
+template <int DT, int ND>
 __device__ __forceinline__ void attend_wide(const SharedArgs& a, char* lds, int set, int h, int rt, int b0, int b1, int64_t row0) {
-    using R = Rows<DT, ND, NR, 0>;
+    using R = Rows<DT, ND, 1, 0>;
     constexpr int TERMS = R::TERMS, NC = R::NC;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n16 = lane & 15, g4 = lane >> 4;
     const int len = clamp_length(a.lengths[0][set], a.nb[0]);
     const int64_t cell0 = ((int64_t)set * a.H + h) * a.nb[0];
-    const int r0 = (rt * kSharedWaves + wave) * NR * 16;
+    const int r0 = (rt * kSharedWaves + wave) * 16;
     const bool rows_here = r0 < a.rows[0];   // the other waves only turn codes
     // where the thread's codes go: keys, row i / (D / 16), pieces 2 (i % (D / 16)) and the next; values, row i / 2, pieces
     // 2 (i % 2) and the next
@@ -555,9 +536,7 @@ __device__ __forceinline__ void attend_wide(const SharedArgs& a, char* lds, int 
         if (step % 64 == 0 && step) load_scales(blk);
         const float ks = lane_value(ks64, step % 64), vs = lane_value(vs64, step % 64);
         if (rows_here) {
-            f32x4 s[NR][2];
-#pragma unroll
-            for (int n = 0; n < NR; ++n) s[n][0] = s[n][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            f32x4 s[1][2] = {};
             auto key_codes = [&](int i) {
                 return *reinterpret_cast<const f16x8*>(tile + (key_at ^ i / 2 * 64) + i % 2 * 4 * kWideRow<ND> * 16);
             };
@@ -567,19 +546,15 @@ __device__ __forceinline__ void attend_wide(const SharedArgs& a, char* lds, int 
                 if (i / 2 * 2 >= ND) continue;   // past the head
                 const f16x8 k = key_codes(i);
 #pragma unroll
-                for (int n = 0; n < NR; ++n)
-#pragma unroll
-                    for (int u = 0; u < TERMS; ++u) s[n][i % 2] = mma(k, rows.qf[n][u][i / 4][i / 2 % 2], s[n][i % 2]);
+                for (int u = 0; u < TERMS; ++u) s[0][i % 2] = mma(k, rows.qf[0][u][i / 4][i / 2 % 2], s[0][i % 2]);
             }
-            f16x8 pf[NR][TERMS];
+            f16x8 pf[1][TERMS];
             rows.weigh(s, ks, vs, blk, lane, pf);
 #pragma unroll
             for (int d = 0; d < ND; ++d) {
                 const f16x8 v = value_codes(d);
 #pragma unroll
-                for (int n = 0; n < NR; ++n)
-#pragma unroll
-                    for (int u = 0; u < TERMS; ++u) rows.o[n][d] = mma(v, pf[n][u], rows.o[n][d]);
+                for (int u = 0; u < TERMS; ++u) rows.o[0][d] = mma(v, pf[0][u], rows.o[0][d]);
             }
         }
         if (blk + 1 < b1) spread_codes<ND>(other, next, to, a.D);
@@ -591,11 +566,8 @@ __device__ __forceinline__ void attend_wide(const SharedArgs& a, char* lds, int 
     }
     if (!rows_here) return;
     rows.finish();
-#pragma unroll
-    for (int n = 0; n < NR; ++n) {
-        rows.rescale(n, rows.m[n]);
-        rows.store(a, n, r0, row0, rows.m[n], rows.l[n], lane);
-    }
+    rows.rescale(0, rows.m[0]);
+    rows.store(a, 0, r0, row0, rows.m[0], rows.l[0], lane);
 }
 
 // NO: 16-row pieces of a sequence's own rows.  A prefix's go 16 to a wave, all four waves' against each block; heads of
@@ -642,7 +614,7 @@ __global__ __launch_bounds__(kSharedThreads, (SharedForm<DT, ND, NO>::kOccupancy
         p = __builtin_amdgcn_readfirstlane(p);
         b0 = __builtin_amdgcn_readfirstlane(b0);
         b1 = __builtin_amdgcn_readfirstlane(b1);
-        if constexpr (F::kWide) attend_wide<DT, ND, 1>(a, lds, p, h, rt, b0, b1, (int64_t)unit * a.rows[0]);
+        if constexpr (F::kWide) attend_wide<DT, ND>(a, lds, p, h, rt, b0, b1, (int64_t)unit * a.rows[0]);
         else attend<DT, ND, F::kPrefix, 0, F::kSlots>(a, lds, p, h, rt, b0, b1, (int64_t)unit * a.rows[0]);
     } else {
         const int i = blockIdx.x - a.prefix_groups, piece = i % a.pieces[1], j = i / a.pieces[1];

@@ -400,6 +400,28 @@ def test_shared_values_of_any_size(size, own, W, dtype):
     assert ref.rel(out.double() / top, want / top) <= _bound(dtype)
 
 
+@pytest.mark.parametrize("D,blocks", [(128, 33000), (256, 16500)])
+@pytest.mark.parametrize("W", [1, 24])
+def test_shared_past_32_bits(W, D, blocks):
+    """Prefixes and own tokens that lie more than 2^32 bytes into their caches."""
+    from axs.unified import AXSKVCacheUnified, axs_cache_append_unified, axs_cache_shared_attention_unified
+
+    dt = torch.bfloat16
+    prefix = AXSKVCacheUnified.empty(3, 12, D, 32 * blocks, dt, DEV)
+    cache = AXSKVCacheUnified.empty(3 * W, 12, D, 32 * blocks // W, dt, DEV)
+    assert prefix.k_codes[2].storage_offset() > 1 << 32 or prefix.k_codes.numel() > 1 << 32
+    values = []
+    for c, tokens, seed in ((prefix, 300, 3), (cache, 40, 4)):
+        k, v = _tokens(c.k_codes.shape[0], tokens, 12, D, dt, seed)
+        axs_cache_append_unified(c, k, v, torch.zeros(k.shape[0], dtype=torch.int64, device=DEV))
+        values.append([(ref.cache_values(k[b]), ref.cache_values(v[b])) for b in range(k.shape[0])])
+    np, n = torch.tensor([300, 7, 290], device=DEV), torch.full((3 * W,), 40, device=DEV)
+    q = torch.randn(3 * W, 1, 12, D, generator=_gen(7)).to(DEV, dt)
+    out = axs_cache_shared_attention_unified(q, prefix, np, cache, n)
+    want = beam_ref.shared_attention(q, values[0], np.tolist(), values[1], n.tolist())
+    assert ref.rel(out[-W:], want[-W:]) <= _bound(dt) and ref.rel(out[:W], want[:W]) <= _bound(dt)
+
+
 @pytest.mark.parametrize("W", [2, 40])
 def test_a_bad_block_counts_where_it_is_seen(W):
     from axs.unified import AXSKVCacheUnified, axs_cache_append_unified, axs_cache_shared_attention_unified
@@ -625,6 +647,8 @@ def test_decode_over_a_prefix(P, W, T):
             m.decode(x, table, cache, n, None, np)
         with pytest.raises(ValueError):
             m.decode(x[1:], table, cache, n[1:], prefix, torch.zeros(4, dtype=torch.int64, device=DEV))
+        with pytest.raises(ValueError):
+            m.decode(x, table, cache, n, type(prefix)(*(t[:0] for t in prefix)), np)
 
 
 class _Reader:
