@@ -21,6 +21,13 @@
 // Turning codes into f16 costs as much as a block's softmax for 32 rows: a prefix's workgroup does it once for its four
 // waves' 64 rows, into LDS; rows of one sequence are few, and there each wave has blocks of its own, whose codes come
 // straight from memory into LDS.
+//
+// Measured (launch + join): a prefix of 32000 tokens for 128 sequences, 32 heads on 8 of 128, bf16, 125 + 9 us, 490
+// TFLOP/s; 8 of 16383 for 8 sequences each, 64 heads on 8, 59 + 9, 3.1 TB/s; 3 of 7777 for 21 sequences of 5 queries, 12
+// heads on 4 of 80, f16, 26 + 9; one of 300 for 4 sequences, f32, 7.5 + 4.5.  At the first: vector instructions (150 a block
+// and 16 rows, 40 of them for the codes) fill 60% of the time, LDS 46%, the matrix cores 23%, and waits for LDS and the
+// others' part of a tile the rest.  16 rows a wave at four workgroups a CU against 32 rows, which read LDS half as often,
+// at two: 140 us against 185.
 #include "kv_attention.h"
 
 namespace axs6 {
@@ -31,7 +38,7 @@ typedef __attribute__((address_space(3))) void lds_void;
 constexpr int kSharedWaves = 4, kSharedThreads = 64 * kSharedWaves;
 constexpr float kSlack = 4.0f;          // in units of log2
 constexpr int kWeightLog2 = 11;         // probabilities go in times 2^11; with 2^kSlack still an f16
-constexpr int kSumLog2 = 20;            // kSumScale
+constexpr int kSumLog2 = 20;            // sums go out divided by 2^20
 constexpr int kMaxEven = 64;            // prefixes whose blocks are shared out evenly
 
 struct SharedArgs {
@@ -287,7 +294,7 @@ struct Rows {
         }
     }
 
-    // The sums of piece n from w to count from ref, in one step: a power of two, and 1 / kSumScale, which keeps sums of the
+    // The sums of piece n from w to count from ref, in one step: a power of two, and 2^-kSumLog2, which keeps sums of the
     // largest values finite, with it (w is -inf where a row saw nothing or values of 0).
     __device__ __forceinline__ void rescale(int n, float ref) {
         const float by = w[n] == -INFINITY ? 0.0f : w[n] - (ref == -INFINITY ? 0.0f : ref), whole_by = floorf(by);
