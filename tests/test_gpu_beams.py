@@ -598,6 +598,52 @@ def test_results_repeat():
         assert all(torch.equal(x, y) for x, y in zip(first[0], again[0])) and torch.equal(first[1], again[1])
 
 
+def test_two_graphs_and_two_streams():
+    """Two searches recorded apart and replayed by turns, then run at once on two streams: neither has the other's
+    workspaces."""
+    def run(a, n):
+        for _ in range(n):
+            _step(a)
+
+    def state(seed):
+        s = _state(2, 4, 90)
+        s["embed"] = torch.randn(90, 128, generator=_gen(seed)).to(DEV)
+        return s
+
+    want = [state(40), state(41)]
+    for w in want:
+        run(w, 5)
+    torch.cuda.synchronize()
+    recorded, graphs = [state(40), state(41)], []
+    for r in recorded:
+        kept = {k: v.clone() for k, v in r.items() if isinstance(v, torch.Tensor)}
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            _step(r)
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            _step(r)
+        graphs.append(graph)
+        for k, v in kept.items():
+            r[k].copy_(v)
+    for _ in range(5):
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+    at_once, streams = [state(40), state(41)], [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for a, stream in zip(at_once, streams):
+            with torch.cuda.stream(stream):
+                _step(a)
+    torch.cuda.synchronize()
+    for w, r, a in zip(want, recorded, at_once):
+        for k in ("scores", "tokens", "finished", "lengths"):
+            assert torch.equal(w[k], r[k]) and torch.equal(w[k], a[k]), k
+
+
 # ---- in the framework's own paths ------------------------------------------------------
 
 
