@@ -514,6 +514,7 @@ __global__ __launch_bounds__(kSelThreads) void beam_select_kernel(BeamArgs a) {
         }
         __syncthreads();
         listed = s.listed <= kList;
+        __syncthreads();   // all have read it: the next turn starts the list anew
         turn = kVectors;
     }
     for (int r = t; r < K; r += kSelThreads) {

@@ -169,6 +169,29 @@ def test_select_among_many_equal_tokens(dtype):
     assert torch.equal(got[2].cpu(), torch.stack([torch.arange(V - 200, V - 72), 5 + 601 * torch.arange(128)]))
 
 
+@pytest.mark.parametrize("dtype", ref.DTYPES)
+@pytest.mark.parametrize("W,ended,V,count", [(8, 4, 5000, 16), (80, 70, 900, 100), (40, 39, 40000, 128)])
+def test_more_equal_tokens_than_are_listed_behind_ended_beams(W, ended, V, count, dtype):
+    """The best segments are ended beams', which have no logits to wait for; of those behind them more tokens are
+    alike than one list holds, so a second choice follows the first at once."""
+    G = 24
+    logits = torch.zeros(G, W, V, device=DEV, dtype=dtype)
+    finished = torch.zeros(G, W, dtype=torch.bool, device=DEV)
+    finished[:, :ended] = True
+    scores = torch.where(finished, 0.0, -1.0)
+    want = beam_ref.select(logits[:1], scores[:1], finished[:1], 9, count)
+    for _ in range(5):
+        got = _beam_select(logits, scores, finished, 9, count)
+        assert torch.equal(got[1].cpu(), want[1].expand(G, -1)) and torch.equal(got[2].cpu(), want[2].expand(G, -1))
+        assert ((got[0].cpu() - want[0]).abs() <= beam_ref.select_bound(want[0], V)).all()
+
+
+def _beam_select(*args):
+    from axs.unified import axs_beam_select_unified
+
+    return axs_beam_select_unified(*args)
+
+
 def axs_select(logits, scores, count):
     from axs.unified import axs_beam_select_unified
 
