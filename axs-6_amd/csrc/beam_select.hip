@@ -162,7 +162,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void beam_rows_kernel(BeamArgs a) {
         const float ref = m == -INFINITY ? 0.0f : m;
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            float part = 0.0f;
+            double part = 0.0;
 #pragma unroll
             for (int j = 0; j < E::V; ++j) part += exp_diff(x[i][j], ref);
             sum += part;

@@ -1,0 +1,59 @@
+"""Beam search's operators on the GPU where single digits, orders or places count: peaked rows, large scores, value
+scales far apart, caches past 32 bits, what a search leaves in its caches."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import beam_ref
+import decoder_ref as ref
+from test_gpu_beams import _check_select, _gen
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+@pytest.mark.parametrize("dtype", ref.DTYPES)
+@pytest.mark.parametrize("V", [512, 4097, 50001])
+def test_peaked_rows_keep_their_order(V, dtype):
+    """Each beam's best token is all but certain, and the beams' scores for it lie 2e-8 apart.  A row's sum is then 1
+    and a rest r < 4e-3, in which each exponential is off by at most (2 + d) 2^-24 of itself, d the units that it lies below
+    the largest, less than 30 for all that count: log(1 + r) is off by 32 r 2^-24 < 8e-9, as long as the sum keeps more digits
+    than its terms."""
+    W, gap = 16, 2e-8
+    g = _gen(V)
+    logits = 2 * torch.randn(3, W, V, generator=g)
+    peak = torch.randint(0, V, (3, W, 1), generator=g)
+    logits = logits.scatter(2, peak, logits.amax(2, keepdim=True) + 11).to(dtype)
+    z = logits.double()
+    total = (z - z.amax(2, keepdim=True)).exp().sum(2).log()
+    assert (total < 4e-3).all()
+    place = torch.stack([torch.randperm(W, generator=g) for _ in range(3)])
+    scores = (total - 0.01 - gap * place).float()            # of about 0.01: steps of 1e-9
+    best = (scores.double() - total).sort(1, descending=True)
+    assert (best.values[:, :-1] - best.values[:, 1:] > 0.8 * gap).all() and torch.equal(best.indices, place.argsort(1))
+    _check_select(logits.to(DEV), scores.to(DEV), count=W)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_largest_vocabulary(dtype):
+    """One row of 2^31 - 1 tokens: its last ones, and more equal ones there than are listed."""
+    from axs.unified import axs_beam_select_unified
+
+    V = 2 ** 31 - 1
+    logits = torch.full((1, 1, V), -math.inf, device=DEV, dtype=dtype)
+    zero = torch.zeros(1, 1, device=DEV)
+    at = [V - 1, 0, V - 8, V - 2049, 1 << 30]
+    logits[0, 0, at] = torch.tensor([5.0, 4.0, 3.0, 2.0, 1.0], device=DEV, dtype=dtype)
+    total = math.log(sum(math.exp(x) for x in range(1, 6)))
+    got = axs_beam_select_unified(logits, zero, count=6)
+    assert got[2].tolist() == [at + [0]] and not got[1].any()
+    want = torch.tensor([[5.0, 4, 3, 2, 1, math.inf]]).double() - total
+    want[0, 5] = -math.inf
+    assert got[0][0, 5] == -math.inf
+    assert ((got[0].cpu() - want)[:, :5].abs() <= beam_ref.select_bound(want, 5)[:, :5]).all()
+    logits[0, 0, -700:] = 6
+    got = axs_beam_select_unified(logits, zero, count=128)
+    assert torch.equal(got[2][0].cpu(), torch.arange(V - 700, V - 572))
