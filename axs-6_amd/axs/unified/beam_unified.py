@@ -63,7 +63,7 @@ def axs_beam_search_unified(
         raise ValueError(f"{beams} beams of {steps} steps")
     G = logits.shape[0]
     scores, parents, tokens = axs_beam_select_unified(
-        logits[:, None], torch.zeros(G, 1, device=logits.device), count=beams)
+        logits[:, None], torch.zeros(G, 1, dtype=torch.float32, device=logits.device), count=beams)
     if starts is None:
         starts = torch.zeros(G * beams, dtype=torch.int64, device=logits.device)
     out = tokens[..., None]

@@ -9,7 +9,7 @@ import torch
 
 import beam_ref
 import decoder_ref as ref
-from test_gpu_beams import _check_select, _gen
+from test_gpu_beams import _check_select, _gen, _Reader
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -57,3 +57,17 @@ def test_the_largest_vocabulary(dtype):
     logits[0, 0, -700:] = 6
     got = axs_beam_select_unified(logits, zero, count=128)
     assert torch.equal(got[2][0].cpu(), torch.arange(V - 700, V - 572))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float64])
+def test_search_under_another_default_dtype(dtype):
+    from axs.unified import axs_beam_search_unified
+
+    m, other = _Reader(2, 3, 40, 0, 5), _Reader(2, 3, 40, 0, 5)
+    want = axs_beam_search_unified(m, m.logits(m.prompt), m.caches, 3, 6)
+    torch.set_default_dtype(dtype)
+    try:
+        got = axs_beam_search_unified(other, other.logits(other.prompt), other.caches, 3, 6)
+    finally:
+        torch.set_default_dtype(torch.float32)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
