@@ -58,7 +58,8 @@ def axs_beam_search_unified(
     that each holds (None: 0).  ``step(tokens (G * beams, 1), starts (G * beams))`` appends those
     tokens to the caches and returns the logits of the next, (G * beams, V) or (G * beams, 1, V);
     it is called ``steps - 1`` times.  A beam that chose ``end`` goes on as it, at its score.
-    Slots for which there is no candidate have the score -inf."""
+    Slots for which there is no candidate have the score -inf.  At the end the caches' sequences
+    are those of the returned beams, without their last tokens: ``steps - 1`` more each."""
     if beams < 1 or steps < 1:
         raise ValueError(f"{beams} beams of {steps} steps")
     G = logits.shape[0]
@@ -76,8 +77,7 @@ def axs_beam_search_unified(
         out = torch.cat([out.gather(1, parents[..., None].expand(-1, -1, i)), tokens[..., None]], -1)
         if end is not None:
             finished = finished.gather(1, parents) | (tokens == end)
-        if i + 1 < steps:
-            for cache in caches:
-                axs_cache_copy_unified(cache, parents, starts)
-            starts = starts.view(G, beams).gather(1, parents).flatten()
+        for cache in caches:
+            axs_cache_copy_unified(cache, parents, starts)
+        starts = starts.view(G, beams).gather(1, parents).flatten()
     return scores, out

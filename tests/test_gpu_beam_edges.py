@@ -71,3 +71,18 @@ def test_search_under_another_default_dtype(dtype):
     finally:
         torch.set_default_dtype(torch.float32)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("G,W,V,steps,starts", [(1, 4, 60, 2, 0), (3, 5, 90, 33, 0), (2, 3, 50, 20, 29)])
+def test_search_leaves_its_beams_in_the_caches(G, W, V, steps, starts):
+    """Each sequence of the caches ends as its returned beam: the prompt and all tokens but the last."""
+    from axs.unified import axs_beam_search_unified, axs_cache_read_unified
+
+    m = _Reader(G, W, V, starts, 7 + V)
+    start = torch.full((G * W,), starts, device=DEV)
+    scores, tokens = axs_beam_search_unified(m, m.logits(m.prompt), m.caches, W, steps, None, start)
+    assert scores.isfinite().all()
+    want = torch.cat([m.prompt.repeat_interleave(W, 0), tokens.cpu().view(G * W, steps)[:, :-1]], 1)
+    for c in m.caches:
+        k, _ = axs_cache_read_unified(c, torch.zeros_like(start), starts + steps - 1)
+        assert torch.equal(k[..., -1, 3].round().long().cpu(), want)
