@@ -73,7 +73,7 @@ def axs_beam_search_unified(
         logits = step(tokens.view(-1, 1), starts)
         starts = starts + 1
         scores, parents, tokens = axs_beam_select_unified(
-            logits.reshape(G, beams, -1), scores, finished, end)
+            logits.reshape(G, beams, logits.shape[-1]), scores, finished, end)
         out = torch.cat([out.gather(1, parents[..., None].expand(-1, -1, i)), tokens[..., None]], -1)
         if end is not None:
             finished = finished.gather(1, parents) | (tokens == end)

@@ -86,3 +86,11 @@ def test_search_leaves_its_beams_in_the_caches(G, W, V, steps, starts):
     for c in m.caches:
         k, _ = axs_cache_read_unified(c, torch.zeros_like(start), starts + steps - 1)
         assert torch.equal(k[..., -1, 3].round().long().cpu(), want)
+
+
+def test_search_of_no_prompts():
+    from axs.unified import AXSKVCacheUnified, axs_beam_search_unified
+
+    cache = AXSKVCacheUnified.empty(0, 2, 16, 40, torch.float32, DEV)
+    scores, tokens = axs_beam_search_unified(lambda t, s: torch.zeros(0, 1, 9, device=DEV), torch.zeros(0, 9, device=DEV), [cache], 3, 5, 4)
+    assert scores.shape == (0, 3) and tokens.shape == (0, 3, 5)
