@@ -212,17 +212,20 @@ struct Rows {
     // Block blk's products s with the queries, of scales ks and vs, to the weights pf of its values.
     __device__ __forceinline__ void weigh(f32x4 (&s)[NR][2], float ks, float vs, int blk, int lane, f16x8 (&pf)[NR][TERMS]) {
         const int g4 = lane >> 4;
-        float c[NR], lv[NR];   // what takes the products to units of log2; log2 of the value scale
+        // log2 of the value scale is le + lm: where a later block, which some rows do not see, has values of the largest
+        // size, vs 2^-unit may be too small for float32, and the sum of both parts has lost digits
+        const float le = (float)(__builtin_amdgcn_frexp_expf(vs) - unit);
+        float c[NR], lm[NR];   // c takes the products to units of log2
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
             c[n] = rs[n] * ks;
             c[n] = c[n] == 0.0f ? 1e-30f : c[n];   // so that it leaves -inf what it is
-            lv[n] = __builtin_amdgcn_logf(ldexpf(vs, -unit));
+            lm[n] = __builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(vs));
         }
         if ((blk + 1) * kKvBlock > whole) {
 #pragma unroll
             for (int n = 0; n < NR; ++n) {
-                if (blk * kKvBlock > last[n]) { c[n] = 1.0f; lv[n] = 0.0f; }   // a row that sees none of it, whatever its scales
+                if (blk * kKvBlock > last[n]) { c[n] = 1.0f; lm[n] = 0.0f; }   // a row that sees none of it, whatever its scales
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                     if (blk * kKvBlock + 8 * g4 + j > last[n]) s[n][j >> 2][j & 3] = -INFINITY;
@@ -236,14 +239,14 @@ struct Rows {
 #pragma unroll
             for (int j = 1; j < 8; ++j) top[n] = fmaxf(top[n], s[n][j >> 2][j & 3]);
             top[n] *= c[n];
-            passed = passed || top[n] > m[n] + kSlack || top[n] + lv[n] > w[n] + kSlack;
+            passed = passed || top[n] > m[n] + kSlack || top[n] + (le + lm[n]) > w[n] + kSlack;
         }
         if (__any(passed)) {
 #pragma unroll
             for (int n = 0; n < NR; ++n) {
                 float mx = fmaxf(top[n], __shfl_xor(top[n], 16, 64));
                 mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-                const float mn = fmaxf(m[n], mx), wn = fmaxf(w[n], mx + lv[n]);
+                const float mn = fmaxf(m[n], mx), wn = fmaxf(w[n], mx + (le + lm[n]));
                 l[n] *= __builtin_amdgcn_exp2f(m[n] - (mn == -INFINITY ? 0.0f : mn));
                 const float alpha = __builtin_amdgcn_exp2f(w[n] - (wn == -INFINITY ? 0.0f : wn));
                 m[n] = mn;
@@ -258,7 +261,7 @@ struct Rows {
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
             const float ref = w[n] == -INFINITY ? 0.0f : w[n], from = m[n] == -INFINITY ? 0.0f : m[n];
-            const float shift = lv[n] - ref, to_l = -from - shift;
+            const float shift = (le - ref) + lm[n], to_l = -from - shift;
             far = far || !(fabsf(to_l) < 60.0f);
             back[n] = __builtin_amdgcn_exp2f(to_l - kWeightLog2);
             float sum = 0.0f, y[8];

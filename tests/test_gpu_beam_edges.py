@@ -9,7 +9,7 @@ import torch
 
 import beam_ref
 import decoder_ref as ref
-from test_gpu_beams import _check_select, _gen, _Reader
+from test_gpu_beams import _bound, _check_select, _gen, _Reader
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -94,3 +94,38 @@ def test_search_of_no_prompts():
     cache = AXSKVCacheUnified.empty(0, 2, 16, 40, torch.float32, DEV)
     scores, tokens = axs_beam_search_unified(lambda t, s: torch.zeros(0, 1, 9, device=DEV), torch.zeros(0, 9, device=DEV), [cache], 3, 5, 4)
     assert scores.shape == (0, 3) and tokens.shape == (0, 3, 5)
+
+
+# ---- attention over a shared prefix ------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("W", [2, 40])
+def test_shared_values_of_the_largest_size_where_they_are_not_seen(W, dtype):
+    """Later tokens of nearly the type's largest size, in the prefix and among a sequence's own: queries before them
+    keep theirs, of 1e-3, to the last digit."""
+    from axs.unified import AXSKVCacheUnified, axs_cache_append_unified, axs_cache_shared_attention_unified
+
+    def filled(B, n, first, seed):
+        g = _gen(seed)
+        k, v = (torch.randn(B, n, 1, 64, generator=g).to(DEV, dtype) for _ in range(2))
+        v *= 1e-3
+        v[:, first:] = 0.9 * torch.finfo(dtype).min
+        c = AXSKVCacheUnified.empty(B, 1, 64, n, dtype, DEV)
+        axs_cache_append_unified(c, k, v, torch.zeros(B, dtype=torch.int64, device=DEV))
+        return c, [(ref.cache_values(x), ref.cache_values(y)) for x, y in zip(k, v)]
+
+    q = torch.randn(W, 40, 2, 64, generator=_gen(3)).to(DEV, dtype)
+    # own tokens from 32 on: of 60, the last 40 are the queries (two blocks are one workgroup's)
+    (prefix, pv), (cache, ov) = filled(1, 64, 64, 1), filled(W, 60, 32, 2)
+    call = axs_cache_shared_attention_unified
+    out = call(q, prefix, torch.tensor([64], device=DEV), cache, torch.full((W,), 60, device=DEV))
+    want = beam_ref.shared_attention(q, pv, [64], ov, [60] * W)
+    assert ref.rel(out[:, :12], want[:, :12]) <= _bound(dtype)
+    assert ref.rel(out[:, 12:].double() / 2e38, want[:, 12:] / 2e38) <= _bound(dtype)
+    # the prefix's from 32 on: of 64 + 1 tokens the last 40 are the queries, the first seven of which stand before them
+    (prefix, pv), (cache, ov) = filled(1, 64, 32, 4), filled(W, 1, 1, 5)
+    out = call(q, prefix, torch.tensor([64], device=DEV), cache, torch.full((W,), 1, device=DEV))
+    want = beam_ref.shared_attention(q, pv, [64], ov, [1] * W)
+    assert ref.rel(out[:, :7], want[:, :7]) <= _bound(dtype)
+    assert ref.rel(out[:, 7:].double() / 2e38, want[:, 7:] / 2e38) <= _bound(dtype)
