@@ -37,6 +37,9 @@ typedef __attribute__((address_space(3))) void lds_void;
 
 constexpr int kSharedWaves = 4, kSharedThreads = 64 * kSharedWaves;
 constexpr float kSlack = 4.0f;          // in units of log2
+// A maximum from which the products first become their distances from it: with the value scale's exponent added at once
+// that would lose its digits (below, 1e-5 of a weight, of which f16 keeps 2^-12; float32's always do).
+constexpr float kLarge = 256.0f;
 constexpr int kWeightLog2 = 11;         // probabilities go in times 2^11; with 2^kSlack still an f16
 constexpr int kSumLog2 = 20;            // sums go out divided by 2^20
 constexpr int kMaxEven = 64;            // prefixes whose blocks are shared out evenly
@@ -256,32 +259,44 @@ struct Rows {
             }
         }
         // exponentials with the value scale in them; l's are the same ones but for a factor, where that is not too far off
-        bool far = false;
-        float back[NR];
+        bool far = false, large = TERMS == 2;
+        float back[NR], from[NR];
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
-            const float ref = w[n] == -INFINITY ? 0.0f : w[n], from = m[n] == -INFINITY ? 0.0f : m[n];
-            const float shift = (le - ref) + lm[n], to_l = -from - shift;
-            far = far || !(fabsf(to_l) < 60.0f);
-            back[n] = __builtin_amdgcn_exp2f(to_l - kWeightLog2);
+            from[n] = m[n] == -INFINITY ? 0.0f : m[n];
+            back[n] = (le - ((w[n] == -INFINITY ? 0.0f : w[n]) - from[n])) + lm[n];
+            far = far || !(fabsf(back[n]) < 60.0f);
+            large = large || !(fabsf(from[n]) < kLarge);
+        }
+        if (TERMS == 2 || __any(large)) {   // the products become their distances from the maximum
+#pragma unroll
+            for (int n = 0; n < NR; ++n) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) s[n][j >> 2][j & 3] = __builtin_fmaf(s[n][j >> 2][j & 3], c[n], -from[n]);
+                c[n] = 1.0f;
+                from[n] = 0.0f;
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+            const float add = back[n] + kWeightLog2, all = add - from[n];
             float sum = 0.0f, y[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                y[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][j >> 2][j & 3], c[n], shift + kWeightLog2));
+                y[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][j >> 2][j & 3], c[n], all));
                 sum += y[j];
                 pf[n][0][j] = (_Float16)y[j];
                 if constexpr (TERMS == 2) pf[n][1][j] = (_Float16)(y[j] - (float)pf[n][0][j]);
             }
-            back[n] *= sum;
+            back[n] = __builtin_amdgcn_exp2f(-add) * sum;
             __builtin_amdgcn_sched_barrier(0);
         }
         if (__any(far)) {
 #pragma unroll
             for (int n = 0; n < NR; ++n) {
-                const float from = m[n] == -INFINITY ? 0.0f : m[n];
                 back[n] = 0.0f;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) back[n] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][j >> 2][j & 3], c[n], -from));
+                for (int j = 0; j < 8; ++j) back[n] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][j >> 2][j & 3], c[n], -from[n]));
             }
         }
 #pragma unroll

@@ -9,7 +9,7 @@ import torch
 
 import beam_ref
 import decoder_ref as ref
-from test_gpu_beams import _bound, _check_select, _gen, _Reader
+from test_gpu_beams import _bound, _check_select, _filled, _gen, _Reader
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -129,3 +129,37 @@ def test_shared_values_of_the_largest_size_where_they_are_not_seen(W, dtype):
     want = beam_ref.shared_attention(q, pv, [64], ov, [1] * W)
     assert ref.rel(out[:, :7], want[:, :7]) <= _bound(dtype)
     assert ref.rel(out[:, 7:].double() / 2e38, want[:, 7:] / 2e38) <= _bound(dtype)
+
+
+@pytest.mark.parametrize("dtype", ref.DTYPES)
+@pytest.mark.parametrize("D", [64, 192])
+@pytest.mark.parametrize("W", [2, 40])
+@pytest.mark.parametrize("size", [64.0, 4000.0, 40000.0, 1e6])
+def test_shared_large_scores(W, size, D, dtype):
+    """Queries of up to `size` along one key each, whose score passes all others by so much that its value alone
+    counts: the output is that value, whatever the score's own size and rounding."""
+    from axs.unified import axs_cache_shared_attention_unified
+
+    if size > torch.finfo(dtype).max:
+        return
+    g = _gen(int(size) + W)
+    prefix, pv = _filled(1, 200, 2, D, dtype, 200, 21)
+    cache, ov = _filled(W, 40, 2, D, dtype, 64, 22)
+    at = torch.randint(0, 240, (W, 1, 4), generator=g)
+    at[:, :, 0] = at[:, :, 0] % 200                      # a prefix's key, and one of the sequence's own
+    at[:, :, 1] = 200 + at[:, :, 1] % 40
+    keys = [torch.cat([pv[0][0], k]) for k, _ in ov]
+    values = [torch.cat([pv[0][1], v]) for _, v in ov]
+    q = torch.stack([torch.stack([keys[b][at[b, 0, h], h // 2] for h in range(4)]) for b in range(W)])[:, None]
+    q = (q / q.norm(dim=-1, keepdim=True) * size * math.sqrt(D) / 8).to(dtype)
+    # what the others' probabilities come to, from the values that the call is given
+    x = torch.stack([torch.einsum("hd,thd->ht", q[b, 0].double(), keys[b].double().repeat_interleave(2, 1)) for b in range(W)]) / math.sqrt(D)
+    best = x.gather(2, at.view(W, 4, 1))
+    rest = (x.scatter(2, at.view(W, 4, 1), -math.inf) - best).exp().sum(2)
+    sure = rest < 1e-8                                   # (a longer key of nearly the same direction may pass it)
+    assert sure.float().mean() > 0.6
+    out = axs_cache_shared_attention_unified(q.to(DEV), prefix, torch.tensor([200], device=DEV), cache,
+                                             torch.full((W,), 40, device=DEV))[:, 0].cpu()
+    want = torch.stack([torch.stack([values[b][at[b, 0, h], h // 2] for h in range(4)]) for b in range(W)])
+    for h in range(4):
+        assert ref.rel(out[:, h][sure[:, h]], want[:, h][sure[:, h]]) <= _bound(dtype), h
