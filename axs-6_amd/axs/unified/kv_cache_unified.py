@@ -98,7 +98,8 @@ def axs_cache_shared_attention_unified(
     query t sees the keys at places j <= prefix + own - Tq + t of them (none: 0).
     -> (B, Tq, Hq, D) of q's dtype, that of both caches' tails.  ``prefix_lengths`` (P) and
     ``lengths`` (B), int64 or int32, are read on the device.  ``scale`` as in
-    :func:`axs_cache_attention_unified`.  No gradient."""
+    :func:`axs_cache_attention_unified`.  No gradient: a ``q`` that records one, or carries a
+    forward-mode tangent, raises."""
     return _lib.ext().kv_shared_attention(q, *prefix, prefix_lengths, *cache, lengths, scale)
 
 

@@ -423,6 +423,7 @@ at::Tensor kv_shared_attention(const at::Tensor& q, const at::Tensor& pk_codes, 
     const Cache c = cache_of(k_codes, k_scales, v_codes, v_scales, k_tail, v_tail, fn);
     check_like(q, c.kt, 4, fn, "q");
     check_like(p.kt, c.kt, 4, fn, "the prefix's tail");
+    TORCH_CHECK(!records(q), fn, ": the cached tokens' attention has no gradient; detach q");
     const int64_t Tq = q.size(1), Hq = q.size(2);
     TORCH_CHECK(p.H == c.H && p.D == c.D && (p.B ? c.B % p.B == 0 : c.B == 0), fn, ": a prefix of ", p.B, " sequences, ", p.H,
                 " heads of ", p.D, " for a cache of ", c.B, " sequences, ", c.H, " heads of ", c.D);

@@ -163,3 +163,26 @@ def test_shared_large_scores(W, size, D, dtype):
     want = torch.stack([torch.stack([values[b][at[b, 0, h], h // 2] for h in range(4)]) for b in range(W)])
     for h in range(4):
         assert ref.rel(out[:, h][sure[:, h]], want[:, h][sure[:, h]]) <= _bound(dtype), h
+
+
+def test_a_gradient_or_tangent_of_no_operator_is_dropped():
+    import torch.autograd.forward_ad as fwAD
+
+    from axs.unified import axs_beam_select_unified, axs_cache_shared_attention_unified
+
+    prefix, _ = _filled(1, 40, 2, 32, torch.float32, 64, 1)
+    cache, _ = _filled(3, 40, 2, 32, torch.float32, 64, 2)
+    n1, n3 = torch.tensor([40], device=DEV), torch.full((3,), 40, device=DEV)
+    q = torch.randn(3, 1, 4, 32, generator=_gen(1)).to(DEV)
+    z, s = torch.randn(2, 3, 10, generator=_gen(2)).to(DEV), torch.zeros(2, 3, device=DEV)
+    attend = lambda x: axs_cache_shared_attention_unified(x, prefix, n1, cache, n3)   # noqa: E731
+    recorded = q.clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="no gradient"):
+        attend(recorded)
+    with torch.no_grad():
+        assert torch.equal(attend(recorded), attend(q))
+    assert torch.equal(attend(recorded.detach()), attend(q))
+    with fwAD.dual_level():
+        for call, x in ((attend, q), (lambda x: axs_beam_select_unified(x, s), z), (lambda x: axs_beam_select_unified(z, x), s)):
+            with pytest.raises(RuntimeError, match="no gradient"):
+                call(fwAD.make_dual(x, torch.ones_like(x)))
