@@ -186,3 +186,33 @@ def test_a_gradient_or_tangent_of_no_operator_is_dropped():
         for call, x in ((attend, q), (lambda x: axs_beam_select_unified(x, s), z), (lambda x: axs_beam_select_unified(z, x), s)):
             with pytest.raises(RuntimeError, match="no gradient"):
                 call(fwAD.make_dual(x, torch.ones_like(x)))
+
+
+# ---- copies ------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+def test_copies_of_sequences_that_start_past_32_bits(in_place):
+    """Five sequences of 1.1e9 bytes of key codes each: the third starts past 2^31 bytes, the fifth past 2^32."""
+    from axs.unified import AXSKVCacheUnified, axs_cache_copy_unified
+
+    blocks, D, B = 137_500, 256, 5
+    assert 2 * blocks * 32 * D > 1 << 31 and 4 * blocks * 32 * D > 1 << 32
+    g = torch.Generator(device=DEV).manual_seed(3)
+    sizes = [((blocks, 32, D), torch.int8), ((blocks,), torch.float32), ((blocks, D, 32), torch.int8), ((blocks,), torch.float32),
+             ((32, D), torch.bfloat16), ((32, D), torch.bfloat16)]
+    big = AXSKVCacheUnified(*(torch.empty(B, 1, *s, dtype=t, device=DEV) for s, t in sizes))
+    for x in big:
+        for y in x:
+            y.random_(-127, 128, generator=g)
+    n = 32 * blocks - 3
+    source = [4, 0, 3, 2, 1]
+    target = big if in_place else AXSKVCacheUnified(*(torch.zeros_like(x) for x in big))
+    old = [x.clone() for x in big]
+    axs_cache_copy_unified(big, torch.tensor(source, device=DEV), torch.full((B,), n, device=DEV), None if in_place else target)
+    for i, p in enumerate(source):
+        for x, y in zip(target[:4], old):
+            assert torch.equal(x[i], y[p])
+        for x, y in zip(target[4:], old[4:]):
+            assert torch.equal(x[i, :, :29], y[p, :, :29])
+            assert torch.equal(x[i, :, 29:], y[i, :, 29:] if in_place else torch.zeros_like(y[i, :, 29:]))
