@@ -25,7 +25,7 @@ def axs_beam_select_unified(
     beams: (scores float32, parents int64, tokens int64), each (G, count), best first.
 
     ``logits`` (G, W, V) float32, bfloat16 or float16, those of the next token after each of W beams
-    (at most 1024) of G sequences, and ``scores`` (G, W) float32, the beams' log probabilities.
+    (at most 1024, and 65535 of all sequences) of G sequences, and ``scores`` (G, W) float32, the beams' log probabilities.
     Token j after beam w scores ``scores[w] + log_softmax(logits[w])[j]``; equal ones stand
     in the order of beam, then token.  ``finished`` (G, W) bool: a beam that has ended goes
     on as one candidate, the token ``end`` with the beam's own score; its logits are not read.
@@ -35,7 +35,9 @@ def axs_beam_select_unified(
     -inf, parent 0 and token 0.  A NaN or +inf in a logit or score that counts makes the
     sequence's scores NaN, its parents and tokens 0.
 
-    Sums and comparisons are in float64, the scores are rounded once.  No gradient."""
+    Exponentials are float32, each off by some 2^-24 of itself; their sums, the scores and comparisons
+    are float64, and the scores are rounded once.  No gradient: logits or scores that record one, or
+    carry a forward-mode tangent, raise."""
     return _lib.ext().beam_select(logits, scores, finished, end, count)
 
 

@@ -21,10 +21,11 @@
 //
 // Bound by HBM where there are many rows, else by the second launch's chain of short steps on one CU a sequence.  Measured
 // (first + second launch): 64 x 8 rows of 128000 bf16, 16 chosen, 29 + 14 us, the first at 4.5 TB/s; 3 x 48 of 50001 f16,
-// 48 chosen, 9 + 16; 8 x 8 of 32000 f32, 16 chosen, 5.5 + 12; 4 rows of 256 4.4 + 8.  Of the second's 15 us at 3 x 48:
-// the rows' sums 2.8, reading and scoring 4704 segments 2, the cut to 160 of them 3, ranking 1.6, their 12288 vectors 4.2,
-// ranking 1.  Eight loads ahead instead of four there, or scoring whole vectors of which one logit counts, took 1 to 5 us
-// more.
+// 48 chosen, 9 + 16; 8 x 8 of 32000 f32, 16 chosen, 5.4 + 12; 4 rows of 256 4.4 + 8.  Of the second's 15 us at 3 x 48:
+// the rows' sums 2.8, reading and scoring 4704 segments 3.1, the cut to 160 of them 2.8, ranking 1, reading and scoring the
+// chosen ones' 3072 vectors, three a thread, 4.2, ranking 1.  Eight loads ahead instead of four there, or scoring whole
+// vectors of which one logit counts, took 1 to 5 us more.  (Eight exponentials added in float32 before the float64 sum:
+// 64 x 8 rows 39.8 us in all for 41.3, and scores of rows with one likely token off by 2e-7.)
 #include <math.h>
 
 #include "axs6_internal.h"
@@ -534,7 +535,8 @@ BeamPlan beam_plan(int64_t rows, int64_t W, int64_t V, int64_t count, int dtype)
     BeamPlan p;
     const int64_t vec = dtype == AXS6_F32 ? 4 : 8, unit = 64 * kLoads * vec;
     p.units = (V + unit - 1) / unit;
-    // eight units a wave, or fewer where the rows are few
+    // eight units a wave, or fewer where that makes less than 2048 workgroups (512: 3 x 48 rows of 50001 24.3 -> 26.0 us;
+    // 8192: 64 x 8 of 128000 41.3 -> 44.2)
     int64_t per = 8 * kRowWaves;
     while (per > kRowWaves && rows * ((p.units + per - 1) / per) < 2048) per /= 2;
     p.chunks = (p.units + per - 1) / per;
@@ -542,6 +544,9 @@ BeamPlan beam_plan(int64_t rows, int64_t W, int64_t V, int64_t count, int dtype)
     // their cut.  Finer segments where that saves a quarter of this work (3 x 48 rows of 50001, an eighth), since
     // they cost the first launch some (64 x 8 of 128000 28.8 -> 31.3), and where there are not four times as many as
     // are chosen: with as many, the last one's maximum is low and most logits pass it.
+    // In vectors' worth of time each further 8192 segments are 4096 (16384: 4 x 200 rows of 32000, 128 chosen, 57 -> 61 us;
+    // 0: the same there, 1 x 64 of 128000 47 -> 41), the cut 2048 (0: 64 x 8 of 128000 41 -> 44, 2 x 2 of 300000 29 -> 27;
+    // 8192: 64 x 64 of 1000 25 -> 27).
     int64_t least = -1;
     for (int level = 2; level >= 0; --level) {
         const int log2 = level == 2 ? 8 : level == 1 ? 6 : 4;

@@ -12,17 +12,19 @@
 // 8 beams, 2047 tokens, 8 heads of 128 (950 MB) in 208 us, 4.6 TB/s; 256 sequences of 375
 // to 1500 tokens closed up, 4 heads of 64 (200 MB), in 43 us, 4.7 TB/s; a prompt of 4001
 // tokens forked 8 ways for 8 groups, 12 heads of 80, in 66 us; four beams of 40 tokens in
-// 5 us, of which the launch and the chain sources - lengths - codes are all.
+// 4 us, of which the launch and the chain sources - lengths - codes are all.
 //
 // - A head's blocks lie behind one another in both caches, so a piece is one run of 16-byte
 //   places and a thread keeps the same sequences through all its pieces: what remains a
 //   piece is a load, in place a barrier, and a store.  (Finding tensor, sequence and length
 //   anew for each value: 96 us for the 256 sequences.)
 // - A workgroup takes 1024 threads where a group is so large that fewer would leave a
-//   sequence less than a cache line of a piece.  Two of 1024 or eight of 256 fit a CU; calls
+//   sequence less than a cache line of a piece (256 sequences closed up 42 us, with 256 threads 58, 1000 of them 202
+//   and 729; 17 sequences 7.7, with 1024 8.2).  Two of 1024 or eight of 256 fit a CU; calls
 //   of few pieces start just as many workgroups as fit (1 x 134 sequences of 288 tokens:
-//   8.8 us, one workgroup a piece 12.0), long ones four times that, so that the last ones
-//   to end are short (32 x 8 beams: 208 us, as many as fit 238).
+//   8.8 us, one workgroup a piece 12.0), those of more than 12 times as
+//   many pieces four times that, so that the last ones to end are short (32 x 8 beams: 208 us, as many as fit 238; from 3
+//   times as many on, 256 sequences closed up 42 -> 47, from 48, the beams 238).
 // - Stores pass the L2 by: what a fork reads stays there for its other sequences (95 us
 //   without, for 66; beams 219 for 214, closing up 45 for 43).
 // - Loading the next piece before this one is stored was slower at all sizes (43 to 48 us

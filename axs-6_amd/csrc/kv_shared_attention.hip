@@ -17,14 +17,18 @@
 // Products as in the cache attention (S^T = K q^T by 16x16x32 f16 instructions in which codes are exact, probabilities
 // stay in their lanes).  A block's value scale goes into its probabilities' exponent, which counts from a reference of
 // its own; the references move only when a score passes them by kSlack, and between that the sums stay where the products
-// add to them.  Probabilities go in as f16 times 2^11 (float32: two terms), 11 bits down to 2^-25 of the largest.
+// add to them.  Probabilities go in as f16 times 2^11 (float32: two terms): 11 bits down to 2^-25 of the largest, and some
+// down to 2^-35 (the cache attention has 2^14, 2^-28 and 2^-38: its reference is the maximum itself).  Beside a bf16
+// output's own rounding that does not count; f16 outputs are off by 2.7e-4 where their rounding alone makes 2.1e-4 (a second
+// term for f16 too would make it that: 32000 tokens for 128 sequences 145 -> 172 us, 3 x 21 of 5 queries 37.7 -> 40.5).
 // Turning codes into f16 costs as much as a block's softmax for 32 rows: a prefix's workgroup does it once for its four
 // waves' 64 rows, into LDS; rows of one sequence are few, and there each wave has blocks of its own, whose codes come
 // straight from memory into LDS.
 //
-// Measured (launch + join): a prefix of 32000 tokens for 128 sequences, 32 heads on 8 of 128, bf16, 125 + 9 us, 490
-// TFLOP/s; 8 of 16383 for 8 sequences each, 64 heads on 8, 59 + 9, 3.1 TB/s; 3 of 7777 for 21 sequences of 5 queries, 12
-// heads on 4 of 80, f16, 26 + 9; one of 300 for 4 sequences, f32, 7.5 + 4.5.  At the first: vector instructions (150 a block
+// Measured (launch + join): a prefix of 32000 tokens for 128 sequences, 32 heads on 8 of 128, bf16, 131 + 9 us, 490
+// TFLOP/s; 8 of 16383 for 8 sequences each, 64 heads on 8, 60 + 9, 3.1 TB/s; 3 of 7777 for 21 sequences of 5 queries, 12
+// heads on 4 of 80, f16, 27.5 + 9.4; one of 300 for 4 sequences, f32, 8.8 + 4.8.  The join takes 9.3 us for 24 MB of sums as
+// for 36: a chain of exponentials and rescaling over a row's 15 to 19 pieces.  At the first: vector instructions (150 a block
 // and 16 rows, 40 of them for the codes) fill 60% of the time, LDS 46%, the matrix cores 23%, and waits for LDS and the
 // others' part of a tile the rest.  16 rows a wave at four workgroups a CU against 32 rows, which read LDS half as often,
 // at two: 140 us against 185.
@@ -36,13 +40,15 @@ namespace {
 typedef __attribute__((address_space(3))) void lds_void;
 
 constexpr int kSharedWaves = 4, kSharedThreads = 64 * kSharedWaves;
-constexpr float kSlack = 4.0f;          // in units of log2
+constexpr float kSlack = 4.0f;          // in units of log2 (0: 32000 tokens for 128 sequences 148 -> 154 us, 2: 149)
 // A maximum from which the products first become their distances from it: with the value scale's exponent added at once
 // that would lose its digits (below, 1e-5 of a weight, of which f16 keeps 2^-12; float32's always do).
 constexpr float kLarge = 256.0f;
 constexpr int kWeightLog2 = 11;         // probabilities go in times 2^11; with 2^kSlack still an f16
 constexpr int kSumLog2 = 20;            // sums go out divided by 2^20
-constexpr int kMaxEven = 64;            // prefixes whose blocks are shared out evenly
+// Prefixes whose blocks are shared out evenly, a lane of a wave each (four of 8000 tokens beside 60 of 300, 4 sequences
+// each: 46 us, by prefix 115; 64 of 1000 50 and 45, for the even cut's own work is 1 us and more).
+constexpr int kMaxEven = 64;
 
 struct SharedArgs {
     const void* q;
@@ -595,8 +601,10 @@ __device__ __forceinline__ void attend_wide(const SharedArgs& a, char* lds, int 
     rows.store(a, 0, r0, row0, rows.m[0], rows.l[0], lane);
 }
 
-// NO: 16-row pieces of a sequence's own rows.  A prefix's go 16 to a wave, all four waves' against each block; heads of
-// more than 128 values, whose tiles of f16 would leave one workgroup a CU, take the form with a ring for 16 (float32) or 32.
+// NO: 16-row pieces of a sequence's own rows.  A prefix's go 16 to a wave, all four waves' against each block.  Heads of
+// more than 128 values take the form with a ring (their tiles of f16, 28 to 32 KB each, are not built), for 16 rows (float32,
+// whose two terms want the registers) or 32 (64 sequences of 4 heads on 8000 tokens, 256 values, 52 us, 16 rows 54; 192 values
+// 43 and 46; where 16 rows are all, 8 sequences on 16000, 34 and 28.5).
 template <int DT, int ND, int NO>
 struct SharedForm {
     static constexpr bool kWide = ND <= 8;
@@ -738,10 +746,13 @@ SharedPlan shared_plan(int dtype, int64_t P, int64_t W, int64_t H, int64_t rows,
                        int64_t blocks) {
     SharedPlan p;
     p.np = D <= 128 ? 4 : dtype == AXS6_F32 ? 1 : 2;
+    // (512 queries of 4 heads, bf16, 45 us, 16 rows a wave 48; float32, 40 rows, 76 and 54)
     p.no = D > 128 || rows <= 16 ? 1 : 2;
     p.row_tiles[0] = (W * rows + 16 * p.np - 1) / (16 * p.np);
     p.row_tiles[1] = (rows + 16 * p.no - 1) / (16 * p.no);
-    // seven of eight workgroups that the card holds, of some blocks each
+    // seven of eight workgroups that the card holds, of some blocks each (four of eight: one prefix of 65536 tokens 37.5 ->
+    // 43.9 us, 32000 for 128 sequences 148 -> 156, 3 x 21 sequences of 5 queries 37.8 -> 35; all of them 8 x 8 sequences on
+    // 16383 75 -> 79; twice as many: hardly a case as short)
     const int64_t most = 224 * (D > 128 ? 1 : dtype == AXS6_F32 ? (p.no == 2 ? 2 : 3) : p.no == 2 ? 3 : 4);
     const int64_t groups = H * p.row_tiles[0], some = P * ((prefix_blocks + kFewest - 1) / kFewest);
     int64_t n = (most + groups - 1) / groups;
@@ -847,6 +858,8 @@ extern "C" int axs6_kv_shared_attention(const void* q, int32_t dtype, int64_t P,
         else if (D <= 192) launch_shared<DT, 12>(a, p, (unsigned)grid, st);
         else launch_shared<DT, 16>(a, p, (unsigned)grid, st);
         const int64_t all = B * H * rows, lanes = D / 4;
+        // a workgroup a row where there are few (one prefix of 65536 tokens, 32 rows: 37.5 us, else 52.8; 4096 rows 27.4, so
+        // 33.1)
         if (all < 1024) kv_shared_join_kernel<DT, true><<<(unsigned)all, kJoinSize, 0, st>>>(a);
         else kv_shared_join_kernel<DT, false><<<(unsigned)((all * lanes + kJoinSize - 1) / kJoinSize), kJoinSize, 0, st>>>(a);
     });

@@ -507,8 +507,8 @@ int axs6_kv_shared_attention(const void* q, int32_t dtype, int64_t P, int64_t W,
  * nonzero where a beam has ended; it offers (w, end) with its own score, its logits are
  * not read.  A logit of -inf is no candidate, nor is any of a beam of score -inf, whose
  * logits are not read.  Slots without a candidate: score -inf, parent and token 0.  A NaN or +inf that
- * counts: the sequence's scores NaN, parents and tokens 0.  Sums in float64; scores
- * rounded once to float32.  Outputs (G, count). */
+ * counts: the sequence's scores NaN, parents and tokens 0.  Exponentials in float32,
+ * sums and comparisons in float64; scores rounded once to float32.  Outputs (G, count). */
 #define AXS6_BEAM_MAX_COUNT 128
 #define AXS6_BEAM_MAX_BEAMS 1024   /* of a sequence; of all 65535 */
 int64_t axs6_beam_select_workspace(int64_t G, int64_t W, int64_t V, int64_t count, int32_t dtype);
